@@ -6,12 +6,12 @@ needs no GPU; calling an operator needs a ROCm device and the in-tree
 """
 from ictc_o3.operators import (EdgeTensorProduct, GraphMessage, PackedGraphMessage, channel_linear,
                                configure_symmetric_contraction, create_symmetric_contraction,
-                               direction_harmonics, normalized_silu)
+                               direction_harmonics, layer_norm, normalized_silu)
 
 __version__ = "0.1.0"
 
 __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
-    "channel_linear", "normalized_silu",
+    "channel_linear", "normalized_silu", "layer_norm",
 ]

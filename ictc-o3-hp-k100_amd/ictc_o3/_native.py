@@ -118,6 +118,11 @@ _SIGNATURES = {
     "ictc_sc_bwd_w": (_i, [_i, _i, _i, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_sc_jvp": (_i, [_i, _i, _i, _i, _p, _p, _i, _p, _i64, _p, _p, _p]),
     "ictc_sc_hvp": (_i, [_i, _i, _i, _i, _p, _p, _i, _p, _i64, _p, _p, _p, _p]),
+    "ictc_layer_norm_workspace_bytes": (_i64, [_i, _i64, _i]),
+    "ictc_layer_norm_fwd": (_i, [_i, _p, _i64, _i64, _i, _p, _p, ctypes.c_float, _p, _p, _p, _p]),
+    "ictc_layer_norm_bwd": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "ictc_layer_norm_bwd2": (_i, [_i, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                  _p]),
     "ictc_sc_bwd_w_jvp": (_i, [_i, _i, _i, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
 }
 

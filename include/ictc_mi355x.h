@@ -33,6 +33,9 @@ enum {
   ICTC_ERR_RUNTIME = -3      /* HIP launch / runtime failure */
 };
 
+/* Element types of the dense-layer entry points. */
+enum { ICTC_F32 = 0, ICTC_BF16 = 1, ICTC_F16 = 2 };
+
 /* Library version (major*10000 + minor*100 + patch). */
 int ictc_version(void);
 
@@ -725,6 +728,29 @@ int ictc_sc_table_bwd_w(int lmax, int target_lmax, int correlation, int channels
                         int64_t nodes, const float* grad, const float* tangent, const int32_t* species_ptr,
                         const int32_t* species_order, float* const* dweights, void* workspace,
                         int64_t workspace_bytes, void* stream);
+
+/* ---- Layer norm -----------------------------------------------------------
+ * y = (x - mean) * rstd * weight + bias over rows of `width` elements (1 to 16384)
+ * at pitch ldx, element type dtype (x, weight, bias, grad and all outputs alike);
+ * statistics and sums in FP32, each output rounded once.  weight / bias NULL: ones /
+ * zeros.  y and the other row outputs are packed [rows, width].  mean and rstd
+ * [rows] FP32 may both be NULL in fwd.  A row with NaN or infinity is NaN throughout.
+ *   bwd:  dx, dweight [width], dbias [width], each NULL to skip; zero rows give zero
+ *         dweight and dbias.
+ *   bwd2: the gradients of <v, dx> + <vweight, dweight> + <vbias, dbias> by x (dx), by
+ *         grad (dgrad) and by weight (dweight); vweight / vbias NULL: absent.
+ * The parameters' gradients are added in a fixed order over a workspace of
+ * ictc_layer_norm_workspace_bytes bytes (-1: an argument out of range).             */
+int64_t ictc_layer_norm_workspace_bytes(int dtype, int64_t rows, int width);
+int ictc_layer_norm_fwd(int dtype, const void* x, int64_t ldx, int64_t rows, int width, const void* weight,
+                        const void* bias, float eps, void* y, float* mean, float* rstd, void* stream);
+int ictc_layer_norm_bwd(int dtype, const void* x, int64_t ldx, const void* grad, int64_t ldg, int64_t rows, int width,
+                        const void* weight, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad, int64_t ldg, const void* v,
+                         int64_t ldv, const void* vweight, const void* vbias, int64_t rows, int width,
+                         const void* weight, const float* mean, const float* rstd, void* dx, void* dgrad,
+                         void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
