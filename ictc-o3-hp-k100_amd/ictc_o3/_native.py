@@ -20,6 +20,7 @@ _lib = None
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
+_d = ctypes.c_double
 
 _SIGNATURES = {
     "ictc_version": (_i, []),
@@ -123,6 +124,10 @@ _SIGNATURES = {
     "ictc_layer_norm_bwd": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_layer_norm_bwd2": (_i, [_i, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64,
                                   _p]),
+    "ictc_gradient_norm_workspace_bytes": (_i64, [_i]),
+    "ictc_gradient_norm": (_i, [_i, _i, _p, _p, _d, _p, _i64, _p]),
+    "ictc_adamw_step": (_i, [_i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _i64, _p, _p]),
+    "ictc_adamw_moments": (_i, [_i, _p, _p, _p, _p, _i64, _p, _p, _p]),
     "ictc_sc_bwd_w_jvp": (_i, [_i, _i, _i, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
 }
 

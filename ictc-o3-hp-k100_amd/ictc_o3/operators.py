@@ -13,11 +13,12 @@ from ictc_o3.basis import tables
 from ictc_o3.basis.ictd_irreps import EdgeWeightedPathPreservingTensorProduct
 from ictc_o3.ops import tensor_product as tpo
 from ictc_o3.ops.harmonics import harmonics_packed
+from ictc_o3.ops.layer_norm import DTYPES as DENSE_DTYPES, layer_norm as _layer_norm
 
 __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
-    "channel_linear", "normalized_silu",
+    "channel_linear", "normalized_silu", "layer_norm",
 ]
 
 
@@ -365,12 +366,11 @@ def configure_symmetric_contraction(module, **kwargs):
 
 
 def _dense_operand(name, value, device, what):
-    from ictc_o3.ops.layer_norm import DTYPES
     if not isinstance(value, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a tensor")
-    if value.device.type != "cuda":
+    if not value.is_cuda:
         raise ValueError(f"{what}: {name} must be on a ROCm (cuda) device")
-    if value.dtype not in DTYPES:
+    if value.dtype not in DENSE_DTYPES:
         raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16")
     if device is not None and value.device != device:
         raise ValueError(f"{what}: {name} must be on {device}")
@@ -383,15 +383,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     are FP32 and each result is rounded once.  Gradients of x, weight and bias, and once more of those (a loss on
     forces), run on kernels; a third derivative raises.  A row that holds NaN or infinity gives NaN."""
     _dense_operand("x", x, None, "layer_norm")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
+    shape = x.shape
+    if len(shape) < 1 or not 1 <= shape[-1] <= 16384:
         raise ValueError("layer_norm: x must have a last axis of 1 to 16384 elements")
     for name, value in (("weight", weight), ("bias", bias)):
-        if value is None:
-            continue
-        _dense_operand(name, value, x.device, "layer_norm")
-        if value.shape != x.shape[-1:] or value.dtype != x.dtype:
-            raise ValueError(f"layer_norm: {name} must have shape [{x.shape[-1]}] and the type of x")
+        if value is not None:
+            _dense_operand(name, value, x.device, "layer_norm")
+            if value.shape != shape[-1:] or value.dtype != x.dtype:
+                raise ValueError(f"layer_norm: {name} must have shape [{shape[-1]}] and the type of x")
     if not isinstance(eps, (int, float)) or isinstance(eps, bool) or not 0.0 <= eps < float("inf"):
         raise ValueError("layer_norm: eps must be a finite number, zero or more")
-    from ictc_o3.ops.layer_norm import layer_norm as impl
-    return impl(x, weight, bias, float(eps))
+    return _layer_norm(x, weight, bias, float(eps))

@@ -752,6 +752,34 @@ int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad
                          const void* weight, const float* mean, const float* rstd, void* dx, void* dgrad,
                          void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- AdamW over a list of tensors ------------------------------------------
+ * One step with decoupled weight decay, in FP32 arithmetic:
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+ *   p = (1 - lr wd) p - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
+ * params, grads, counts and starts are HOST arrays: device addresses (as integers) and
+ * element counts of `tensors` packed tensors of element type dtype (any element
+ * alignment), and where the moments of each begin in m and v, which are flat over all
+ * tensors (starts: ascending multiples of 256; NULL: each at the next multiple of 256).
+ * A tensor's moments take whole blocks of 256 elements, kept zero past its end;
+ * state_elements is what m and v hold.  bits 32: FP32 moments, scales NULL.  bits 8: one
+ * byte an element and an FP32 power-of-two scale per block: m in E4M3, v with five
+ * exponent and three mantissa bits (code c > 0 is (1 + (c mod 8) / 8) 2^(c div 8 - 31)
+ * scale).  norm: NULL, or what ictc_gradient_norm left in its workspace: the gradients
+ * are then taken times norm[1].  ictc_adamw_moments writes 8-bit moments as values.
+ *
+ * ictc_gradient_norm: workspace[0] = the 2-norm over all gradients, workspace[1] =
+ * min(1, max_norm / (norm + 1e-6)), both FP32 (sums in FP64 above 2,048 elements, in a
+ * fixed order); ictc_gradient_norm_workspace_bytes bytes.                            */
+int64_t ictc_gradient_norm_workspace_bytes(int tensors);
+int ictc_gradient_norm(int dtype, int tensors, const int64_t* grads, const int64_t* counts, double max_norm,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int ictc_adamw_step(int dtype, int bits, int tensors, const int64_t* params, const int64_t* grads,
+                    const int64_t* counts, const int64_t* starts, void* m, void* v, float* m_scale, float* v_scale,
+                    int64_t state_elements, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    int64_t step, const float* norm, void* stream);
+int ictc_adamw_moments(int dtype, const void* m, const void* v, const float* m_scale, const float* v_scale,
+                       int64_t elements, void* m_out, void* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,382 @@
+"""AdamW over many tensors against its formula in float64, its 8-bit moments against codes made by torch, the optimizer
+class against torch.optim.AdamW in float64, and refusals.
+
+Bounds: a moment takes at most seven roundings of FP32 (three of them the gradient's factor), a parameter nine, each
+2^-24 of a value no larger than the largest term: 9 * 2^-24 = 5.4e-7; the bound is 1e-6 of the largest value, times the
+number of steps taken.  A bfloat16 or float16 parameter is rounded once more: 2^-9 or 2^-11, the bounds are twice that.
+Codes and scales have to be equal, bit by bit: without a norm bound every operation on the moments is rounded alone.
+"""
+import copy
+
+import pytest
+import torch
+
+from helpers import rel_err
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.float32: 1e-6, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -10}
+HYPER = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.05)
+SIZES = [1, 3, 255, 256, 257, 64, 2047, 2048, 2049, 10000, 0, 17]
+
+
+def _formula(p, g, m, v, step, max_norm=None, *, lr, betas, eps, weight_decay):
+    norm = torch.cat([x.flatten() for x in g]).norm() if max_norm is not None else None
+    c = min(1.0, max_norm / (float(norm) + 1e-6)) if max_norm is not None else 1.0
+    out = []
+    for a, b, i, j in zip(p, g, m, v):
+        b = b * c
+        i = betas[0] * i + (1 - betas[0]) * b
+        j = betas[1] * j + (1 - betas[1]) * b * b
+        up = i / (1 - betas[0] ** step) / ((j / (1 - betas[1] ** step)).sqrt() + eps)
+        out.append((a * (1 - lr * weight_decay) - lr * up, i, j))
+    return [list(t) for t in zip(*out)], norm
+
+
+def _lists(sizes, dtype, seed, device, odd=False):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for scale in (0.3, 0.02):
+        ts = []
+        for n in sizes:
+            t = (scale * torch.randn(n + 1, generator=g)).to(dtype).to(device)
+            ts.append(t[1:] if odd else t[:-1].clone())
+        out.append(ts)
+    return out
+
+
+def _segments(flat, starts, sizes):
+    return [flat[a:a + n] for a, n in zip(starts, sizes)]
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.05, 1e6])
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_step_against_the_formula(device, dtype, odd, max_norm):
+    from ictc_o3 import adamw_segments, adamw_step
+    ps, gs = _lists(SIZES, dtype, 1, device, odd)
+    starts, total = adamw_segments(SIZES)
+    assert starts[:5] == [0, 256, 512, 768, 1024] and total % 256 == 0
+    m, v = torch.zeros(total, device=device), torch.zeros(total, device=device)
+    for step in (1, 2, 700):
+        old = [[t.double() for t in ts] for ts in (ps, gs, _segments(m, starts, SIZES), _segments(v, starts, SIZES))]
+        before = [t.clone() for t in gs]
+        norm = adamw_step(ps, gs, m, v, step=step, max_norm=max_norm, **HYPER)
+        (P, M, V), N = _formula(*old, step, max_norm, **HYPER)
+        assert all(torch.equal(a, b) for a, b in zip(gs, before))
+        assert (norm is None) == (max_norm is None)
+        if norm is not None:
+            assert norm.dtype == torch.float32 and norm.shape == () and abs(float(norm) - float(N)) < 1e-6 * float(N)
+        for got, ref, tol in ((ps, P, TOL[dtype]), (_segments(m, starts, SIZES), M, 1e-6),
+                              (_segments(v, starts, SIZES), V, 1e-6)):
+            assert rel_err(torch.cat([t.flatten() for t in got]), torch.cat(ref)) < tol
+        filled = torch.zeros(total, dtype=torch.bool, device=device)
+        for a, n in zip(starts, SIZES):
+            filled[a:a + n] = True
+        assert m[~filled].abs().max() == 0 and v[~filled].abs().max() == 0
+
+
+def test_more_tensors_than_one_launch_takes(device):
+    from ictc_o3 import adamw_segments, adamw_step
+    sizes = [1 + (i * 97) % 700 for i in range(263)]
+    ps, gs = _lists(sizes, torch.float32, 2, device)
+    starts, total = adamw_segments(sizes)
+    m, v = torch.zeros(total, device=device), torch.zeros(total, device=device)
+    old = [[t.double() for t in ts] for ts in (ps, gs, _segments(m, starts, sizes), _segments(v, starts, sizes))]
+    norm = adamw_step(ps, gs, m, v, step=1, max_norm=0.1, **HYPER)
+    (P, M, V), N = _formula(*old, 1, 0.1, **HYPER)
+    assert abs(float(norm) - float(N)) < 1e-6 * float(N)
+    assert rel_err(torch.cat(ps), torch.cat(P)) < 1e-6
+    assert rel_err(torch.cat(_segments(v, starts, sizes)), torch.cat(V)) < 1e-6
+
+
+# ---------------------------------------------------------------------------
+# 8 bits
+# ---------------------------------------------------------------------------
+
+
+def _encode(m, v):
+    """Codes and scales of FP32 moments [blocks, 256] by torch on the CPU."""
+    m, v = m.cpu().view(-1, 256), v.cpu().view(-1, 256)
+    em = (torch.frexp(m.abs().amax(1)).exponent - 8).clamp(-126, 126)
+    sm = torch.tensor([2.0 ** int(e) for e in em])
+    cm = (m.double() / sm.double()[:, None]).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    scale, codes = [], []
+    for row in v.double():
+        top = float(row.max())
+        mant, e = torch.frexp(torch.tensor(top, dtype=torch.float64))
+        e = int(e) - 1 + (1 if float(mant) >= 31.0 / 32.0 else 0)      # the maximum rounds up to the next power of two
+        e = max(-126, min(126, e)) if top > 0 else -126
+        y = row / 2.0 ** e
+        mant, k = torch.frexp(y)
+        q = torch.round(mant * 16)                                     # 8 .. 16, ties to even
+        k = k - 1 + (q == 16)
+        q = torch.where(q == 16, torch.full_like(q, 8.0), q)
+        c = ((k + 31) * 8 + q - 8).clamp(1, 255)
+        codes.append(torch.where(row > 0, c, torch.zeros_like(c)).to(torch.uint8))
+        scale.append(2.0 ** e)
+    return cm.view(-1), sm, torch.stack(codes).view(-1), torch.tensor(scale)
+
+
+def _values(c, s):
+    x = c.double()
+    return torch.where(x > 0, (1 + x % 8 / 8) * 2.0 ** (torch.div(x, 8, rounding_mode="floor") - 31), 0 * x) \
+        * s.double().repeat_interleave(256)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_codes_of_8_bit_moments(device, dtype):
+    from ictc_o3 import adamw_moments, adamw_segments, adamw_step
+    sizes = [300, 256, 5, 2304, 1, 700]
+    ps, gs = _lists(sizes, dtype, 3, device)
+    gs[1].mul_(1e6)
+    gs[2].zero_()
+    gs[3] *= torch.exp2(-torch.arange(2304, device=device) / 64).to(dtype)     # 36 binades within nine blocks
+    gs[5][::3] = 0
+    starts, total = adamw_segments(sizes)
+    m8 = torch.zeros(total, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    v8 = torch.zeros(total, dtype=torch.uint8, device=device)
+    sm, sv = torch.ones(total // 256, device=device), torch.ones(total // 256, device=device)
+    m, v = torch.zeros(total), torch.zeros(total)
+    b1, b2 = HYPER["betas"]
+    f = torch.float32
+    for step in range(1, 5):
+        old_p = torch.cat([p.double().flatten() for p in ps]).cpu()
+        adamw_step(ps, gs, m8, v8, step=step, exp_avg_scale=sm, exp_avg_sq_scale=sv, **HYPER)
+        for a, n, g in zip(starts, sizes, gs):
+            g = g.cpu().float()
+            m[a:a + n] = m[a:a + n] * torch.tensor(b1, dtype=f) + g * torch.tensor(1 - b1, dtype=f)
+            v[a:a + n] = v[a:a + n] * torch.tensor(b2, dtype=f) + g * g * torch.tensor(1 - b2, dtype=f)
+        new = []
+        for a, n in zip(starts, sizes):
+            up = m[a:a + n].double() / (1 - b1 ** step) / ((v[a:a + n].double() / (1 - b2 ** step)).sqrt() + 1e-8)
+            new.append(up)
+        ref = old_p * (1 - HYPER["lr"] * HYPER["weight_decay"]) - HYPER["lr"] * torch.cat(new)
+        assert rel_err(torch.cat([p.flatten() for p in ps]), ref) < TOL[dtype]
+        cm, cs, cv, vs = _encode(m, v)
+        assert torch.equal(m8.view(torch.uint8).cpu(), cm) and torch.equal(v8.cpu(), cv)
+        live = m.view(-1, 256).abs().amax(1) > 0
+        assert torch.equal(sm.cpu()[live], cs[live]) and torch.equal(sv.cpu()[live], vs[live])
+        assert ((v8.cpu() > 0) == (v > 0)).all()                               # nothing small became zero
+        for kind in (torch.float32, torch.bfloat16):
+            dm, dv = adamw_moments(m8, v8, sm, sv, dtype=kind)
+            m = (cm.view(torch.float8_e4m3fn).double() * cs.double().repeat_interleave(256)).float()
+            assert torch.equal(dm.cpu().float()[live.repeat_interleave(256)], m[live.repeat_interleave(256)])
+            v = _values(cv, vs).float()
+            assert torch.equal(dv.cpu().float(), v)
+
+
+def test_8_bit_moments_of_extreme_gradients(device):
+    """Values near both ends of FP32: scales are held to 2^-126 .. 2^126 and nothing becomes NaN."""
+    from ictc_o3 import adamw_moments, adamw_step
+    for size in (1e-38, 1e-25, 1e-12, 1e12, 1.5e19):
+        g = torch.full((256,), size, device=device)
+        p = torch.zeros(256, device=device)
+        m8 = torch.zeros(256, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        v8 = torch.zeros(256, dtype=torch.uint8, device=device)
+        sm, sv = torch.ones(1, device=device), torch.ones(1, device=device)
+        adamw_step([p], [g], m8, v8, step=1, exp_avg_scale=sm, exp_avg_sq_scale=sv, **{**HYPER, "eps": 0.0 if size > 1e-15 else 1e-8})
+        m, v = adamw_moments(m8, v8, sm, sv)
+        assert torch.isfinite(p).all() and torch.isfinite(m).all() and torch.isfinite(v).all()
+        assert abs(float(m[0]) / (0.1 * size) - 1) < 1 / 16 or size < 1e-36
+        if size * size > 1e-35:
+            assert abs(float(v[0]) / (0.01 * size * size) - 1) < 1 / 16
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nan_and_infinity_reach_only_their_own(device, bits):
+    from ictc_o3 import AdamW
+    for bad in (float("nan"), float("inf")):
+        ps = [torch.nn.Parameter(torch.ones(n, device=device)) for n in (700, 40)]
+        opt = AdamW(ps, state_bits=bits)
+        for p in ps:
+            p.grad = torch.full_like(p, 0.5)
+        ps[0].grad[300] = bad
+        opt.step()
+        fine = torch.ones(700, dtype=torch.bool, device=device)
+        fine[300] = False
+        assert torch.isfinite(ps[0][fine]).all() and not torch.isfinite(ps[0][300]) and torch.isfinite(ps[1]).all()
+        ps[0].grad[300] = 0.5
+        opt.step()
+        if bits == 8:     # the block's scale is lost with it: loud, and the other blocks go on
+            fine[256:512] = False
+        assert torch.isfinite(ps[0][fine]).all() and not torch.isfinite(ps[0][300])
+        assert torch.isfinite(ps[1]).all()
+
+
+def test_a_bound_with_a_non_finite_norm_is_loud(device):
+    from ictc_o3 import adamw_step
+    p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+    g[7] = float("nan")
+    m, v = torch.zeros(512, device=device), torch.zeros(512, device=device)
+    norm = adamw_step([p], [g], m, v, step=1, max_norm=1.0)
+    assert torch.isnan(norm) and torch.isnan(p).all()
+
+
+def test_offsets_past_32_bits(device):
+    """2^31 + 777 bfloat16 parameters with 8-bit moments: elements at both ends, against a small tensor's."""
+    from ictc_o3 import adamw_segments, adamw_step
+    n = 2 ** 31 + 777
+    _, total = adamw_segments([n])
+
+    def state(total):
+        return (torch.zeros(total, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                torch.zeros(total, dtype=torch.uint8, device=device), torch.ones(total // 256, device=device),
+                torch.ones(total // 256, device=device))
+
+    p = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    g = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    ends = torch.randn(1000, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(device)
+    p[:1000], g[:1000], p[-1000:], g[-1000:] = ends, ends.flip(0), ends, ends.flip(0)
+    m, v, sm, sv = state(total)
+    norm = adamw_step([p], [g], m, v, step=1, exp_avg_scale=sm, exp_avg_sq_scale=sv, max_norm=1e9, **HYPER)
+    small = ends.clone()
+    m2, v2, sm2, sv2 = state(1024)
+    adamw_step([small], [ends.flip(0)], m2, v2, step=1, exp_avg_scale=sm2, exp_avg_sq_scale=sv2, **HYPER)
+    assert torch.equal(p[:1000], small) and torch.equal(p[-1000:], small)
+    assert p[1000:2000].abs().max() == 0
+    assert abs(float(norm) - 2 ** 0.5 * float(ends.double().norm())) < 1e-5 * float(norm)
+
+
+# ---------------------------------------------------------------------------
+# The optimizer
+# ---------------------------------------------------------------------------
+
+
+def _pair(device, shapes, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    start = [torch.randn(s, generator=g, dtype=torch.float64) for s in shapes]
+    return ([torch.nn.Parameter(t.float().to(device)) for t in start],
+            [torch.nn.Parameter(t.float().double()) for t in start])
+
+
+def test_optimizer_against_torch(device):
+    """Eight steps with two groups, a learning rate schedule and a parameter that some steps give no gradient."""
+    from ictc_o3 import AdamW
+    ps, rs = _pair(device, [(7, 5), (300,), (2, 3, 64), (1,), (500,)])
+    groups = lambda q: [dict(params=q[:3], weight_decay=0.1), dict(params=q[3:], lr=1e-2)]  # noqa: E731
+    opt = AdamW(groups(ps), lr=1e-3, max_norm=0.7)
+    ref = torch.optim.AdamW(groups(rs), lr=1e-3, eps=1e-8)
+    sched = [torch.optim.lr_scheduler.StepLR(o, 3, 0.5) for o in (opt, ref)]
+    gen = torch.Generator().manual_seed(9)
+    for k in range(8):
+        for i, (p, r) in enumerate(zip(ps, rs)):
+            grad = torch.randn(r.shape, generator=gen)
+            skip = i == 1 and k in (0, 3)
+            p.grad, r.grad = (None, None) if skip else (grad.to(device), grad.double())
+        norm = torch.nn.utils.clip_grad_norm_([r for r in rs if r.grad is not None], 0.7)
+        opt.step()
+        ref.step()
+        for s in sched:
+            s.step()
+        assert abs(float(opt.grad_norm) - float(norm)) < 1e-6 * float(norm)
+    for p, r in zip(ps, rs):
+        assert rel_err(p, r) < 8e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_saved_state_continues_bit_by_bit(device, bits, dtype, tmp_path):
+    from ictc_o3 import AdamW
+    ps = [torch.nn.Parameter(p.detach().to(dtype)) for p in _pair(device, [(600,), (33, 9)])[0]]
+    opt = AdamW(ps, lr=1e-2, state_bits=bits)
+    gen = torch.Generator().manual_seed(4)
+    grads = [[torch.randn(p.shape, generator=gen).to(dtype).to(device) for p in ps] for _ in range(6)]
+
+    def steps(opt, ps, which):
+        for k in which:
+            for p, g in zip(ps, grads[k]):
+                p.grad = g
+            opt.step()
+
+    steps(opt, ps, range(3))
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    for how in ("file", "copy"):
+        qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+        if how == "file":
+            other = AdamW(qs, lr=1.0, state_bits=bits)
+            other.load_state_dict(torch.load(tmp_path / "opt.pt", weights_only=True))
+            assert other.param_groups[0]["lr"] == 1e-2
+        else:
+            other = copy.deepcopy(opt)
+            qs = other.param_groups[0]["params"]
+        keep = [p.detach().clone() for p in ps]
+        state = copy.deepcopy(opt.state_dict())
+        steps(other, qs, range(3, 6))
+        assert all(torch.equal(a, b) for a, b in zip(keep, ps))                 # the first one was left alone
+        mine = AdamW([torch.nn.Parameter(t) for t in keep], lr=1e-2, state_bits=bits)
+        mine.load_state_dict(state)
+        again = mine.param_groups[0]["params"]
+        steps(mine, again, range(3, 6))
+        assert all(torch.equal(a, b) for a, b in zip(again, qs)), how
+    wrong = AdamW([torch.nn.Parameter(p.detach().clone()) for p in ps], state_bits=40 - bits)
+    state = opt.state_dict()
+    state["param_groups"][0]["state_bits"] = 40 - bits
+    wrong.load_state_dict(state)
+    for p, g in zip(wrong.param_groups[0]["params"], grads[0]):
+        p.grad = g
+    with pytest.raises(ValueError, match="state"):
+        wrong.step()
+
+
+def test_8_bits_fit_as_well_as_32(device):
+    """A least-squares fit: both kinds of moments come down to the same loss within a tenth."""
+    from ictc_o3 import AdamW
+    g = torch.Generator().manual_seed(0)
+    A = torch.randn(512, 300, generator=g).to(device)
+    y = A @ torch.randn(300, 4, generator=g).to(device) + 0.5 * torch.randn(512, 4, generator=g).to(device)
+    loss = {}
+    for bits in (32, 8):
+        w = torch.nn.Parameter(torch.zeros(300, 4, device=device))
+        opt = AdamW([w], lr=2e-2, weight_decay=0.0, state_bits=bits)
+        for _ in range(400):
+            opt.zero_grad()
+            out = (A @ w - y).square().mean()
+            out.backward()
+            opt.step()
+        loss[bits] = float(out)
+    assert loss[8] < 1.1 * loss[32] < 0.2
+
+
+def test_a_step_outdates_what_was_read_of_a_parameter(device):
+    """Cached weight copies and saved graph inputs go by a tensor's version: a step has to change it."""
+    from ictc_o3 import AdamW
+    p = torch.nn.Parameter(torch.ones(64, 64, device=device))
+    x = torch.ones(2, 64, device=device, requires_grad=True)
+    y = (x @ p).sum()
+    before = p._version
+    p.grad = torch.ones_like(p)
+    AdamW([p]).step()
+    assert p._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_gradients_of_any_layout_and_other_streams(device):
+    from ictc_o3 import AdamW
+    ps = [torch.nn.Parameter(torch.ones(40, 30, device=device)) for _ in range(2)]
+    grad = torch.randn(30, 40, device=device)
+    ps[0].grad, ps[1].grad = grad.t(), grad.t().contiguous()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt = AdamW(ps)
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(ps[0], ps[1]) and not torch.equal(ps[0], torch.ones_like(ps[0]))
+
+
+def test_refusals(device):
+    from ictc_o3 import adamw_step
+    p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+    m, v = torch.zeros(512, device=device), torch.zeros(512, device=device)
+    bad = [dict(params=[p], grads=[]), dict(grads=[g.double()]), dict(grads=[g[:299]]), dict(params=[p.cpu()]),
+           dict(params=[torch.ones(600, device=device)[::2]]), dict(exp_avg=m[:256]), dict(exp_avg=m[:256], exp_avg_sq=v[:256]),
+           dict(exp_avg=m.double()), dict(step=0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(lr=float("nan")),
+           dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(exp_avg_scale=torch.ones(2, device=device))]
+    for change in bad:
+        args = dict(params=[p], grads=[g], exp_avg=m, exp_avg_sq=v, step=1)
+        args.update(change)
+        with pytest.raises(ValueError):
+            adamw_step(**args)
+    assert torch.equal(p, torch.ones_like(p))
+    assert adamw_step([], [], m, v, step=1) is None
