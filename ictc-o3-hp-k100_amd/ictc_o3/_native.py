@@ -124,6 +124,9 @@ _SIGNATURES = {
     "ictc_layer_norm_bwd": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_layer_norm_bwd2": (_i, [_i, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64,
                                   _p]),
+    "ictc_expert_linear": (_i, [_i, _p, _i64, _i64, _i, _p, _p, _i, _i, _p, _p, _i, _p, _p]),
+    "ictc_expert_outer_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i]),
+    "ictc_expert_outer": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_gradient_norm_workspace_bytes": (_i64, [_i]),
     "ictc_gradient_norm": (_i, [_i, _i, _p, _p, _d, _p, _i64, _p]),
     "ictc_adamw_step": (_i, [_i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _i64, _p, _p]),

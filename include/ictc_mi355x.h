@@ -752,6 +752,27 @@ int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad
                          const void* weight, const float* mean, const float* rstd, void* dx, void* dgrad,
                          void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Linears chosen per row by an expert id --------------------------------
+ * out[n] = W[e] x[n] + bias[e] with e the expert of row n, W [experts, outputs, inputs]
+ * (transpose == 0); or out[n] = W[e]^T x[n] with W [experts, inputs, outputs] read in
+ * place (transpose != 0, the adjoint by rows: `inputs` is always x's width and `outputs`
+ * out's).  Element type dtype throughout, FP32 sums, results rounded once; x at row pitch
+ * ldx, the other operands packed, any element alignment.  perm [rows] and offsets
+ * [experts + 2] as ictc_csr_build(ids, rows, experts) gives them; a row whose id is
+ * outside [0, experts) gets a zero row.  bias may be NULL.
+ *
+ * ictc_expert_outer: dweight[e] = sum over the rows of expert e of grad[n] x[n]^T
+ * ([experts, outputs, inputs]) and dbias[e] = sum of grad[n] (NULL: absent); zeros for an
+ * expert without rows; sums in a fixed order over a workspace of
+ * ictc_expert_outer_workspace_bytes bytes (0: none needed, -1: out of range).          */
+int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int inputs, const void* weight,
+                       const void* bias, int outputs, int experts, const int32_t* perm, const int32_t* offsets,
+                       int transpose, void* out, void* stream);
+int64_t ictc_expert_outer_workspace_bytes(int dtype, int64_t rows, int inputs, int outputs, int experts);
+int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int inputs,
+                      int outputs, int experts, const int32_t* perm, const int32_t* offsets, void* dweight,
+                      void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- AdamW over a list of tensors ------------------------------------------
  * One step with decoupled weight decay, in FP32 arithmetic:
  *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
