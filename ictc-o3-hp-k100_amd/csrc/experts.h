@@ -1,0 +1,139 @@
+// What the expert linears' kernels share: matrix instructions, runs of sorted rows, the order of blocks.
+#pragma once
+#include "dense.h"
+#include "split_bf16.h"
+
+namespace {
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ v4f mma(u32x4 a, u32x4 b, v4f c) {
+  if constexpr (sizeof(T) == 2 && !__is_same(T, bf16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+// Run `t` of groups 0 .. G - 1 cut into runs of `rows` sorted rows: its group, first sorted row and row count.  False
+// past the last run.  The same values in every lane of the wave, which has to be whole.
+struct Run {
+  int group, start, count;
+};
+
+// Sum over the wave's lanes up to each lane.
+__device__ __forceinline__ int scan_lanes(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(x, d);
+    if (lane >= d) x += up;
+  }
+  return x;
+}
+
+// `unit` of groups 0 .. G - 1 cut into units of `rows` sorted rows: its group, the group's first unit, sorted rows
+// and units.  False past the last unit, and then `first` is their number.
+struct Place {
+  int group, first, lo, count, units;
+};
+
+__device__ __forceinline__ bool find_unit(const int* __restrict__ off, int G, int rows, int unit, Place& p) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int s0 = 0; s0 < G; s0 += 64) {
+    const int s = s0 + lane;
+    int lo = 0, n = 0;
+    if (s < G) {
+      lo = off[s];
+      n = off[s + 1] - lo;
+    }
+    const int units = (n + rows - 1) / rows, sum = scan_lanes(units);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
+    if (unit < base + total) {
+      const int f = __builtin_ctzll(__ballot(base + sum > unit));
+      p.group = s0 + f;
+      p.units = __builtin_amdgcn_readlane(units, f);
+      p.first = base + __builtin_amdgcn_readlane(sum, f) - p.units;
+      p.lo = __builtin_amdgcn_readlane(lo, f);
+      p.count = __builtin_amdgcn_readlane(n, f);
+      return true;
+    }
+    base += total;
+  }
+  p.first = base;
+  return false;
+}
+
+__device__ __forceinline__ bool find_run(const int* __restrict__ off, int G, int rows, int t, Run& r) {
+  Place p;
+  if (!find_unit(off, G, rows, t, p)) return false;
+  const int at = (t - p.first) * rows;
+  r.group = p.group;
+  r.start = p.lo + at;
+  r.count = min(rows, p.count - at);
+  return true;
+}
+
+// The weights' gradient: the sorted rows of all experts, in steps of `rows` of one expert, are cut into `ranges` of
+// equal length; a block takes one tile of the output over one range and meets the experts in it in turn.  An expert
+// that lies within a range is done there; one that continues into others leaves FP32 partial sums, in slot 0 of each
+// range, or in slot 1 of the range that it begins in behind another.  Every range costs the same whatever the
+// experts' sizes, and there are as many partial sums as ranges and experts that cross them, not more.
+struct Ranges {
+  int steps, per;   // of all experts; of a range
+};
+
+__device__ __forceinline__ Ranges find_ranges(const int* __restrict__ off, int experts, int rows, int ranges) {
+  Place p;
+  find_unit(off, experts, rows, INT32_MAX, p);
+  return {p.first, max(1, (p.first + ranges - 1) / ranges)};
+}
+
+struct Segment {
+  int expert, start, count;   // sorted rows
+  int steps;                  // of this segment
+  bool whole;                 // the expert has no other
+  int slot;
+};
+
+// The segment that begins at step `u` of the range q = [q per, q per + per).
+__device__ __forceinline__ bool find_segment(const int* __restrict__ off, int experts, int rows, const Ranges& r,
+                                             int q, int u, Segment& s) {
+  Place p;
+  const int end = min(r.steps, (q + 1) * r.per);
+  if (u >= end || !find_unit(off, experts, rows, u, p)) return false;
+  const int last = min(end, p.first + p.units);
+  s.expert = p.group;
+  s.steps = last - u;
+  s.start = p.lo + (u - p.first) * rows;
+  s.count = min(s.steps * rows, p.count - (u - p.first) * rows);
+  s.whole = u == p.first && last == p.first + p.units;
+  s.slot = u > q * r.per;
+  return true;
+}
+
+// Block `b` of `blocks` in an order that gives each of the eight dies (blocks go to them in turn) a contiguous part.
+__device__ __forceinline__ int die_order(int b, int blocks) {
+  const int per = blocks / 8, rest = blocks % 8, die = b & 7;
+  return die * per + min(die, rest) + (b >> 3);
+}
+
+}  // namespace
+
+// The kernels of 16-bit types on aligned rows (experts_direct.hip).
+bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
+                         int N, int experts, const int* perm, const int* off, bool transpose, void* out,
+                         hipStream_t st);
+
+// Where the weights' gradient takes them, how it is cut: `tile` columns a side, `rows` of a step, `ranges`.
+struct OuterPlan {
+  bool direct;
+  int tile, rows, ranges;
+};
+bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K);
+void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,
+                          int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
+                          float* part, hipStream_t st);

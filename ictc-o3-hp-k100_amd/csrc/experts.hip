@@ -13,14 +13,11 @@
 // operands of a step are staged in LDS as [row][reduction index], 16-byte chunks XORed with the row so that neither
 // the stores nor the fragment reads share banks.  An operand whose memory runs along the other axis (the weights of
 // gx, both operands of gW) is transposed in registers on its way to LDS: eight rows of a few columns per thread.
-#include "dense.h"
-#include "split_bf16.h"
-
 #include <algorithm>
 
-namespace {
+#include "experts.h"
 
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+namespace {
 
 constexpr int kTile = 128;   // rows and columns of an output tile: four waves of 64 x 64
 
@@ -96,16 +93,6 @@ __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch,
   }
 }
 
-template <typename T>
-__device__ __forceinline__ v4f mma(u32x4 a, u32x4 b, v4f c) {
-  if constexpr (sizeof(T) == 2 && !__is_same(T, bf16))
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
-                                                  0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
-}
-
 // The product of one 16 x 16 block over 32 reduction indices from the operands' parts.
 template <typename T>
 __device__ __forceinline__ v4f product(const u32x4 (&a)[Config<T>::NP], const u32x4 (&b)[Config<T>::NP], v4f c) {
@@ -144,53 +131,6 @@ __device__ __forceinline__ void step(const uint16_t* __restrict__ A, const uint1
       for (int i = 0; i < 4; ++i) acc[i][j] = product<T>(a[i], b, acc[i][j]);
     }
   }
-}
-
-// Run `t` of groups 0 .. G - 1 cut into runs of `rows` sorted rows: its group, first row, row count, index within
-// the group and the group's runs.  ONE: a group without rows has one empty run.  False past the last run.  The same
-// values in every lane of the wave, which has to be whole.
-struct Run {
-  int group, start, count, index, runs;
-};
-
-template <bool ONE>
-__device__ __forceinline__ bool find_run(const int* __restrict__ off, int G, int rows, int t, Run& r) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int s0 = 0; s0 < G; s0 += 64) {
-    const int s = s0 + lane;
-    int lo = 0, n = 0, runs = 0;
-    if (s < G) {
-      lo = off[s];
-      n = off[s + 1] - lo;
-      runs = (n + rows - 1) / rows;
-      if (ONE && runs == 0) runs = 1;
-    }
-    int sum = runs;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(sum, d);
-      if (lane >= d) sum += up;
-    }
-    const int total = __builtin_amdgcn_readlane(sum, 63);
-    if (t < base + total) {
-      const int f = __builtin_ctzll(__ballot(base + sum > t));
-      r.group = s0 + f;
-      r.runs = __builtin_amdgcn_readlane(runs, f);
-      r.index = t - (base + __builtin_amdgcn_readlane(sum, f) - r.runs);
-      r.start = __builtin_amdgcn_readlane(lo, f) + r.index * rows;
-      r.count = min(rows, __builtin_amdgcn_readlane(n, f) - r.index * rows);
-      return true;
-    }
-    base += total;
-  }
-  return false;
-}
-
-// Block `b` of `blocks` in an order that gives each of the eight dies (blocks go to them in turn) a contiguous part.
-__device__ __forceinline__ int die_order(int b, int blocks) {
-  const int per = blocks / 8, rest = blocks % 8, die = b & 7;
-  return die * per + min(die, rest) + (b >> 3);
 }
 
 // A 128-row operand whose rows run along the reduction index.
@@ -249,7 +189,7 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
   const int columns = (N + kTile - 1) / kTile;
   const int b = die_order(blockIdx.x, gridDim.x);
   Run run;
-  if (!find_run<false>(off, experts + 1, kTile, b / columns, run)) return;
+  if (!find_run(off, experts + 1, kTile, b / columns, run)) return;
   const int n0 = b % columns * kTile;
   if (run.group == experts) {   // ids outside [0, experts): zero rows
     const int width = min(kTile, N - n0);
@@ -299,20 +239,29 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
     step<T>(As, Bs, wave >> 1, wave & 1, acc);
     __syncthreads();
   }
+  // all of the bias and row numbers are asked for before the first is needed
+  T bv[4][4];
+  T* row[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = n0 + 64 * (wave >> 1) + 16 * i + 4 * g;
-    float bv[4];
+    const T* bp = bias + (int64_t)run.group * N + c;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) bv[r] = bias && c + r < N ? (float)bias[(int64_t)run.group * N + c + r] : 0.f;
+    for (int q = 0; q < 4; ++q) bv[i][q] = bias && c + q < N ? bp[q] : (T)0.f;
+    const int r = 64 * (wave & 1) + 16 * i + li;
+    row[i] = out + (int64_t)perm[run.start + (r < run.count ? r : 0)] * N;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = 64 * (wave & 1) + 16 * j + li;
-      if (r >= run.count || c >= N) continue;
-      T* o = out + (int64_t)perm[run.start + r] * N + c;
+  for (int j = 0; j < 4; ++j) {
+    if (64 * (wave & 1) + 16 * j + li >= run.count) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = n0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+      if (c >= N) continue;
+      T* o = row[j] + c;
       T v[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = (T)(acc[i][j][q] + bv[q]);
+      for (int q = 0; q < 4; ++q) v[q] = (T)(acc[i][j][q] + (float)bv[i][q]);
       if (c + 4 <= N) {
         if constexpr (sizeof(T) == 4)
           *reinterpret_cast<u32x4_any*>(o) = *reinterpret_cast<const u32x4*>(v);
@@ -327,126 +276,149 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
   }
 }
 
-// Partial gradients of one run of an expert's rows: [M, K] of W (g^T x) and [M] of b (the blocks of column tile 0:
-// the product of g with ones).  A group of one run is done; the others leave FP32 sums, run by run, in `part`.
+// Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
+// over one range of rows.
 template <typename T>
-__global__ __launch_bounds__(256) void experts_outer_kernel(const T* __restrict__ gy, int64_t ldg, int M,
+__global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restrict__ gy, int64_t ldg, int M,
                                                             const T* __restrict__ x, int64_t ldx, int K, int experts,
-                                                            int rows, const int* __restrict__ perm,
+                                                            int ranges, const int* __restrict__ perm,
                                                             const int* __restrict__ off, T* __restrict__ gW,
                                                             T* __restrict__ gb, float* __restrict__ part) {
   using C = Config<T>;
   __shared__ __attribute__((aligned(16))) uint16_t As[C::NP * C::PART];
   __shared__ __attribute__((aligned(16))) uint16_t Bs[C::NP * C::PART];
   const int ct = (K + kTile - 1) / kTile, tiles = ct * ((M + kTile - 1) / kTile);
-  const int b = die_order(blockIdx.x, gridDim.x), t = b / tiles;
-  Run run;
-  if (!find_run<true>(off, experts, rows, t, run)) return;
+  const int b = die_order(blockIdx.x, gridDim.x), q = b / tiles;
   const int k0 = b % tiles % ct * kTile, m0 = b % tiles / ct * kTile;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-  Across<T> xs, gs;
-  const int cx = k0 + xs.column(), cg = m0 + gs.column(), r0 = 8 * xs.block();
-  auto load = [&](int s) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = s + r0 + j;
-      const bool ok = r < run.count;
-      const int64_t node = ok ? perm[run.start + r] : 0;
-      xs.v[j] = load_few(x + node * ldx + cx, ok ? K - cx : 0);
-      gs.v[j] = load_few(gy + node * ldg + cg, ok ? M - cg : 0);
-    }
-  };
+  const int64_t MK = (int64_t)M * K;
   const bool bias = gb != nullptr && k0 == 0 && wave < 2;
   const uint32_t one = sizeof(T) == 4 || __is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u;
-  v4f acc[4][4], accb[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    accb[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  // experts without rows: zeros, shared out over the ranges
+  for (int e = q; e < experts; e += ranges) {
+    if (off[e + 1] != off[e]) continue;
+    for (int i = threadIdx.x; i < kTile * kTile; i += 256)
+      if (m0 + i / kTile < M && k0 + i % kTile < K) gW[e * MK + (int64_t)(m0 + i / kTile) * K + k0 + i % kTile] = (T)0.f;
+    if (gb && k0 == 0 && threadIdx.x < kTile && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
   }
-  load(0);
-  for (int s = 0; s < run.count; s += C::BK) {
-    xs.store(As);
-    gs.store(Bs);
-    __syncthreads();
-    if (s + C::BK < run.count) load(s + C::BK);
-    step<T>(As, Bs, wave >> 1, wave & 1, acc);
-    if (bias) {
+  const Ranges r = find_ranges(off, experts, C::BK, ranges);
+  Across<T> xs, gs;
+  const int cx = k0 + xs.column(), cg = m0 + gs.column(), r0 = 8 * xs.block();
+  Segment s;
+  for (int u = q * r.per; find_segment(off, experts, C::BK, r, q, u, s); u += s.steps) {
+    int node[8];   // the row numbers of a step are read one step before its rows
+    auto name = [&](int row) {
 #pragma unroll
-      for (int kk = 0; kk < C::BK / 32; ++kk)
+      for (int j = 0; j < 8; ++j) node[j] = row + r0 + j < s.count ? perm[s.start + row + r0 + j] : -1;
+    };
+    auto load = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32x4 f[C::NP];
-          fragment<T>(Bs, 64 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
-#pragma unroll
-          for (int p = C::NP - 1; p >= 0; --p) accb[j] = mma<T>(u32x4{one, one, one, one}, f[p], accb[j]);
-        }
-    }
-    __syncthreads();
-  }
-  const bool whole = run.runs == 1;
-  const int64_t MK = (int64_t)M * K;
-  float* pw = part + (int64_t)t * (MK + M);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = m0 + 64 * (wave & 1) + 16 * j + li;
-    if (m >= M) continue;
-    if (bias && g == 0) {
-      if (whole)
-        gb[(int64_t)run.group * M + m] = (T)accb[j][0];
-      else
-        pw[MK + m] = accb[j][0];
-    }
+      for (int j = 0; j < 8; ++j) {
+        const int64_t n = max(node[j], 0);
+        xs.v[j] = load_few(x + n * ldx + cx, node[j] >= 0 ? K - cx : 0);
+        gs.v[j] = load_few(gy + n * ldg + cg, node[j] >= 0 ? M - cg : 0);
+      }
+    };
+    v4f acc[4][4], accb[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int k = k0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+      accb[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (k + q >= K) continue;
-        if (whole)
-          gW[(int64_t)run.group * MK + (int64_t)m * K + k + q] = (T)acc[i][j][q];
+      for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    name(0);
+    load();
+    name(C::BK);
+    for (int row = 0; row < s.count; row += C::BK) {
+      xs.store(As);
+      gs.store(Bs);
+      __syncthreads();
+      if (row + C::BK < s.count) {
+        load();
+        name(row + 2 * C::BK);
+      }
+      step<T>(As, Bs, wave >> 1, wave & 1, acc);
+      if (bias) {
+#pragma unroll
+        for (int kk = 0; kk < C::BK / 32; ++kk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            u32x4 f[C::NP];
+            fragment<T>(Bs, 64 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
+#pragma unroll
+            for (int p = C::NP - 1; p >= 0; --p) accb[j] = mma<T>(u32x4{one, one, one, one}, f[p], accb[j]);
+          }
+      }
+      __syncthreads();
+    }
+    float* pw = part + (int64_t)(2 * q + s.slot) * (MK + M);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + 64 * (wave & 1) + 16 * j + li;
+      if (m >= M) continue;
+      if (bias && g == 0) {
+        if (s.whole)
+          gb[(int64_t)s.expert * M + m] = (T)accb[j][0];
         else
-          pw[(int64_t)m * K + k + q] = acc[i][j][q];
+          pw[MK + m] = accb[j][0];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (k + e >= K) continue;
+          if (s.whole)
+            gW[(int64_t)s.expert * MK + (int64_t)m * K + k + e] = (T)acc[i][j][e];
+          else
+            pw[(int64_t)m * K + k + e] = acc[i][j][e];
+        }
       }
     }
   }
 }
 
-// Sums of the runs' partial gradients in run order, for experts of more than one run.
+// Sums of the ranges' partial gradients in order, for the experts that cross ranges.
 template <typename T>
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restrict__ part, int64_t MK, int M,
-                                                          const int* __restrict__ off, int rows, T* __restrict__ gW,
-                                                          T* __restrict__ gb) {
+                                                          const int* __restrict__ off, int experts, int rows,
+                                                          int ranges, T* __restrict__ gW, T* __restrict__ gb) {
   const int s = blockIdx.y, lane = threadIdx.x & 63;
-  const int runs = (off[s + 1] - off[s] + rows - 1) / rows;
-  if (runs < 2) return;
-  int first = 0;   // runs of the experts before this one
-  for (int e = lane; e < s; e += 64) first += max(1, (off[e + 1] - off[e] + rows - 1) / rows);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) first += __shfl_xor(first, d);
+  const int units = (off[s + 1] - off[s] + rows - 1) / rows;
+  if (units < 2) return;
+  const Ranges r = find_ranges(off, experts, rows, ranges);
+  int first = 0;   // steps of the experts before this one
+  for (int e = lane; e < s; e += 64) first += (off[e + 1] - off[e] + rows - 1) / rows;
+  first = __builtin_amdgcn_readlane(scan_lanes(first), 63);
+  const int q0 = first / r.per, q1 = (first + units - 1) / r.per;
+  if (q0 == q1) return;
   const int64_t size = MK + M, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= size || (i >= MK && !gb)) return;
-  const float* p = part + (int64_t)first * size + i;
-  float a = 0.f;
+  float a = part[(int64_t)(2 * q0 + (first > q0 * r.per)) * size + i];
 #pragma unroll 4
-  for (int r = 0; r < runs; ++r) a += p[(int64_t)r * size];
+  for (int q = q0 + 1; q <= q1; ++q) a += part[(int64_t)(2 * q) * size + i];
   if (i < MK)
     gW[(int64_t)s * MK + i] = (T)a;
   else
     gb[(int64_t)s * M + i - MK] = (T)a;
 }
 
-// Rows of a run of the weight gradient: enough runs to fill the card where there are few tiles, but no run so short
-// that its partial sums (4 bytes a weight) cost more than its rows.
-int outer_rows(int64_t n, int experts, int M, int K) {
-  const int64_t tiles = (int64_t)((M + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
-  const int64_t wanted = std::max<int64_t>(1, 1024 / tiles);
-  const int64_t rows = std::max<int64_t>(512, (n + wanted - 1) / wanted);
-  return (int)std::min<int64_t>((rows + 63) / 64 * 64, int64_t(1) << 30);
+// As many ranges as fill the card's block slots together with the tiles, none of fewer than 256 rows (their partial
+// sums, 4 bytes a weight and range, would cost more than the rows).
+OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K) {
+  OuterPlan p;
+  p.direct = direct;
+  p.rows = dtype == ICTC_F32 ? Config<float>::BK : Config<bf16>::BK;
+  p.tile = direct && M > 128 && K > 128 && n >= 32768 ? 256 : kTile;
+  const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((K + p.tile - 1) / p.tile);
+  const int64_t most = std::max<int64_t>(1, n / 256);
+  p.ranges = (int)std::min<int64_t>(most, std::max<int64_t>(1, (p.tile == 256 ? 256 : 512) / tiles));
+  return p;
 }
 
-int64_t outer_runs(int64_t n, int experts, int rows) { return n / rows + experts; }
+int64_t outer_bytes(const OuterPlan& p, int M, int K) {
+  return p.ranges > 1 ? 2 * (int64_t)p.ranges * ((int64_t)M * K + M) * (int64_t)sizeof(float) : 0;
+}
 
 const char* bad_sizes(int dtype, int64_t rows, int64_t inputs, int64_t outputs, int experts) {
   if (dtype < ICTC_F32 || dtype > ICTC_F16) return "expert_linear: dtype must be ICTC_F32, ICTC_BF16 or ICTC_F16";
@@ -468,16 +440,19 @@ void launch_rows(const void* x, int64_t ldx, int K, const void* W, const void* b
 }
 
 template <typename T>
-void launch_outer(const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K, int64_t n, int experts,
-                  int rows, const int* perm, const int* off, void* gW, void* gb, float* part, unsigned blocks,
-                  hipStream_t st) {
-  hipLaunchKernelGGL(experts_outer_kernel<T>, dim3(blocks), dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
-                     K, experts, rows, perm, off, (T*)gW, (T*)gb, part);
-  if (n > rows) {   // an expert may have several runs
-    const int64_t MK = (int64_t)M * K;
-    hipLaunchKernelGGL(experts_sum_kernel<T>, dim3((unsigned)((MK + M + 255) / 256), (unsigned)experts), dim3(256), 0,
-                       st, part, MK, M, off, rows, (T*)gW, (T*)gb);
-  }
+void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
+                  int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
+  const int64_t tiles = (int64_t)((M + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
+  hipLaunchKernelGGL(experts_outer_kernel<T>, dim3((unsigned)(plan.ranges * tiles)), dim3(256), 0, st, (const T*)gy,
+                     ldg, M, (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+}
+
+template <typename T>
+void launch_sum(const OuterPlan& plan, int M, int K, int experts, const int* off, void* gW, void* gb, const float* part,
+                hipStream_t st) {
+  const int64_t MK = (int64_t)M * K;
+  hipLaunchKernelGGL(experts_sum_kernel<T>, dim3((unsigned)((MK + M + 255) / 256), (unsigned)experts), dim3(256), 0, st,
+                     part, MK, M, off, experts, plan.rows, plan.ranges, (T*)gW, (T*)gb);
 }
 
 }  // namespace
@@ -494,6 +469,9 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   const int64_t blocks = (rows / kTile + experts + 1) * ((outputs + kTile - 1) / kTile);
   if (blocks >= (int64_t(1) << 31)) return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: too many tiles");
   hipStream_t st = (hipStream_t)stream;
+  if (experts_direct_rows(dtype, x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose != 0,
+                          out, st))
+    return dense_status("expert_linear launch");
   if (dtype == ICTC_F32)
     launch_rows<float>(x, ldx, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, (unsigned)blocks, st);
   else if (dtype == ICTC_BF16)
@@ -505,8 +483,8 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
 
 int64_t ictc_expert_outer_workspace_bytes(int dtype, int64_t rows, int inputs, int outputs, int experts) {
   if (bad_sizes(dtype, rows, inputs, outputs, experts)) return -1;
-  const int run = outer_rows(rows, experts, outputs, inputs);
-  return rows > run ? outer_runs(rows, experts, run) * ((int64_t)outputs * inputs + outputs) * (int64_t)sizeof(float) : 0;
+  return std::max(outer_bytes(outer_plan(false, dtype, rows, outputs, inputs), outputs, inputs),
+                  outer_bytes(outer_plan(true, dtype, rows, outputs, inputs), outputs, inputs));
 }
 
 int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int inputs,
@@ -517,21 +495,30 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: row pitch below the row");
   if (!offsets || !dweight || (rows > 0 && (!grad || !x || !perm)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
-  const int64_t need = ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts);
-  if (need > 0 && (!workspace || workspace_bytes < need))
+  const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, grad, ldg, outputs, x, ldx, inputs),
+                                    dtype, rows, outputs, inputs);
+  if (outer_bytes(plan, outputs, inputs) > 0 &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: workspace smaller than ictc_expert_outer_workspace_bytes");
-  const int run = outer_rows(rows, experts, outputs, inputs);
-  const int64_t tiles = (int64_t)((outputs + kTile - 1) / kTile) * ((inputs + kTile - 1) / kTile);
-  const int64_t blocks = outer_runs(rows, experts, run) * tiles;
-  if (blocks >= (int64_t(1) << 31)) return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_outer: too many tiles");
   hipStream_t st = (hipStream_t)stream;
   float* part = (float*)workspace;
-  if (dtype == ICTC_F32)
-    launch_outer<float>(grad, ldg, outputs, x, ldx, inputs, rows, experts, run, perm, offsets, dweight, dbias, part, (unsigned)blocks, st);
+  if (plan.direct)
+    experts_direct_outer(dtype, plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part,
+                         st);
+  else if (dtype == ICTC_F32)
+    launch_outer<float>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
   else if (dtype == ICTC_BF16)
-    launch_outer<bf16>(grad, ldg, outputs, x, ldx, inputs, rows, experts, run, perm, offsets, dweight, dbias, part, (unsigned)blocks, st);
+    launch_outer<bf16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
   else
-    launch_outer<f16>(grad, ldg, outputs, x, ldx, inputs, rows, experts, run, perm, offsets, dweight, dbias, part, (unsigned)blocks, st);
+    launch_outer<f16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
+  if (plan.ranges > 1) {
+    if (dtype == ICTC_F32)
+      launch_sum<float>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+    else if (dtype == ICTC_BF16)
+      launch_sum<bf16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+    else
+      launch_sum<f16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+  }
   return dense_status("expert_outer launch");
 }
 

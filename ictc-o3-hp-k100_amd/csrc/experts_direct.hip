@@ -1,0 +1,391 @@
+// The expert linears' products for bfloat16 and FP16 operands on 16-byte aligned rows: the tiles go from memory to
+// LDS without passing through registers (global_load_lds, 16 bytes a lane), one step of 64 reduction indices ahead of
+// the matrix instructions.
+//
+// A tile of an operand whose rows run along the reduction index is kept [row][64]; one whose memory runs along the
+// rows is kept as it lies, [64][row], and its fragments are transposed as they are read (ds_read_b64_tr_b16: sixteen
+// lanes read four rows of sixteen values and receive four of a column each).  A load writes lane l's 16 bytes at
+// base + 16 l, so the exchange of chunks that spreads the fragment reads over the banks is made by the lanes' source
+// addresses.  Chunks past the end of the reduction come from a block of zeros; rows and columns past the tile's end
+// repeat valid ones and are not stored.
+//
+// 256 x 256 tiles of eight waves (128 x 64 each: 12 fragments for 32 matrix instructions, so LDS is read for three
+// quarters of the time that those take) where they fill the card, 128 x 128 of four waves otherwise.
+#include <algorithm>
+
+#include "experts.h"
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kStep = 64;   // reduction indices of a step
+
+__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ void to_lds(const void* p, uint16_t* lds) {
+  __builtin_amdgcn_global_load_lds((global_void*)p, (lds_void*)lds, 16, 0, 0);
+}
+
+// Chunk exchange of row `r` of an operand kept [64][R]: pairs of chunks (16 columns) XORed with this.
+__device__ __forceinline__ int pair_swap(int r) { return (r & 3) | ((r >> 3) & 1) << 2; }
+
+// Loads of an operand of R rows by a wave: R / 8 blocks of 1 KB over WAVES waves.
+template <int R, int WAVES>
+constexpr int kLoads = R / 8 / WAVES;
+
+// Where a lane's part of a fragment lies: 16 x 32 values at rows r0 .. r0 + 15 of an operand, reduction indices
+// 32 kk ..., r0 a multiple of 16.  Kept [R][64]: + r0 * 64.
+__device__ __forceinline__ int straight_at(int kk) {
+  const int lane = threadIdx.x & 63, li = lane & 15;
+  return li * 64 + (((4 * kk + (lane >> 4)) ^ (li & 7)) * 8);
+}
+
+__device__ __forceinline__ u32x4 straight_fragment(const uint16_t* lds, int at, int r0) {
+  return *reinterpret_cast<const u32x4*>(lds + at + r0 * 64);
+}
+
+// Kept [64][R]: the lane's row of the tile and its exchange; ^ the first column, a multiple of 16 below R.
+template <int R>
+__device__ __forceinline__ int across_at() {
+  const int lane = threadIdx.x & 63, i = lane & 15, k = 8 * (lane >> 4) + (i >> 2);
+  return k * R + pair_swap(k) * 16 + (i & 3) * 4;
+}
+
+template <int R>
+__device__ __forceinline__ u32x4 across_fragment(const uint16_t* p) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * R));
+  const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+  return u32x4{l[0], l[1], h[0], h[1]};
+}
+
+// N fragments of an operand of R rows from row 16 N w on.
+template <bool ACROSS, int R, int N>
+__device__ __forceinline__ void fragments(const uint16_t* lds, int kk, int w, u32x4 (&f)[N]) {
+  if (ACROSS) {
+    int at = across_at<R>() ^ (w * N * 16);
+    asm volatile("" : "+v"(at));   // (keeps one address in a register, not one for each fragment over the whole loop)
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = across_fragment<R>(lds + (at ^ (i * 16)) + kk * 32 * R);
+  } else {
+    const int at = straight_at(kk) + w * N * 16 * 64;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = straight_fragment(lds, at, i * 16);
+  }
+}
+
+// ones: the sums of operand B's rows over the step are added to accb too.
+template <typename T, bool ACROSS_A, bool ACROSS_B, int TA, int TB, int GA, int GB, bool SUMS>
+__device__ __forceinline__ void direct_step(const uint16_t* A, const uint16_t* B, int wa, int wb,
+                                            v4f (&acc)[TA / GA / 16][TB / GB / 16], bool ones,
+                                            v4f (&accb)[SUMS ? TB / GB / 16 : 1]) {
+  constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
+#pragma unroll
+  for (int kk = 0; kk < kStep / 32; ++kk) {
+    u32x4 a[NA], b[NB];
+    fragments<ACROSS_B, TB, NB>(B, kk, wb, b);
+    fragments<ACROSS_A, TA, NA>(A, kk, wa, a);
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = mma<T>(a[i], b[j], acc[i][j]);
+    if (SUMS && ones) {
+      constexpr uint32_t one = __is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) accb[j] = mma<T>(u32x4{one, one, one, one}, b[j], accb[j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (the next half's fragments would not fit the registers beside these)
+  }
+}
+
+// All of this wave's loads have reached LDS, and then all waves'.
+__device__ __forceinline__ void landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// out[perm[r]] = M x[perm[r]] + b, M = W[e] [N, K] or, TRANS, the transpose of W[e] [K, N].  Operand A is the
+// weights (TA output columns), operand B the rows (TB of them).
+template <typename T, bool TRANS, int TA, int TB, int GA, int GB>
+__global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_kernel(
+    const T* __restrict__ x, int64_t ldx, int K, const T* __restrict__ W, const T* __restrict__ bias, int N,
+    int experts, const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ out) {
+  constexpr int WAVES = GA * GB, LA = kLoads<TA, WAVES>, LB = kLoads<TB, WAVES>;
+  constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * kStep], A1[TA * kStep], B0[TB * kStep], B1[TB * kStep];
+  const int columns = (N + TA - 1) / TA;
+  const int blk = die_order(blockIdx.x, gridDim.x);
+  Run run;
+  if (!find_run(off, experts + 1, TB, blk / columns, run)) return;
+  const int n0 = blk % columns * TA;
+  if (run.group == experts) {   // ids outside [0, experts): zero rows
+    const int width = min(TA, N - n0);
+    for (int i = threadIdx.x; i < run.count * TA; i += WAVES * 64)
+      if (i % TA < width) out[(int64_t)perm[run.start + i / TA] * N + n0 + i % TA] = (T)0.f;
+    return;
+  }
+  const T* w = W + (int64_t)run.group * N * K;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wa = wave / GB, wb = wave % GB;
+  // the lanes' source addresses at step 0, and the reduction index that each stands at
+  const T *pa[LA], *pb[LB];
+  int ka[LA];
+  const int kb = ((lane & 7) ^ (lane >> 3)) * 8;
+#pragma unroll
+  for (int i = 0; i < LA; ++i) {
+    const int block = wave * LA + i;
+    if (TRANS) {
+      constexpr int CH = TA / 8;   // chunks of a row of 64
+      const int r = block * (64 / CH) + lane / CH, c = (lane % CH) ^ (pair_swap(r) << 1);
+      ka[i] = r;
+      pa[i] = w + (int64_t)r * N + (n0 + 8 * c < N ? n0 + 8 * c : n0);
+    } else {
+      const int r = block * 8 + (lane >> 3);
+      ka[i] = kb;
+      pa[i] = w + (int64_t)(n0 + r < N ? n0 + r : n0) * K + kb;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < LB; ++i) {
+    const int r = (wave * LB + i) * 8 + (lane >> 3);
+    pb[i] = x + (int64_t)perm[run.start + (r < run.count ? r : 0)] * ldx + kb;
+  }
+  auto load = [&](uint16_t* A, uint16_t* B, int k0) {
+    const int left = K - k0;   // reduction indices from here on
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+      const T* p = pa[i] + (TRANS ? (int64_t)k0 * N : (int64_t)k0);
+      to_lds(ka[i] < left ? (const void*)p : (const void*)kZeros, A + (wave * LA + i) * 512);
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      to_lds(kb < left ? (const void*)(pb[i] + k0) : (const void*)kZeros, B + (wave * LB + i) * 512);
+  };
+  v4f acc[NA][NB], none[1];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  load(A0, B0, 0);
+  for (int k0 = 0; k0 < K; k0 += 2 * kStep) {
+    landed();
+    if (k0 + kStep < K) load(A1, B1, k0 + kStep);
+    direct_step<T, TRANS, false, TA, TB, GA, GB, false>(A0, B0, wa, wb, acc, false, none);
+    if (k0 + kStep < K) {
+      landed();
+      if (k0 + 2 * kStep < K) load(A0, B0, k0 + 2 * kStep);
+      direct_step<T, TRANS, false, TA, TB, GA, GB, false>(A1, B1, wa, wb, acc, false, none);
+    }
+  }
+  // all of the bias and row numbers are asked for before the first is needed
+  T bv[NA][4];
+  T* row[NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    const int c = n0 + (wa * NA + i) * 16 + 4 * g;
+    const T* bp = bias + (int64_t)run.group * N + c;
+    if (bias && c + 4 <= N) {
+      *reinterpret_cast<u32x2*>(bv[i]) = *reinterpret_cast<const u32x2_any*>(bp);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bv[i][q] = bias && c + q < N ? bp[q] : (T)0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int r = (wb * NB + j) * 16 + li;
+    row[j] = out + (int64_t)perm[run.start + (r < run.count ? r : 0)] * N;
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    if ((wb * NB + j) * 16 + li >= run.count) continue;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int c = n0 + (wa * NA + i) * 16 + 4 * g;
+      if (c >= N) continue;
+      T v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = (T)(acc[i][j][q] + (float)bv[i][q]);
+      if (c + 4 <= N) {
+        *reinterpret_cast<u32x2_any*>(row[j] + c) = *reinterpret_cast<const u32x2*>(v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (c + q < N) row[j][c + q] = v[q];
+      }
+    }
+  }
+}
+
+template <typename T, bool TRANS, int TA, int TB, int GA, int GB>
+void launch_direct(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
+                   const int* perm, const int* off, void* out, hipStream_t st) {
+  const int64_t blocks = (rows / TB + experts + 1) * ((N + TA - 1) / TA);
+  hipLaunchKernelGGL((experts_direct_kernel<T, TRANS, TA, TB, GA, GB>), dim3((unsigned)blocks), dim3(GA * GB * 64), 0,
+                     st, (const T*)x, ldx, K, (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
+}
+
+template <typename T>
+void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
+                 const int* perm, const int* off, bool transpose, void* out, hipStream_t st) {
+  const bool big = (rows / 256) * ((N + 255) / 256) >= 512;
+  if (big && transpose)
+    launch_direct<T, true, 256, 256, 2, 4>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  else if (big)
+    launch_direct<T, false, 256, 256, 2, 4>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  else if (transpose)
+    launch_direct<T, true, 128, 128, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  else
+    launch_direct<T, false, 128, 128, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+}
+
+// Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
+// range of rows: see experts_outer_kernel.
+template <typename T, int TA, int TB, int GA, int GB>
+__global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
+    const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, int K, int experts, int ranges,
+    const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ gW, T* __restrict__ gb,
+    float* __restrict__ part) {
+  static_assert(TA == TB, "one row number serves both operands");
+  constexpr int WAVES = GA * GB, L = kLoads<TA, WAVES>, CH = TA / 8, PER = 64 / CH;
+  constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * kStep], A1[TA * kStep], B0[TB * kStep], B1[TB * kStep];
+  const int ct = (K + TA - 1) / TA, tiles = ct * ((M + TB - 1) / TB);
+  const int blk = die_order(blockIdx.x, gridDim.x), q = blk / tiles;
+  const int k0 = blk % tiles % ct * TA, m0 = blk % tiles / ct * TB;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wa = wave / GB, wb = wave % GB;
+  const int64_t MK = (int64_t)M * K;
+  const bool bias = gb != nullptr && k0 == 0 && wa == 0;
+  for (int e = q; e < experts; e += ranges) {   // experts without rows: zeros, shared out over the ranges
+    if (off[e + 1] != off[e]) continue;
+    for (int i = threadIdx.x; i < TA * TB; i += WAVES * 64)
+      if (m0 + i / TA < M && k0 + i % TA < K) gW[e * MK + (int64_t)(m0 + i / TA) * K + k0 + i % TA] = (T)0.f;
+    if (gb && k0 == 0 && threadIdx.x < TB && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
+  }
+  const Ranges range = find_ranges(off, experts, kStep, ranges);
+  // this lane's row within a load, and its columns of both operands
+  const int sub = lane / CH;
+  Segment s;
+  for (int u = q * range.per; find_segment(off, experts, kStep, range, q, u, s); u += s.steps) {
+    int node[L];   // row numbers, read a step before their rows
+    auto name = [&](int row) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int r = row + (wave * L + i) * PER + sub;
+        node[i] = r < s.count ? perm[s.start + r] : -1;
+      }
+    };
+    auto load = [&](uint16_t* A, uint16_t* B) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int c = ((lane % CH) ^ (pair_swap((wave * L + i) * PER + sub) << 1)) * 8;
+        const int ca = k0 + c < K ? k0 + c : k0, cb = m0 + c < M ? m0 + c : m0;
+        const bool ok = node[i] >= 0;
+        to_lds(ok ? (const void*)(x + (int64_t)node[i] * ldx + ca) : (const void*)kZeros, A + (wave * L + i) * 512);
+        to_lds(ok ? (const void*)(gy + (int64_t)node[i] * ldg + cb) : (const void*)kZeros, B + (wave * L + i) * 512);
+      }
+    };
+    v4f acc[NA][NB], accb[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      accb[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NA; ++i) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    name(0);
+    load(A0, B0);
+    name(kStep);
+    for (int row = 0; row < s.count; row += 2 * kStep) {
+      landed();
+      if (row + kStep < s.count) {
+        load(A1, B1);
+        name(row + 2 * kStep);
+      }
+      direct_step<T, true, true, TA, TB, GA, GB, true>(A0, B0, wa, wb, acc, bias, accb);
+      if (row + kStep < s.count) {
+        landed();
+        if (row + 2 * kStep < s.count) {
+          load(A0, B0);
+          name(row + 3 * kStep);
+        }
+        direct_step<T, true, true, TA, TB, GA, GB, true>(A1, B1, wa, wb, acc, bias, accb);
+      }
+    }
+    __syncthreads();   // the next segment's first load overwrites what a wave may still read
+    float* pw = part + (int64_t)(2 * q + s.slot) * (MK + M);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int m = m0 + (wb * NB + j) * 16 + li;
+      if (m >= M) continue;
+      if (bias && g == 0) {
+        if (s.whole)
+          gb[(int64_t)s.expert * M + m] = (T)accb[j][0];
+        else
+          pw[MK + m] = accb[j][0];
+      }
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int k = k0 + (wa * NA + i) * 16 + 4 * g;
+        if (k >= K) continue;   // (K is a multiple of 8: four columns are in or out together)
+        if (s.whole) {
+          T v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][e];
+          *reinterpret_cast<u32x2_any*>(gW + (int64_t)s.expert * MK + (int64_t)m * K + k) =
+              *reinterpret_cast<const u32x2*>(v);
+        } else {
+          *reinterpret_cast<v4f*>(pw + (int64_t)m * K + k) = acc[i][j];
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
+                  int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
+  const int64_t tiles = (int64_t)((M + plan.tile - 1) / plan.tile) * ((K + plan.tile - 1) / plan.tile);
+  const dim3 grid((unsigned)(plan.ranges * tiles));
+  if (plan.tile == 256)
+    hipLaunchKernelGGL((experts_direct_outer_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, (const T*)gy, ldg, M,
+                       (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  else
+    hipLaunchKernelGGL((experts_direct_outer_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
+                       (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+}
+
+bool whole16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
+                         int N, int experts, const int* perm, const int* off, bool transpose, void* out,
+                         hipStream_t st) {
+  // 16-byte chunks of x, and of the weights along their memory, have to be whole and aligned
+  if (dtype == ICTC_F32 || !whole16(x) || ldx % 8 || K % 8 || !whole16(W) || (transpose && N % 8)) return false;
+  if (dtype == ICTC_BF16)
+    direct_rows<bf16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+  else
+    direct_rows<f16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+  return true;
+}
+
+bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K) {
+  return dtype != ICTC_F32 && whole16(gy) && whole16(x) && ldg % 8 == 0 && ldx % 8 == 0 && M % 8 == 0 && K % 8 == 0;
+}
+
+void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,
+                          int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
+                          float* part, hipStream_t st) {
+  if (dtype == ICTC_BF16)
+    direct_outer<bf16>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+  else
+    direct_outer<f16>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+}
