@@ -128,10 +128,10 @@ bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st);
 
-// Where the weights' gradient takes them, how it is cut: `tile` columns a side, `rows` of a step, `ranges`.
+// How the weights' gradient is cut: `rows` of a step, `ranges`; `direct`: by the kernel of experts_direct.hip.
 struct OuterPlan {
   bool direct;
-  int tile, rows, ranges;
+  int rows, ranges;
 };
 bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K);
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,

@@ -14,6 +14,7 @@
 // the stores nor the fragment reads share banks.  An operand whose memory runs along the other axis (the weights of
 // gx, both operands of gW) is transposed in registers on its way to LDS: eight rows of a few columns per thread.
 #include <algorithm>
+#include <cmath>
 
 #include "experts.h"
 
@@ -403,16 +404,16 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
     gb[(int64_t)s * M + i - MK] = (T)a;
 }
 
-// As many ranges as fill the card's block slots together with the tiles, none of fewer than 256 rows (their partial
-// sums, 4 bytes a weight and range, would cost more than the rows).
+// As many ranges as fill the card's block slots (two a unit) together with the tiles, unless the rows are few: R rows
+// take a block about R / 32 us, and n / R ranges of M K partial sums are written and read at about 3 TB/s, which is
+// least at R = sqrt(n M K 8.5e-5).
 OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K) {
   OuterPlan p;
   p.direct = direct;
   p.rows = dtype == ICTC_F32 ? Config<float>::BK : Config<bf16>::BK;
-  p.tile = direct && M > 128 && K > 128 && n >= 32768 ? 256 : kTile;
-  const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((K + p.tile - 1) / p.tile);
-  const int64_t most = std::max<int64_t>(1, n / 256);
-  p.ranges = (int)std::min<int64_t>(most, std::max<int64_t>(1, (p.tile == 256 ? 256 : 512) / tiles));
+  const int64_t tiles = (int64_t)((M + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
+  const double rows = std::max(64.0, std::sqrt(8.5e-5 * (double)n * M * K));
+  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, (int64_t)((double)n / rows)));
   return p;
 }
 

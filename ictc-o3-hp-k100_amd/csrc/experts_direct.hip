@@ -9,8 +9,11 @@
 // addresses.  Chunks past the end of the reduction come from a block of zeros; rows and columns past the tile's end
 // repeat valid ones and are not stored.
 //
-// 256 x 256 tiles of eight waves (128 x 64 each: 12 fragments for 32 matrix instructions, so LDS is read for three
-// quarters of the time that those take) where they fill the card, 128 x 128 of four waves otherwise.
+// Tiles of 128 x 128 by four waves of 64 x 64.  For the rows' products a step has 32 reduction indices, so that four
+// blocks share a compute unit and one's first loads and last stores run under another's products: at 131,072 rows of
+// 512 -> 1,024 bfloat16 this measured 216 us and its adjoint 168 us (1,024 -> 512), against 204 / 188 us with 256 x 256
+// tiles (one block of eight waves, steps of 64), which lose a factor of two at 128 -> 128 (41 against 17 us).  For the
+// weights' gradient a step has 64 rows and two blocks share a unit.
 #include <algorithm>
 
 #include "experts.h"
@@ -22,8 +25,6 @@ typedef const __attribute__((address_space(1))) void global_void;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int kStep = 64;   // reduction indices of a step
-
 __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ void to_lds(const void* p, uint16_t* lds) {
@@ -33,22 +34,23 @@ __device__ __forceinline__ void to_lds(const void* p, uint16_t* lds) {
 // Chunk exchange of row `r` of an operand kept [64][R]: pairs of chunks (16 columns) XORed with this.
 __device__ __forceinline__ int pair_swap(int r) { return (r & 3) | ((r >> 3) & 1) << 2; }
 
-// Loads of an operand of R rows by a wave: R / 8 blocks of 1 KB over WAVES waves.
-template <int R, int WAVES>
-constexpr int kLoads = R / 8 / WAVES;
+// Loads of an operand of R rows by a wave: blocks of 1 KB of a step of S reduction indices over WAVES waves.
+template <int R, int S, int WAVES>
+constexpr int kLoads = R * S / 512 / WAVES;
+
+// Chunk exchange of row `r` of an operand kept [R][S], S = 64 (eight chunks a row) or 32 (four).
+template <int S>
+__device__ __forceinline__ int row_swap(int r) { return S == 64 ? r & 7 : (r >> 2) & 3; }
 
 // Where a lane's part of a fragment lies: 16 x 32 values at rows r0 .. r0 + 15 of an operand, reduction indices
-// 32 kk ..., r0 a multiple of 16.  Kept [R][64]: + r0 * 64.
+// 32 kk ..., r0 a multiple of 16.  Kept [R][S]: + r0 * S.
+template <int S>
 __device__ __forceinline__ int straight_at(int kk) {
   const int lane = threadIdx.x & 63, li = lane & 15;
-  return li * 64 + (((4 * kk + (lane >> 4)) ^ (li & 7)) * 8);
+  return li * S + (((4 * kk + (lane >> 4)) ^ row_swap<S>(li)) * 8);
 }
 
-__device__ __forceinline__ u32x4 straight_fragment(const uint16_t* lds, int at, int r0) {
-  return *reinterpret_cast<const u32x4*>(lds + at + r0 * 64);
-}
-
-// Kept [64][R]: the lane's row of the tile and its exchange; ^ the first column, a multiple of 16 below R.
+// Kept [S][R]: the lane's row of the tile and its exchange; ^ the first column, a multiple of 16 below R.
 template <int R>
 __device__ __forceinline__ int across_at() {
   const int lane = threadIdx.x & 63, i = lane & 15, k = 8 * (lane >> 4) + (i >> 2);
@@ -64,7 +66,7 @@ __device__ __forceinline__ u32x4 across_fragment(const uint16_t* p) {
 }
 
 // N fragments of an operand of R rows from row 16 N w on.
-template <bool ACROSS, int R, int N>
+template <bool ACROSS, int R, int S, int N>
 __device__ __forceinline__ void fragments(const uint16_t* lds, int kk, int w, u32x4 (&f)[N]) {
   if (ACROSS) {
     int at = across_at<R>() ^ (w * N * 16);
@@ -72,23 +74,23 @@ __device__ __forceinline__ void fragments(const uint16_t* lds, int kk, int w, u3
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = across_fragment<R>(lds + (at ^ (i * 16)) + kk * 32 * R);
   } else {
-    const int at = straight_at(kk) + w * N * 16 * 64;
+    const uint16_t* p = lds + straight_at<S>(kk) + w * N * 16 * S;
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = straight_fragment(lds, at, i * 16);
+    for (int i = 0; i < N; ++i) f[i] = *reinterpret_cast<const u32x4*>(p + i * 16 * S);
   }
 }
 
 // ones: the sums of operand B's rows over the step are added to accb too.
-template <typename T, bool ACROSS_A, bool ACROSS_B, int TA, int TB, int GA, int GB, bool SUMS>
+template <typename T, bool ACROSS_A, bool ACROSS_B, int TA, int TB, int S, int GA, int GB, bool SUMS>
 __device__ __forceinline__ void direct_step(const uint16_t* A, const uint16_t* B, int wa, int wb,
                                             v4f (&acc)[TA / GA / 16][TB / GB / 16], bool ones,
                                             v4f (&accb)[SUMS ? TB / GB / 16 : 1]) {
   constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
 #pragma unroll
-  for (int kk = 0; kk < kStep / 32; ++kk) {
+  for (int kk = 0; kk < S / 32; ++kk) {
     u32x4 a[NA], b[NB];
-    fragments<ACROSS_B, TB, NB>(B, kk, wb, b);
-    fragments<ACROSS_A, TA, NA>(A, kk, wa, a);
+    fragments<ACROSS_B, TB, S, NB>(B, kk, wb, b);
+    fragments<ACROSS_A, TA, S, NA>(A, kk, wa, a);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
 #pragma unroll
@@ -102,21 +104,26 @@ __device__ __forceinline__ void direct_step(const uint16_t* A, const uint16_t* B
   }
 }
 
-// All of this wave's loads have reached LDS, and then all waves'.
-__device__ __forceinline__ void landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+// All waves are here, with their reads of LDS behind them and, LOADS, this wave's loads in LDS.  (The wait is the
+// builtin's: the compiler then knows of it and adds none of its own before the fragment reads.)
+template <bool LOADS>
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(LOADS ? 0x0070 : 0xc07f);   // vmcnt(0) lgkmcnt(0); lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // out[perm[r]] = M x[perm[r]] + b, M = W[e] [N, K] or, TRANS, the transpose of W[e] [K, N].  Operand A is the
 // weights (TA output columns), operand B the rows (TB of them).
-template <typename T, bool TRANS, int TA, int TB, int GA, int GB>
-__global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_kernel(
+template <typename T, bool TRANS, int TA, int TB, int S, int GA, int GB>
+__global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_kernel(
     const T* __restrict__ x, int64_t ldx, int K, const T* __restrict__ W, const T* __restrict__ bias, int N,
     int experts, const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ out) {
-  constexpr int WAVES = GA * GB, LA = kLoads<TA, WAVES>, LB = kLoads<TB, WAVES>;
+  constexpr int WAVES = GA * GB, LA = kLoads<TA, S, WAVES>, LB = kLoads<TB, S, WAVES>;
   constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
-  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * kStep], A1[TA * kStep], B0[TB * kStep], B1[TB * kStep];
+  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * S], A1[TA * S], B0[TB * S], B1[TB * S];
+  __shared__ __attribute__((aligned(16))) uint16_t stage[WAVES * NA * 256];
   const int columns = (N + TA - 1) / TA;
   const int blk = die_order(blockIdx.x, gridDim.x);
   Run run;
@@ -135,24 +142,25 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_kernel(
   // the lanes' source addresses at step 0, and the reduction index that each stands at
   const T *pa[LA], *pb[LB];
   int ka[LA];
-  const int kb = ((lane & 7) ^ (lane >> 3)) * 8;
+  constexpr int RC = S / 8, RR = 64 / RC;   // chunks of a row kept [R][S], rows of a load
+  const int kb = ((lane % RC) ^ row_swap<S>(lane / RC)) * 8;
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
     const int block = wave * LA + i;
     if (TRANS) {
-      constexpr int CH = TA / 8;   // chunks of a row of 64
+      constexpr int CH = TA / 8;   // chunks of a row kept [S][R]
       const int r = block * (64 / CH) + lane / CH, c = (lane % CH) ^ (pair_swap(r) << 1);
       ka[i] = r;
       pa[i] = w + (int64_t)r * N + (n0 + 8 * c < N ? n0 + 8 * c : n0);
     } else {
-      const int r = block * 8 + (lane >> 3);
+      const int r = block * RR + lane / RC;
       ka[i] = kb;
       pa[i] = w + (int64_t)(n0 + r < N ? n0 + r : n0) * K + kb;
     }
   }
 #pragma unroll
   for (int i = 0; i < LB; ++i) {
-    const int r = (wave * LB + i) * 8 + (lane >> 3);
+    const int r = (wave * LB + i) * RR + lane / RC;
     pb[i] = x + (int64_t)perm[run.start + (r < run.count ? r : 0)] * ldx + kb;
   }
   auto load = [&](uint16_t* A, uint16_t* B, int k0) {
@@ -172,22 +180,22 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_kernel(
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   load(A0, B0, 0);
-  for (int k0 = 0; k0 < K; k0 += 2 * kStep) {
-    landed();
-    if (k0 + kStep < K) load(A1, B1, k0 + kStep);
-    direct_step<T, TRANS, false, TA, TB, GA, GB, false>(A0, B0, wa, wb, acc, false, none);
-    if (k0 + kStep < K) {
-      landed();
-      if (k0 + 2 * kStep < K) load(A0, B0, k0 + 2 * kStep);
-      direct_step<T, TRANS, false, TA, TB, GA, GB, false>(A1, B1, wa, wb, acc, false, none);
+  for (int k0 = 0; k0 < K; k0 += 2 * S) {   // the two buffers are separate objects: a step's reads wait for no load
+    meet<true>();
+    if (k0 + S < K) load(A1, B1, k0 + S);
+    direct_step<T, TRANS, false, TA, TB, S, GA, GB, false>(A0, B0, wa, wb, acc, false, none);
+    if (k0 + S < K) {
+      meet<true>();
+      if (k0 + 2 * S < K) load(A0, B0, k0 + 2 * S);
+      direct_step<T, TRANS, false, TA, TB, S, GA, GB, false>(A1, B1, wa, wb, acc, false, none);
     }
   }
-  // all of the bias and row numbers are asked for before the first is needed
-  T bv[NA][4];
-  T* row[NB];
+  // The results go through LDS, 16 rows of this wave's columns at a time, so that a store writes runs of them.
+  const int c0 = n0 + wa * NA * 16;
+  T bv[NA][4];   // all of the bias and row numbers are asked for before the first is needed
 #pragma unroll
   for (int i = 0; i < NA; ++i) {
-    const int c = n0 + (wa * NA + i) * 16 + 4 * g;
+    const int c = c0 + 16 * i + 4 * g;
     const T* bp = bias + (int64_t)run.group * N + c;
     if (bias && c + 4 <= N) {
       *reinterpret_cast<u32x2*>(bv[i]) = *reinterpret_cast<const u32x2_any*>(bp);
@@ -196,65 +204,80 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_kernel(
       for (int q = 0; q < 4; ++q) bv[i][q] = bias && c + q < N ? bp[q] : (T)0.f;
     }
   }
+  constexpr int CH = NA * 2, PER = 64 / CH;   // chunks of a row here; rows of a store
+  // An output larger than the caches is not kept in them (131,072 x 1,024: 233 us without, 216 us with).
+  const bool stream = (int64_t)off[experts + 1] * N * (int64_t)sizeof(T) > (int64_t(1) << 27);
+  const int cc = c0 + lane % CH * 8;
+  int at[NB][16 / PER];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int h = 0; h < 16 / PER; ++h) {
+      const int r = (wb * NB + j) * 16 + h * PER + lane / CH;
+      at[j][h] = r < run.count ? perm[run.start + r] : -1;
+    }
+  uint16_t* st = stage + wave * NA * 256;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int r = (wb * NB + j) * 16 + li;
-    row[j] = out + (int64_t)perm[run.start + (r < run.count ? r : 0)] * N;
-  }
-#pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    if ((wb * NB + j) * 16 + li >= run.count) continue;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      const int c = n0 + (wa * NA + i) * 16 + 4 * g;
-      if (c >= N) continue;
       T v[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = (T)(acc[i][j][q] + (float)bv[i][q]);
-      if (c + 4 <= N) {
-        *reinterpret_cast<u32x2_any*>(row[j] + c) = *reinterpret_cast<const u32x2*>(v);
+      *reinterpret_cast<u32x2*>(st + (li * CH + ((2 * i + (g >> 1)) ^ (li % CH))) * 8 + (g & 1) * 4) =
+          *reinterpret_cast<const u32x2*>(v);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 16 / PER; ++h) {
+      const int r = h * PER + lane / CH;
+      Chunk<T> v;
+      v.raw = *reinterpret_cast<const u32x4*>(st + (r * CH + ((lane % CH) ^ (r % CH))) * 8);
+      if (at[j][h] < 0) continue;
+      T* o = out + (int64_t)at[j][h] * N + cc;
+      if (cc + 8 <= N) {
+        if (stream)
+          __builtin_nontemporal_store(v.raw, reinterpret_cast<u32x4_any*>(o));
+        else
+          *reinterpret_cast<u32x4_any*>(o) = v.raw;
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (c + q < N) row[j][c + q] = v[q];
+        for (int q = 0; q < 8; ++q)
+          if (cc + q < N) o[q] = v.e[q];
       }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-template <typename T, bool TRANS, int TA, int TB, int GA, int GB>
+template <typename T, bool TRANS, int TA, int TB, int S, int GA, int GB>
 void launch_direct(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                    const int* perm, const int* off, void* out, hipStream_t st) {
   const int64_t blocks = (rows / TB + experts + 1) * ((N + TA - 1) / TA);
-  hipLaunchKernelGGL((experts_direct_kernel<T, TRANS, TA, TB, GA, GB>), dim3((unsigned)blocks), dim3(GA * GB * 64), 0,
+  hipLaunchKernelGGL((experts_direct_kernel<T, TRANS, TA, TB, S, GA, GB>), dim3((unsigned)blocks), dim3(GA * GB * 64), 0,
                      st, (const T*)x, ldx, K, (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
 }
 
 template <typename T>
 void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, bool transpose, void* out, hipStream_t st) {
-  const bool big = (rows / 256) * ((N + 255) / 256) >= 512;
-  if (big && transpose)
-    launch_direct<T, true, 256, 256, 2, 4>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
-  else if (big)
-    launch_direct<T, false, 256, 256, 2, 4>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
-  else if (transpose)
-    launch_direct<T, true, 128, 128, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  if (transpose)
+    launch_direct<T, true, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else
-    launch_direct<T, false, 128, 128, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    launch_direct<T, false, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
 }
 
 // Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
 // range of rows: see experts_outer_kernel.
-template <typename T, int TA, int TB, int GA, int GB>
+template <typename T, int TA, int TB, int S, int GA, int GB>
 __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, int K, int experts, int ranges,
     const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ gW, T* __restrict__ gb,
     float* __restrict__ part) {
   static_assert(TA == TB, "one row number serves both operands");
-  constexpr int WAVES = GA * GB, L = kLoads<TA, WAVES>, CH = TA / 8, PER = 64 / CH;
+  constexpr int WAVES = GA * GB, L = kLoads<TA, S, WAVES>, CH = TA / 8, PER = 64 / CH;
   constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
-  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * kStep], A1[TA * kStep], B0[TB * kStep], B1[TB * kStep];
+  __shared__ __attribute__((aligned(16))) uint16_t A0[TA * S], A1[TA * S], B0[TB * S], B1[TB * S];
   const int ct = (K + TA - 1) / TA, tiles = ct * ((M + TB - 1) / TB);
   const int blk = die_order(blockIdx.x, gridDim.x), q = blk / tiles;
   const int k0 = blk % tiles % ct * TA, m0 = blk % tiles / ct * TB;
@@ -269,17 +292,17 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
       if (m0 + i / TA < M && k0 + i % TA < K) gW[e * MK + (int64_t)(m0 + i / TA) * K + k0 + i % TA] = (T)0.f;
     if (gb && k0 == 0 && threadIdx.x < TB && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
   }
-  const Ranges range = find_ranges(off, experts, kStep, ranges);
+  const Ranges range = find_ranges(off, experts, S, ranges);
   // this lane's row within a load, and its columns of both operands
   const int sub = lane / CH;
-  Segment s;
-  for (int u = q * range.per; find_segment(off, experts, kStep, range, q, u, s); u += s.steps) {
+  Segment seg;
+  for (int u = q * range.per; find_segment(off, experts, S, range, q, u, seg); u += seg.steps) {
     int node[L];   // row numbers, read a step before their rows
     auto name = [&](int row) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         const int r = row + (wave * L + i) * PER + sub;
-        node[i] = r < s.count ? perm[s.start + r] : -1;
+        node[i] = r < seg.count ? perm[seg.start + r] : -1;
       }
     };
     auto load = [&](uint16_t* A, uint16_t* B) {
@@ -301,32 +324,32 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     }
     name(0);
     load(A0, B0);
-    name(kStep);
-    for (int row = 0; row < s.count; row += 2 * kStep) {
-      landed();
-      if (row + kStep < s.count) {
+    name(S);
+    for (int row = 0; row < seg.count; row += 2 * S) {
+      meet<true>();
+      if (row + S < seg.count) {
         load(A1, B1);
-        name(row + 2 * kStep);
+        name(row + 2 * S);
       }
-      direct_step<T, true, true, TA, TB, GA, GB, true>(A0, B0, wa, wb, acc, bias, accb);
-      if (row + kStep < s.count) {
-        landed();
-        if (row + 2 * kStep < s.count) {
+      direct_step<T, true, true, TA, TB, S, GA, GB, true>(A0, B0, wa, wb, acc, bias, accb);
+      if (row + S < seg.count) {
+        meet<true>();
+        if (row + 2 * S < seg.count) {
           load(A0, B0);
-          name(row + 3 * kStep);
+          name(row + 3 * S);
         }
-        direct_step<T, true, true, TA, TB, GA, GB, true>(A1, B1, wa, wb, acc, bias, accb);
+        direct_step<T, true, true, TA, TB, S, GA, GB, true>(A1, B1, wa, wb, acc, bias, accb);
       }
     }
-    __syncthreads();   // the next segment's first load overwrites what a wave may still read
-    float* pw = part + (int64_t)(2 * q + s.slot) * (MK + M);
+    meet<false>();   // the next segment's first load overwrites what a wave may still read
+    float* pw = part + (int64_t)(2 * q + seg.slot) * (MK + M);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int m = m0 + (wb * NB + j) * 16 + li;
       if (m >= M) continue;
       if (bias && g == 0) {
-        if (s.whole)
-          gb[(int64_t)s.expert * M + m] = (T)accb[j][0];
+        if (seg.whole)
+          gb[(int64_t)seg.expert * M + m] = (T)accb[j][0];
         else
           pw[MK + m] = accb[j][0];
       }
@@ -334,11 +357,11 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
       for (int i = 0; i < NA; ++i) {
         const int k = k0 + (wa * NA + i) * 16 + 4 * g;
         if (k >= K) continue;   // (K is a multiple of 8: four columns are in or out together)
-        if (s.whole) {
+        if (seg.whole) {
           T v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][e];
-          *reinterpret_cast<u32x2_any*>(gW + (int64_t)s.expert * MK + (int64_t)m * K + k) =
+          *reinterpret_cast<u32x2_any*>(gW + (int64_t)seg.expert * MK + (int64_t)m * K + k) =
               *reinterpret_cast<const u32x2*>(v);
         } else {
           *reinterpret_cast<v4f*>(pw + (int64_t)m * K + k) = acc[i][j];
@@ -351,13 +374,9 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
 template <typename T>
 void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
-  const int64_t tiles = (int64_t)((M + plan.tile - 1) / plan.tile) * ((K + plan.tile - 1) / plan.tile);
+  const int64_t tiles = (int64_t)((M + 127) / 128) * ((K + 127) / 128);
   const dim3 grid((unsigned)(plan.ranges * tiles));
-  if (plan.tile == 256)
-    hipLaunchKernelGGL((experts_direct_outer_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, (const T*)gy, ldg, M,
-                       (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
-  else
-    hipLaunchKernelGGL((experts_direct_outer_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
+  hipLaunchKernelGGL((experts_direct_outer_kernel<T, 128, 128, 64, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
                        (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
 
