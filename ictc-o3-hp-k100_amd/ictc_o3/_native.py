@@ -4,18 +4,24 @@ The library is built in-tree by ``csrc/build.py``.  There is no fallback:
 if the library is missing, or the tensors are not on a ROCm device, every
 entry point raises.  Launches go on torch's current HIP stream of the
 operand's device, so they order correctly with surrounding torch work.
+
+``ops()`` is the compiled torch layer over the same C ABI (csrc/torch_ops.cpp,
+built beside the library) for the dense-layer operators.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 import torch
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libictc_mi355x.so")
+_OPS_PATH = os.path.join(os.path.dirname(_LIB_PATH), "ictc_torch.so")
 _lock = threading.Lock()
 _lib = None
+_ops = None
 
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -159,6 +165,23 @@ def lib():
                     fn.restype, fn.argtypes = res, args
                 _lib = handle
     return _lib
+
+
+def ops():
+    """The compiled torch layer (ictc_torch.so), loaded once; raises if it was not built."""
+    global _ops
+    if _ops is None:
+        lib()
+        with _lock:
+            if _ops is None:
+                if not os.path.isfile(_OPS_PATH):
+                    raise RuntimeError(f"ictc_torch.so is not built ({_OPS_PATH}); run "
+                                       "`python ictc-o3-hp-k100_amd/csrc/build.py` (or __graft_entry__.build())")
+                spec = importlib.util.spec_from_file_location("ictc_torch", _OPS_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _ops = module
+    return _ops
 
 
 def exported_symbols():

@@ -9,12 +9,12 @@ from __future__ import annotations
 
 import torch
 
+from ictc_o3 import _native as nat
 from ictc_o3.basis import tables
 from ictc_o3.basis.ictd_irreps import EdgeWeightedPathPreservingTensorProduct
 from ictc_o3.ops import tensor_product as tpo
-from ictc_o3.ops.experts import ExpertOrder, expert_linear as _expert_linear
+from ictc_o3.ops.experts import ExpertOrder
 from ictc_o3.ops.harmonics import harmonics_packed
-from ictc_o3.ops.layer_norm import DTYPES as DENSE_DTYPES, layer_norm as _layer_norm
 
 __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
@@ -366,44 +366,20 @@ def configure_symmetric_contraction(module, **kwargs):
     return impl(module, **kwargs)
 
 
-def _dense_operand(name, value, device, what):
-    if not isinstance(value, torch.Tensor):
-        raise TypeError(f"{what}: {name} must be a tensor")
-    if not value.is_cuda:
-        raise ValueError(f"{what}: {name} must be on a ROCm (cuda) device")
-    if value.dtype not in DENSE_DTYPES:
-        raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16")
-    if device is not None and value.device != device:
-        raise ValueError(f"{what}: {name} must be on {device}")
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm of the last axis of x [..., C], C up to 16384: (x - mean) / sqrt(var + eps) * weight + bias.
 
     x is float32, bfloat16 or float16, weight and bias [C] of the same type (None: ones / zeros).  Statistics and sums
     are FP32 and each result is rounded once.  Gradients of x, weight and bias, and once more of those (a loss on
     forces), run on kernels; a third derivative raises.  A row that holds NaN or infinity gives NaN."""
-    _dense_operand("x", x, None, "layer_norm")
-    shape = x.shape
-    if len(shape) < 1 or not 1 <= shape[-1] <= 16384:
-        raise ValueError("layer_norm: x must have a last axis of 1 to 16384 elements")
-    for name, value in (("weight", weight), ("bias", bias)):
-        if value is not None:
-            _dense_operand(name, value, x.device, "layer_norm")
-            if value.shape != shape[-1:] or value.dtype != x.dtype:
-                raise ValueError(f"layer_norm: {name} must have shape [{shape[-1]}] and the type of x")
-    if not isinstance(eps, (int, float)) or isinstance(eps, bool) or not 0.0 <= eps < float("inf"):
-        raise ValueError("layer_norm: eps must be a finite number, zero or more")
-    return _layer_norm(x, weight, bias, float(eps))
+    return nat.ops().layer_norm(x, weight, bias, eps)
 
 
 def expert_order(ids, experts):
     """The order of rows by expert that ``expert_linear`` takes: ids int64 [N] on the device (an atom's compact element
     index, say), `experts` how many there are.  Rows whose id is outside [0, experts) belong to none.  It holds the
     ids as they are now; make it anew when they change."""
-    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int64 or ids.dim() != 1 or not ids.is_cuda:
-        raise ValueError("expert_order: ids must be an int64 vector on a ROCm (cuda) device")
-    if not isinstance(experts, int) or isinstance(experts, bool) or not 1 <= experts <= 65535:
+    if not isinstance(experts, int):
         raise ValueError("expert_order: experts must be an integer from 1 to 65535")
     return ExpertOrder(ids, experts)
 
@@ -415,20 +391,6 @@ def expert_linear(x, weight, order, bias=None):
     Sums are FP32 (FP32 operands keep FP32 accuracy; a row with infinities may give NaN) and each result is rounded
     once.  A row of no expert gives a zero row and adds to no gradient; an expert without rows has zero gradients.
     Differentiable to any order in x, weight and bias; every sum has a fixed order."""
-    _dense_operand("x", x, None, "expert_linear")
-    _dense_operand("weight", weight, x.device, "expert_linear")
     if not isinstance(order, ExpertOrder):
         raise TypeError("expert_linear: order must come from expert_order")
-    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or 0 in weight.shape:
-        raise ValueError("expert_linear: expected x [N, inputs] and weight [experts, outputs, inputs]")
-    if max(weight.shape) > 65536:
-        raise ValueError("expert_linear: up to 65536 inputs and outputs")
-    if x.dtype != weight.dtype:
-        raise ValueError("expert_linear: x and weight must have one type")
-    if order.rows != x.shape[0] or order.experts != weight.shape[0] or order.device != x.device:
-        raise ValueError("expert_linear: the order is of other rows, experts or another device")
-    if bias is not None:
-        _dense_operand("bias", bias, x.device, "expert_linear")
-        if bias.shape != weight.shape[:2] or bias.dtype != x.dtype:
-            raise ValueError("expert_linear: bias must have shape [experts, outputs] and the type of x")
-    return _expert_linear(x, weight, order, bias)
+    return nat.ops().expert_linear(x, weight, bias, order.perm, order.offsets, order.rows)

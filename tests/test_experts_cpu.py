@@ -9,7 +9,7 @@ def test_python_refusals():
     from ictc_o3 import expert_linear, expert_order
     with pytest.raises(ValueError, match="device"):
         expert_order(torch.zeros(3, dtype=torch.int64), 2)
-    with pytest.raises(ValueError, match="device"):
+    with pytest.raises(TypeError, match="order"):
         expert_linear(torch.zeros(3, 4), torch.zeros(2, 4, 4), None)
 
 
