@@ -1,5 +1,7 @@
 // What the expert linears' kernels share: matrix instructions, runs of sorted rows, the order of blocks.
 #pragma once
+#include <algorithm>
+
 #include "dense.h"
 #include "split_bf16.h"
 
@@ -128,10 +130,16 @@ bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st);
 
-// How the weights' gradient is cut: `rows` of a step, `ranges`; `direct`: by the kernel of experts_direct.hip.
+// Whether tiles of 128 x 128 are too few to occupy the card's 256 units.
+inline bool experts_few_tiles(int64_t rows, int N, int experts) {
+  return (rows / 128 + std::min<int64_t>(rows, experts)) * ((N + 127) / 128) < 256;
+}
+
+// How the weights' gradient is cut: `tile` columns a side, `rows` of a step, `ranges`; `direct`: by the kernel of
+// experts_direct.hip.
 struct OuterPlan {
   bool direct;
-  int rows, ranges;
+  int tile, rows, ranges;
 };
 bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K);
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,

@@ -20,16 +20,17 @@
 
 namespace {
 
-constexpr int kTile = 128;   // rows and columns of an output tile: four waves of 64 x 64
-
-template <typename T>
+// Tiles of 128 x 128 outputs by four waves of 64 x 64; or, where those are fewer than the card's units, of 64 x 64
+// by waves of 32 x 32.
+template <typename T, int TILE>
 struct Config {
-  static constexpr int NP = sizeof(T) == 4 ? 3 : 1;    // parts of an operand in LDS
-  static constexpr int BK = sizeof(T) == 4 ? 32 : 64;  // reduction indices of a step
-  static constexpr int CH = BK / 8;                    // chunks of a row in LDS
-  static constexpr int PER = kTile * CH / 256;         // chunks staged by a thread
-  static constexpr int NC = BK / 16;                   // columns per thread of a transposed operand
-  static constexpr int PART = kTile * BK;              // 16-bit values of a part of an operand
+  static constexpr int NP = sizeof(T) == 4 ? 3 : 1;                     // parts of an operand in LDS
+  static constexpr int BK = sizeof(T) == 4 && TILE == 128 ? 32 : 64;    // reduction indices of a step
+  static constexpr int CH = BK / 8;                                     // chunks of a row in LDS
+  static constexpr int PER = TILE * CH / 256;                           // chunks staged by a thread
+  static constexpr int NC = TILE * BK / 2048;                           // columns per thread of a transposed operand
+  static constexpr int PART = TILE * BK;                                // 16-bit values of a part of an operand
+  static constexpr int NI = TILE / 32;                                  // blocks of 16 a side of a wave's tile
 };
 
 template <typename T>
@@ -55,49 +56,53 @@ __device__ __forceinline__ Eight<T> load8(const T* __restrict__ p, int n) {
   return r;
 }
 
-// NC (2 or 4) values, 8 bytes
-template <typename T>
-struct alignas(8) Few {
-  T e[Config<T>::NC];
+// NC (2 or 4) values, 4 or 8 bytes
+template <typename T, int NC>
+struct alignas(NC * sizeof(T)) Few {
+  T e[NC];
 };
 
-template <typename T>
-__device__ __forceinline__ Few<T> load_few(const T* __restrict__ p, int n) {
-  Few<T> r;
-  if (n >= Config<T>::NC) {
-    *reinterpret_cast<u32x2*>(&r) = *reinterpret_cast<const u32x2_any*>(p);
+template <typename T, int NC>
+__device__ __forceinline__ Few<T, NC> load_few(const T* __restrict__ p, int n) {
+  typedef uint32_t u32_any __attribute__((aligned(2)));
+  Few<T, NC> r;
+  if (n >= NC) {
+    if constexpr (NC * sizeof(T) == 8)
+      *reinterpret_cast<u32x2*>(&r) = *reinterpret_cast<const u32x2_any*>(p);
+    else
+      *reinterpret_cast<uint32_t*>(&r) = *reinterpret_cast<const u32_any*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < Config<T>::NC; ++i) r.e[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < NC; ++i) r.e[i] = i < n ? p[i] : (T)0.f;
   }
   return r;
 }
 
 // 16-bit offset of chunk `ch` of row `row` in a part of an operand
-template <typename T>
+template <int CH>
 __device__ __forceinline__ int lds_at(int row, int ch) {
-  constexpr int CH = Config<T>::CH;
   const int swz = CH == 8 ? (row ^ (row >> 3)) & 7 : (row >> 2) & 3;
   return (row * CH + (ch ^ swz)) * 8;
 }
 
-template <typename T>
+template <typename T, int TILE>
 __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch, const Eight<T>& v) {
-  uint16_t* at = lds + lds_at<T>(row, ch);
+  using C = Config<T, TILE>;
+  uint16_t* at = lds + lds_at<C::CH>(row, ch);
   if constexpr (sizeof(T) == 4) {
     const Split s = split8(v.e);
     *reinterpret_cast<bf16x8*>(at) = s.hi;
-    *reinterpret_cast<bf16x8*>(at + Config<T>::PART) = s.mid;
-    *reinterpret_cast<bf16x8*>(at + 2 * Config<T>::PART) = s.lo;
+    *reinterpret_cast<bf16x8*>(at + C::PART) = s.mid;
+    *reinterpret_cast<bf16x8*>(at + 2 * C::PART) = s.lo;
   } else {
     *reinterpret_cast<u32x4*>(at) = *reinterpret_cast<const u32x4*>(&v.e[0]);
   }
 }
 
 // The product of one 16 x 16 block over 32 reduction indices from the operands' parts.
-template <typename T>
-__device__ __forceinline__ v4f product(const u32x4 (&a)[Config<T>::NP], const u32x4 (&b)[Config<T>::NP], v4f c) {
-  if constexpr (sizeof(T) == 4) {
+template <typename T, int NP>
+__device__ __forceinline__ v4f product(const u32x4 (&a)[NP], const u32x4 (&b)[NP], v4f c) {
+  if constexpr (NP == 3) {
     c = mma<T>(a[2], b[0], c);
     c = mma<T>(a[0], b[2], c);
     c = mma<T>(a[1], b[1], c);
@@ -107,64 +112,68 @@ __device__ __forceinline__ v4f product(const u32x4 (&a)[Config<T>::NP], const u3
   return mma<T>(a[0], b[0], c);
 }
 
-template <typename T>
-__device__ __forceinline__ void fragment(const uint16_t* __restrict__ lds, int row, int ch, u32x4 (&f)[Config<T>::NP]) {
-  const uint16_t* at = lds + lds_at<T>(row, ch);
+template <typename T, int TILE>
+__device__ __forceinline__ void fragment(const uint16_t* __restrict__ lds, int row, int ch,
+                                         u32x4 (&f)[Config<T, TILE>::NP]) {
+  using C = Config<T, TILE>;
+  const uint16_t* at = lds + lds_at<C::CH>(row, ch);
 #pragma unroll
-  for (int p = 0; p < Config<T>::NP; ++p) f[p] = *reinterpret_cast<const u32x4*>(at + p * Config<T>::PART);
+  for (int p = 0; p < C::NP; ++p) f[p] = *reinterpret_cast<const u32x4*>(at + p * C::PART);
 }
 
-// acc[i][j] += the block's step: rows 64 wa + 16 i of operand A by rows 64 wb + 16 j of operand B.
-template <typename T>
+// acc[i][j] += the block's step: rows 16 (wa NI + i) of operand A by rows 16 (wb NI + j) of operand B.
+template <typename T, int TILE>
 __device__ __forceinline__ void step(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int wa, int wb,
-                                     v4f (&acc)[4][4]) {
+                                     v4f (&acc)[Config<T, TILE>::NI][Config<T, TILE>::NI]) {
+  using C = Config<T, TILE>;
   const int li = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int kk = 0; kk < Config<T>::BK / 32; ++kk) {
-    u32x4 a[4][Config<T>::NP];
+  for (int kk = 0; kk < C::BK / 32; ++kk) {
+    u32x4 a[C::NI][C::NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fragment<T>(A, 64 * wa + 16 * i + li, 4 * kk + g, a[i]);
+    for (int i = 0; i < C::NI; ++i) fragment<T, TILE>(A, 16 * (wa * C::NI + i) + li, 4 * kk + g, a[i]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u32x4 b[Config<T>::NP];
-      fragment<T>(B, 64 * wb + 16 * j + li, 4 * kk + g, b);
+    for (int j = 0; j < C::NI; ++j) {
+      u32x4 b[C::NP];
+      fragment<T, TILE>(B, 16 * (wb * C::NI + j) + li, 4 * kk + g, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i][j] = product<T>(a[i], b, acc[i][j]);
+      for (int i = 0; i < C::NI; ++i) acc[i][j] = product<T>(a[i], b, acc[i][j]);
     }
   }
 }
 
-// A 128-row operand whose rows run along the reduction index.
-template <typename T>
+// An operand whose rows run along the reduction index.
+template <typename T, int TILE>
 struct Straight {
-  const T* row[Config<T>::PER];
-  bool ok[Config<T>::PER];
-  Eight<T> v[Config<T>::PER];
+  using C = Config<T, TILE>;
+  const T* row[C::PER];
+  bool ok[C::PER];
+  Eight<T> v[C::PER];
 
-  static __device__ __forceinline__ int row_of(int i) { return (i * 256 + (int)threadIdx.x) / Config<T>::CH; }
-  static __device__ __forceinline__ int chunk_of(int i) { return (i * 256 + (int)threadIdx.x) % Config<T>::CH; }
+  static __device__ __forceinline__ int row_of(int i) { return (i * 256 + (int)threadIdx.x) / C::CH; }
+  static __device__ __forceinline__ int chunk_of(int i) { return (i * 256 + (int)threadIdx.x) % C::CH; }
 
   __device__ __forceinline__ void load(int k0, int K) {
 #pragma unroll
-    for (int i = 0; i < Config<T>::PER; ++i) {
+    for (int i = 0; i < C::PER; ++i) {
       const int k = k0 + 8 * chunk_of(i);
       v[i] = load8(row[i] + k, ok[i] ? K - k : 0);
     }
   }
   __device__ __forceinline__ void store(uint16_t* lds) const {
 #pragma unroll
-    for (int i = 0; i < Config<T>::PER; ++i) put(lds, row_of(i), chunk_of(i), v[i]);
+    for (int i = 0; i < C::PER; ++i) put<T, TILE>(lds, row_of(i), chunk_of(i), v[i]);
   }
 };
 
-// An operand whose memory runs along its 128 rows: thread (kb, cg) takes reduction indices 8 kb .. and rows NC cg ...
-template <typename T>
+// An operand whose memory runs along its rows: thread (kb, cg) takes reduction indices 8 kb .. and rows NC cg ...
+template <typename T, int TILE>
 struct Across {
-  static constexpr int NC = Config<T>::NC;
-  Few<T> v[8];
+  static constexpr int NC = Config<T, TILE>::NC;
+  Few<T, NC> v[8];
 
-  static __device__ __forceinline__ int column() { return (int)threadIdx.x % (kTile / NC) * NC; }
-  static __device__ __forceinline__ int block() { return (int)threadIdx.x / (kTile / NC); }
+  static __device__ __forceinline__ int column() { return (int)threadIdx.x % (TILE / NC) * NC; }
+  static __device__ __forceinline__ int block() { return (int)threadIdx.x / (TILE / NC); }
 
   __device__ __forceinline__ void store(uint16_t* lds) const {
 #pragma unroll
@@ -172,36 +181,36 @@ struct Across {
       Eight<T> e;
 #pragma unroll
       for (int j = 0; j < 8; ++j) e.e[j] = v[j].e[c];
-      put(lds, column() + c, block(), e);
+      put<T, TILE>(lds, column() + c, block(), e);
     }
   }
 };
 
-// out[perm[r]] = M x[perm[r]] + b over the 128 columns of a block, M = W[e] [N, K] or, TRANS, the transpose of
+// out[perm[r]] = M x[perm[r]] + b over the columns of a tile, M = W[e] [N, K] or, TRANS, the transpose of
 // W[e] [K, N].  Operand A is the weights, so a lane ends with four consecutive columns of one row.
-template <typename T, bool TRANS>
+template <typename T, bool TRANS, int TILE>
 __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__ x, int64_t ldx, int K,
                                                            const T* __restrict__ W, const T* __restrict__ bias, int N,
                                                            int experts, const int* __restrict__ perm,
                                                            const int* __restrict__ off, T* __restrict__ out) {
-  using C = Config<T>;
+  using C = Config<T, TILE>;
   __shared__ __attribute__((aligned(16))) uint16_t As[C::NP * C::PART];
   __shared__ __attribute__((aligned(16))) uint16_t Bs[C::NP * C::PART];
-  const int columns = (N + kTile - 1) / kTile;
+  const int columns = (N + TILE - 1) / TILE;
   const int b = die_order(blockIdx.x, gridDim.x);
   Run run;
-  if (!find_run(off, experts + 1, kTile, b / columns, run)) return;
-  const int n0 = b % columns * kTile;
+  if (!find_run(off, experts + 1, TILE, b / columns, run)) return;
+  const int n0 = b % columns * TILE;
   if (run.group == experts) {   // ids outside [0, experts): zero rows
-    const int width = min(kTile, N - n0);
-    for (int i = threadIdx.x; i < run.count * kTile; i += 256)
-      if (i % kTile < width) out[(int64_t)perm[run.start + i / kTile] * N + n0 + i % kTile] = (T)0.f;
+    const int width = min(TILE, N - n0);
+    for (int i = threadIdx.x; i < run.count * TILE; i += 256)
+      if (i % TILE < width) out[(int64_t)perm[run.start + i / TILE] * N + n0 + i % TILE] = (T)0.f;
     return;
   }
   const T* w = W + (int64_t)run.group * N * K;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-  Straight<T> xs, ws;
-  Across<T> wt;
+  Straight<T, TILE> xs, ws;
+  Across<T, TILE> wt;
 #pragma unroll
   for (int i = 0; i < C::PER; ++i) {
     const int r = xs.row_of(i);
@@ -219,15 +228,15 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = k0 + 8 * wt.block() + j;
-        wt.v[j] = load_few(w + (int64_t)k * N + c, k < K ? N - c : 0);
+        wt.v[j] = load_few<T, C::NC>(w + (int64_t)k * N + c, k < K ? N - c : 0);
       }
     }
   };
-  v4f acc[4][4];
+  v4f acc[C::NI][C::NI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < C::NI; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   load(0);
   for (int k0 = 0; k0 < K; k0 += C::BK) {
     xs.store(Bs);
@@ -237,27 +246,27 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
       ws.store(As);
     __syncthreads();
     if (k0 + C::BK < K) load(k0 + C::BK);
-    step<T>(As, Bs, wave >> 1, wave & 1, acc);
+    step<T, TILE>(As, Bs, wave >> 1, wave & 1, acc);
     __syncthreads();
   }
   // all of the bias and row numbers are asked for before the first is needed
-  T bv[4][4];
-  T* row[4];
+  T bv[C::NI][4];
+  T* row[C::NI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = n0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+  for (int i = 0; i < C::NI; ++i) {
+    const int c = n0 + TILE / 2 * (wave >> 1) + 16 * i + 4 * g;
     const T* bp = bias + (int64_t)run.group * N + c;
 #pragma unroll
     for (int q = 0; q < 4; ++q) bv[i][q] = bias && c + q < N ? bp[q] : (T)0.f;
-    const int r = 64 * (wave & 1) + 16 * i + li;
+    const int r = TILE / 2 * (wave & 1) + 16 * i + li;
     row[i] = out + (int64_t)perm[run.start + (r < run.count ? r : 0)] * N;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (64 * (wave & 1) + 16 * j + li >= run.count) continue;
+  for (int j = 0; j < C::NI; ++j) {
+    if (TILE / 2 * (wave & 1) + 16 * j + li >= run.count) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = n0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+    for (int i = 0; i < C::NI; ++i) {
+      const int c = n0 + TILE / 2 * (wave >> 1) + 16 * i + 4 * g;
       if (c >= N) continue;
       T* o = row[j] + c;
       T v[4];
@@ -277,20 +286,84 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
   }
 }
 
+// The stable order of up to kOrderRows rows by expert (ids outside [0, experts) last) by one block: each wave counts
+// the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves go over
+// their rows again and place them.  Lanes of one expert find each other by one ballot for each bit of the id.
+constexpr int kOrderRows = 16384, kOrderExperts = 1023, kOrderWaves = 16;
+
+__global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __restrict__ ids, int n, int experts,
+                                                             int bits, int* __restrict__ off, int* __restrict__ perm) {
+  __shared__ int count[kOrderWaves][kOrderExperts + 1];
+  __shared__ int wave_total[kOrderWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = experts + 1;
+  for (int i = threadIdx.x; i < kOrderWaves * groups; i += 1024) count[i / groups][i % groups] = 0;
+  __syncthreads();
+  const int per = ((n + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
+  const int begin = wave * per, end = min(n, begin + per);
+  auto peers = [&](int row, int& key) -> uint64_t {   // the lanes whose row has this lane's expert
+    const int64_t id = row < end ? ids[row] : -1;
+    key = id >= 0 && id < experts ? (int)id : experts;
+    uint64_t m = __ballot(row < end);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot(key >> b & 1);
+      m &= key >> b & 1 ? set : ~set;
+    }
+    return m;
+  };
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  for (int r0 = begin; r0 < end; r0 += 64) {
+    int key;
+    const uint64_t m = peers(r0 + lane, key);
+    if (r0 + lane < end && (m & below) == 0) count[wave][key] += __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  int total = 0;
+  if ((int)threadIdx.x < groups) {
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) {
+      const int c = count[w][threadIdx.x];
+      count[w][threadIdx.x] = total;
+      total += c;
+    }
+  }
+  int sum = scan_lanes(total);
+  if (lane == 63) wave_total[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += wave_total[w];
+  if ((int)threadIdx.x < groups) {
+    off[threadIdx.x] = sum - total;
+    if ((int)threadIdx.x == experts) off[groups] = n;
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) count[w][threadIdx.x] += sum - total;
+  }
+  __syncthreads();
+  for (int r0 = begin; r0 < end; r0 += 64) {
+    int key;
+    const uint64_t m = peers(r0 + lane, key);
+    if (r0 + lane < end) perm[count[wave][key] + __popcll(m & below)] = r0 + lane;
+    __builtin_amdgcn_wave_barrier();
+    if (r0 + lane < end && (m & below) == 0) count[wave][key] += __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+bool small_order(int64_t rows, int experts) { return rows <= kOrderRows && experts <= kOrderExperts; }
+
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
 // over one range of rows.
-template <typename T>
+template <typename T, int TILE>
 __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restrict__ gy, int64_t ldg, int M,
                                                             const T* __restrict__ x, int64_t ldx, int K, int experts,
                                                             int ranges, const int* __restrict__ perm,
                                                             const int* __restrict__ off, T* __restrict__ gW,
                                                             T* __restrict__ gb, float* __restrict__ part) {
-  using C = Config<T>;
+  using C = Config<T, TILE>;
   __shared__ __attribute__((aligned(16))) uint16_t As[C::NP * C::PART];
   __shared__ __attribute__((aligned(16))) uint16_t Bs[C::NP * C::PART];
-  const int ct = (K + kTile - 1) / kTile, tiles = ct * ((M + kTile - 1) / kTile);
+  const int ct = (K + TILE - 1) / TILE, tiles = ct * ((M + TILE - 1) / TILE);
   const int b = die_order(blockIdx.x, gridDim.x), q = b / tiles;
-  const int k0 = b % tiles % ct * kTile, m0 = b % tiles / ct * kTile;
+  const int k0 = b % tiles % ct * TILE, m0 = b % tiles / ct * TILE;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
   const int64_t MK = (int64_t)M * K;
   const bool bias = gb != nullptr && k0 == 0 && wave < 2;
@@ -298,12 +371,12 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
   // experts without rows: zeros, shared out over the ranges
   for (int e = q; e < experts; e += ranges) {
     if (off[e + 1] != off[e]) continue;
-    for (int i = threadIdx.x; i < kTile * kTile; i += 256)
-      if (m0 + i / kTile < M && k0 + i % kTile < K) gW[e * MK + (int64_t)(m0 + i / kTile) * K + k0 + i % kTile] = (T)0.f;
-    if (gb && k0 == 0 && threadIdx.x < kTile && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
+    for (int i = threadIdx.x; i < TILE * TILE; i += 256)
+      if (m0 + i / TILE < M && k0 + i % TILE < K) gW[e * MK + (int64_t)(m0 + i / TILE) * K + k0 + i % TILE] = (T)0.f;
+    if (gb && k0 == 0 && threadIdx.x < TILE && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
   }
   const Ranges r = find_ranges(off, experts, C::BK, ranges);
-  Across<T> xs, gs;
+  Across<T, TILE> xs, gs;
   const int cx = k0 + xs.column(), cg = m0 + gs.column(), r0 = 8 * xs.block();
   Segment s;
   for (int u = q * r.per; find_segment(off, experts, C::BK, r, q, u, s); u += s.steps) {
@@ -316,16 +389,16 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int64_t n = max(node[j], 0);
-        xs.v[j] = load_few(x + n * ldx + cx, node[j] >= 0 ? K - cx : 0);
-        gs.v[j] = load_few(gy + n * ldg + cg, node[j] >= 0 ? M - cg : 0);
+        xs.v[j] = load_few<T, C::NC>(x + n * ldx + cx, node[j] >= 0 ? K - cx : 0);
+        gs.v[j] = load_few<T, C::NC>(gy + n * ldg + cg, node[j] >= 0 ? M - cg : 0);
       }
     };
-    v4f acc[4][4], accb[4];
+    v4f acc[C::NI][C::NI], accb[C::NI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < C::NI; ++i) {
       accb[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < C::NI; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
     name(0);
     load();
@@ -338,14 +411,14 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
         load();
         name(row + 2 * C::BK);
       }
-      step<T>(As, Bs, wave >> 1, wave & 1, acc);
+      step<T, TILE>(As, Bs, wave >> 1, wave & 1, acc);
       if (bias) {
 #pragma unroll
         for (int kk = 0; kk < C::BK / 32; ++kk)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < C::NI; ++j) {
             u32x4 f[C::NP];
-            fragment<T>(Bs, 64 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
+            fragment<T, TILE>(Bs, TILE / 2 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
 #pragma unroll
             for (int p = C::NP - 1; p >= 0; --p) accb[j] = mma<T>(u32x4{one, one, one, one}, f[p], accb[j]);
           }
@@ -354,8 +427,8 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
     }
     float* pw = part + (int64_t)(2 * q + s.slot) * (MK + M);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + 64 * (wave & 1) + 16 * j + li;
+    for (int j = 0; j < C::NI; ++j) {
+      const int m = m0 + TILE / 2 * (wave & 1) + 16 * j + li;
       if (m >= M) continue;
       if (bias && g == 0) {
         if (s.whole)
@@ -364,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
           pw[MK + m] = accb[j][0];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = k0 + 64 * (wave >> 1) + 16 * i + 4 * g;
+      for (int i = 0; i < C::NI; ++i) {
+        const int k = k0 + TILE / 2 * (wave >> 1) + 16 * i + 4 * g;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (k + e >= K) continue;
@@ -404,16 +477,23 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
     gb[(int64_t)s * M + i - MK] = (T)a;
 }
 
+int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
+
 // As many ranges as fill the card's block slots (two a unit) together with the tiles, unless the rows are few: R rows
 // take a block about R / 32 us, and n / R ranges of M K partial sums are written and read at about 3 TB/s, which is
 // least at R = sqrt(n M K 8.5e-5).
 OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K) {
   OuterPlan p;
   p.direct = direct;
-  p.rows = dtype == ICTC_F32 ? Config<float>::BK : Config<bf16>::BK;
-  const int64_t tiles = (int64_t)((M + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
+  p.tile = 128;
   const double rows = std::max(64.0, std::sqrt(8.5e-5 * (double)n * M * K));
-  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, (int64_t)((double)n / rows)));
+  int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128), most = std::max<int64_t>(1, (int64_t)((double)n / rows));
+  if (!direct && tiles * std::min<int64_t>(512 / tiles, most) < 256) {   // too few blocks: smaller tiles
+    p.tile = 64;
+    tiles = tiles_of(M, 64) * tiles_of(K, 64);
+  }
+  p.rows = p.tile == 128 && dtype == ICTC_F32 ? Config<float, 128>::BK : 64;
+  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, most));
   return p;
 }
 
@@ -429,23 +509,37 @@ const char* bad_sizes(int dtype, int64_t rows, int64_t inputs, int64_t outputs, 
   return nullptr;
 }
 
-template <typename T>
-void launch_rows(const void* x, int64_t ldx, int K, const void* W, const void* bias, int N, int experts,
-                 const int* perm, const int* off, int transpose, void* out, unsigned blocks, hipStream_t st) {
+template <typename T, int TILE>
+void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
+                 const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
+  const dim3 grid((unsigned)((rows / TILE + experts + 1) * tiles_of(N, TILE)));
   if (transpose)
-    hipLaunchKernelGGL((experts_rows_kernel<T, true>), dim3(blocks), dim3(256), 0, st, (const T*)x, ldx, K,
-                       (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
+    hipLaunchKernelGGL((experts_rows_kernel<T, true, TILE>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+                       (const T*)bias, N, experts, perm, off, (T*)out);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<T, false>), dim3(blocks), dim3(256), 0, st, (const T*)x, ldx, K,
-                       (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
+    hipLaunchKernelGGL((experts_rows_kernel<T, false, TILE>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+                       (const T*)bias, N, experts, perm, off, (T*)out);
+}
+
+template <typename T>
+void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
+                 const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
+  if (experts_few_tiles(rows, N, experts))
+    launch_rows<T, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+  else
+    launch_rows<T, 128>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
 }
 
 template <typename T>
 void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
-  const int64_t tiles = (int64_t)((M + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
-  hipLaunchKernelGGL(experts_outer_kernel<T>, dim3((unsigned)(plan.ranges * tiles)), dim3(256), 0, st, (const T*)gy,
-                     ldg, M, (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  const dim3 grid((unsigned)(plan.ranges * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
+  if (plan.tile == 64)
+    hipLaunchKernelGGL((experts_outer_kernel<T, 64>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
+                       K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  else
+    hipLaunchKernelGGL((experts_outer_kernel<T, 128>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
+                       K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
 
 template <typename T>
@@ -460,6 +554,25 @@ void launch_sum(const OuterPlan& plan, int M, int K, int experts, const int* off
 
 extern "C" {
 
+int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts) {
+  if (bad_sizes(ICTC_F32, rows, 1, 1, experts)) return -1;
+  return small_order(rows, experts) ? 0 : ictc_csr_workspace_bytes(rows, experts);
+}
+
+int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  if (const char* e = bad_sizes(ICTC_F32, rows, 1, 1, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
+  if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: null operand");
+  // One launch for few rows (5 rows: 3 us, 8,192: 11 us); the counting sort's three (3 to 6 us each) for more.
+  if (!small_order(rows, experts))
+    return ictc_csr_build(ids, rows, experts, offsets, perm, workspace, workspace_bytes, stream);
+  int bits = 1;
+  while (experts >> bits) ++bits;
+  hipLaunchKernelGGL(experts_order_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, ids, (int)rows, experts, bits,
+                     offsets, perm);
+  return dense_status("expert_order launch");
+}
+
 int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int inputs, const void* weight,
                        const void* bias, int outputs, int experts, const int32_t* perm, const int32_t* offsets,
                        int transpose, void* out, void* stream) {
@@ -467,18 +580,18 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   if (rows == 0) return ICTC_OK;
   if (ldx < inputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: row pitch below the inputs");
   if (!x || !weight || !perm || !offsets || !out) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: null operand");
-  const int64_t blocks = (rows / kTile + experts + 1) * ((outputs + kTile - 1) / kTile);
-  if (blocks >= (int64_t(1) << 31)) return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: too many tiles");
+  if ((rows / 64 + experts + 1) * tiles_of(outputs, 64) >= (int64_t(1) << 31))
+    return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: too many tiles");
   hipStream_t st = (hipStream_t)stream;
   if (experts_direct_rows(dtype, x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose != 0,
                           out, st))
     return dense_status("expert_linear launch");
   if (dtype == ICTC_F32)
-    launch_rows<float>(x, ldx, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, (unsigned)blocks, st);
+    choose_rows<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   else if (dtype == ICTC_BF16)
-    launch_rows<bf16>(x, ldx, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, (unsigned)blocks, st);
+    choose_rows<bf16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   else
-    launch_rows<f16>(x, ldx, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, (unsigned)blocks, st);
+    choose_rows<f16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   return dense_status("expert_linear launch");
 }
 

@@ -31,8 +31,9 @@ __device__ __forceinline__ void to_lds(const void* p, uint16_t* lds) {
   __builtin_amdgcn_global_load_lds((global_void*)p, (lds_void*)lds, 16, 0, 0);
 }
 
-// Chunk exchange of row `r` of an operand kept [64][R]: pairs of chunks (16 columns) XORed with this.
-__device__ __forceinline__ int pair_swap(int r) { return (r & 3) | ((r >> 3) & 1) << 2; }
+// Chunk exchange of row `r` of an operand kept [S][R]: pairs of chunks (16 columns, R / 16 of them) XORed with this.
+template <int R>
+__device__ __forceinline__ int pair_swap(int r) { return ((r & 3) | ((r >> 3) & 1) << 2) & (R / 16 - 1); }
 
 // Loads of an operand of R rows by a wave: blocks of 1 KB of a step of S reduction indices over WAVES waves.
 template <int R, int S, int WAVES>
@@ -54,7 +55,7 @@ __device__ __forceinline__ int straight_at(int kk) {
 template <int R>
 __device__ __forceinline__ int across_at() {
   const int lane = threadIdx.x & 63, i = lane & 15, k = 8 * (lane >> 4) + (i >> 2);
-  return k * R + pair_swap(k) * 16 + (i & 3) * 4;
+  return k * R + pair_swap<R>(k) * 16 + (i & 3) * 4;
 }
 
 template <int R>
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
     const int block = wave * LA + i;
     if (TRANS) {
       constexpr int CH = TA / 8;   // chunks of a row kept [S][R]
-      const int r = block * (64 / CH) + lane / CH, c = (lane % CH) ^ (pair_swap(r) << 1);
+      const int r = block * (64 / CH) + lane / CH, c = (lane % CH) ^ (pair_swap<TA>(r) << 1);
       ka[i] = r;
       pa[i] = w + (int64_t)r * N + (n0 + 8 * c < N ? n0 + 8 * c : n0);
     } else {
@@ -261,7 +262,12 @@ void launch_direct(const void* x, int64_t ldx, int64_t rows, int K, const void* 
 template <typename T>
 void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, bool transpose, void* out, hipStream_t st) {
-  if (transpose)
+  const bool few = experts_few_tiles(rows, N, experts);
+  if (few && transpose)
+    launch_direct<T, true, 64, 64, 64, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  else if (few)
+    launch_direct<T, false, 64, 64, 64, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  else if (transpose)
     launch_direct<T, true, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else
     launch_direct<T, false, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
@@ -308,7 +314,7 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     auto load = [&](uint16_t* A, uint16_t* B) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const int c = ((lane % CH) ^ (pair_swap((wave * L + i) * PER + sub) << 1)) * 8;
+        const int c = ((lane % CH) ^ (pair_swap<TA>((wave * L + i) * PER + sub) << 1)) * 8;
         const int ca = k0 + c < K ? k0 + c : k0, cb = m0 + c < M ? m0 + c : m0;
         const bool ok = node[i] >= 0;
         to_lds(ok ? (const void*)(x + (int64_t)node[i] * ldx + ca) : (const void*)kZeros, A + (wave * L + i) * 512);

@@ -257,12 +257,13 @@ std::pair<Tensor, Tensor> expert_order(const Tensor& ids_, int64_t experts) {
   TORCH_CHECK_VALUE(ids_.size(0) < (int64_t(1) << 31) - 2, "expert_order: up to 2^31 - 3 rows");
   const c10::DeviceGuard guard(ids_.device());
   const Tensor ids = packed(ids_);
-  const int64_t N = ids.size(0), bytes = ictc_csr_workspace_bytes(N, experts);
+  const int64_t N = ids.size(0), bytes = ictc_expert_order_workspace_bytes(N, (int)experts);
   const auto ints = ids.options().dtype(at::kInt);
   const Tensor perm = at::empty({std::max<int64_t>(N, 1)}, ints), offsets = at::empty({experts + 2}, ints);
-  const Tensor ws = at::empty({std::max<int64_t>(bytes, 1)}, ids.options().dtype(at::kByte));
-  done(ictc_csr_build(ids.const_data_ptr<int64_t>(), N, experts, offsets.mutable_data_ptr<int>(),
-                      perm.mutable_data_ptr<int>(), ptr(ws), bytes, stream_of(ids)),
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, ids.options().dtype(at::kByte));
+  done(ictc_expert_order(ids.const_data_ptr<int64_t>(), N, (int)experts, perm.mutable_data_ptr<int>(),
+                         offsets.mutable_data_ptr<int>(), ptr(ws), bytes, stream_of(ids)),
        "expert_order");
   return {perm, offsets};
 }

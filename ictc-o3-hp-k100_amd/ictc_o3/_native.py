@@ -130,6 +130,8 @@ _SIGNATURES = {
     "ictc_layer_norm_bwd": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_layer_norm_bwd2": (_i, [_i, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i, _p, _p, _p, _p, _p, _p, _p, _i64,
                                   _p]),
+    "ictc_expert_order_workspace_bytes": (_i64, [_i64, _i]),
+    "ictc_expert_order": (_i, [_p, _i64, _i, _p, _p, _p, _i64, _p]),
     "ictc_expert_linear": (_i, [_i, _p, _i64, _i64, _i, _p, _p, _i, _i, _p, _p, _i, _p, _p]),
     "ictc_expert_outer_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i]),
     "ictc_expert_outer": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _p, _p, _i64, _p]),

@@ -757,14 +757,20 @@ int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad
  * (transpose == 0); or out[n] = W[e]^T x[n] with W [experts, inputs, outputs] read in
  * place (transpose != 0, the adjoint by rows: `inputs` is always x's width and `outputs`
  * out's).  Element type dtype throughout, FP32 sums, results rounded once; x at row pitch
- * ldx, the other operands packed, any element alignment.  perm [rows] and offsets
- * [experts + 2] as ictc_csr_build(ids, rows, experts) gives them; a row whose id is
- * outside [0, experts) gets a zero row.  bias may be NULL.
+ * ldx, the other operands packed, any element alignment.  bias may be NULL.
+ *
+ * ictc_expert_order: perm [rows], the rows sorted by their id (stable), and offsets
+ * [experts + 2]: expert e has sorted rows offsets[e] .. offsets[e + 1], and the rows
+ * whose id is outside [0, experts), which get zero rows, come last; what
+ * ictc_csr_build gives too.  ictc_expert_order_workspace_bytes bytes (0: none needed).
  *
  * ictc_expert_outer: dweight[e] = sum over the rows of expert e of grad[n] x[n]^T
  * ([experts, outputs, inputs]) and dbias[e] = sum of grad[n] (NULL: absent); zeros for an
  * expert without rows; sums in a fixed order over a workspace of
  * ictc_expert_outer_workspace_bytes bytes (0: none needed, -1: out of range).          */
+int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts);
+int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int inputs, const void* weight,
                        const void* bias, int outputs, int experts, const int32_t* perm, const int32_t* offsets,
                        int transpose, void* out, void* stream);

@@ -67,7 +67,8 @@ def _reference(ids, x, W, b, gy):
 
 
 SHAPES = [(1, 1, 1, 1), (3, 2, 5, 7), (130, 4, 64, 64), (257, 3, 33, 129), (1000, 10, 128, 128), (700, 89, 200, 333),
-          (2000, 5, 96, 1), (900, 7, 1, 160), (515, 1, 256, 255), (1500, 70, 127, 16), (4000, 3, 144, 272)]
+          (2000, 5, 96, 1), (900, 7, 1, 160), (515, 1, 256, 255), (1500, 70, 127, 16), (4000, 3, 144, 272),
+          (40000, 9, 80, 24), (33000, 6, 257, 40)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -231,6 +232,24 @@ def test_graph_replays(device):
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(i, j) for i, j in zip(held, eager)), k
+
+
+@pytest.mark.parametrize("rows", [0, 1, 63, 64, 65, 1000, 1025, 8191, 16384, 16385, 40000])
+@pytest.mark.parametrize("experts", [1, 2, 10, 89, 1023, 1024, 5000])
+def test_order(device, rows, experts):
+    """The stable order of the ids, those of no expert last."""
+    from ictc_o3 import expert_order
+    g = torch.Generator().manual_seed(rows + experts)
+    ids = torch.randint(-2, experts + 2, (rows,), generator=g)
+    if rows > 100:
+        ids[:50] = experts - 1
+        ids[60] = 2 ** 40
+    order = expert_order(ids.to(device), experts)
+    key = torch.where((ids >= 0) & (ids < experts), ids, torch.full_like(ids, experts))
+    ref = torch.sort(key, stable=True).indices
+    assert torch.equal(order.perm[:rows].cpu().long(), ref)
+    starts = torch.searchsorted(key[ref], torch.arange(experts + 1))
+    assert torch.equal(order.offsets.cpu().long(), torch.cat([starts, torch.tensor([rows])]))
 
 
 def test_refusals(device):
