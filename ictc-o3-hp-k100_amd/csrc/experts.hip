@@ -466,15 +466,29 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
   first = __builtin_amdgcn_readlane(scan_lanes(first), 63);
   const int q0 = first / r.per, q1 = (first + units - 1) / r.per;
   if (q0 == q1) return;
-  const int64_t size = MK + M, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= size || (i >= MK && !gb)) return;
-  float a = part[(int64_t)(2 * q0 + (first > q0 * r.per)) * size + i];
+  const int64_t size = MK + M, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int n = (int)min<int64_t>(4, size - i);   // this thread's sums
+  if (n <= 0) return;
+  const bool four = n == 4 && size % 4 == 0;
+  auto read = [&](int slot) {
+    const float* p = part + (int64_t)slot * size + i;
+    if (four) return *reinterpret_cast<const v4f*>(p);
+    v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : 0.f;
+    return v;
+  };
+  v4f a = read(2 * q0 + (first > q0 * r.per));
 #pragma unroll 4
-  for (int q = q0 + 1; q <= q1; ++q) a += part[(int64_t)(2 * q) * size + i];
-  if (i < MK)
-    gW[(int64_t)s * MK + i] = (T)a;
-  else
-    gb[(int64_t)s * M + i - MK] = (T)a;
+  for (int q = q0 + 1; q <= q1; ++q) a += read(2 * q);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (e >= n) continue;
+    if (i + e < MK)
+      gW[(int64_t)s * MK + i + e] = (T)a[e];
+    else if (gb)
+      gb[(int64_t)s * M + i + e - MK] = (T)a[e];
+  }
 }
 
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
@@ -546,7 +560,7 @@ template <typename T>
 void launch_sum(const OuterPlan& plan, int M, int K, int experts, const int* off, void* gW, void* gb, const float* part,
                 hipStream_t st) {
   const int64_t MK = (int64_t)M * K;
-  hipLaunchKernelGGL(experts_sum_kernel<T>, dim3((unsigned)((MK + M + 255) / 256), (unsigned)experts), dim3(256), 0, st,
+  hipLaunchKernelGGL(experts_sum_kernel<T>, dim3((unsigned)((MK + M + 1023) / 1024), (unsigned)experts), dim3(256), 0, st,
                      part, MK, M, off, experts, plan.rows, plan.ranges, (T*)gW, (T*)gb);
 }
 
