@@ -31,34 +31,48 @@ union Chunk {
   __device__ Chunk() {}
 };
 
-// v[0 .. kChunk) = p[0 .. n), zero past n (n may be zero or negative).
+// p[0 .. n), zero past n (n may be zero or negative; lanes that all are skip the element loop).
+template <typename T>
+__device__ __forceinline__ u32x4 load_raw(const T* __restrict__ p, int n) {
+  constexpr int V = kChunk<T>;
+  if (n >= V) return *reinterpret_cast<const u32x4_any*>(p);
+  Chunk<T> c;
+  c.raw = u32x4{0, 0, 0, 0};
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) c.e[i] = p[i];
+  }
+  return c.raw;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(u32x4 raw, float* v) {
+  Chunk<T> c;
+  c.raw = raw;
+#pragma unroll
+  for (int i = 0; i < kChunk<T>; ++i) v[i] = (float)c.e[i];
+}
+
 template <typename T>
 __device__ __forceinline__ void load_chunk(const T* __restrict__ p, int n, float* v) {
-  constexpr int V = kChunk<T>;
-  if (n >= V) {
-    Chunk<T> c;
-    c.raw = *reinterpret_cast<const u32x4_any*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (float)c.e[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.f;
-  }
+  widen<T>(load_raw(p, n), v);
 }
 
 // p[0 .. n) = v, each value rounded to T once (to nearest even).
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const float* v) {
   constexpr int V = kChunk<T>;
-  if (n >= V) {
-    Chunk<T> c;
+  if (n <= 0) return;
+  Chunk<T> c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) c.e[i] = (T)v[i];
+  for (int i = 0; i < V; ++i) c.e[i] = (T)v[i];
+  if (n >= V) {
     *reinterpret_cast<u32x4_any*>(p) = c.raw;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = (T)v[i];
+      if (i < n) p[i] = c.e[i];
   }
 }
 

@@ -10,9 +10,10 @@
 // (t is the gradient by h with r held fixed; dr/dx = -r^2 h / width gives the last term).
 //
 // All three are bound by memory: each element of each operand is read once and each output written once.  A row is
-// held in the registers of a team of 8 to 1024 lanes as 16-byte chunks, so the mean is subtracted before the
-// squares are added (no cancellation) and nothing is read twice; teams of up to 64 lanes need no barrier.  The
-// gradients by w and b are added per lane over the rows that a team takes, then over the teams of a block in LDS,
+// held in the registers of a team of 8 to 512 lanes as 16-byte chunks, so the mean is subtracted before the
+// squares are added (no cancellation) and nothing is read twice; teams of up to 64 lanes need no barrier.  Teams of
+// 64 and more ask for their next row before they work on the present one (a team of 16 has three neighbours in its
+// wave to wait with).  The gradients by w and b are added per lane over the rows that a team takes, then over the teams of a block in LDS,
 // and the blocks' partial sums by a second kernel, always in the same order.
 #include "dense.h"
 
@@ -49,6 +50,29 @@ __device__ __forceinline__ void team_sum(float (&s)[K], float* lds) {
 template <int TEAM>
 constexpr int kThreads = TEAM > 256 ? TEAM : 256;
 
+// Whether a kernel reads one row ahead: where the registers for it are there.  (8,191 x 2,176 bfloat16: gradients 50
+// us without, 36 us with; 2,048 x 8,192: 61 and 37 us.)
+template <int TEAM, int EPL>
+constexpr bool kAhead = TEAM >= 64 && EPL <= 16;
+
+// A row's chunks as a lane of its team holds them.
+template <typename T, int TEAM, int EPL>
+struct Row {
+  static constexpr int V = kChunk<T>, N = EPL / V;
+  u32x4 raw[N];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int width, int lane) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = (n * TEAM + lane) * V;
+      raw[n] = load_raw(row + c, width - c);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[EPL]) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) widen<T>(raw[n], v + n * V);
+  }
+};
+
 template <typename T, int TEAM, int EPL>
 __global__ __launch_bounds__(kThreads<TEAM>) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                                 int width, const T* __restrict__ weight,
@@ -71,15 +95,17 @@ __global__ __launch_bounds__(kThreads<TEAM>) void ln_fwd_kernel(const T* __restr
       if (!bias) b[n * V + e] = 0.f;
     }
   }
-  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < rows; row += (int64_t)gridDim.x * TEAMS) {
+  const int64_t gap = (int64_t)gridDim.x * TEAMS;
+  int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+  Row<T, TEAM, EPL> next;
+  if (kAhead<TEAM, EPL> && row < rows) next.load(x + row * ldx, width, lane);
+  for (; row < rows; row += gap) {
     float v[EPL], s[1] = {0.f};
+    if (!kAhead<TEAM, EPL>) next.load(x + row * ldx, width, lane);
+    next.get(v);
+    if (kAhead<TEAM, EPL> && row + gap < rows) next.load(x + (row + gap) * ldx, width, lane);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int c = (n * TEAM + lane) * V;
-      load_chunk(x + row * ldx + c, width - c, v + n * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += v[n * V + e];
-    }
+    for (int i = 0; i < EPL; ++i) s[0] += v[i];
     team_sum<TEAM>(s, lds);
     const float mu = s[0] * inv;
     s[0] = 0.f;
@@ -156,24 +182,32 @@ __global__ __launch_bounds__(kThreads<TEAM>) void ln_bwd_kernel(
       dw[n * V + e] = db[n * V + e] = 0.f;
     }
   }
-  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < rows; row += (int64_t)gridDim.x * TEAMS) {
+  const int64_t gap = (int64_t)gridDim.x * TEAMS;
+  int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+  Row<T, TEAM, EPL> nx, ng;
+  float mu_next = 0.f, r_next = 0.f;
+  auto load = [&](int64_t at) {
+    nx.load(x + at * ldx, width, lane);
+    ng.load(g + at * ldg, width, lane);
+    mu_next = mean[at];
+    r_next = rstd[at];
+  };
+  if (kAhead<TEAM, EPL> && row < rows) load(row);
+  for (; row < rows; row += gap) {
     float h[EPL], u[EPL], s[2] = {0.f, 0.f};
-    const float mu = mean[row], r = rstd[row];
+    if (!kAhead<TEAM, EPL>) load(row);
+    nx.get(h);
+    ng.get(u);
+    const float mu = mu_next, r = r_next;
+    if (kAhead<TEAM, EPL> && row + gap < rows) load(row + gap);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int c = (n * TEAM + lane) * V;
-      load_chunk(x + row * ldx + c, width - c, h + n * V);
-      load_chunk(g + row * ldg + c, width - c, u + n * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int i = n * V + e;
-        h[i] = (h[i] - mu) * r;
-        dw[i] += u[i] * h[i];
-        db[i] += u[i];
-        u[i] *= w[i];
-        s[0] += u[i];
-        s[1] += u[i] * h[i];
-      }
+    for (int i = 0; i < EPL; ++i) {
+      h[i] = (h[i] - mu) * r;
+      dw[i] += u[i] * h[i];
+      db[i] += u[i];
+      u[i] *= w[i];
+      s[0] += u[i];
+      s[1] += u[i] * h[i];
     }
     if (dx) {
       team_sum<TEAM>(s, lds);
@@ -204,16 +238,30 @@ __global__ __launch_bounds__(kThreads<TEAM>) void ln_bwd2_kernel(
   float dw[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) dw[i] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < rows; row += (int64_t)gridDim.x * TEAMS) {
+  const int64_t gap = (int64_t)gridDim.x * TEAMS;
+  int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+  Row<T, TEAM, EPL> nx, ng, nv;
+  float mu_next = 0.f, r_next = 0.f;
+  auto load = [&](int64_t at) {
+    nx.load(x + at * ldx, width, lane);
+    ng.load(g + at * ldg, width, lane);
+    nv.load(v + at * ldv, width, lane);
+    mu_next = mean[at];
+    r_next = rstd[at];
+  };
+  if (kAhead<TEAM, EPL> && row < rows) load(row);
+  for (; row < rows; row += gap) {
     float h[EPL], gr[EPL], vr[EPL], s[7] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float mu = mean[row], r = rstd[row];
+    if (!kAhead<TEAM, EPL>) load(row);
+    nx.get(h);
+    ng.get(gr);
+    nv.get(vr);
+    const float mu = mu_next, r = r_next;
+    if (kAhead<TEAM, EPL> && row + gap < rows) load(row + gap);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int c = (n * TEAM + lane) * V;
       float w[V], q[V];
-      load_chunk(x + row * ldx + c, width - c, h + n * V);
-      load_chunk(g + row * ldg + c, width - c, gr + n * V);
-      load_chunk(v + row * ldv + c, width - c, vr + n * V);
       if (weight) load_chunk(weight + c, width - c, w);
       if (vw) load_chunk(vw + c, width - c, q);
 #pragma unroll
@@ -284,7 +332,7 @@ __global__ __launch_bounds__(256) void ln_param_kernel(const float* __restrict__
   }
 }
 
-// Lanes and elements per lane that hold a row, and the blocks of 256 threads (1024 for the widest) that take `rows`.
+// Lanes and elements per lane that hold a row.
 struct Shape {
   int team, epl;
 };
@@ -297,8 +345,8 @@ Shape shape_of(int width, int chunk) {
   if (width <= 1024) return {64, 16};
   if (width <= 2048) return {64, 32};
   if (width <= 4096) return {256, 16};
-  if (width <= 8192) return {256, 32};
-  return {1024, 16};
+  if (width <= 8192) return {512, 16};
+  return {512, 32};
 }
 
 int64_t blocks_of(int64_t rows, int team, int64_t most) {
@@ -307,9 +355,11 @@ int64_t blocks_of(int64_t rows, int team, int64_t most) {
 }
 
 constexpr int64_t kFwdBlocks = 2048;
-// The blocks of the gradient kernels each leave a partial row per parameter: fewer of them for wide rows.
+// The blocks of the gradient kernels each leave a partial row per parameter: fewer of them for wide rows.  Measured at
+// 256 / 512 / 1,024 blocks: 425,991 x 64 FP32 103 / 65 / 67 us, 8,191 x 2,176 bfloat16 44 / 36 / 45 us, 2,048 x 8,192
+// bfloat16 37 / 53 / 83 us.
 int64_t grad_blocks(int64_t rows, int width, int chunk) {
-  return blocks_of(rows, shape_of(width, chunk).team, width <= 1024 ? 1024 : 512);
+  return blocks_of(rows, shape_of(width, chunk).team, width <= 256 ? 1024 : width <= 4096 ? 512 : 256);
 }
 
 #define LN_CASE(TEAM_, EPL_, ...)                      \
@@ -323,7 +373,7 @@ int64_t grad_blocks(int64_t rows, int width, int chunk) {
     else LN_CASE(16, 8, __VA_ARGS__) else LN_CASE(16, 16, __VA_ARGS__)         \
     else LN_CASE(64, 8, __VA_ARGS__) else LN_CASE(64, 16, __VA_ARGS__)         \
     else LN_CASE(64, 32, __VA_ARGS__) else LN_CASE(256, 16, __VA_ARGS__)       \
-    else LN_CASE(256, 32, __VA_ARGS__) else LN_CASE(1024, 16, __VA_ARGS__)     \
+    else LN_CASE(512, 16, __VA_ARGS__) else LN_CASE(512, 32, __VA_ARGS__)     \
   }
 
 template <typename T>
