@@ -241,28 +241,48 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table t, Hyper h, void* __re
   }
 }
 
-// part[block] = sum of squares of the gradients of this launch's runs blockIdx, blockIdx + gridDim, ...: FP32 over
-// the eight elements of a thread's run, FP64 above.
+// part[block] = sum of squares of the gradients of this launch's runs blockIdx, blockIdx + gridDim, ...: FP32 over the
+// eight elements of a thread's run, FP64 above.  Four runs are asked for before the first is added.
 template <typename T>
 __global__ __launch_bounds__(256) void grad_norm_kernel(Table t, double* __restrict__ part) {
+  constexpr int V = kChunk<T>, L = kRun / 256 / V, AHEAD = 4;
   __shared__ double lds[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double sum = 0.0;
-  for (int b = blockIdx.x; b < t.runs; b += gridDim.x) {
-    const int k = find_tensor(t, b);
-    const int64_t start = (int64_t)(b - (int)t.first[k]) * kRun;
-    const int64_t n = t.n[k] - start;
-    const T* g = reinterpret_cast<const T*>(t.g[k]) + start;
-    float s = 0.f;
+  int k = 0;
+  for (int64_t b0 = blockIdx.x; b0 < t.runs; b0 += (int64_t)AHEAD * gridDim.x) {
+    u32x4 raw[AHEAD][L];
 #pragma unroll
-    for (int j = 0; j < kRun / 1024; ++j) {
-      const int at = j * 1024 + threadIdx.x * 4;
-      float gv[4];
-      load4(g + at, (int)min<int64_t>(4, n - at), gv);
+    for (int a = 0; a < AHEAD; ++a) {
+      const int64_t b = b0 + (int64_t)a * gridDim.x;
+      const bool in = b < t.runs;
+      while (in && k + 1 < t.tensors && t.first[k + 1] <= (uint32_t)b) ++k;
+      const int64_t start = (b - t.first[k]) * kRun, left = in ? t.n[k] - start : 0;
+      const T* g = reinterpret_cast<const T*>(t.g[k]) + start;
+      if (left >= kRun) {   // (the same in every lane: a whole run needs no checks)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += gv[i] * gv[i];
+        for (int j = 0; j < L; ++j)
+          raw[a][j] = *reinterpret_cast<const u32x4_any*>(g + (j * 256 + (int)threadIdx.x) * V);
+      } else {
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          const int at = (j * 256 + (int)threadIdx.x) * V;
+          raw[a][j] = load_raw(g + at, (int)max<int64_t>(0, min<int64_t>(V, left - at)));
+        }
+      }
     }
-    sum += (double)s;
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        float v[V];
+        widen<T>(raw[a][j], v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += v[i] * v[i];
+      }
+      sum += (double)s;
+    }
   }
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
