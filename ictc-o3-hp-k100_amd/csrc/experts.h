@@ -123,10 +123,25 @@ __device__ __forceinline__ int die_order(int b, int blocks) {
   return die * per + min(die, rest) + (b >> 3);
 }
 
+// Zeros in the tile at (m0, k0) of gW [M, K] and, of the first column tile, of gb [M].
+template <typename T, int TILE, int THREADS>
+__device__ __forceinline__ void zero_tile(T* __restrict__ gW, T* __restrict__ gb, int M, int K, int m0, int k0) {
+  constexpr int V = kChunk<T>, CH = TILE / V;
+  const float zero[V] = {};
+  for (int i = threadIdx.x; i < TILE * CH; i += THREADS) {
+    const int m = m0 + i / CH, k = k0 + i % CH * V;
+    if (m < M) store_chunk(gW + (int64_t)m * K + k, K - k, zero);
+  }
+  if (gb && k0 == 0)
+    for (int i = threadIdx.x; i < TILE; i += THREADS)
+      if (m0 + i < M) gb[m0 + i] = (T)0.f;
+}
+
 }  // namespace
 
-// The kernels of 16-bit types on aligned rows (experts_direct.hip).
-bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
+// The kernels of 16-bit types on aligned rows (experts_direct.hip), and whether they take these.
+bool experts_direct_rows_fit(int dtype, const void* x, int64_t ldx, int K, const void* W, int N, bool transpose);
+void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st);
 
@@ -135,11 +150,11 @@ inline bool experts_few_tiles(int64_t rows, int N, int experts) {
   return (rows / 128 + std::min<int64_t>(rows, experts)) * ((N + 127) / 128) < 256;
 }
 
-// How the weights' gradient is cut: `tile` columns a side, `rows` of a step, `ranges`; `direct`: by the kernel of
-// experts_direct.hip.
+// How the weights' gradient is cut: `tile` columns a side, `rows` of a step, `ranges`; `fill` blocks of a tile share the
+// zeros of experts without rows; `sums`: an expert may cross ranges; `direct`: by the kernel of experts_direct.hip.
 struct OuterPlan {
-  bool direct;
-  int tile, rows, ranges;
+  bool direct, sums;
+  int tile, rows, ranges, fill;
 };
 bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K);
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,

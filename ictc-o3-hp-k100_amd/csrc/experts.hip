@@ -286,6 +286,87 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
   }
 }
 
+// The same for few rows: a block takes 16 rows of an expert and 32 columns, its eight waves share the reduction, and
+// every lane reads its fragments' values from memory itself, so a call is one round of loads, not a chain of steps (1
+// row of 1,024 -> 1,024 FP32: 33 us in tiles of 64).  The waves' sums are added in order.
+constexpr int kFewRows = 16, kFewColumns = 32, kFewWaves = 8;
+
+template <typename T>
+__device__ __forceinline__ void parts(const Eight<T>& v, u32x4 (&f)[sizeof(T) == 4 ? 3 : 1]) {
+  if constexpr (sizeof(T) == 4) {
+    const Split s = split8(v.e);
+    f[0] = __builtin_bit_cast(u32x4, s.hi);
+    f[1] = __builtin_bit_cast(u32x4, s.mid);
+    f[2] = __builtin_bit_cast(u32x4, s.lo);
+  } else {
+    f[0] = *reinterpret_cast<const u32x4*>(&v.e[0]);
+  }
+}
+
+template <typename T, bool TRANS>
+__global__ __launch_bounds__(kFewWaves * 64) void experts_few_kernel(const T* __restrict__ x, int64_t ldx, int K,
+                                                                    const T* __restrict__ W,
+                                                                    const T* __restrict__ bias, int N, int experts,
+                                                                    const int* __restrict__ perm,
+                                                                    const int* __restrict__ off,
+                                                                    T* __restrict__ out) {
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1, AHEAD = 4;
+  __shared__ v4f sums[kFewWaves][2][64];
+  const int columns = (N + kFewColumns - 1) / kFewColumns;
+  Run run;
+  if (!find_run(off, experts + 1, kFewRows, blockIdx.x / columns, run)) return;
+  const int n0 = blockIdx.x % columns * kFewColumns;
+  const bool valid = run.group < experts;   // rows of no expert: zeros
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* w = W + (int64_t)(valid ? run.group : 0) * N * K;
+  const bool row = valid && li < run.count;
+  const T* xr = x + (row ? (int64_t)perm[run.start + li] * ldx : 0);
+  const int per = (K + kFewWaves * 32 - 1) / (kFewWaves * 32) * 32, end = min(K, (wave + 1) * per);
+  v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+  for (int k0 = wave * per; valid && k0 < end; k0 += 32 * AHEAD) {
+    Eight<T> xv[AHEAD], wv[AHEAD][2];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const int k = k0 + 32 * s + 8 * g, left = end - k;
+      xv[s] = load8(xr + k, row ? left : 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = n0 + 16 * i + li;
+        if (!TRANS) {
+          wv[s][i] = load8(w + (int64_t)c * K + k, c < N ? left : 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wv[s][i].e[e] = c < N && e < left ? w[(int64_t)(k + e) * N + c] : (T)0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      u32x4 b[NP];
+      parts(xv[s], b);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u32x4 a[NP];
+        parts(wv[s][i], a);
+        acc[i] = product<T>(a, b, acc[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) sums[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave >= 2 || li >= run.count) return;   // wave i adds the column block i: four columns of one row a lane
+  v4f t = sums[0][wave][lane];
+#pragma unroll
+  for (int v = 1; v < kFewWaves; ++v) t += sums[v][wave][lane];
+  const int c = n0 + 16 * wave + 4 * g;
+  T* o = out + (int64_t)perm[run.start + li] * N + c;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (c + q < N) o[q] = valid ? (T)(t[q] + (bias ? (float)bias[(int64_t)run.group * N + c + q] : 0.f)) : (T)0.f;
+}
+
 // The stable order of up to kOrderRows rows by expert (ids outside [0, experts) last) by one block: each wave counts
 // the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves go over
 // their rows again and place them.  Lanes of one expert find each other by one ballot for each bit of the id.
@@ -368,22 +449,26 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
   const int64_t MK = (int64_t)M * K;
   const bool bias = gb != nullptr && k0 == 0 && wave < 2;
   const uint32_t one = sizeof(T) == 4 || __is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u;
-  // experts without rows: zeros, shared out over the ranges
-  for (int e = q; e < experts; e += ranges) {
-    if (off[e + 1] != off[e]) continue;
-    for (int i = threadIdx.x; i < TILE * TILE; i += 256)
-      if (m0 + i / TILE < M && k0 + i % TILE < K) gW[e * MK + (int64_t)(m0 + i / TILE) * K + k0 + i % TILE] = (T)0.f;
-    if (gb && k0 == 0 && threadIdx.x < TILE && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
-  }
+  const int parts = gridDim.x / tiles;
+  for (int e = q; e < experts; e += parts)   // experts without rows: zeros, shared out over the blocks of a tile
+    if (off[e + 1] == off[e]) zero_tile<T, TILE, 256>(gW + e * MK, gb ? gb + (int64_t)e * M : nullptr, M, K, m0, k0);
+  if (q >= ranges) return;
   const Ranges r = find_ranges(off, experts, C::BK, ranges);
   Across<T, TILE> xs, gs;
   const int cx = k0 + xs.column(), cg = m0 + gs.column(), r0 = 8 * xs.block();
   Segment s;
   for (int u = q * r.per; find_segment(off, experts, C::BK, r, q, u, s); u += s.steps) {
-    int node[8];   // the row numbers of a step are read one step before its rows
+    alignas(16) int node[8];   // the row numbers of a step are read one step before its rows
     auto name = [&](int row) {
+      typedef u32x4 u32x4_int __attribute__((aligned(4)));
+      const int* p = perm + s.start + row + r0;
+      if (row + r0 + 8 <= s.count) {
+        *reinterpret_cast<u32x4*>(node) = *reinterpret_cast<const u32x4_int*>(p);
+        *reinterpret_cast<u32x4*>(node + 4) = *reinterpret_cast<const u32x4_int*>(p + 4);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) node[j] = row + r0 + j < s.count ? perm[s.start + row + r0 + j] : -1;
+        for (int j = 0; j < 8; ++j) node[j] = row + r0 + j < s.count ? p[j] : -1;
+      }
     };
     auto load = [&]() {
 #pragma unroll
@@ -493,10 +578,25 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
 
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
+// Most groups of kFewRows rows of one expert (or of none).
+int64_t few_groups(int64_t rows, int experts) { return rows / kFewRows + std::min<int64_t>(rows, experts + 1); }
+
+// Whether `blocks` of experts_few_kernel beat tiles of 64 x 64.  Both measured in us: a round of its blocks (256 FP32,
+// 512 16-bit) takes 7 to 9 / 5 to 6; the tiles take 6.7 / 17.5 / 33 at 128 / 512 / 1,024 inputs in FP32, 4.5 / 9.3 /
+// 15.4 in 16 bits (7 / 18 / 32 through the transpose), 3.5 / 5.5 / 7.7 where they go to LDS directly, up to some
+// thousand rows.
+bool few_is_faster(int dtype, bool direct, bool transpose, int64_t blocks, int inputs) {
+  const bool f32 = dtype == ICTC_F32;
+  const double few = f32 ? 8.0 * (double)((blocks + 255) / 256) : 5.3 * (double)((blocks + 511) / 512);
+  const double tiles = f32 ? 3.0 + inputs / 36.0
+                       : direct ? 3.0 + inputs / 210.0 : transpose ? 4.0 + inputs / 36.0 : 2.5 + inputs / 80.0;
+  return blocks <= 1024 && few < tiles;
+}
+
 // As many ranges as fill the card's block slots (two a unit) together with the tiles, unless the rows are few: R rows
 // take a block about R / 32 us, and n / R ranges of M K partial sums are written and read at about 3 TB/s, which is
 // least at R = sqrt(n M K 8.5e-5).
-OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K) {
+OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K, int experts) {
   OuterPlan p;
   p.direct = direct;
   p.tile = 128;
@@ -508,11 +608,17 @@ OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K) {
   }
   p.rows = p.tile == 128 && dtype == ICTC_F32 ? Config<float, 128>::BK : 64;
   p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, most));
+  // Experts of few rows: a range for each of them, not several one after another (64 rows of ten experts, 128 -> 128
+  // FP32: 58 us in one range).
+  if (n < 256 * (int64_t)experts)
+    p.ranges = (int)std::max<int64_t>(p.ranges, std::min(std::min<int64_t>(n, experts), 2048 / tiles));
+  p.sums = p.ranges > 1 && n > p.rows;   // (an expert of one step lies within a range)
+  p.fill = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, experts));
   return p;
 }
 
 int64_t outer_bytes(const OuterPlan& p, int M, int K) {
-  return p.ranges > 1 ? 2 * (int64_t)p.ranges * ((int64_t)M * K + M) * (int64_t)sizeof(float) : 0;
+  return p.sums ? 2 * (int64_t)p.ranges * ((int64_t)M * K + M) * (int64_t)sizeof(float) : 0;
 }
 
 const char* bad_sizes(int dtype, int64_t rows, int64_t inputs, int64_t outputs, int experts) {
@@ -536,6 +642,18 @@ void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W,
 }
 
 template <typename T>
+void launch_few(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
+                const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
+  const dim3 grid((unsigned)(few_groups(rows, experts) * tiles_of(N, kFewColumns))), block(kFewWaves * 64);
+  if (transpose)
+    hipLaunchKernelGGL((experts_few_kernel<T, true>), grid, block, 0, st, (const T*)x, ldx, K, (const T*)W,
+                       (const T*)bias, N, experts, perm, off, (T*)out);
+  else
+    hipLaunchKernelGGL((experts_few_kernel<T, false>), grid, block, 0, st, (const T*)x, ldx, K, (const T*)W,
+                       (const T*)bias, N, experts, perm, off, (T*)out);
+}
+
+template <typename T>
 void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
   if (experts_few_tiles(rows, N, experts))
@@ -547,7 +665,7 @@ void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W,
 template <typename T>
 void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
-  const dim3 grid((unsigned)(plan.ranges * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
+  const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
   if (plan.tile == 64)
     hipLaunchKernelGGL((experts_outer_kernel<T, 64>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
                        K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
@@ -597,10 +715,20 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   if ((rows / 64 + experts + 1) * tiles_of(outputs, 64) >= (int64_t(1) << 31))
     return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: too many tiles");
   hipStream_t st = (hipStream_t)stream;
-  if (experts_direct_rows(dtype, x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose != 0,
-                          out, st))
+  const bool direct = experts_direct_rows_fit(dtype, x, ldx, inputs, weight, outputs, transpose != 0);
+  if (few_is_faster(dtype, direct, transpose != 0, few_groups(rows, experts) * tiles_of(outputs, kFewColumns), inputs)) {
+    if (dtype == ICTC_F32)
+      launch_few<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
+    else if (dtype == ICTC_BF16)
+      launch_few<bf16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
+    else
+      launch_few<f16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
     return dense_status("expert_linear launch");
-  if (dtype == ICTC_F32)
+  }
+  if (direct)
+    experts_direct_rows(dtype, x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose != 0, out,
+                        st);
+  else if (dtype == ICTC_F32)
     choose_rows<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   else if (dtype == ICTC_BF16)
     choose_rows<bf16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
@@ -611,8 +739,8 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
 
 int64_t ictc_expert_outer_workspace_bytes(int dtype, int64_t rows, int inputs, int outputs, int experts) {
   if (bad_sizes(dtype, rows, inputs, outputs, experts)) return -1;
-  return std::max(outer_bytes(outer_plan(false, dtype, rows, outputs, inputs), outputs, inputs),
-                  outer_bytes(outer_plan(true, dtype, rows, outputs, inputs), outputs, inputs));
+  return std::max(outer_bytes(outer_plan(false, dtype, rows, outputs, inputs, experts), outputs, inputs),
+                  outer_bytes(outer_plan(true, dtype, rows, outputs, inputs, experts), outputs, inputs));
 }
 
 int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int inputs,
@@ -624,7 +752,7 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
   if (!offsets || !dweight || (rows > 0 && (!grad || !x || !perm)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
   const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, grad, ldg, outputs, x, ldx, inputs),
-                                    dtype, rows, outputs, inputs);
+                                    dtype, rows, outputs, inputs, experts);
   if (outer_bytes(plan, outputs, inputs) > 0 &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: workspace smaller than ictc_expert_outer_workspace_bytes");
@@ -639,7 +767,7 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
     launch_outer<bf16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
   else
     launch_outer<f16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
-  if (plan.ranges > 1) {
+  if (plan.sums) {
     if (dtype == ICTC_F32)
       launch_sum<float>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
     else if (dtype == ICTC_BF16)

@@ -292,12 +292,11 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
   const int wa = wave / GB, wb = wave % GB;
   const int64_t MK = (int64_t)M * K;
   const bool bias = gb != nullptr && k0 == 0 && wa == 0;
-  for (int e = q; e < experts; e += ranges) {   // experts without rows: zeros, shared out over the ranges
-    if (off[e + 1] != off[e]) continue;
-    for (int i = threadIdx.x; i < TA * TB; i += WAVES * 64)
-      if (m0 + i / TA < M && k0 + i % TA < K) gW[e * MK + (int64_t)(m0 + i / TA) * K + k0 + i % TA] = (T)0.f;
-    if (gb && k0 == 0 && threadIdx.x < TB && m0 + threadIdx.x < M) gb[(int64_t)e * M + m0 + threadIdx.x] = (T)0.f;
-  }
+  const int parts = gridDim.x / tiles;
+  for (int e = q; e < experts; e += parts)   // experts without rows: zeros, shared out over the blocks of a tile
+    if (off[e + 1] == off[e])
+      zero_tile<T, TA, WAVES * 64>(gW + e * MK, gb ? gb + (int64_t)e * M : nullptr, M, K, m0, k0);
+  if (q >= ranges) return;
   const Ranges range = find_ranges(off, experts, S, ranges);
   // this lane's row within a load, and its columns of both operands
   const int sub = lane / CH;
@@ -381,7 +380,7 @@ template <typename T>
 void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const int64_t tiles = (int64_t)((M + 127) / 128) * ((K + 127) / 128);
-  const dim3 grid((unsigned)(plan.ranges * tiles));
+  const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles));
   hipLaunchKernelGGL((experts_direct_outer_kernel<T, 128, 128, 64, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
                        (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
@@ -390,16 +389,18 @@ bool whole16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 
 }  // namespace
 
-bool experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
+bool experts_direct_rows_fit(int dtype, const void* x, int64_t ldx, int K, const void* W, int N, bool transpose) {
+  // 16-byte chunks of x, and of the weights along their memory, have to be whole and aligned
+  return dtype != ICTC_F32 && whole16(x) && ldx % 8 == 0 && K % 8 == 0 && whole16(W) && (!transpose || N % 8 == 0);
+}
+
+void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st) {
-  // 16-byte chunks of x, and of the weights along their memory, have to be whole and aligned
-  if (dtype == ICTC_F32 || !whole16(x) || ldx % 8 || K % 8 || !whole16(W) || (transpose && N % 8)) return false;
   if (dtype == ICTC_BF16)
     direct_rows<bf16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
   else
     direct_rows<f16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
-  return true;
 }
 
 bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K) {

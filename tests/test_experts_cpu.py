@@ -27,7 +27,7 @@ def test_native_refusals():
             rows(**bad)
     rows(n=0, x=None)
     size = nat.lib().ictc_expert_outer_workspace_bytes
-    assert size(0, 100, 8, 8, 2) == 0 and size(0, 100000, 8, 8, 2) > 0
+    assert size(0, 50, 8, 8, 2) == 0 and size(0, 100000, 8, 8, 2) > 0
     assert size(0, -1, 8, 8, 2) == -1 and size(7, 1, 8, 8, 2) == -1 and size(0, 1, 8, 0, 2) == -1
     with pytest.raises(ValueError, match="workspace"):
         nat.call("ictc_expert_outer", 0, 16, 8, 16, 8, 100000, 8, 8, 2, 16, 16, 16, None, 16, 8, None)

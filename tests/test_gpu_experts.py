@@ -68,7 +68,7 @@ def _reference(ids, x, W, b, gy):
 
 SHAPES = [(1, 1, 1, 1), (3, 2, 5, 7), (130, 4, 64, 64), (257, 3, 33, 129), (1000, 10, 128, 128), (700, 89, 200, 333),
           (2000, 5, 96, 1), (900, 7, 1, 160), (515, 1, 256, 255), (1500, 70, 127, 16), (4000, 3, 144, 272),
-          (40000, 9, 80, 24), (33000, 6, 257, 40)]
+          (40000, 9, 80, 24), (33000, 6, 257, 40), (1, 8, 1024, 300), (40, 3, 1000, 130), (200, 60, 520, 136), (17, 2, 77, 33)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
