@@ -145,9 +145,9 @@ void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st);
 
-// Whether tiles of 128 x 128 are too few to occupy the card's 256 units.
-inline bool experts_few_tiles(int64_t rows, int N, int experts) {
-  return (rows / 128 + std::min<int64_t>(rows, experts)) * ((N + 127) / 128) < 256;
+// About as many tiles of 128 x 128 as the rows' product has.
+inline int64_t experts_tiles(int64_t rows, int N, int experts) {
+  return (rows / 128 + std::min<int64_t>(rows, experts)) * ((N + 127) / 128);
 }
 
 // How the weights' gradient is cut: `tile` columns a side, `rows` of a step, `ranges`; `fill` blocks of a tile share the

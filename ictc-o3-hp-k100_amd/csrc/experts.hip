@@ -14,14 +14,12 @@
 // the stores nor the fragment reads share banks.  An operand whose memory runs along the other axis (the weights of
 // gx, both operands of gW) is transposed in registers on its way to LDS: eight rows of a few columns per thread.
 #include <algorithm>
-#include <cmath>
 
 #include "experts.h"
 
 namespace {
 
-// Tiles of 128 x 128 outputs by four waves of 64 x 64; or, where those are fewer than the card's units, of 64 x 64
-// by waves of 32 x 32.
+// Tiles of 128 x 128 outputs by four waves of 64 x 64, or of 64 x 64 by waves of 32 x 32.
 template <typename T, int TILE>
 struct Config {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;                     // parts of an operand in LDS
@@ -593,21 +591,24 @@ bool few_is_faster(int dtype, bool direct, bool transpose, int64_t blocks, int i
   return blocks <= 1024 && few < tiles;
 }
 
-// As many ranges as fill the card's block slots (two a unit) together with the tiles, unless the rows are few: R rows
-// take a block about R / 32 us, and n / R ranges of M K partial sums are written and read at about 3 TB/s, which is
-// least at R = sqrt(n M K 8.5e-5).
+// Ranges of the weights' gradient: as many blocks as the card has units (256), or twice that where each still gets a
+// thousand rows, and no range shorter than a step.  Measured, in us, at 256 / 512 blocks: 30,000 rows of 256 -> 256
+// bfloat16 18.2 / 18.8, 131,072 of 128 -> 128 20.3 / 22.4, 131,072 of 512 -> 512 146 / 99, 8,192 of 1,024 -> 1,024 48 /
+// 39.  FP32 in tiles of 64 where a block of 128 x 128 would have under 256 rows (2,000 of 336 -> 520 FP32: 34 against 45
+// us; 8,192 of 1,024 -> 1,024 220 against 165); 16-bit tiles of 64 would read four bytes a lane and are not built.
 OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K, int experts) {
   OuterPlan p;
   p.direct = direct;
   p.tile = 128;
-  const double rows = std::max(64.0, std::sqrt(8.5e-5 * (double)n * M * K));
-  int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128), most = std::max<int64_t>(1, (int64_t)((double)n / rows));
-  if (!direct && tiles * std::min<int64_t>(512 / tiles, most) < 256) {   // too few blocks: smaller tiles
+  int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128), blocks = n * tiles >= 512 * 1024 ? 512 : 256;
+  if (dtype == ICTC_F32 && n * tiles < 512 * 256) {
     p.tile = 64;
     tiles = tiles_of(M, 64) * tiles_of(K, 64);
+    blocks = 512;
   }
   p.rows = p.tile == 128 && dtype == ICTC_F32 ? Config<float, 128>::BK : 64;
-  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, most));
+  const int64_t steps = n / p.rows + std::min<int64_t>(n, experts);   // about as many as there are
+  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(blocks / tiles, steps));
   // Experts of few rows: a range for each of them, not several one after another (64 rows of ten experts, 128 -> 128
   // FP32: 58 us in one range).
   if (n < 256 * (int64_t)experts)
@@ -656,7 +657,12 @@ void launch_few(const void* x, int64_t ldx, int64_t rows, int K, const void* W, 
 template <typename T>
 void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  if (experts_few_tiles(rows, N, experts))
+  // Tiles of 64 x 64 until those of 128 x 128 fill the card's 512 slots several times over.  Both in us: FP32 131,072
+  // rows of 512 -> 512 575 / 404, 40,000 of 90 experts 191 / 170, 8,192 of 1,024 -> 1,024 146 / 154, 30,000 of 256 ->
+  // 256 41 / 48; 16 bits 131,072 of 512 -> 512 160 / 144, 30,000 of 256 -> 256 17 / 22; through the transpose, where
+  // tiles of 64 read four bytes a lane, 314 / 157 and 34 / 24, 8,192 of 128 -> 128 8 / 9.
+  const int64_t most = sizeof(T) == 4 ? 1024 : transpose ? 256 : 2048;
+  if (N <= 64 || experts_tiles(rows, N, experts) < most)
     launch_rows<T, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
   else
     launch_rows<T, 128>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
@@ -666,9 +672,9 @@ template <typename T>
 void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
-  if (plan.tile == 64)
-    hipLaunchKernelGGL((experts_outer_kernel<T, 64>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
-                       K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  if (sizeof(T) == 4 && plan.tile == 64)
+    hipLaunchKernelGGL((experts_outer_kernel<float, 64>), grid, dim3(256), 0, st, (const float*)gy, ldg, M,
+                       (const float*)x, ldx, K, experts, plan.ranges, perm, off, (float*)gW, (float*)gb, part);
   else
     hipLaunchKernelGGL((experts_outer_kernel<T, 128>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
                        K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);

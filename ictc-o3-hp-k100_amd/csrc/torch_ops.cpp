@@ -495,11 +495,13 @@ std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const 
 }  // namespace
 
 PYBIND11_MODULE(ictc_torch, mod) {
-  mod.def("layer_norm", &layer_norm);
-  mod.def("expert_order", &expert_order);
-  mod.def("expert_linear", &expert_linear);
-  mod.def("gradient_norm", &gradient_norm);
-  mod.def("adamw_update", &adamw_update);
-  mod.def("adamw_step", &adamw_step);
-  mod.def("adamw_moments", &adamw_moments);
+  // Launches may wait for room in a queue: other Python threads run meanwhile.
+  using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
+  mod.def("layer_norm", &layer_norm, Free());
+  mod.def("expert_order", &expert_order, Free());
+  mod.def("expert_linear", &expert_linear, Free());
+  mod.def("gradient_norm", &gradient_norm, Free());
+  mod.def("adamw_update", &adamw_update, Free());
+  mod.def("adamw_step", &adamw_step, Free());
+  mod.def("adamw_moments", &adamw_moments, Free());
 }
