@@ -34,7 +34,7 @@ def test_native_refusals():
 
     def step(dtype=0, bits=32, tensors=1, counts=n, starts=None, m=16, state=512, lr=1e-3, b1=0.9, b2=0.9, eps=1e-8,
              step=1, params=one):
-        nat.call("ictc_adamw_step", dtype, bits, tensors, at(params), at(one), at(counts),
+        nat.call("ictc_adamw_step", dtype, bits, tensors, at(params), at(params), at(counts),
                  None if starts is None else at(starts), m, 16, None, None, state, lr, b1, b2, eps, 0.0, step, None,
                  None)
 
