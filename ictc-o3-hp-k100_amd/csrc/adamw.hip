@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(Table t, double* __restr
   __shared__ double lds[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double sum = 0.0;
-  int k = 0;
+  int k = find_tensor(t, blockIdx.x);   // (1.3 M elements in 40 tensors: 5.5 us, walking there from tensor 0 7.9)
   for (int64_t b0 = blockIdx.x; b0 < t.runs; b0 += (int64_t)AHEAD * gridDim.x) {
     u32x4 raw[AHEAD][L];
 #pragma unroll

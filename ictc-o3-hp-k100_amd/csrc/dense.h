@@ -94,6 +94,14 @@ __device__ __forceinline__ float lane_sum(float x) {
   return x;
 }
 
+// Lanes of a wave that hand values to each other through LDS: what was written before is seen after.  (LDS serves a
+// wave's accesses in order, so this holds the compiler only.)
+__device__ __forceinline__ void wave_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 inline int dense_fail(int code, const char* msg) { return ictc::set_error(code, msg); }
 
 inline int dense_status(const char* what) {

@@ -366,35 +366,48 @@ __global__ __launch_bounds__(kFewWaves * 64) void experts_few_kernel(const T* __
 }
 
 // The stable order of up to kOrderRows rows by expert (ids outside [0, experts) last) by one block: each wave counts
-// the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves go over
-// their rows again and place them.  Lanes of one expert find each other by one ballot for each bit of the id.
-constexpr int kOrderRows = 16384, kOrderExperts = 1023, kOrderWaves = 16;
+// the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves place their
+// rows.  Lanes of one expert find each other by one ballot for each bit of the id.  What a row needs for its place, the
+// expert, the lanes of it below and how many there are, is kept in one register, so the ids are read once, all of a lane's
+// at once.
+constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16;
+constexpr int kOrderRows = kOrderWaves * kOrderAtOnce * 64;
 
 __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __restrict__ ids, int n, int experts,
                                                              int bits, int* __restrict__ off, int* __restrict__ perm) {
   __shared__ int count[kOrderWaves][kOrderExperts + 1];
   __shared__ int wave_total[kOrderWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = experts + 1;
+  const int lane = threadIdx.x & 63, groups = experts + 1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int i = threadIdx.x; i < kOrderWaves * groups; i += 1024) count[i / groups][i % groups] = 0;
   __syncthreads();
   const int per = ((n + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
   const int begin = wave * per, end = min(n, begin + per);
-  auto peers = [&](int row, int& key) -> uint64_t {   // the lanes whose row has this lane's expert
-    const int64_t id = row < end ? ids[row] : -1;
-    key = id >= 0 && id < experts ? (int)id : experts;
-    uint64_t m = __ballot(row < end);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot(key >> b & 1);
-      m &= key >> b & 1 ? set : ~set;
+  int* mine = count[wave];
+  uint32_t place[kOrderAtOnce];   // expert | lanes below << 10 | lanes << 16
+  int64_t id[kOrderAtOnce];
+#pragma unroll
+  for (int i = 0; i < kOrderAtOnce; ++i) {
+    const int row = begin + i * 64 + lane;
+    id[i] = row < end ? ids[row] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kOrderAtOnce; ++i) {
+    const int r0 = begin + i * 64;
+    if (r0 >= end) break;
+    const uint32_t key = (uint64_t)id[i] < (uint64_t)experts ? (uint32_t)id[i] : (uint32_t)experts;
+    const uint64_t in = __ballot(r0 + lane < end);
+    uint32_t lo = (uint32_t)in, hi = (uint32_t)(in >> 32);   // the lanes whose row has this lane's expert
+    int x = (int)(key << (32 - bits));
+    for (int b = 0; b < bits; ++b, x <<= 1) {
+      const uint64_t set = __ballot(x < 0);
+      lo &= ~((uint32_t)set ^ (uint32_t)(x >> 31));
+      hi &= ~((uint32_t)(set >> 32) ^ (uint32_t)(x >> 31));
     }
-    return m;
-  };
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int r0 = begin; r0 < end; r0 += 64) {
-    int key;
-    const uint64_t m = peers(r0 + lane, key);
-    if (r0 + lane < end && (m & below) == 0) count[wave][key] += __popcll(m);
-    __builtin_amdgcn_wave_barrier();
+    const uint64_t m = (uint64_t)hi << 32 | lo;
+    const int below = __popcll(m & ((uint64_t(1) << lane) - 1)), lanes = __popcll(m);
+    place[i] = key | below << 10 | lanes << 16;
+    if (r0 + lane < end && below == 0) atomicAdd(&mine[key], lanes);
   }
   __syncthreads();
   int total = 0;
@@ -417,17 +430,30 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
     for (int w = 0; w < kOrderWaves; ++w) count[w][threadIdx.x] += sum - total;
   }
   __syncthreads();
-  for (int r0 = begin; r0 < end; r0 += 64) {
-    int key;
-    const uint64_t m = peers(r0 + lane, key);
-    if (r0 + lane < end) perm[count[wave][key] + __popcll(m & below)] = r0 + lane;
-    __builtin_amdgcn_wave_barrier();
-    if (r0 + lane < end && (m & below) == 0) count[wave][key] += __popcll(m);
-    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < kOrderAtOnce; ++i) {
+    const int r0 = begin + i * 64;
+    if (r0 >= end) break;
+    const bool in = r0 + lane < end;
+    const int key = place[i] & 1023u, below = place[i] >> 10 & 63u, lanes = place[i] >> 16;
+    if (in) perm[mine[key] + below] = r0 + lane;
+    wave_meet();
+    if (in && below == 0) atomicAdd(&mine[key], lanes);   // (before the next rows' reads: LDS keeps a wave's order)
+    wave_meet();
   }
 }
 
-bool small_order(int64_t rows, int experts) { return rows <= kOrderRows && experts <= kOrderExperts; }
+int id_bits(int experts) {
+  int bits = 1;
+  while (experts >> bits) ++bits;
+  return bits;
+}
+
+// Whether one block beats the counting sort's three launches.  Both in us, with ten experts: 5 rows 4.5 / 10, 8,192 7.9
+// / 10.7, 16,384 12.8 / 10.7; with 89 9,000 rows 10.6 / 11; with 300 (a counting sort of another kind) 16,384 19.6 / 29.
+bool small_order(int64_t rows, int experts) {
+  return rows <= kOrderRows && experts <= kOrderExperts && (experts > 255 || rows * (3 + id_bits(experts)) <= 90000);
+}
 
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
 // over one range of rows.
@@ -701,13 +727,10 @@ int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* pe
                       int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(ICTC_F32, rows, 1, 1, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: null operand");
-  // One launch for few rows (5 rows: 3 us, 8,192: 11 us); the counting sort's three (3 to 6 us each) for more.
   if (!small_order(rows, experts))
     return ictc_csr_build(ids, rows, experts, offsets, perm, workspace, workspace_bytes, stream);
-  int bits = 1;
-  while (experts >> bits) ++bits;
-  hipLaunchKernelGGL(experts_order_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, ids, (int)rows, experts, bits,
-                     offsets, perm);
+  hipLaunchKernelGGL(experts_order_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, ids, (int)rows, experts,
+                     id_bits(experts), offsets, perm);
   return dense_status("expert_order launch");
 }
 
@@ -718,8 +741,9 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   if (rows == 0) return ICTC_OK;
   if (ldx < inputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: row pitch below the inputs");
   if (!x || !weight || !perm || !offsets || !out) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: null operand");
-  if ((rows / 64 + experts + 1) * tiles_of(outputs, 64) >= (int64_t(1) << 31))
-    return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: too many tiles");
+  const int tile = outputs <= 64 || experts_tiles(rows, outputs, experts) < 2048 ? 64 : 128;   // the least that is taken
+  if ((rows / tile + experts + 1) * tiles_of(outputs, tile) >= (int64_t(1) << 24))
+    return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: more than 2^24 tiles");
   hipStream_t st = (hipStream_t)stream;
   const bool direct = experts_direct_rows_fit(dtype, x, ldx, inputs, weight, outputs, transpose != 0);
   if (few_is_faster(dtype, direct, transpose != 0, few_groups(rows, experts) * tiles_of(outputs, kFewColumns), inputs)) {

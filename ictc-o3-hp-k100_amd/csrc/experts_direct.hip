@@ -228,7 +228,7 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
       *reinterpret_cast<u32x2*>(st + (li * CH + ((2 * i + (g >> 1)) ^ (li % CH))) * 8 + (g & 1) * 4) =
           *reinterpret_cast<const u32x2*>(v);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_meet();
 #pragma unroll
     for (int h = 0; h < 16 / PER; ++h) {
       const int r = h * PER + lane / CH;
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
           if (cc + q < N) o[q] = v.e[q];
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_meet();
   }
 }
 
