@@ -139,11 +139,16 @@ __device__ __forceinline__ void zero_tile(T* __restrict__ gW, T* __restrict__ gb
 
 }  // namespace
 
-// The kernels of 16-bit types on aligned rows (experts_direct.hip), and whether they take these.
-bool experts_direct_rows_fit(int dtype, const void* x, int64_t ldx, int K, const void* W, int N, bool transpose);
+// The kernels of 16-bit types (experts_direct.hip), and whether they take these: rows of eight elements or more.
+bool experts_direct_rows_fit(int dtype, int K, int N, bool transpose);
 void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st);
+
+// Most runs of up to `tile` rows of one expert (or of none).
+inline int64_t most_runs(int64_t rows, int experts, int tile) {
+  return rows / tile + std::min<int64_t>(rows, experts + 1);
+}
 
 // About as many tiles of 128 x 128 as the rows' product has.
 inline int64_t experts_tiles(int64_t rows, int N, int experts) {
@@ -156,7 +161,7 @@ struct OuterPlan {
   bool direct, sums;
   int tile, rows, ranges, fill;
 };
-bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K);
+bool experts_direct_outer_fits(int dtype, int M, int K);
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,
                           int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
                           float* part, hipStream_t st);

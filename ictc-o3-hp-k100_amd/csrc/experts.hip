@@ -6,7 +6,7 @@
 // Rows come in expert order (perm, offsets: ictc_csr_build), so a tile of 128 rows has one expert and its product is
 // an ordinary matrix product; the gather and the scatter of the rows happen in the tile's own loads and stores.  The
 // tile list is implicit: a block finds its (expert, first row) by a scan of the group sizes, one expert a lane, so
-// nothing is counted on the host and the grid is the upper bound rows / 128 + experts.
+// nothing is counted on the host and the grid is an upper bound (most_runs).
 //
 // Products run on v_mfma_f32_16x16x32; FP32 operands are split exactly into three bfloat16 parts of which the six
 // leading products are kept (FP32-level accuracy, see split_bf16.h; an infinite FP32 input may give NaN).  Both
@@ -602,26 +602,20 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
 
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Most groups of kFewRows rows of one expert (or of none).
-int64_t few_groups(int64_t rows, int experts) { return rows / kFewRows + std::min<int64_t>(rows, experts + 1); }
-
 // Whether `blocks` of experts_few_kernel beat tiles of 64 x 64.  Both measured in us: a round of its blocks (256 FP32,
-// 512 16-bit) takes 7 to 9 / 5 to 6; the tiles take 6.7 / 17.5 / 33 at 128 / 512 / 1,024 inputs in FP32, 4.5 / 9.3 /
-// 15.4 in 16 bits (7 / 18 / 32 through the transpose), 3.5 / 5.5 / 7.7 where they go to LDS directly, up to some
-// thousand rows.
-bool few_is_faster(int dtype, bool direct, bool transpose, int64_t blocks, int inputs) {
+// 512 16-bit) takes 7 to 9 / 5 to 6; the tiles take 6.7 / 17.5 / 33 at 128 / 512 / 1,024 inputs in FP32, 3.5 / 5.5 / 7.7
+// in 16 bits, up to some thousand rows.
+bool few_is_faster(int dtype, int64_t blocks, int inputs) {
   const bool f32 = dtype == ICTC_F32;
   const double few = f32 ? 8.0 * (double)((blocks + 255) / 256) : 5.3 * (double)((blocks + 511) / 512);
-  const double tiles = f32 ? 3.0 + inputs / 36.0
-                       : direct ? 3.0 + inputs / 210.0 : transpose ? 4.0 + inputs / 36.0 : 2.5 + inputs / 80.0;
-  return blocks <= 1024 && few < tiles;
+  return blocks <= 1024 && few < 3.0 + inputs / (f32 ? 36.0 : 210.0);
 }
 
 // Ranges of the weights' gradient: as many blocks as the card has units (256), or twice that where each still gets a
 // thousand rows, and no range shorter than a step.  Measured, in us, at 256 / 512 blocks: 30,000 rows of 256 -> 256
 // bfloat16 18.2 / 18.8, 131,072 of 128 -> 128 20.3 / 22.4, 131,072 of 512 -> 512 146 / 99, 8,192 of 1,024 -> 1,024 48 /
 // 39.  FP32 in tiles of 64 where a block of 128 x 128 would have under 256 rows (2,000 of 336 -> 520 FP32: 34 against 45
-// us; 8,192 of 1,024 -> 1,024 220 against 165); 16-bit tiles of 64 would read four bytes a lane and are not built.
+// us; 8,192 of 1,024 -> 1,024 220 against 165).
 OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K, int experts) {
   OuterPlan p;
   p.direct = direct;
@@ -659,7 +653,7 @@ const char* bad_sizes(int dtype, int64_t rows, int64_t inputs, int64_t outputs, 
 template <typename T, int TILE>
 void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  const dim3 grid((unsigned)((rows / TILE + experts + 1) * tiles_of(N, TILE)));
+  const dim3 grid((unsigned)(most_runs(rows, experts, TILE) * tiles_of(N, TILE)));
   if (transpose)
     hipLaunchKernelGGL((experts_rows_kernel<T, true, TILE>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
@@ -671,7 +665,7 @@ void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W,
 template <typename T>
 void launch_few(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                 const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  const dim3 grid((unsigned)(few_groups(rows, experts) * tiles_of(N, kFewColumns))), block(kFewWaves * 64);
+  const dim3 grid((unsigned)(most_runs(rows, experts, kFewRows) * tiles_of(N, kFewColumns))), block(kFewWaves * 64);
   if (transpose)
     hipLaunchKernelGGL((experts_few_kernel<T, true>), grid, block, 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
@@ -683,14 +677,12 @@ void launch_few(const void* x, int64_t ldx, int64_t rows, int K, const void* W, 
 template <typename T>
 void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  // Tiles of 64 x 64 until those of 128 x 128 fill the card's 512 slots several times over.  Both in us: FP32 131,072
-  // rows of 512 -> 512 575 / 404, 40,000 of 90 experts 191 / 170, 8,192 of 1,024 -> 1,024 146 / 154, 30,000 of 256 ->
-  // 256 41 / 48; 16 bits 131,072 of 512 -> 512 160 / 144, 30,000 of 256 -> 256 17 / 22; through the transpose, where
-  // tiles of 64 read four bytes a lane, 314 / 157 and 34 / 24, 8,192 of 128 -> 128 8 / 9.
-  const int64_t most = sizeof(T) == 4 ? 1024 : transpose ? 256 : 2048;
-  if (N <= 64 || experts_tiles(rows, N, experts) < most)
+  // FP32: tiles of 64 x 64 until those of 128 x 128 fill the card's 512 slots twice.  Both in us: 131,072 rows of 512 ->
+  // 512 575 / 404, 40,000 of 90 experts 191 / 170, 8,192 of 1,024 -> 1,024 146 / 154, 30,000 of 256 -> 256 41 / 48.
+  // (16 bits: rows of under eight elements, always 64.)
+  if (sizeof(T) == 2 || N <= 64 || experts_tiles(rows, N, experts) < 1024)
     launch_rows<T, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
-  else
+  else if constexpr (sizeof(T) == 4)
     launch_rows<T, 128>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
 }
 
@@ -741,12 +733,13 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   if (rows == 0) return ICTC_OK;
   if (ldx < inputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: row pitch below the inputs");
   if (!x || !weight || !perm || !offsets || !out) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: null operand");
-  const int tile = outputs <= 64 || experts_tiles(rows, outputs, experts) < 2048 ? 64 : 128;   // the least that is taken
-  if ((rows / tile + experts + 1) * tiles_of(outputs, tile) >= (int64_t(1) << 24))
+  const bool direct = experts_direct_rows_fit(dtype, inputs, outputs, transpose != 0);
+  const bool wide = outputs > 64 && experts_tiles(rows, outputs, experts) >= 1024 && (direct || dtype == ICTC_F32);
+  const int tile = wide ? 128 : 64;   // the least that is taken
+  if (most_runs(rows, experts, tile) * tiles_of(outputs, tile) >= (int64_t(1) << 24))
     return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: more than 2^24 tiles");
   hipStream_t st = (hipStream_t)stream;
-  const bool direct = experts_direct_rows_fit(dtype, x, ldx, inputs, weight, outputs, transpose != 0);
-  if (few_is_faster(dtype, direct, transpose != 0, few_groups(rows, experts) * tiles_of(outputs, kFewColumns), inputs)) {
+  if (few_is_faster(dtype, most_runs(rows, experts, kFewRows) * tiles_of(outputs, kFewColumns), inputs)) {
     if (dtype == ICTC_F32)
       launch_few<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
     else if (dtype == ICTC_BF16)
@@ -781,7 +774,7 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: row pitch below the row");
   if (!offsets || !dweight || (rows > 0 && (!grad || !x || !perm)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
-  const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, grad, ldg, outputs, x, ldx, inputs),
+  const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, outputs, inputs),
                                     dtype, rows, outputs, inputs, experts);
   if (outer_bytes(plan, outputs, inputs) > 0 &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))

@@ -1,6 +1,6 @@
-// The expert linears' products for bfloat16 and FP16 operands on 16-byte aligned rows: the tiles go from memory to
-// LDS without passing through registers (global_load_lds, 16 bytes a lane), one step of 64 reduction indices ahead of
-// the matrix instructions.
+// The expert linears' products for bfloat16 and FP16 operands with rows of eight elements or more: where all rows begin
+// at multiples of 16 bytes the tiles go from memory to LDS without passing through registers (global_load_lds, 16 bytes a
+// lane), one step ahead of the matrix instructions; else through registers (load_chunk_of), at 0.6 to 0.75 of the speed.
 //
 // A tile of an operand whose rows run along the reduction index is kept [row][64]; one whose memory runs along the
 // rows is kept as it lies, [64][row], and its fragments are transposed as they are read (ds_read_b64_tr_b16: sixteen
@@ -13,7 +13,8 @@
 // blocks share a compute unit and one's first loads and last stores run under another's products: at 131,072 rows of
 // 512 -> 1,024 bfloat16 this measured 216 us and its adjoint 168 us (1,024 -> 512), against 204 / 188 us with 256 x 256
 // tiles (one block of eight waves, steps of 64), which lose a factor of two at 128 -> 128 (41 against 17 us).  For the
-// weights' gradient a step has 64 rows and two blocks share a unit.
+// weights' gradient a step has 64 rows and two blocks share a unit.  Through registers, 131,072 rows of 511 -> 511 FP16:
+// rows 149 us, adjoint 177, weights' gradient 185 (512 -> 512 direct: 99, 99 and 123).
 #include <algorithm>
 
 #include "experts.h"
@@ -29,6 +30,25 @@ __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ void to_lds(const void* p, uint16_t* lds) {
   __builtin_amdgcn_global_load_lds((global_void*)p, (lds_void*)lds, 16, 0, 0);
+}
+
+// Rows that do not begin at multiples of 16 bytes go through registers, to the same places.  The chunk at p has `n`
+// elements of its row left: of a chunk that passes the row's end the eight last elements of the row are read (a row has
+// eight or more) and moved down, and what has none left reads zeros; so no load passes a row's end.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk_of(const T* p, int n) {
+  const T* at = n <= 0 ? reinterpret_cast<const T*>(kZeros) : p - max(0, 8 - n);
+  return *reinterpret_cast<const u32x4_any*>(at);
+}
+__device__ __forceinline__ u32x4 move_chunk(u32x4 raw, int n) {
+  if (n > 0 && n < 8) {
+    const int s = 16 * (8 - n);
+    uint64_t lo = (uint64_t)raw[1] << 32 | raw[0], hi = (uint64_t)raw[3] << 32 | raw[2];
+    lo = s >= 64 ? hi >> (s - 64) : lo >> s | hi << (64 - s);
+    hi = s >= 64 ? 0 : hi >> s;
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+  return raw;
 }
 
 // Chunk exchange of row `r` of an operand kept [S][R]: pairs of chunks (16 columns, R / 16 of them) XORed with this.
@@ -117,7 +137,7 @@ __device__ __forceinline__ void meet() {
 
 // out[perm[r]] = M x[perm[r]] + b, M = W[e] [N, K] or, TRANS, the transpose of W[e] [K, N].  Operand A is the
 // weights (TA output columns), operand B the rows (TB of them).
-template <typename T, bool TRANS, int TA, int TB, int S, int GA, int GB>
+template <typename T, bool ALIGNED, bool TRANS, int TA, int TB, int S, int GA, int GB>
 __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_kernel(
     const T* __restrict__ x, int64_t ldx, int K, const T* __restrict__ W, const T* __restrict__ bias, int N,
     int experts, const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ out) {
@@ -142,7 +162,7 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
   const int wa = wave / GB, wb = wave % GB;
   // the lanes' source addresses at step 0, and the reduction index that each stands at
   const T *pa[LA], *pb[LB];
-  int ka[LA];
+  int ka[LA], na[LA];   // (na: TRANS, the weights' columns from there on)
   constexpr int RC = S / 8, RR = 64 / RC;   // chunks of a row kept [R][S], rows of a load
   const int kb = ((lane % RC) ^ row_swap<S>(lane / RC)) * 8;
 #pragma unroll
@@ -152,7 +172,8 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
       constexpr int CH = TA / 8;   // chunks of a row kept [S][R]
       const int r = block * (64 / CH) + lane / CH, c = (lane % CH) ^ (pair_swap<TA>(r) << 1);
       ka[i] = r;
-      pa[i] = w + (int64_t)r * N + (n0 + 8 * c < N ? n0 + 8 * c : n0);
+      na[i] = N - n0 - 8 * c;
+      pa[i] = w + (int64_t)r * N + (na[i] > 0 ? n0 + 8 * c : n0);
     } else {
       const int r = block * RR + lane / RC;
       ka[i] = kb;
@@ -164,16 +185,33 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
     const int r = (wave * LB + i) * RR + lane / RC;
     pb[i] = x + (int64_t)perm[run.start + (r < run.count ? r : 0)] * ldx + kb;
   }
+  u32x4 ra[LA], rb[LB];   // (not ALIGNED)
   auto load = [&](uint16_t* A, uint16_t* B, int k0) {
     const int left = K - k0;   // reduction indices from here on
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
       const T* p = pa[i] + (TRANS ? (int64_t)k0 * N : (int64_t)k0);
-      to_lds(ka[i] < left ? (const void*)p : (const void*)kZeros, A + (wave * LA + i) * 512);
+      if (ALIGNED)
+        to_lds(ka[i] < left ? (const void*)p : (const void*)kZeros, A + (wave * LA + i) * 512);
+      else
+        ra[i] = load_chunk_of(p, TRANS ? (ka[i] < left ? na[i] : 0) : left - kb);
     }
 #pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      if (ALIGNED)
+        to_lds(kb < left ? (const void*)(pb[i] + k0) : (const void*)kZeros, B + (wave * LB + i) * 512);
+      else
+        rb[i] = load_chunk_of(pb[i] + k0, left - kb);
+    }
+  };
+  auto put = [&](uint16_t* A, uint16_t* B, int k0) {   // not ALIGNED: what load read
+    const int left = K - k0;
+#pragma unroll
+    for (int i = 0; i < LA; ++i)
+      *reinterpret_cast<u32x4*>(A + (wave * LA + i) * 512 + lane * 8) = move_chunk(ra[i], TRANS ? na[i] : left - kb);
+#pragma unroll
     for (int i = 0; i < LB; ++i)
-      to_lds(kb < left ? (const void*)(pb[i] + k0) : (const void*)kZeros, B + (wave * LB + i) * 512);
+      *reinterpret_cast<u32x4*>(B + (wave * LB + i) * 512 + lane * 8) = move_chunk(rb[i], left - kb);
   };
   v4f acc[NA][NB], none[1];
 #pragma unroll
@@ -181,14 +219,17 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   load(A0, B0, 0);
+  if (!ALIGNED) put(A0, B0, 0);
   for (int k0 = 0; k0 < K; k0 += 2 * S) {   // the two buffers are separate objects: a step's reads wait for no load
-    meet<true>();
+    meet<ALIGNED>();
     if (k0 + S < K) load(A1, B1, k0 + S);
     direct_step<T, TRANS, false, TA, TB, S, GA, GB, false>(A0, B0, wa, wb, acc, false, none);
     if (k0 + S < K) {
-      meet<true>();
+      if (!ALIGNED) put(A1, B1, k0 + S);
+      meet<ALIGNED>();
       if (k0 + 2 * S < K) load(A0, B0, k0 + 2 * S);
       direct_step<T, TRANS, false, TA, TB, S, GA, GB, false>(A1, B1, wa, wb, acc, false, none);
+      if (!ALIGNED && k0 + 2 * S < K) put(A0, B0, k0 + 2 * S);
     }
   }
   // The results go through LDS, 16 rows of this wave's columns at a time, so that a store writes runs of them.
@@ -251,33 +292,34 @@ __global__ __launch_bounds__(GA * GB * 64, S == 32 ? 4 : 2) void experts_direct_
   }
 }
 
-template <typename T, bool TRANS, int TA, int TB, int S, int GA, int GB>
+template <typename T, bool ALIGNED, bool TRANS, int TILE, int S>
 void launch_direct(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                    const int* perm, const int* off, void* out, hipStream_t st) {
-  const int64_t blocks = (rows / TB + experts + 1) * ((N + TA - 1) / TA);
-  hipLaunchKernelGGL((experts_direct_kernel<T, TRANS, TA, TB, S, GA, GB>), dim3((unsigned)blocks), dim3(GA * GB * 64), 0,
+  const int64_t blocks = most_runs(rows, experts, TILE) * ((N + TILE - 1) / TILE);
+  hipLaunchKernelGGL((experts_direct_kernel<T, ALIGNED, TRANS, TILE, TILE, S, 2, 2>), dim3((unsigned)blocks), dim3(256), 0,
                      st, (const T*)x, ldx, K, (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
 }
 
-template <typename T>
+template <typename T, bool ALIGNED>
 void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, bool transpose, void* out, hipStream_t st) {
   // Tiles of 64 x 64 where those of 128 x 128 are fewer than the card's units or half empty: 8,192 rows of 128 -> 128 4.4
   // against 6.2 us, 131,072 of 64 -> 64 11 against 15; 16,384 of 256 -> 256 10.1 against 9.6.
+  constexpr int S = ALIGNED ? 32 : 64;   // (transposed: four blocks a unit leave too few registers to load through)
   const bool few = N <= 64 || experts_tiles(rows, N, experts) < 256;
   if (few && transpose)
-    launch_direct<T, true, 64, 64, 64, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    launch_direct<T, ALIGNED, true, 64, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else if (few)
-    launch_direct<T, false, 64, 64, 64, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    launch_direct<T, ALIGNED, false, 64, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else if (transpose)
-    launch_direct<T, true, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    launch_direct<T, ALIGNED, true, 128, S>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else
-    launch_direct<T, false, 128, 128, 32, 2, 2>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    launch_direct<T, ALIGNED, false, 128, 32>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
 }
 
 // Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
 // range of rows: see experts_outer_kernel.
-template <typename T, int TA, int TB, int S, int GA, int GB>
+template <typename T, bool ALIGNED, int TA, int TB, int S, int GA, int GB>
 __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, int K, int experts, int ranges,
     const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ gW, T* __restrict__ gb,
@@ -312,14 +354,28 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
         node[i] = r < seg.count ? perm[seg.start + r] : -1;
       }
     };
+    u32x4 ra[L], rb[L];   // (not ALIGNED)
+    auto column = [&](int i) { return ((lane % CH) ^ (pair_swap<TA>((wave * L + i) * PER + sub) << 1)) * 8; };
     auto load = [&](uint16_t* A, uint16_t* B) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const int c = ((lane % CH) ^ (pair_swap<TA>((wave * L + i) * PER + sub) << 1)) * 8;
-        const int ca = k0 + c < K ? k0 + c : k0, cb = m0 + c < M ? m0 + c : m0;
+        const int c = column(i), ca = k0 + c < K ? k0 + c : k0, cb = m0 + c < M ? m0 + c : m0;
         const bool ok = node[i] >= 0;
-        to_lds(ok ? (const void*)(x + (int64_t)node[i] * ldx + ca) : (const void*)kZeros, A + (wave * L + i) * 512);
-        to_lds(ok ? (const void*)(gy + (int64_t)node[i] * ldg + cb) : (const void*)kZeros, B + (wave * L + i) * 512);
+        const T *px = x + (int64_t)node[i] * ldx + ca, *pg = gy + (int64_t)node[i] * ldg + cb;
+        if (ALIGNED) {
+          to_lds(ok ? (const void*)px : (const void*)kZeros, A + (wave * L + i) * 512);
+          to_lds(ok ? (const void*)pg : (const void*)kZeros, B + (wave * L + i) * 512);
+        } else {
+          ra[i] = load_chunk_of(px, ok ? K - k0 - c : 0);
+          rb[i] = load_chunk_of(pg, ok ? M - m0 - c : 0);
+        }
+      }
+    };
+    auto put = [&](uint16_t* A, uint16_t* B) {   // not ALIGNED: what load read
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        *reinterpret_cast<u32x4*>(A + (wave * L + i) * 512 + lane * 8) = move_chunk(ra[i], K - k0 - column(i));
+        *reinterpret_cast<u32x4*>(B + (wave * L + i) * 512 + lane * 8) = move_chunk(rb[i], M - m0 - column(i));
       }
     };
     v4f acc[NA][NB], accb[NB];
@@ -331,21 +387,24 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     }
     name(0);
     load(A0, B0);
+    if (!ALIGNED) put(A0, B0);
     name(S);
     for (int row = 0; row < seg.count; row += 2 * S) {
-      meet<true>();
+      meet<ALIGNED>();
       if (row + S < seg.count) {
         load(A1, B1);
         name(row + 2 * S);
       }
       direct_step<T, true, true, TA, TB, S, GA, GB, true>(A0, B0, wa, wb, acc, bias, accb);
       if (row + S < seg.count) {
-        meet<true>();
+        if (!ALIGNED) put(A1, B1);
+        meet<ALIGNED>();
         if (row + 2 * S < seg.count) {
           load(A0, B0);
           name(row + 3 * S);
         }
         direct_step<T, true, true, TA, TB, S, GA, GB, true>(A1, B1, wa, wb, acc, bias, accb);
+        if (!ALIGNED && row + 2 * S < seg.count) put(A0, B0);
       }
     }
     meet<false>();   // the next segment's first load overwrites what a wave may still read
@@ -363,57 +422,82 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
 #pragma unroll
       for (int i = 0; i < NA; ++i) {
         const int k = k0 + (wa * NA + i) * 16 + 4 * g;
-        if (k >= K) continue;   // (K is a multiple of 8: four columns are in or out together)
-        if (seg.whole) {
-          T v[4];
+        if (k >= K) continue;
+        T* w = gW + (int64_t)seg.expert * MK + (int64_t)m * K + k;
+        float* p = pw + (int64_t)m * K + k;
+        T v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][e];
-          *reinterpret_cast<u32x2_any*>(gW + (int64_t)seg.expert * MK + (int64_t)m * K + k) =
-              *reinterpret_cast<const u32x2*>(v);
+        for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][e];
+        if (ALIGNED || k + 4 <= K) {   // (ALIGNED: K is a multiple of 8)
+          if (seg.whole)
+            *reinterpret_cast<u32x2_any*>(w) = *reinterpret_cast<const u32x2*>(v);
+          else
+            *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, acc[i][j]);
         } else {
-          *reinterpret_cast<v4f*>(pw + (int64_t)m * K + k) = acc[i][j];
+#pragma unroll
+          for (int e = 0; e < 3; ++e) {
+            if (k + e >= K) continue;
+            if (seg.whole)
+              w[e] = v[e];
+            else
+              p[e] = acc[i][j][e];
+          }
         }
       }
     }
   }
 }
 
-template <typename T>
+template <typename T, bool ALIGNED>
 void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const int64_t tiles = (int64_t)((M + 127) / 128) * ((K + 127) / 128);
   const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles));
-  hipLaunchKernelGGL((experts_direct_outer_kernel<T, 128, 128, 64, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
+  hipLaunchKernelGGL((experts_direct_outer_kernel<T, ALIGNED, 128, 128, 64, 2, 2>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
                        (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
 
 bool whole16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+template <bool ALIGNED, typename... A>
+void typed_rows(int dtype, A... a) {
+  if (dtype == ICTC_BF16)
+    direct_rows<bf16, ALIGNED>(a...);
+  else
+    direct_rows<f16, ALIGNED>(a...);
+}
+
+template <bool ALIGNED, typename... A>
+void typed_outer(int dtype, A... a) {
+  if (dtype == ICTC_BF16)
+    direct_outer<bf16, ALIGNED>(a...);
+  else
+    direct_outer<f16, ALIGNED>(a...);
+}
+
 }  // namespace
 
-bool experts_direct_rows_fit(int dtype, const void* x, int64_t ldx, int K, const void* W, int N, bool transpose) {
-  // 16-byte chunks of x, and of the weights along their memory, have to be whole and aligned
-  return dtype != ICTC_F32 && whole16(x) && ldx % 8 == 0 && K % 8 == 0 && whole16(W) && (!transpose || N % 8 == 0);
+bool experts_direct_rows_fit(int dtype, int K, int N, bool transpose) {
+  return dtype != ICTC_F32 && K >= 8 && (!transpose || N >= 8);
 }
 
 void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,
                          hipStream_t st) {
-  if (dtype == ICTC_BF16)
-    direct_rows<bf16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+  // 16-byte chunks of x, and of the weights along their memory, whole and aligned
+  if (whole16(x) && ldx % 8 == 0 && K % 8 == 0 && whole16(W) && (!transpose || N % 8 == 0))
+    typed_rows<true>(dtype, x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
   else
-    direct_rows<f16>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+    typed_rows<false>(dtype, x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
 }
 
-bool experts_direct_outer_fits(int dtype, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K) {
-  return dtype != ICTC_F32 && whole16(gy) && whole16(x) && ldg % 8 == 0 && ldx % 8 == 0 && M % 8 == 0 && K % 8 == 0;
-}
+bool experts_direct_outer_fits(int dtype, int M, int K) { return dtype != ICTC_F32 && M >= 8 && K >= 8; }
 
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,
                           int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
                           float* part, hipStream_t st) {
-  if (dtype == ICTC_BF16)
-    direct_outer<bf16>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+  if (whole16(gy) && whole16(x) && ldg % 8 == 0 && ldx % 8 == 0 && M % 8 == 0 && K % 8 == 0)
+    typed_outer<true>(dtype, plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
   else
-    direct_outer<f16>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    typed_outer<false>(dtype, plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
 }

@@ -96,6 +96,25 @@ def test_many_rows_repeat_bit_by_bit(device, rows, experts, K, M, dtype):
     assert torch.equal(y, y2) and all(torch.equal(i, j) for i, j in zip(got, again))
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("rows,experts,K,M", [(30000, 5, 9, 131), (30000, 3, 131, 9), (30000, 4, 65, 193), (20000, 3, 8, 300),
+                                              (30000, 2, 300, 7), (26000, 3, 127, 130), (18000, 2, 200, 15)])
+def test_rows_that_end_inside_a_chunk(device, rows, experts, K, M, dtype):
+    """Many rows whose ends, beginnings and pitches are no multiples of 16 bytes, between NaN."""
+    from ictc_o3 import expert_linear, expert_order
+    ids, x, W, b, gy = _inputs(rows, experts, K, M, dtype, rows + K, device)
+    _, Y, ref = _reference(ids, x, W, b, gy)
+    order = expert_order(ids, experts)
+    for front in (0, 3):
+        def held(t):
+            wide = torch.full((rows, t.shape[1] + front + 4), float("nan"), dtype=dtype, device=device)
+            wide[:, front:front + t.shape[1]] = t
+            return wide[:, front:front + t.shape[1]]
+        args = [held(x).requires_grad_(), W.clone().requires_grad_(), b.clone().requires_grad_()]
+        y = expert_linear(args[0], args[1], order, args[2])
+        _check((y, *torch.autograd.grad(y, args, held(gy))), (Y, *ref), ("y", "gx", "gW", "gb"))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_gradients_of_gradients(device, dtype):
     data = _inputs(300, 4, 40, 72, dtype, 2, device)
