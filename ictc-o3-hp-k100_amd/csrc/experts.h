@@ -19,6 +19,47 @@ __device__ __forceinline__ v4f mma(u32x4 a, u32x4 b, v4f c) {
                                                    0, 0);
 }
 
+// split8 (split_bf16.h) with each remainder by one instruction, the pair's dot product with (-1, 0) or (0, -1) added to
+// the value: it is exact as the subtraction is (checked over a million bit patterns), and where one value of a pair is
+// beyond bfloat16's range the other's remainder is NaN too.
+__device__ __forceinline__ Split split8_pairs(const float* v) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first));   // (registers: as an inline constant of a pair -1 would stand for another)
+  asm("" : "+s"(second));
+  const bf16x2 m0 = __builtin_bit_cast(bf16x2, first), m1 = __builtin_bit_cast(bf16x2, second);
+  Split s;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const bf16x2 h = {(__bf16)v[e], (__bf16)v[e + 1]};
+    const float r0 = __builtin_amdgcn_fdot2_f32_bf16(h, m0, v[e], false);
+    const float r1 = __builtin_amdgcn_fdot2_f32_bf16(h, m1, v[e + 1], false);
+    const bf16x2 m = {(__bf16)r0, (__bf16)r1};
+    const bf16x2 l = {(__bf16)__builtin_amdgcn_fdot2_f32_bf16(m, m0, r0, false),
+                      (__bf16)__builtin_amdgcn_fdot2_f32_bf16(m, m1, r1, false)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s.hi[e + i] = h[i];
+      s.mid[e + i] = m[i];
+      s.lo[e + i] = l[i];
+    }
+  }
+  return s;
+}
+
+// The product of one 16 x 16 block over 32 reduction indices from the operands' parts.
+template <typename T, int NP>
+__device__ __forceinline__ v4f product(const u32x4 (&a)[NP], const u32x4 (&b)[NP], v4f c) {
+  if constexpr (NP == 3) {
+    c = mma<T>(a[2], b[0], c);
+    c = mma<T>(a[0], b[2], c);
+    c = mma<T>(a[1], b[1], c);
+    c = mma<T>(a[1], b[0], c);
+    c = mma<T>(a[0], b[1], c);
+  }
+  return mma<T>(a[0], b[0], c);
+}
+
 // Run `t` of groups 0 .. G - 1 cut into runs of `rows` sorted rows: its group, first sorted row and row count.  False
 // past the last run.  The same values in every lane of the wave, which has to be whole.
 struct Run {
@@ -139,7 +180,7 @@ __device__ __forceinline__ void zero_tile(T* __restrict__ gW, T* __restrict__ gb
 
 }  // namespace
 
-// The kernels of 16-bit types (experts_direct.hip), and whether they take these: rows of eight elements or more.
+// The kernels of experts_direct.hip, and whether they take these: rows of 16 bytes or more.
 bool experts_direct_rows_fit(int dtype, int K, int N, bool transpose);
 void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias,
                          int N, int experts, const int* perm, const int* off, bool transpose, void* out,

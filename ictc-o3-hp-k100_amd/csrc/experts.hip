@@ -3,27 +3,29 @@
 //   gW[e] = sum over its rows gy[n] x[n]^T,   gb[e] = sum over its rows gy[n],
 // W [experts, outputs, inputs] of any width, FP32, bfloat16 or FP16, FP32 sums, each result rounded once.
 //
-// Rows come in expert order (perm, offsets: ictc_csr_build), so a tile of 128 rows has one expert and its product is
-// an ordinary matrix product; the gather and the scatter of the rows happen in the tile's own loads and stores.  The
-// tile list is implicit: a block finds its (expert, first row) by a scan of the group sizes, one expert a lane, so
-// nothing is counted on the host and the grid is an upper bound (most_runs).
+// Rows come in expert order (perm, offsets: ictc_expert_order), so a tile of rows has one expert and its product is an
+// ordinary matrix product; the gather and the scatter of the rows happen in the tile's own loads and stores.  The tile
+// list is implicit: a block finds its (expert, first row) by a scan of the group sizes, one expert a lane, so nothing is
+// counted on the host and the grid is an upper bound (most_runs).
 //
 // Products run on v_mfma_f32_16x16x32; FP32 operands are split exactly into three bfloat16 parts of which the six
-// leading products are kept (FP32-level accuracy, see split_bf16.h; an infinite FP32 input may give NaN).  Both
-// operands of a step are staged in LDS as [row][reduction index], 16-byte chunks XORed with the row so that neither
-// the stores nor the fragment reads share banks.  An operand whose memory runs along the other axis (the weights of
-// gx, both operands of gW) is transposed in registers on its way to LDS: eight rows of a few columns per thread.
+// leading products are kept (FP32-level accuracy, see split_bf16.h; an infinite FP32 input may give NaN).  Here are the
+// order, the products of few rows, the sums of partial gradients, the choice among the kernels, and kernels for rows of
+// under 16 bytes; those of experts_direct.hip take the rest.  Both operands of a step here are staged in LDS as
+// [row][reduction index], 16-byte chunks XORed with the row so that neither the stores nor the fragment reads share
+// banks.  An operand whose memory runs along the other axis (the weights of gx, both operands of gW) is transposed in
+// registers on its way to LDS: eight rows of a few columns per thread.
 #include <algorithm>
 
 #include "experts.h"
 
 namespace {
 
-// Tiles of 128 x 128 outputs by four waves of 64 x 64, or of 64 x 64 by waves of 32 x 32.
+// Tiles of 64 x 64 outputs by four waves of 32 x 32, or of 128 x 128 (the weights' gradient in 16 bits).
 template <typename T, int TILE>
 struct Config {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;                     // parts of an operand in LDS
-  static constexpr int BK = sizeof(T) == 4 && TILE == 128 ? 32 : 64;    // reduction indices of a step
+  static constexpr int BK = 64;                                         // reduction indices of a step
   static constexpr int CH = BK / 8;                                     // chunks of a row in LDS
   static constexpr int PER = TILE * CH / 256;                           // chunks staged by a thread
   static constexpr int NC = TILE * BK / 2048;                           // columns per thread of a transposed operand
@@ -77,18 +79,14 @@ __device__ __forceinline__ Few<T, NC> load_few(const T* __restrict__ p, int n) {
 }
 
 // 16-bit offset of chunk `ch` of row `row` in a part of an operand
-template <int CH>
-__device__ __forceinline__ int lds_at(int row, int ch) {
-  const int swz = CH == 8 ? (row ^ (row >> 3)) & 7 : (row >> 2) & 3;
-  return (row * CH + (ch ^ swz)) * 8;
-}
+__device__ __forceinline__ int lds_at(int row, int ch) { return (row * 8 + (ch ^ ((row ^ (row >> 3)) & 7))) * 8; }
 
 template <typename T, int TILE>
 __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch, const Eight<T>& v) {
   using C = Config<T, TILE>;
-  uint16_t* at = lds + lds_at<C::CH>(row, ch);
+  uint16_t* at = lds + lds_at(row, ch);
   if constexpr (sizeof(T) == 4) {
-    const Split s = split8(v.e);
+    const Split s = split8_pairs(v.e);
     *reinterpret_cast<bf16x8*>(at) = s.hi;
     *reinterpret_cast<bf16x8*>(at + C::PART) = s.mid;
     *reinterpret_cast<bf16x8*>(at + 2 * C::PART) = s.lo;
@@ -97,24 +95,11 @@ __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch,
   }
 }
 
-// The product of one 16 x 16 block over 32 reduction indices from the operands' parts.
-template <typename T, int NP>
-__device__ __forceinline__ v4f product(const u32x4 (&a)[NP], const u32x4 (&b)[NP], v4f c) {
-  if constexpr (NP == 3) {
-    c = mma<T>(a[2], b[0], c);
-    c = mma<T>(a[0], b[2], c);
-    c = mma<T>(a[1], b[1], c);
-    c = mma<T>(a[1], b[0], c);
-    c = mma<T>(a[0], b[1], c);
-  }
-  return mma<T>(a[0], b[0], c);
-}
-
 template <typename T, int TILE>
 __device__ __forceinline__ void fragment(const uint16_t* __restrict__ lds, int row, int ch,
                                          u32x4 (&f)[Config<T, TILE>::NP]) {
   using C = Config<T, TILE>;
-  const uint16_t* at = lds + lds_at<C::CH>(row, ch);
+  const uint16_t* at = lds + lds_at(row, ch);
 #pragma unroll
   for (int p = 0; p < C::NP; ++p) f[p] = *reinterpret_cast<const u32x4*>(at + p * C::PART);
 }
@@ -285,14 +270,14 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
 }
 
 // The same for few rows: a block takes 16 rows of an expert and 32 columns, its eight waves share the reduction, and
-// every lane reads its fragments' values from memory itself, so a call is one round of loads, not a chain of steps (1
-// row of 1,024 -> 1,024 FP32: 33 us in tiles of 64).  The waves' sums are added in order.
+// every lane reads its fragments' values from memory itself, so a call is one round of loads, not a chain of steps (1 row
+// of 1,024 -> 1,024 FP32: 7.8 us, 24 in tiles of 64).  The waves' sums are added in order.  Two blocks share a unit.
 constexpr int kFewRows = 16, kFewColumns = 32, kFewWaves = 8;
 
 template <typename T>
 __device__ __forceinline__ void parts(const Eight<T>& v, u32x4 (&f)[sizeof(T) == 4 ? 3 : 1]) {
   if constexpr (sizeof(T) == 4) {
-    const Split s = split8(v.e);
+    const Split s = split8_pairs(v.e);
     f[0] = __builtin_bit_cast(u32x4, s.hi);
     f[1] = __builtin_bit_cast(u32x4, s.mid);
     f[2] = __builtin_bit_cast(u32x4, s.lo);
@@ -302,7 +287,7 @@ __device__ __forceinline__ void parts(const Eight<T>& v, u32x4 (&f)[sizeof(T) ==
 }
 
 template <typename T, bool TRANS>
-__global__ __launch_bounds__(kFewWaves * 64) void experts_few_kernel(const T* __restrict__ x, int64_t ldx, int K,
+__global__ __launch_bounds__(kFewWaves * 64, 4) void experts_few_kernel(const T* __restrict__ x, int64_t ldx, int K,
                                                                     const T* __restrict__ W,
                                                                     const T* __restrict__ bias, int N, int experts,
                                                                     const int* __restrict__ perm,
@@ -602,31 +587,33 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
 
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Whether `blocks` of experts_few_kernel beat tiles of 64 x 64.  Both measured in us: a round of its blocks (256 FP32,
-// 512 16-bit) takes 7 to 9 / 5 to 6; the tiles take 6.7 / 17.5 / 33 at 128 / 512 / 1,024 inputs in FP32, 3.5 / 5.5 / 7.7
-// in 16 bits, up to some thousand rows.
+// Whether `blocks` of experts_few_kernel beat tiles of 64 x 64, from both measured in us (straight and transposed within
+// 0.5): tiles of FP32 5.8 / 13.8 / 24 / 45 at 128 / 512 / 1,024 / 2,048 inputs, of 16 bits 3.8 / 5.5 / 7.9 / 12.7, up to
+// some thousand rows; the others at those inputs, of one round (256 blocks) FP32 6.2 / 7.5 / 9.6 / 16 and 16 bits 5.2 / 5.5
+// / 5.7 / 8.4, of two rounds FP32 7.2 / 10.4 / 15.4 / 26 and 16 bits 5.5 / 6.8 / 8.3 / 13.9.
 bool few_is_faster(int dtype, int64_t blocks, int inputs) {
-  const bool f32 = dtype == ICTC_F32;
-  const double few = f32 ? 8.0 * (double)((blocks + 255) / 256) : 5.3 * (double)((blocks + 511) / 512);
-  return blocks <= 1024 && few < 3.0 + inputs / (f32 ? 36.0 : 210.0);
+  const double rounds = (double)((blocks + 255) / 256), k = inputs;
+  return dtype == ICTC_F32 ? 5.0 + rounds * (1.0 + k / 230.0) < 3.2 + k / 49.0
+                           : 4.2 + rounds * k / 450.0 < 3.3 + k / 230.0;
 }
 
-// Ranges of the weights' gradient: as many blocks as the card has units (256), or twice that where each still gets a
-// thousand rows, and no range shorter than a step.  Measured, in us, at 256 / 512 blocks: 30,000 rows of 256 -> 256
-// bfloat16 18.2 / 18.8, 131,072 of 128 -> 128 20.3 / 22.4, 131,072 of 512 -> 512 146 / 99, 8,192 of 1,024 -> 1,024 48 /
-// 39.  FP32 in tiles of 64 where a block of 128 x 128 would have under 256 rows (2,000 of 336 -> 520 FP32: 34 against 45
-// us; 8,192 of 1,024 -> 1,024 220 against 165).
+// Ranges of the weights' gradient: two blocks for each of the card's 256 units; one in 16 bits where a block would have
+// under a thousand rows, unless experts have so few; and no range shorter than a step.  Measured, in us, at 256 / 512
+// blocks: bfloat16 131,072 rows of 128 -> 128 20.3 / 22.4, of 512 -> 512 146 / 99, 30,000 of 512 -> 512 over 40 experts 80
+// / 62; FP32 30,000 of 512 -> 512 over 40 experts 223 / 136, 16,384 of 512 -> 512 over ten 90 / 82.  FP32 in tiles of 64
+// where a block of 128 x 128 would have under 256 rows (2,000 of 336 -> 520 34 against 45 us; 16,384 of 512 -> 512 100
+// against 82).
 OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K, int experts) {
   OuterPlan p;
   p.direct = direct;
   p.tile = 128;
-  int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128), blocks = n * tiles >= 512 * 1024 ? 512 : 256;
-  if (dtype == ICTC_F32 && n * tiles < 512 * 256) {
+  int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128);
+  const int64_t blocks = dtype == ICTC_F32 || n * tiles >= 512 * 1024 || n < 1024 * (int64_t)experts ? 512 : 256;
+  if (dtype == ICTC_F32 && (!direct || n * tiles < 512 * 256)) {
     p.tile = 64;
     tiles = tiles_of(M, 64) * tiles_of(K, 64);
-    blocks = 512;
   }
-  p.rows = p.tile == 128 && dtype == ICTC_F32 ? Config<float, 128>::BK : 64;
+  p.rows = p.tile == 128 && dtype == ICTC_F32 ? 32 : 64;
   const int64_t steps = n / p.rows + std::min<int64_t>(n, experts);   // about as many as there are
   p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(blocks / tiles, steps));
   // Experts of few rows: a range for each of them, not several one after another (64 rows of ten experts, 128 -> 128
@@ -650,15 +637,15 @@ const char* bad_sizes(int dtype, int64_t rows, int64_t inputs, int64_t outputs, 
   return nullptr;
 }
 
-template <typename T, int TILE>
+template <typename T>
 void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  const dim3 grid((unsigned)(most_runs(rows, experts, TILE) * tiles_of(N, TILE)));
+  const dim3 grid((unsigned)(most_runs(rows, experts, 64) * tiles_of(N, 64)));
   if (transpose)
-    hipLaunchKernelGGL((experts_rows_kernel<T, true, TILE>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+    hipLaunchKernelGGL((experts_rows_kernel<T, true, 64>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<T, false, TILE>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+    hipLaunchKernelGGL((experts_rows_kernel<T, false, 64>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
 }
 
@@ -675,27 +662,11 @@ void launch_few(const void* x, int64_t ldx, int64_t rows, int K, const void* W, 
 }
 
 template <typename T>
-void choose_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
-                 const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
-  // FP32: tiles of 64 x 64 until those of 128 x 128 fill the card's 512 slots twice.  Both in us: 131,072 rows of 512 ->
-  // 512 575 / 404, 40,000 of 90 experts 191 / 170, 8,192 of 1,024 -> 1,024 146 / 154, 30,000 of 256 -> 256 41 / 48.
-  // (16 bits: rows of under eight elements, always 64.)
-  if (sizeof(T) == 2 || N <= 64 || experts_tiles(rows, N, experts) < 1024)
-    launch_rows<T, 64>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
-  else if constexpr (sizeof(T) == 4)
-    launch_rows<T, 128>(x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
-}
-
-template <typename T>
 void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
-  if (sizeof(T) == 4 && plan.tile == 64)
-    hipLaunchKernelGGL((experts_outer_kernel<float, 64>), grid, dim3(256), 0, st, (const float*)gy, ldg, M,
-                       (const float*)x, ldx, K, experts, plan.ranges, perm, off, (float*)gW, (float*)gb, part);
-  else
-    hipLaunchKernelGGL((experts_outer_kernel<T, 128>), grid, dim3(256), 0, st, (const T*)gy, ldg, M, (const T*)x, ldx,
-                       K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  hipLaunchKernelGGL((experts_outer_kernel<T, (sizeof(T) == 4 ? 64 : 128)>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
+                     (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
 
 template <typename T>
@@ -734,7 +705,7 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
   if (ldx < inputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: row pitch below the inputs");
   if (!x || !weight || !perm || !offsets || !out) return dense_fail(ICTC_ERR_ARGUMENT, "expert_linear: null operand");
   const bool direct = experts_direct_rows_fit(dtype, inputs, outputs, transpose != 0);
-  const bool wide = outputs > 64 && experts_tiles(rows, outputs, experts) >= 1024 && (direct || dtype == ICTC_F32);
+  const bool wide = outputs > 64 && experts_tiles(rows, outputs, experts) >= 1024 && direct;
   const int tile = wide ? 128 : 64;   // the least that is taken
   if (most_runs(rows, experts, tile) * tiles_of(outputs, tile) >= (int64_t(1) << 24))
     return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_linear: more than 2^24 tiles");
@@ -752,11 +723,11 @@ int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int 
     experts_direct_rows(dtype, x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose != 0, out,
                         st);
   else if (dtype == ICTC_F32)
-    choose_rows<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
+    launch_rows<float>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   else if (dtype == ICTC_BF16)
-    choose_rows<bf16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
+    launch_rows<bf16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   else
-    choose_rows<f16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
+    launch_rows<f16>(x, ldx, rows, inputs, weight, bias, outputs, experts, perm, offsets, transpose, out, st);
   return dense_status("expert_linear launch");
 }
 
