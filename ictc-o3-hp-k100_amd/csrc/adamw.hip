@@ -13,7 +13,10 @@
 // linear grid, and a nonzero value never becomes zero: a step would blow up on the next small gradient.  A block
 // with NaN or infinity gets a NaN scale: the parameters it feeds become NaN, as they do with FP32 moments.
 //
-// Bound by memory: p and g in, p out, both moments in and out, 28 bytes an element in FP32, 16 with 8-bit moments.
+// Bound by memory: p and g in, p out, both moments in and out, 28 bytes an element in FP32, 16 with 8-bit moments; the
+// norm reads g once more before.  Measured: 80 M bfloat16 parameters with FP32 moments 313 us (5.6 TB/s) and 64 us for
+// the norm; 100 M FP32 with 8-bit moments 318 us (5.0 TB/s) and 127 us (3.2 TB/s: the moments that the update wrote are
+// still on their way to memory); 1.2 M FP32 in 42 tensors 7.2 and 5 us.
 // A block of 256 threads takes a run of 2,048 elements of one tensor; the tensors' pointers travel in the kernel's
 // arguments, so no table is copied to the device.  A wave holds one 256-element block of the state, four elements
 // a lane, so its largest value is a wave reduction.

