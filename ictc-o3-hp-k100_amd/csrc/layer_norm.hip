@@ -359,7 +359,11 @@ int64_t blocks_of(int64_t rows, int team, int64_t most) {
   return std::max<int64_t>(1, std::min<int64_t>(most, (rows + teams - 1) / teams));
 }
 
-constexpr int64_t kFwdBlocks = 2048;
+// Blocks of the forward kernel: four a unit, two for the widest rows.  Measured at 512 / 1,024 / 2,048 blocks: 425,991 x 64
+// FP32 56 / 41 / 44 us, 8,191 x 2,176 FP32 32 / 30 / 35, bfloat16 26 / 20 / 21, 2,048 x 8,192 bfloat16 14 / 16 / 18, FP32
+// 28 / 29 / 36; 32,768 x 500 bfloat16, the other way, 30 / 20 / 17.
+int64_t fwd_blocks(int64_t rows, int team, int width) { return blocks_of(rows, team, width <= 4096 ? 1024 : 512); }
+
 // The blocks of the gradient kernels each leave a partial row per parameter: fewer of them for wide rows.  Measured at
 // 256 / 512 / 1,024 blocks: 425,991 x 64 FP32 103 / 65 / 67 us, 8,191 x 2,176 bfloat16 44 / 36 / 45 us, 2,048 x 8,192
 // bfloat16 37 / 53 / 83 us.
@@ -385,7 +389,7 @@ template <typename T>
 int run_fwd(const void* x, int64_t ldx, int64_t rows, int width, const void* weight, const void* bias, float eps,
             void* y, float* mean, float* rstd, hipStream_t st) {
   const Shape s = shape_of(width, kChunk<T>);
-  const dim3 grid((unsigned)blocks_of(rows, s.team, kFwdBlocks));
+  const dim3 grid((unsigned)fwd_blocks(rows, s.team, width));
   LN_DISPATCH(T, hipLaunchKernelGGL((ln_fwd_kernel<T, TEAM, EPL>), grid, dim3(kThreads<TEAM>), 0, st, (const T*)x,
                                     ldx, rows, width, (const T*)weight, (const T*)bias, eps, (T*)y, mean, rstd))
   return dense_status("layer_norm_fwd launch");
