@@ -350,24 +350,54 @@ __global__ __launch_bounds__(kFewWaves * 64, 4) void experts_few_kernel(const T*
     if (c + q < N) o[q] = valid ? (T)(t[q] + (bias ? (float)bias[(int64_t)run.group * N + c + q] : 0.f)) : (T)0.f;
 }
 
-// The stable order of up to kOrderRows rows by expert (ids outside [0, experts) last) by one block: each wave counts
-// the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves place their
-// rows.  Lanes of one expert find each other by one ballot for each bit of the id.  What a row needs for its place, the
-// expert, the lanes of it below and how many there are, is kept in one register, so the ids are read once, all of a lane's
-// at once.
-constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16;
+// The stable order of the rows by expert (ids outside [0, experts) last).  A block takes up to kOrderRows of them: each
+// wave counts the experts of a run of rows, the counts are scanned expert by expert and wave by wave, and the waves place
+// their rows.  Lanes of one expert find each other by one ballot for each bit of the id.  What a row needs for its place,
+// the expert, the lanes of it below and how many there are, is kept in one register, so the ids are read once, all of a
+// lane's at once.  One block does it alone; of several, each has `span` rows and adds up, from all blocks' counts
+// ([blocks, experts + 1], the kernel below), what lies before its own.
+constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16, kOrderBlocks = 256;
 constexpr int kOrderRows = kOrderWaves * kOrderAtOnce * 64;
 
+__global__ __launch_bounds__(1024) void experts_count_kernel(const int64_t* __restrict__ ids, int n, int experts,
+                                                             int span, int* __restrict__ counts) {
+  __shared__ int count[kOrderExperts + 1];
+  if ((int)threadIdx.x <= experts) count[threadIdx.x] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * span, end = min(n, begin + span);
+  for (int r0 = begin + (int)threadIdx.x; r0 < end; r0 += 4096) {
+    int64_t id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = r0 + i * 1024 < end ? ids[r0 + i * 1024] : -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r0 + i * 1024 < end) atomicAdd(&count[(uint64_t)id[i] < (uint64_t)experts ? (int)id[i] : experts], 1);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x <= experts) counts[blockIdx.x * (experts + 1) + threadIdx.x] = count[threadIdx.x];
+}
+
 __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __restrict__ ids, int n, int experts,
-                                                             int bits, int* __restrict__ off, int* __restrict__ perm) {
+                                                             int bits, int span, const int* __restrict__ counts,
+                                                             int* __restrict__ off, int* __restrict__ perm) {
   __shared__ int count[kOrderWaves][kOrderExperts + 1];
   __shared__ int wave_total[kOrderWaves];
-  const int lane = threadIdx.x & 63, groups = experts + 1;
+  const int lane = threadIdx.x & 63, groups = experts + 1, group = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int i = threadIdx.x; i < kOrderWaves * groups; i += 1024) count[i / groups][i % groups] = 0;
+  int total = 0, before = 0;   // of this group: all rows, and those of the blocks before
+  if (counts && group < groups) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int c = counts[b * groups + group];
+      total += c;
+      before += b < (int)blockIdx.x ? c : 0;
+    }
+  }
   __syncthreads();
-  const int per = ((n + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
-  const int begin = wave * per, end = min(n, begin + per);
+  const int first = blockIdx.x * span, rows = min(span, n - first);
+  const int per = ((rows + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
+  const int begin = first + wave * per, end = min(first + rows, begin + per);
   int* mine = count[wave];
   uint32_t place[kOrderAtOnce];   // expert | lanes below << 10 | lanes << 16
   int64_t id[kOrderAtOnce];
@@ -395,24 +425,26 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
     if (r0 + lane < end && below == 0) atomicAdd(&mine[key], lanes);
   }
   __syncthreads();
-  int total = 0;
-  if ((int)threadIdx.x < groups) {
+  int here = 0;
+  if (group < groups) {
 #pragma unroll
     for (int w = 0; w < kOrderWaves; ++w) {
-      const int c = count[w][threadIdx.x];
-      count[w][threadIdx.x] = total;
-      total += c;
+      const int c = count[w][group];
+      count[w][group] = here;
+      here += c;
     }
   }
+  if (!counts) total = here;
   int sum = scan_lanes(total);
   if (lane == 63) wave_total[wave] = sum;
   __syncthreads();
   for (int w = 0; w < wave; ++w) sum += wave_total[w];
-  if ((int)threadIdx.x < groups) {
-    off[threadIdx.x] = sum - total;
-    if ((int)threadIdx.x == experts) off[groups] = n;
+  if (group < groups) {
+    const int start = sum - total;
+    if (blockIdx.x == 0) off[group] = start;
+    if (blockIdx.x == 0 && group == experts) off[groups] = n;
 #pragma unroll
-    for (int w = 0; w < kOrderWaves; ++w) count[w][threadIdx.x] += sum - total;
+    for (int w = 0; w < kOrderWaves; ++w) count[w][group] += start + before;
   }
   __syncthreads();
 #pragma unroll
@@ -428,16 +460,21 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
   }
 }
 
+int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
+
 int id_bits(int experts) {
   int bits = 1;
   while (experts >> bits) ++bits;
   return bits;
 }
 
-// Whether one block beats the counting sort's three launches.  Both in us, with ten experts: 5 rows 4.5 / 10, 8,192 7.9
-// / 10.7, 16,384 12.8 / 10.7; with 89 9,000 rows 10.6 / 11; with 300 (a counting sort of another kind) 16,384 19.6 / 29.
-bool small_order(int64_t rows, int experts) {
-  return rows <= kOrderRows && experts <= kOrderExperts && (experts > 255 || rows * (3 + id_bits(experts)) <= 90000);
+// Rows of a block: all of few rows; 4,096; more once those would be more than 64 blocks; and zero: the general sort.  Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5, 16,384 12.9 / 9.0; 89 experts
+// 6,000 rows 8.2 / 8.7, 16,384 16.4 / 10.1.  Several / the general sort, ten experts: 30,011 rows
+// 8.8 / 10.8, 262,145 11.8 / 106, 4.2 million 32 / 83.
+int order_span(int64_t rows, int experts) {
+  if (experts > kOrderExperts || rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
+  if (rows <= kOrderRows && rows * (3 + id_bits(experts)) <= 60000) return (int)std::max<int64_t>(rows, 1);
+  return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(4096, (rows / 64 + 1023) / 1024 * 1024));
 }
 
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
@@ -585,8 +622,6 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
   }
 }
 
-int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
-
 // Whether `blocks` of experts_few_kernel beat tiles of 64 x 64, from both measured in us (straight and transposed within
 // 0.5): tiles of FP32 5.8 / 13.8 / 24 / 45 at 128 / 512 / 1,024 / 2,048 inputs, of 16 bits 3.8 / 5.5 / 7.9 / 12.7, up to
 // some thousand rows; the others at those inputs, of one round (256 blocks) FP32 6.2 / 7.5 / 9.6 / 16 and 16 bits 5.2 / 5.5
@@ -683,17 +718,28 @@ extern "C" {
 
 int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts) {
   if (bad_sizes(ICTC_F32, rows, 1, 1, experts)) return -1;
-  return small_order(rows, experts) ? 0 : ictc_csr_workspace_bytes(rows, experts);
+  const int span = order_span(rows, experts);
+  if (span == 0) return ictc_csr_workspace_bytes(rows, experts);
+  return rows <= span ? 0 : tiles_of(rows, span) * (experts + 1) * (int64_t)sizeof(int);
 }
 
 int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
                       int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(ICTC_F32, rows, 1, 1, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: null operand");
-  if (!small_order(rows, experts))
-    return ictc_csr_build(ids, rows, experts, offsets, perm, workspace, workspace_bytes, stream);
-  hipLaunchKernelGGL(experts_order_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, ids, (int)rows, experts,
-                     id_bits(experts), offsets, perm);
+  const int span = order_span(rows, experts);
+  if (span == 0) return ictc_csr_build(ids, rows, experts, offsets, perm, workspace, workspace_bytes, stream);
+  const bool several = rows > span;
+  if (several && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) ||
+                  workspace_bytes < ictc_expert_order_workspace_bytes(rows, experts)))
+    return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: workspace smaller than ictc_expert_order_workspace_bytes");
+  const dim3 blocks((unsigned)std::max<int64_t>(1, tiles_of(rows, span)));
+  int* counts = several ? (int*)workspace : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (several)
+    hipLaunchKernelGGL(experts_count_kernel, blocks, dim3(1024), 0, st, ids, (int)rows, experts, span, counts);
+  hipLaunchKernelGGL(experts_order_kernel, blocks, dim3(1024), 0, st, ids, (int)rows, experts, id_bits(experts), span,
+                     counts, offsets, perm);
   return dense_status("expert_order launch");
 }
 

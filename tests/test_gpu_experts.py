@@ -271,6 +271,21 @@ def test_order(device, rows, experts):
     assert torch.equal(order.offsets.cpu().long(), torch.cat([starts, torch.tensor([rows])]))
 
 
+@pytest.mark.parametrize("rows", [8571, 8572, 12288, 65537, 262145, 1048577, 4194305])
+@pytest.mark.parametrize("experts", [1, 10, 300, 1023])
+def test_order_of_many_rows(device, rows, experts):
+    """Blocks that each place a part of the rows, whole parts and a last one of one row."""
+    from ictc_o3 import expert_order
+    ids = torch.randint(-1, experts + 1, (rows,), device=device, generator=torch.Generator(device).manual_seed(rows + experts))
+    order = expert_order(ids, experts)
+    key = torch.where((ids >= 0) & (ids < experts), ids, torch.full_like(ids, experts))
+    placed = order.perm[:rows].long()
+    assert torch.equal(torch.bincount(placed, minlength=rows), torch.ones(rows, dtype=torch.int64, device=device))
+    assert (torch.diff(key[placed] * rows + placed) > 0).all()   # by expert, then by row
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64, device=device), torch.bincount(key, minlength=experts + 1).cumsum(0)])
+    assert torch.equal(order.offsets.long(), starts)
+
+
 def test_refusals(device):
     from ictc_o3 import expert_linear, expert_order
     ids = torch.zeros(6, dtype=torch.int64, device=device)
