@@ -107,19 +107,22 @@ def train(steps=300, cells=4, n=3, state_bits=32, lr=4e-3, seed=0, device="cuda"
     order = expert_order(data["element"], ELEMENTS)
     atoms = data["pos"].shape[0] // cells
     history = []
-    for k in range(steps):
-        pos = data["pos"].requires_grad_()
-        energy = model(pos, data["element"], order, data["src"], data["dst"], data["shift"])
-        forces = -torch.autograd.grad(energy.sum(), pos, create_graph=True)[0]
-        e_loss = ((energy.view(cells, -1).sum(1) - data["energy"]) / atoms).square().mean()
-        f_loss = (forces - data["forces"]).square().mean()
-        opt.zero_grad()
-        (e_loss + 10 * f_loss).backward(inputs=[p for p in model.parameters() if p.requires_grad])
-        opt.step()
-        history.append(torch.stack([e_loss.detach(), f_loss.detach(), opt.grad_norm]))
-        if log and (k % 50 == 0 or k == steps - 1):
-            e, f, norm = history[-1].tolist()
-            log(f"step {k:4d}  energy loss {e:.5f} per atom^2  force loss {f:.5f}  gradient norm {norm:.3f}")
+    # A system as small as these is bound by its host: backward passes in this thread, not handed over to the engine's
+    # (3.6 to 4.5 ms a step with it, 2.8 to 3.0 without).
+    with torch.autograd.set_multithreading_enabled(False):
+        for k in range(steps):
+            pos = data["pos"].requires_grad_()
+            energy = model(pos, data["element"], order, data["src"], data["dst"], data["shift"])
+            forces = -torch.autograd.grad(energy.sum(), pos, create_graph=True)[0]
+            e_loss = ((energy.view(cells, -1).sum(1) - data["energy"]) / atoms).square().mean()
+            f_loss = (forces - data["forces"]).square().mean()
+            opt.zero_grad()
+            (e_loss + 10 * f_loss).backward(inputs=[p for p in model.parameters() if p.requires_grad])
+            opt.step()
+            history.append(torch.stack([e_loss.detach(), f_loss.detach(), opt.grad_norm]))
+            if log and (k % 50 == 0 or k == steps - 1):
+                e, f, norm = history[-1].tolist()
+                log(f"step {k:4d}  energy loss {e:.5f} per atom^2  force loss {f:.5f}  gradient norm {norm:.3f}")
     return model, torch.stack(history).cpu()
 
 

@@ -17,7 +17,7 @@
 // teams of a block in LDS, and the blocks' partial sums by a second kernel, always in the same order.
 //
 // Measured: 425,991 rows of 64 FP32 forward 38 us (5.7 TB/s), gradients 54 us (6.1 TB/s) and 4.7 us for the blocks'
-// sums; 131,072 of 128 FP32 second derivative 58 us (5.8 TB/s); 8,191 of 2,176 bfloat16 forward 20 us and gradients
+// sums; 131,072 of 128 FP32 second derivative 55 us (6.1 TB/s); 8,191 of 2,176 bfloat16 forward 20 us and gradients
 // 29 us (3.6 TB/s: a few rows a block, whose first loads and last stores wait for nothing else); 257 of 64 about 3 us
 // each, the latency of a launch.  A large copy reaches 5.1 TB/s; operands that the caches still hold come faster.
 #include "dense.h"
