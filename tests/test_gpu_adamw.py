@@ -203,6 +203,21 @@ def test_nan_and_infinity_reach_only_their_own(device, bits):
         assert torch.isfinite(ps[1]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[1], [0, 5, 0], [2048 * 8], [2048 * 8 + 1], [2048] * 8, [300] * 9, [1] * 121, [2049, 7, 6000]])
+def test_norms_of_few_elements(device, dtype, counts):
+    """Squares and eight of them are added in FP32, under five units of 2^-24 of the norm, and the norm is rounded."""
+    from ictc_o3 import AdamW
+    g = torch.Generator().manual_seed(sum(counts))
+    ps = [torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=device)) for n in counts]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g).to(dtype).to(device)
+    opt = AdamW(ps, max_norm=0.5)
+    opt.step()
+    ref = torch.cat([p.grad.double() for p in ps]).norm()
+    assert abs(float(opt.grad_norm) - float(ref)) < 1e-6 * float(ref)
+
+
 def test_a_bound_with_a_non_finite_norm_is_loud(device):
     from ictc_o3 import adamw_step
     p, g = torch.ones(300, device=device), torch.ones(300, device=device)

@@ -302,3 +302,23 @@ def test_refusals(device):
     for bad in ((ids.int(), 2), (ids.view(2, 3), 2), (ids, 0), (ids, 70000), (ids, 2.0), (ids.cpu(), 2)):
         with pytest.raises(ValueError):
             expert_order(*bad)
+
+
+@pytest.mark.parametrize("dtype,K,M", [(torch.bfloat16, 1000, 72), (torch.float16, 17, 1001)])
+def test_offsets_past_32_bits(device, dtype, K, M):
+    """Rows or outputs of more than 2^31 elements: the first and last rows, and their gradients alone."""
+    from ictc_o3 import expert_linear, expert_order
+    N, E = 2200000, 5
+    g = torch.Generator(device).manual_seed(1)
+    x = torch.randn(N, K, device=device, dtype=dtype, generator=g).requires_grad_()
+    ids = torch.randint(0, E, (N,), device=device, generator=g)
+    W = (torch.randn(E, M, K, device=device, generator=g) / math.sqrt(K)).to(dtype).requires_grad_()
+    y = expert_linear(x, W, expert_order(ids, E))
+    ends = torch.cat([torch.arange(0, 200, device=device), torch.arange(N - 200, N, device=device)])
+    gy = torch.zeros(N, M, device=device, dtype=dtype)
+    gy[ends] = torch.randn(400, M, device=device, generator=g).to(dtype)
+    gx, gW = torch.autograd.grad(y, (x, W), gy)
+    few = [t.detach().double().requires_grad_() for t in (x[ends], W)]
+    Y = _formula(*few, None, ids[ends])
+    _check((y[ends], gx[ends], gW), (Y, *torch.autograd.grad(Y, few, gy[ends].double())), ("y", "gx", "gW"))
+    assert gx[200:400].abs().max() == 0

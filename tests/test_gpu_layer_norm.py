@@ -227,3 +227,22 @@ def test_graph_replays_and_side_streams(device):
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(i, j) for i, j in zip(held, eager)), k
+
+
+def test_offsets_past_32_bits(device):
+    """More than 2^31 elements: the first and last rows and their gradients alone."""
+    from ictc_o3 import layer_norm
+    N, C = 34000000, 64
+    g = torch.Generator(device).manual_seed(1)
+    x = torch.randn(N, C, device=device, generator=g).requires_grad_()
+    w, b = (torch.randn(C, device=device, generator=g).requires_grad_() for _ in range(2))
+    y = layer_norm(x, w, b)
+    ends = torch.cat([torch.arange(0, 200, device=device), torch.arange(N - 200, N, device=device)])
+    gy = torch.zeros(N, C, device=device)
+    gy[ends] = torch.randn(400, C, device=device, generator=g)
+    got = torch.autograd.grad(y, (x, w, b), gy)
+    few = [t.detach().double().requires_grad_() for t in (x[ends], w, b)]
+    Y = torch.nn.functional.layer_norm(few[0], (C,), few[1], few[2])
+    ref = torch.autograd.grad(Y, few, gy[ends].double())
+    for a, r in zip((y[ends], got[0][ends], got[1], got[2]), (Y, *ref)):
+        assert rel_err(a, r) < TOL[torch.float32]
