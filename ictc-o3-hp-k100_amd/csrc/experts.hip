@@ -21,8 +21,10 @@
 
 namespace {
 
-// Tiles of 64 x 64 outputs by four waves of 32 x 32, or of 128 x 128 (the weights' gradient in 16 bits).
-template <typename T, int TILE>
+// Rows of under 16 bytes: tiles of 64 x 64 outputs by four waves of 32 x 32.
+constexpr int TILE = 64;
+
+template <typename T>
 struct Config {
   static constexpr int NP = sizeof(T) == 4 ? 3 : 1;                     // parts of an operand in LDS
   static constexpr int BK = 64;                                         // reduction indices of a step
@@ -81,9 +83,9 @@ __device__ __forceinline__ Few<T, NC> load_few(const T* __restrict__ p, int n) {
 // 16-bit offset of chunk `ch` of row `row` in a part of an operand
 __device__ __forceinline__ int lds_at(int row, int ch) { return (row * 8 + (ch ^ ((row ^ (row >> 3)) & 7))) * 8; }
 
-template <typename T, int TILE>
+template <typename T>
 __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch, const Eight<T>& v) {
-  using C = Config<T, TILE>;
+  using C = Config<T>;
   uint16_t* at = lds + lds_at(row, ch);
   if constexpr (sizeof(T) == 4) {
     const Split s = split8_pairs(v.e);
@@ -95,30 +97,30 @@ __device__ __forceinline__ void put(uint16_t* __restrict__ lds, int row, int ch,
   }
 }
 
-template <typename T, int TILE>
+template <typename T>
 __device__ __forceinline__ void fragment(const uint16_t* __restrict__ lds, int row, int ch,
-                                         u32x4 (&f)[Config<T, TILE>::NP]) {
-  using C = Config<T, TILE>;
+                                         u32x4 (&f)[Config<T>::NP]) {
+  using C = Config<T>;
   const uint16_t* at = lds + lds_at(row, ch);
 #pragma unroll
   for (int p = 0; p < C::NP; ++p) f[p] = *reinterpret_cast<const u32x4*>(at + p * C::PART);
 }
 
 // acc[i][j] += the block's step: rows 16 (wa NI + i) of operand A by rows 16 (wb NI + j) of operand B.
-template <typename T, int TILE>
+template <typename T>
 __device__ __forceinline__ void step(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int wa, int wb,
-                                     v4f (&acc)[Config<T, TILE>::NI][Config<T, TILE>::NI]) {
-  using C = Config<T, TILE>;
+                                     v4f (&acc)[Config<T>::NI][Config<T>::NI]) {
+  using C = Config<T>;
   const int li = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int kk = 0; kk < C::BK / 32; ++kk) {
     u32x4 a[C::NI][C::NP];
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i) fragment<T, TILE>(A, 16 * (wa * C::NI + i) + li, 4 * kk + g, a[i]);
+    for (int i = 0; i < C::NI; ++i) fragment<T>(A, 16 * (wa * C::NI + i) + li, 4 * kk + g, a[i]);
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {
       u32x4 b[C::NP];
-      fragment<T, TILE>(B, 16 * (wb * C::NI + j) + li, 4 * kk + g, b);
+      fragment<T>(B, 16 * (wb * C::NI + j) + li, 4 * kk + g, b);
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) acc[i][j] = product<T>(a[i], b, acc[i][j]);
     }
@@ -126,9 +128,9 @@ __device__ __forceinline__ void step(const uint16_t* __restrict__ A, const uint1
 }
 
 // An operand whose rows run along the reduction index.
-template <typename T, int TILE>
+template <typename T>
 struct Straight {
-  using C = Config<T, TILE>;
+  using C = Config<T>;
   const T* row[C::PER];
   bool ok[C::PER];
   Eight<T> v[C::PER];
@@ -145,14 +147,14 @@ struct Straight {
   }
   __device__ __forceinline__ void store(uint16_t* lds) const {
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) put<T, TILE>(lds, row_of(i), chunk_of(i), v[i]);
+    for (int i = 0; i < C::PER; ++i) put<T>(lds, row_of(i), chunk_of(i), v[i]);
   }
 };
 
 // An operand whose memory runs along its rows: thread (kb, cg) takes reduction indices 8 kb .. and rows NC cg ...
-template <typename T, int TILE>
+template <typename T>
 struct Across {
-  static constexpr int NC = Config<T, TILE>::NC;
+  static constexpr int NC = Config<T>::NC;
   Few<T, NC> v[8];
 
   static __device__ __forceinline__ int column() { return (int)threadIdx.x % (TILE / NC) * NC; }
@@ -164,19 +166,19 @@ struct Across {
       Eight<T> e;
 #pragma unroll
       for (int j = 0; j < 8; ++j) e.e[j] = v[j].e[c];
-      put<T, TILE>(lds, column() + c, block(), e);
+      put<T>(lds, column() + c, block(), e);
     }
   }
 };
 
 // out[perm[r]] = M x[perm[r]] + b over the columns of a tile, M = W[e] [N, K] or, TRANS, the transpose of
 // W[e] [K, N].  Operand A is the weights, so a lane ends with four consecutive columns of one row.
-template <typename T, bool TRANS, int TILE>
+template <typename T, bool TRANS>
 __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__ x, int64_t ldx, int K,
                                                            const T* __restrict__ W, const T* __restrict__ bias, int N,
                                                            int experts, const int* __restrict__ perm,
                                                            const int* __restrict__ off, T* __restrict__ out) {
-  using C = Config<T, TILE>;
+  using C = Config<T>;
   __shared__ __attribute__((aligned(16))) uint16_t As[C::NP * C::PART];
   __shared__ __attribute__((aligned(16))) uint16_t Bs[C::NP * C::PART];
   const int columns = (N + TILE - 1) / TILE;
@@ -192,8 +194,8 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
   }
   const T* w = W + (int64_t)run.group * N * K;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-  Straight<T, TILE> xs, ws;
-  Across<T, TILE> wt;
+  Straight<T> xs, ws;
+  Across<T> wt;
 #pragma unroll
   for (int i = 0; i < C::PER; ++i) {
     const int r = xs.row_of(i);
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
       ws.store(As);
     __syncthreads();
     if (k0 + C::BK < K) load(k0 + C::BK);
-    step<T, TILE>(As, Bs, wave >> 1, wave & 1, acc);
+    step<T>(As, Bs, wave >> 1, wave & 1, acc);
     __syncthreads();
   }
   // all of the bias and row numbers are asked for before the first is needed
@@ -270,8 +272,9 @@ __global__ __launch_bounds__(256) void experts_rows_kernel(const T* __restrict__
 }
 
 // The same for few rows: a block takes 16 rows of an expert and 32 columns, its eight waves share the reduction, and
-// every lane reads its fragments' values from memory itself, so a call is one round of loads, not a chain of steps (1 row
-// of 1,024 -> 1,024 FP32: 7.8 us, 24 in tiles of 64).  The waves' sums are added in order.  Two blocks share a unit.
+// every lane reads its fragments' values from memory itself, so a call is one round of loads, not a chain of steps (16
+// rows of 1,024 -> 1,024 FP32 over eight experts: 8.9 us, 25 in tiles of 64).  The waves' sums are added in order.  Two
+// blocks share a unit.
 constexpr int kFewRows = 16, kFewColumns = 32, kFewWaves = 8;
 
 template <typename T>
@@ -468,9 +471,10 @@ int id_bits(int experts) {
   return bits;
 }
 
-// Rows of a block: all of few rows; 4,096; more once those would be more than 64 blocks; and zero: the general sort.  Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5, 16,384 12.9 / 9.0; 89 experts
-// 6,000 rows 8.2 / 8.7, 16,384 16.4 / 10.1.  Several / the general sort, ten experts: 30,011 rows
-// 8.8 / 10.8, 262,145 11.8 / 106, 4.2 million 32 / 83.
+// Rows of a block: all of few rows; 4,096; more once those would be more than 64 blocks; and zero: the general sort.
+// Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5, 16,384 12.9 / 9.0; 89 experts 6,000
+// rows 8.2 / 8.7, 16,384 16.4 / 10.1.  Several / the general sort, ten experts: 30,011 rows 8.8 / 10.8, 262,145 11.8 / 106,
+// 4.2 million 32 / 83.
 int order_span(int64_t rows, int experts) {
   if (experts > kOrderExperts || rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
   if (rows <= kOrderRows && rows * (3 + id_bits(experts)) <= 60000) return (int)std::max<int64_t>(rows, 1);
@@ -479,13 +483,13 @@ int order_span(int64_t rows, int experts) {
 
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
 // over one range of rows.
-template <typename T, int TILE>
+template <typename T>
 __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restrict__ gy, int64_t ldg, int M,
                                                             const T* __restrict__ x, int64_t ldx, int K, int experts,
                                                             int ranges, const int* __restrict__ perm,
                                                             const int* __restrict__ off, T* __restrict__ gW,
                                                             T* __restrict__ gb, float* __restrict__ part) {
-  using C = Config<T, TILE>;
+  using C = Config<T>;
   __shared__ __attribute__((aligned(16))) uint16_t As[C::NP * C::PART];
   __shared__ __attribute__((aligned(16))) uint16_t Bs[C::NP * C::PART];
   const int ct = (K + TILE - 1) / TILE, tiles = ct * ((M + TILE - 1) / TILE);
@@ -500,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
     if (off[e + 1] == off[e]) zero_tile<T, TILE, 256>(gW + e * MK, gb ? gb + (int64_t)e * M : nullptr, M, K, m0, k0);
   if (q >= ranges) return;
   const Ranges r = find_ranges(off, experts, C::BK, ranges);
-  Across<T, TILE> xs, gs;
+  Across<T> xs, gs;
   const int cx = k0 + xs.column(), cg = m0 + gs.column(), r0 = 8 * xs.block();
   Segment s;
   for (int u = q * r.per; find_segment(off, experts, C::BK, r, q, u, s); u += s.steps) {
@@ -542,14 +546,14 @@ __global__ __launch_bounds__(256, 2) void experts_outer_kernel(const T* __restri
         load();
         name(row + 2 * C::BK);
       }
-      step<T, TILE>(As, Bs, wave >> 1, wave & 1, acc);
+      step<T>(As, Bs, wave >> 1, wave & 1, acc);
       if (bias) {
 #pragma unroll
         for (int kk = 0; kk < C::BK / 32; ++kk)
 #pragma unroll
           for (int j = 0; j < C::NI; ++j) {
             u32x4 f[C::NP];
-            fragment<T, TILE>(Bs, TILE / 2 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
+            fragment<T>(Bs, TILE / 2 * (wave & 1) + 16 * j + li, 4 * kk + g, f);
 #pragma unroll
             for (int p = C::NP - 1; p >= 0; --p) accb[j] = mma<T>(u32x4{one, one, one, one}, f[p], accb[j]);
           }
@@ -644,7 +648,7 @@ OuterPlan outer_plan(bool direct, int dtype, int64_t n, int M, int K, int expert
   p.tile = 128;
   int64_t tiles = tiles_of(M, 128) * tiles_of(K, 128);
   const int64_t blocks = dtype == ICTC_F32 || n * tiles >= 512 * 1024 || n < 1024 * (int64_t)experts ? 512 : 256;
-  if (dtype == ICTC_F32 && (!direct || n * tiles < 512 * 256)) {
+  if (!direct || (dtype == ICTC_F32 && n * tiles < 512 * 256)) {
     p.tile = 64;
     tiles = tiles_of(M, 64) * tiles_of(K, 64);
   }
@@ -677,10 +681,10 @@ void launch_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W,
                  const int* perm, const int* off, int transpose, void* out, hipStream_t st) {
   const dim3 grid((unsigned)(most_runs(rows, experts, 64) * tiles_of(N, 64)));
   if (transpose)
-    hipLaunchKernelGGL((experts_rows_kernel<T, true, 64>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+    hipLaunchKernelGGL((experts_rows_kernel<T, true>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<T, false, 64>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
+    hipLaunchKernelGGL((experts_rows_kernel<T, false>), grid, dim3(256), 0, st, (const T*)x, ldx, K, (const T*)W,
                        (const T*)bias, N, experts, perm, off, (T*)out);
 }
 
@@ -700,7 +704,7 @@ template <typename T>
 void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
                   int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles_of(M, plan.tile) * tiles_of(K, plan.tile)));
-  hipLaunchKernelGGL((experts_outer_kernel<T, (sizeof(T) == 4 ? 64 : 128)>), grid, dim3(256), 0, st, (const T*)gy, ldg, M,
+  hipLaunchKernelGGL(experts_outer_kernel<T>, grid, dim3(256), 0, st, (const T*)gy, ldg, M,
                      (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
 }
 
@@ -794,7 +798,8 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
   const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, outputs, inputs),
                                     dtype, rows, outputs, inputs, experts);
   if (outer_bytes(plan, outputs, inputs) > 0 &&
-      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+       workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
     return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: workspace smaller than ictc_expert_outer_workspace_bytes");
   hipStream_t st = (hipStream_t)stream;
   float* part = (float*)workspace;
