@@ -322,3 +322,20 @@ def test_offsets_past_32_bits(device, dtype, K, M):
     Y = _formula(*few, None, ids[ends])
     _check((y[ends], gx[ends], gW), (Y, *torch.autograd.grad(Y, few, gy[ends].double())), ("y", "gx", "gW"))
     assert gx[200:400].abs().max() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,K,M", [(40, 300, 64), (1000, 128, 72), (1000, 65, 33), (900, 5, 7)])
+def test_non_finite_rows_stay_alone(device, rows, K, M, dtype):
+    """Infinities and NaN in some rows change neither other rows' results nor other experts' gradients."""
+    ids, x, W, b, gy = _inputs(rows, 4, K, M, dtype, 21, device)
+    bad = x.clone()
+    bad[5, K // 2], bad[9, 0], bad[rows // 2], bad[rows - 1] = float("inf"), float("-inf"), float("nan"), float("nan")
+    ids[5], ids[9], ids[rows // 2] = 0, 0, 0
+    _, y0, clean = _run(ids, x, W, b, gy)
+    _, y1, got = _run(ids, bad, W, b, gy)
+    others = torch.ones(rows, dtype=torch.bool, device=device)
+    others[[5, 9, rows // 2]] = False          # (the last row belongs to no expert)
+    assert torch.equal(y1[others], y0[others]) and not torch.isfinite(y1[~others]).all(1).any()
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+    assert torch.equal(got[1][1:], clean[1][1:]) and not torch.isfinite(got[1][0]).all()
