@@ -69,6 +69,14 @@ Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.option
 
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+// Whether an operator's call has to leave a node behind.  Without (inference) it goes past autograd, and layer norm writes
+// no statistics: order and expert linear of 5 rows 10.7 -> 8.9 us, layer norm of one 5.5 -> 3.8.
+bool tracked(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
+  return false;
+}
+
 // Which of a node's inputs the running backward pass asks for; inputs without a variable have no edge.
 std::vector<bool> wanted(AutogradContext* ctx, std::initializer_list<bool> present) {
   std::vector<bool> out;
@@ -193,19 +201,24 @@ struct LayerNormGrad : Function<LayerNormGrad> {
   }
 };
 
+// stats: the rows' mean and 1 / deviation, or undefined
+Tensor norm_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, const Tensor& stats) {
+  const Tensor x = rows_of(x_), w = packed(w_), b = packed(b_);
+  const int64_t N = x.size(0), C = x.size(1);
+  Tensor y = at::empty({N, C}, x.options());
+  float* st = stats.defined() ? stats.mutable_data_ptr<float>() : nullptr;
+  done(ictc_layer_norm_fwd(dtype_of(x), ptr(x), pitch(x), N, (int)C, ptr(w), ptr(b), (float)eps, ptr(y), st,
+                           st ? st + N : nullptr, stream_of(x)),
+       "layer_norm");
+  return y;
+}
+
 struct LayerNorm : Function<LayerNorm> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps) {
-    const Tensor x = rows_of(x_), w = packed(value(w_)), b = packed(value(b_));
-    const int64_t N = x.size(0), C = x.size(1);
-    Tensor y = at::empty({N, C}, x.options());
-    const Tensor stats = floats(2 * N, x);   // the rows' mean and 1 / deviation
-    float* st = stats.mutable_data_ptr<float>();
-    done(ictc_layer_norm_fwd(dtype_of(x), ptr(x), pitch(x), N, (int)C, ptr(w), ptr(b), (float)eps, ptr(y), st, st + N,
-                             stream_of(x)),
-         "layer_norm");
-    ctx->save_for_backward({x_, value(w_), stats});
-    ctx->saved_data["bias"] = b.defined();
-    return y;
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+    const Tensor stats = floats(2 * x.size(0), x);
+    ctx->save_for_backward({x, value(w), stats});
+    ctx->saved_data["bias"] = b.has_value();
+    return norm_forward(x, value(w), value(b), eps, stats);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
@@ -241,8 +254,10 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
   }
   TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "layer_norm: eps must be a finite number, zero or more");
   const c10::DeviceGuard guard(x.device());
-  if (x.dim() == 2) return LayerNorm::apply(x, w, b, eps);
-  return LayerNorm::apply(x.reshape({x.numel() / C, C}), w, b, eps).view(x.sizes());
+  const Tensor rows = x.dim() == 2 ? x : x.reshape({x.numel() / C, C}), wv = value(w), bv = value(b);
+  const Tensor y = tracked({&rows, &wv, &bv}) ? LayerNorm::apply(rows, w, b, eps)
+                                              : norm_forward(rows, wv, bv, eps, Tensor());
+  return x.dim() == 2 ? y : y.view(x.sizes());
 }
 
 // ---------------------------------------------------------------------------
@@ -375,7 +390,9 @@ Tensor expert_linear(const Tensor& x, const Tensor& W, const OptTensor& b, const
                       "expert_linear: bias must have shape [experts, outputs]");
   }
   const c10::DeviceGuard guard(x.device());
-  return ExpertLinear::apply(x, W, b, perm, off, false);
+  const Tensor bv = value(b);
+  return tracked({&x, &W, &bv}) ? ExpertLinear::apply(x, W, b, perm, off, false)
+                                : linear_rows(x, W, bv, perm, off, false);
 }
 
 // ---------------------------------------------------------------------------

@@ -339,3 +339,16 @@ def test_non_finite_rows_stay_alone(device, rows, K, M, dtype):
     assert torch.equal(y1[others], y0[others]) and not torch.isfinite(y1[~others]).all(1).any()
     assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
     assert torch.equal(got[1][1:], clean[1][1:]) and not torch.isfinite(got[1][0]).all()
+
+
+def test_the_same_without_a_graph(device):
+    from ictc_o3 import expert_linear, expert_order
+    ids, x, W, b, _ = _inputs(60, 3, 40, 24, torch.float32, 6, device)
+    order = expert_order(ids, 3)
+    plain, kept = expert_linear(x, W, order, b), expert_linear(x, W, order, b.clone().requires_grad_())
+    with torch.no_grad():
+        off = expert_linear(x.clone().requires_grad_(), W, order, b)
+    with torch.inference_mode():
+        inference = expert_linear(x, W, expert_order(ids, 3), b)
+    assert kept.requires_grad and not plain.requires_grad and not off.requires_grad
+    assert all(torch.equal(t, kept) for t in (plain, off, inference))

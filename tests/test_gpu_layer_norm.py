@@ -246,3 +246,17 @@ def test_offsets_past_32_bits(device):
     ref = torch.autograd.grad(Y, few, gy[ends].double())
     for a, r in zip((y[ends], got[0][ends], got[1], got[2]), (Y, *ref)):
         assert rel_err(a, r) < TOL[torch.float32]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_same_without_a_graph(device, dtype):
+    from ictc_o3 import layer_norm
+    x, w, b, _, _ = _inputs(77, 130, dtype, 5, device)
+    plain = layer_norm(x, w, b)
+    kept = layer_norm(x, w.clone().requires_grad_(), b)
+    with torch.no_grad():
+        off = layer_norm(x.clone().requires_grad_(), w, b)
+    with torch.inference_mode():
+        inference = layer_norm(x, w, b)
+    assert kept.requires_grad and not plain.requires_grad and not off.requires_grad
+    assert all(torch.equal(t, kept) for t in (plain, off, inference))
