@@ -12,14 +12,15 @@
 // than the 6 bytes that split values would take in LDS (30,000 rows of 256 -> 256, split on their way there: rows 43
 // against 38 us, weights' gradient 77 against 59).
 //
-// Tiles of 128 x 128 by four waves of 64 x 64.  For the rows' products in 16 bits a step has 32 reduction indices, so
-// that four blocks share a compute unit and one's first loads and last stores run under another's products: at 131,072
-// rows of 512 -> 1,024 bfloat16 this measured 216 us and its adjoint 168 us (1,024 -> 512), against 204 / 188 us with 256
-// x 256 tiles (one block of eight waves, steps of 64), which lose a factor of two at 128 -> 128 (41 against 17 us).  For
-// the weights' gradient a step has 64 rows and two blocks share a unit.
+// Tiles of 128 x 128 by four waves of 64 x 64, or of 256 columns by eight.  For the rows' products in 16 bits a step has 32
+// reduction indices, so that sixteen waves share a compute unit and one block's first loads and last stores run under
+// another's products: at 131,072 rows of 512 -> 1,024 bfloat16 in tiles of 128 x 128 this measured 211 us and its adjoint
+// 182 us (1,024 -> 512).  256 x 256 tiles, one block of eight waves and steps of 64, took 204 / 188 us there and lost a
+// factor of two at 128 -> 128 (41 against 17 us).  For the weights' gradient a step has 64 rows and two blocks share a
+// unit.
 //
-// At 131,072 rows of 512 -> 512 over ten experts, rows / adjoint / weights' gradient in us: bfloat16 103 / 100 / 123 (667,
-// 687 and 559 TFLOP/s), FP32 520 / 520 / 485 (132 to 142 TFLOP/s, six times that on the matrix cores), bound by the
+// At 131,072 rows of 512 -> 512 over ten experts, rows / adjoint / weights' gradient in us: bfloat16 97 / 99 / 118 (709,
+// 694 and 582 TFLOP/s), FP32 520 / 520 / 485 (132 to 142 TFLOP/s, six times that on the matrix cores), bound by the
 // matrix cores' rate at the clock that they leave; 511 -> 511 FP16, through registers, 149 / 177 / 185.
 #include <algorithm>
 #include <type_traits>
@@ -361,30 +362,40 @@ __global__ __launch_bounds__(GA * GB * 64, sizeof(T) == 2 && S == 32 ? 4 : 2) vo
   }
 }
 
-template <typename T, bool ALIGNED, bool TRANS, int TILE, int S>
+template <typename T, bool ALIGNED, bool TRANS, int TA, int TB, int S>
 void launch_direct(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
                    const int* perm, const int* off, void* out, hipStream_t st) {
-  const int64_t blocks = most_runs(rows, experts, TILE) * ((N + TILE - 1) / TILE);
-  hipLaunchKernelGGL((experts_direct_kernel<T, ALIGNED, TRANS, TILE, TILE, S, 2, 2>), dim3((unsigned)blocks), dim3(256), 0,
-                     st, (const T*)x, ldx, K, (const T*)W, (const T*)bias, N, experts, perm, off, (T*)out);
+  constexpr int GA = TA == 256 ? 4 : 2;
+  const int64_t blocks = most_runs(rows, experts, TB) * ((N + TA - 1) / TA);
+  hipLaunchKernelGGL((experts_direct_kernel<T, ALIGNED, TRANS, TA, TB, S, GA, 2>), dim3((unsigned)blocks),
+                     dim3(GA * 128), 0, st, (const T*)x, ldx, K, (const T*)W, (const T*)bias, N, experts, perm, off,
+                     (T*)out);
 }
 
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, bool TRANS>
 void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W, const void* bias, int N, int experts,
-                 const int* perm, const int* off, bool transpose, void* out, hipStream_t st) {
+                 const int* perm, const int* off, void* out, hipStream_t st) {
   // Tiles of 64 x 64 where those of 128 x 128 are fewer than the card's units or half empty: 8,192 rows of 128 -> 128 4.4
-  // against 6.2 us, 131,072 of 64 -> 64 11 against 15; 16,384 of 256 -> 256 10.1 against 9.6.
+  // against 6.2 us, 131,072 of 64 -> 64 11 against 15; 16,384 of 256 -> 256 10.1 against 9.6.  (FP32: 30,000 of 256 -> 256
+  // 38 against 45, 16,384 of 512 -> 512 72 against 75, 8,192 of 1,024 -> 1,024 141 both.)
   constexpr int SMALL = sizeof(T) == 4 ? 32 : 64;
-  constexpr int BACK = sizeof(T) == 4 || ALIGNED ? 32 : 64;   // (four blocks a unit leave too few registers to load through)
-  const bool few = N <= 64 || experts_tiles(rows, N, experts) < (sizeof(T) == 4 ? 1024 : 256);
-  if (few && transpose)
-    launch_direct<T, ALIGNED, true, 64, SMALL>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
-  else if (few)
-    launch_direct<T, ALIGNED, false, 64, SMALL>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
-  else if (transpose)
-    launch_direct<T, ALIGNED, true, 128, BACK>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
-  else
-    launch_direct<T, ALIGNED, false, 128, 32>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+  // (transposed through registers: four blocks a unit leave too few for the loads)
+  constexpr int LARGE = sizeof(T) == 4 || ALIGNED || !TRANS ? 32 : 64;
+  const int64_t tiles = experts_tiles(rows, N, experts);
+  if (N <= 64 || tiles < (sizeof(T) == 4 ? 1024 : 256)) {
+    launch_direct<T, ALIGNED, TRANS, 64, 64, SMALL>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+    return;
+  }
+  // 16 bits, aligned: 256 columns by eight waves where those tiles are as full and there are many.  Both in us: 131,072 rows
+  // of 512 -> 1,024 211 / 204, of 512 -> 512 103 / 99, 60,000 of 512 -> 512 over 40 experts 50 / 45; the other way 131,072 of
+  // 256 -> 256 37 / 39, of 128 -> 512 39 / 41, 20,000 of 512 -> 1,024 35 / 37.
+  if constexpr (sizeof(T) == 2 && ALIGNED) {
+    if (N > 256 && K >= 256 && (N + 127) / 128 % 2 == 0 && tiles >= 1536) {
+      launch_direct<T, ALIGNED, TRANS, 256, 128, 32>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
+      return;
+    }
+  }
+  launch_direct<T, ALIGNED, TRANS, 128, 128, LARGE>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
 }
 
 // Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
@@ -541,14 +552,22 @@ void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, con
 
 bool whole16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <bool ALIGNED, typename... A>
+template <bool ALIGNED, bool TRANS, typename... A>
 void typed_rows(int dtype, A... a) {
   if (dtype == ICTC_F32)
-    direct_rows<float, ALIGNED>(a...);
+    direct_rows<float, ALIGNED, TRANS>(a...);
   else if (dtype == ICTC_BF16)
-    direct_rows<bf16, ALIGNED>(a...);
+    direct_rows<bf16, ALIGNED, TRANS>(a...);
   else
-    direct_rows<f16, ALIGNED>(a...);
+    direct_rows<f16, ALIGNED, TRANS>(a...);
+}
+
+template <bool ALIGNED, typename... A>
+void either_rows(int dtype, bool transpose, A... a) {
+  if (transpose)
+    typed_rows<ALIGNED, true>(dtype, a...);
+  else
+    typed_rows<ALIGNED, false>(dtype, a...);
 }
 
 template <bool ALIGNED, typename... A>
@@ -575,9 +594,9 @@ void experts_direct_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
   // 16-byte chunks of x, and of the weights along their memory, whole and aligned
   const int v = chunk_of(dtype);
   if (whole16(x) && ldx % v == 0 && K % v == 0 && whole16(W) && (!transpose || N % v == 0))
-    typed_rows<true>(dtype, x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+    either_rows<true>(dtype, transpose, x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
   else
-    typed_rows<false>(dtype, x, ldx, rows, K, W, bias, N, experts, perm, off, transpose, out, st);
+    either_rows<false>(dtype, transpose, x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
 }
 
 bool experts_direct_outer_fits(int dtype, int M, int K) { return M >= chunk_of(dtype) && K >= chunk_of(dtype); }

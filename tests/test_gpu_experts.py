@@ -341,6 +341,16 @@ def test_non_finite_rows_stay_alone(device, rows, K, M, dtype):
     assert torch.equal(got[1][1:], clean[1][1:]) and not torch.isfinite(got[1][0]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("K,M", [(264, 504), (504, 264), (256, 1000)])
+def test_many_rows_and_columns(device, dtype, K, M):
+    """Rows and columns enough for the largest tiles, straight and transposed, the last ones part full."""
+    data = _inputs(50021, 3, K, M, dtype, K, device)
+    _, y, got = _run(*data)
+    _, Y, ref = _reference(*data)
+    _check((y, *got), (Y, *ref), ("y", "gx", "gW", "gb"))
+
+
 def test_the_same_without_a_graph(device):
     from ictc_o3 import expert_linear, expert_order
     ids, x, W, b, _ = _inputs(60, 3, 40, 24, torch.float32, 6, device)
