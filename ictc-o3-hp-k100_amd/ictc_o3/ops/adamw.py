@@ -52,7 +52,7 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits 32 or 8 chooses the type of the moments.  max_norm bounds the 2-norm over the gradients of all groups;
     the norm before the bound is left in ``grad_norm`` (a device scalar).  A parameter without a gradient is skipped:
-    its moments and its count of steps stay as they are."""
+    its moments and its count of steps stay as they are.  A group's list of parameters may change between steps."""
 
     _MOMENTS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
@@ -76,10 +76,14 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm, self._flat = None, {}   # (a copy gathers its moments anew from its per-parameter state)
 
     def _moments(self, index):
-        """The flat moments of a group, whose segments are its parameters' state; made at the first step."""
-        if index not in self._flat:
-            group = self.param_groups[index]
-            ps, eight = group["params"], group["state_bits"] == 8
+        """The flat moments of a group, whose segments are its parameters' state.  Made at the first step, and anew from
+        that state whenever the group's parameters (which ones, their order, size and device) or its type of moments
+        are no longer those that they were made for."""
+        group = self.param_groups[index]
+        ps, eight = group["params"], group["state_bits"] == 8
+        made_for = (eight, ps[0].device, [(id(p), p.numel()) for p in ps])   # (kept parameters keep their ids)
+        if index not in self._flat or self._flat[index][2] != made_for:
+            self._flat.pop(index, None)   # (a fault below leaves the state as the only source)
             starts, total = adamw_segments([p.numel() for p in ps])
             device = ps[0].device
             if eight:
@@ -102,8 +106,8 @@ class AdamW(torch.optim.Optimizer):
                         raw = segment.view(torch.uint8) if segment.element_size() == 1 else segment
                         raw.copy_(state[name].view(raw.dtype))
                     state[name] = segment
-            self._flat[index] = (flat, starts)
-        return self._flat[index]
+            self._flat[index] = (flat, starts, made_for, list(ps))
+        return self._flat[index][:2]
 
     def load_state_dict(self, state_dict):
         """torch.optim's, but the moments keep their type whatever the parameters' is."""

@@ -395,3 +395,37 @@ def test_refusals(device):
             adamw_step(**args)
     assert torch.equal(p, torch.ones_like(p))
     assert adamw_step([], [], m, v, step=1) is None
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_join_leave_and_move(device, bits):
+    """A group's list of parameters may change between steps: each keeps its own moments and count of steps, as with
+    torch.optim.AdamW.  (8 bits against a run in which every parameter has an optimizer of its own.)"""
+    from ictc_o3 import AdamW
+    ps, rs = _pair(device, [(300,), (5,), (300,), (20, 30)])
+    hyper = dict(lr=1e-2, weight_decay=0.05)
+    opt = AdamW(ps[:3], state_bits=bits, **hyper)
+    if bits == 32:
+        refs = [torch.optim.AdamW([r], eps=1e-8, **hyper) for r in rs]
+    else:
+        rs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+        refs = [AdamW([r], state_bits=bits, **hyper) for r in rs]
+    gen = torch.Generator().manual_seed(2)
+    group = opt.param_groups[0]
+    for members in ([0, 1, 2], [0, 1, 2, 3], [1, 2, 3], [3, 2, 1], [2], [0, 2, 1, 3]):
+        group["params"][:] = [ps[i] for i in members]
+        for _ in range(2):
+            for p in ps:
+                p.grad = None
+            for i in members:
+                grad = torch.randn(rs[i].shape, generator=gen)
+                ps[i].grad, rs[i].grad = grad.to(device), grad.to(rs[i])
+            opt.step()
+            for i in members:
+                refs[i].step()
+        for p, r in zip(ps, rs):
+            assert torch.equal(p, r) if bits == 8 else rel_err(p, r) < 12e-6
+        if bits == 32:
+            for i in members:
+                m = opt.state[ps[i]]["exp_avg"][:ps[i].numel()]
+                assert rel_err(m, refs[i].state[rs[i]]["exp_avg"].flatten()) < 12e-6
