@@ -245,17 +245,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table t, Hyper h, void* __re
   }
 }
 
-// out[0] = the norm, out[1] = the factor that holds it to `bound`.  NaN stays NaN.
+// out[0] = the norm, out[1] = the factor that holds it to `bound`, from the norm in FP64: one past FP32 still has one.
+// NaN stays NaN.
 __device__ __forceinline__ void write_norm(double squares, float bound, float* __restrict__ out) {
-  const float norm = (float)sqrt(squares);
-  const float f = bound / (norm + 1e-6f);
-  out[0] = norm;
-  out[1] = f >= 1.f ? 1.f : f;
+  const double norm = sqrt(squares), f = (double)bound / (norm + 1e-6);
+  out[0] = (float)norm;
+  out[1] = f >= 1.0 ? 1.f : (float)f;
 }
 
 // part[block] = sum of squares of the gradients of this launch's runs blockIdx, blockIdx + gridDim, ...: FP32 over the
-// eight elements of a thread's run, FP64 above.  Four runs are asked for before the first is added.  `out`: there is one
-// block, which writes the norm and the factor too.
+// eight elements of a thread's run, FP64 above; and FP64 at once where the eight's sum is not well inside FP32's range
+// (past it, or under 2^-100, to which squares below FP32's smallest still belong: any finite gradients have a norm).  Four
+// runs are asked for before the first is added.  `out`: there is one block, which writes the norm and the factor too.
 template <typename T>
 __global__ __launch_bounds__(256) void grad_norm_kernel(Table t, double* __restrict__ part, float bound,
                                                         float* __restrict__ out) {
@@ -295,7 +296,20 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(Table t, double* __restr
 #pragma unroll
         for (int i = 0; i < V; ++i) s += v[i] * v[i];
       }
-      sum += (double)s;
+      double d = (double)s;
+      if (sizeof(T) == 4 || __is_same(T, bf16)) {   // (FP16's squares are all in the range)
+        if (!(s >= 0x1p-100f && s < bits_float(kInf))) {
+          d = 0.0;
+#pragma unroll
+          for (int j = 0; j < L; ++j) {
+            float v[V];
+            widen<T>(raw[a][j], v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) d += (double)v[i] * (double)v[i];
+          }
+        }
+      }
+      sum += d;
     }
   }
 #pragma unroll

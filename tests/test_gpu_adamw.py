@@ -429,3 +429,47 @@ def test_parameters_that_join_leave_and_move(device, bits):
             for i in members:
                 m = opt.state[ps[i]]["exp_avg"][:ps[i].numel()]
                 assert rel_err(m, refs[i].state[rs[i]]["exp_avg"].flatten()) < 12e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e25, 1e19, 1e-19, 1e-25, 1e-36])
+@pytest.mark.parametrize("counts", [[700], [3000, 5, 20000, 9000]])
+def test_norms_whose_squares_leave_the_range(device, dtype, size, counts):
+    from ictc_o3 import adamw_segments, adamw_step
+    ps, gs = _lists(counts, dtype, 3, device)
+    for k, g in enumerate(gs):
+        g.mul_(size)
+        if k == 1:
+            g.mul_(1e-3)
+    starts, total = adamw_segments(counts)
+    m, v = torch.zeros(total, device=device), torch.zeros(total, device=device)
+    old = [[t.double() for t in ts] for ts in (ps, gs, _segments(m, starts, counts), _segments(v, starts, counts))]
+    norm = adamw_step(ps, gs, m, v, step=1, max_norm=0.5, **HYPER)
+    (P, _, _), N = _formula(*old, 1, 0.5, **HYPER)
+    assert abs(float(norm) - float(N)) < 1e-6 * float(N)
+    assert rel_err(torch.cat(ps), torch.cat(P)) < TOL[dtype]
+
+
+def test_a_norm_beyond_the_type_still_scales(device):
+    """Every gradient is finite and their norm is past FP32: it is reported as infinite, and the step is the bound's.
+    The factor, 2e-41, has 14 bits, and the first step hardly depends on it; the bound is 1e-4."""
+    from ictc_o3 import adamw_step
+    g = 3e38 * torch.sign(torch.randn(16384, generator=torch.Generator().manual_seed(0))).to(device)
+    p, m, v = torch.zeros(16384, device=device), torch.zeros(16384, device=device), torch.zeros(16384, device=device)
+    norm = adamw_step([p], [g], m, v, step=1, max_norm=1.0, **HYPER)
+    assert torch.isinf(norm)
+    assert rel_err(p, -HYPER["lr"] * torch.sign(g).double()) < 1e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_norm_of_several_large_tensors(device, dtype):
+    from ictc_o3 import adamw_step
+    counts = [3000001, 2500000, 7, 4100003, 300, 6000000, 2048, 5000011]
+    gen = torch.Generator(device).manual_seed(1)
+    gs = [(torch.randn(n, device=device, generator=gen) * (1 + i)).to(dtype) for i, n in enumerate(counts)]
+    ps = [torch.zeros_like(g) for g in gs]
+    total = sum(-(-n // 256) * 256 for n in counts)
+    m, v = torch.zeros(total, device=device), torch.zeros(total, device=device)
+    norm = adamw_step(ps, gs, m, v, step=1, max_norm=1.0, **HYPER)
+    ref = sum(g.double().square().sum() for g in gs).sqrt()
+    assert abs(float(norm) - float(ref)) < 1e-6 * float(ref)
