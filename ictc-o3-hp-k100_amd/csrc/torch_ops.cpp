@@ -463,7 +463,12 @@ void adamw_update(const std::vector<Tensor>& params, const std::vector<Tensor>& 
   check_moments(m, v, ms, vs);
   TORCH_CHECK_VALUE(params.size() == grads.size(), "adamw: as many gradients as parameters are needed");
   TORCH_CHECK_VALUE(starts.empty() || starts.size() == params.size(), "adamw: a segment per parameter is needed");
-  if (params.empty()) return;
+  if (params.empty()) {   // the call's other arguments are checked all the same
+    done(ictc_adamw_step(ICTC_F32, 32, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, lr,
+                         beta1, beta2, eps, decay, step, nullptr, nullptr),
+         "adamw");
+    return;
+  }
   const c10::DeviceGuard guard(m.device());
   const List p = list_of(params, m, "parameters"), g = list_of(grads, m, "gradients");
   TORCH_CHECK_VALUE(p.dtype == g.dtype, "adamw: gradients must have the type of their parameters");
@@ -488,8 +493,7 @@ OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor
   OptTensor norm;
   if (max_norm.has_value()) {
     TORCH_CHECK_VALUE(*max_norm >= 0.0, "adamw: max_norm must be zero or more");
-    if (grads.empty()) return at::zeros({}, m.options().dtype(at::kFloat));
-    norm = gradient_norm(grads, *max_norm);
+    norm = grads.empty() ? at::zeros({1}, m.options().dtype(at::kFloat)) : gradient_norm(grads, *max_norm);
   }
   adamw_update(params, grads, m, v, ms, vs, {}, step, lr, beta1, beta2, eps, decay, norm);
   return norm.has_value() ? OptTensor(norm->select(0, 0)) : OptTensor();

@@ -473,3 +473,15 @@ def test_norm_of_several_large_tensors(device, dtype):
     norm = adamw_step(ps, gs, m, v, step=1, max_norm=1.0, **HYPER)
     ref = sum(g.double().square().sum() for g in gs).sqrt()
     assert abs(float(norm) - float(ref)) < 1e-6 * float(ref)
+
+
+def test_a_bound_does_not_let_a_bad_call_pass(device):
+    from ictc_o3 import adamw_step
+    p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+    m, v = torch.zeros(512, device=device), torch.zeros(512, device=device)
+    for bad in (dict(params=[p]), dict(step=0), dict(betas=(1.0, 0.9)), dict(lr=float("nan"))):
+        for bound in (None, 1.0):
+            with pytest.raises(ValueError):
+                adamw_step(**{**dict(params=[], grads=[], exp_avg=m, exp_avg_sq=v, step=1, max_norm=bound), **bad})
+    norm = adamw_step([], [], m, v, step=1, max_norm=1.0)
+    assert norm.shape == () and float(norm) == 0
