@@ -11,6 +11,7 @@
 #include <limits>
 #include <optional>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "../../include/ictc_mi355x.h"
@@ -443,60 +444,99 @@ List list_of(const std::vector<Tensor>& ts, const Tensor& like, const char* name
 }
 
 // [0] the norm over the gradients, [1] the factor that holds it to max_norm (ictc_gradient_norm's workspace).
-Tensor gradient_norm(const std::vector<Tensor>& grads, double max_norm) {
-  TORCH_CHECK_VALUE(max_norm >= 0.0, "adamw: max_norm must be zero or more");
-  TORCH_CHECK_VALUE(!grads.empty() && grads[0].is_cuda(), "adamw: tensors must be on a ROCm (cuda) device");
-  const c10::DeviceGuard guard(grads[0].device());
-  const List l = list_of(grads, grads[0], "gradients");
-  const int64_t bytes = ictc_gradient_norm_workspace_bytes((int)grads.size());
-  const Tensor ws = floats(bytes / 4, grads[0]);
-  done(ictc_gradient_norm(l.dtype, (int)grads.size(), l.at.data(), l.count.data(), max_norm, ptr(ws), bytes,
-                          stream_of(ws)),
+Tensor gradient_norm(const List& grads, double max_norm, const Tensor& like) {
+  const int64_t bytes = ictc_gradient_norm_workspace_bytes((int)grads.at.size());
+  const Tensor ws = floats(bytes / 4, like);
+  done(ictc_gradient_norm(grads.dtype, (int)grads.at.size(), grads.at.data(), grads.count.data(), max_norm, ptr(ws),
+                          bytes, stream_of(ws)),
        "adamw");
   return ws;
 }
 
-void adamw_update(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const Tensor& m,
-                  const Tensor& v, const OptTensor& ms, const OptTensor& vs, const std::vector<int64_t>& starts,
-                  int64_t step, double lr, double beta1, double beta2, double eps, double decay,
-                  const OptTensor& norm) {
-  check_moments(m, v, ms, vs);
-  TORCH_CHECK_VALUE(params.size() == grads.size(), "adamw: as many gradients as parameters are needed");
-  TORCH_CHECK_VALUE(starts.empty() || starts.size() == params.size(), "adamw: a segment per parameter is needed");
-  if (params.empty()) {   // the call's other arguments are checked all the same
-    done(ictc_adamw_step(ICTC_F32, 32, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, lr,
-                         beta1, beta2, eps, decay, step, nullptr, nullptr),
-         "adamw");
-    return;
-  }
-  const c10::DeviceGuard guard(m.device());
-  const List p = list_of(params, m, "parameters"), g = list_of(grads, m, "gradients");
-  TORCH_CHECK_VALUE(p.dtype == g.dtype, "adamw: gradients must have the type of their parameters");
-  TORCH_CHECK_VALUE(p.count == g.count, "adamw: a gradient must have its parameter's shape");
-  done(ictc_adamw_step(p.dtype, ms.has_value() ? 8 : 32, (int)params.size(), p.at.data(), g.at.data(), p.count.data(),
-                       starts.empty() ? nullptr : starts.data(), ptr(m), ptr(v), (float*)ptr(value(ms)),
-                       (float*)ptr(value(vs)), m.numel(), lr, beta1, beta2, eps, decay, step,
-                       (const float*)ptr(value(norm)), stream_of(m)),
+// One step of a list of parameters, whose moments begin at `starts` (empty: one behind another); the caller's lists.
+struct Step {
+  const std::vector<Tensor>&params, &grads;
+  const Tensor &m, &v;
+  const OptTensor &ms, &vs;
+  const std::vector<int64_t>& starts;
+  int64_t step;
+  double lr, beta1, beta2, eps, decay;
+};
+
+struct Lists {
+  List p, g;
+};
+
+// Everything that can be wrong with a step, found before anything of it is done.
+Lists check_step(const Step& s) {
+  check_moments(s.m, s.v, s.ms, s.vs);
+  TORCH_CHECK_VALUE(s.params.size() == s.grads.size(), "adamw: as many gradients as parameters are needed");
+  TORCH_CHECK_VALUE(s.starts.empty() || s.starts.size() == s.params.size(), "adamw: a segment per parameter is needed");
+  const Lists l = {list_of(s.params, s.m, "parameters"), list_of(s.grads, s.m, "gradients")};
+  TORCH_CHECK_VALUE(l.p.dtype == l.g.dtype, "adamw: gradients must have the type of their parameters");
+  TORCH_CHECK_VALUE(l.p.count == l.g.count, "adamw: a gradient must have its parameter's shape");
+  done(ictc_adamw_step(ICTC_F32, 32, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, s.lr,
+                       s.beta1, s.beta2, s.eps, s.decay, s.step, nullptr, nullptr),   // (of no tensors: the numbers)
+       "adamw");
+  return l;
+}
+
+void launch_step(const Step& s, const Lists& l, const OptTensor& norm) {
+  if (s.params.empty()) return;
+  const c10::DeviceGuard guard(s.m.device());
+  done(ictc_adamw_step(l.p.dtype, s.ms.has_value() ? 8 : 32, (int)s.params.size(), l.p.at.data(), l.g.at.data(),
+                       l.p.count.data(), s.starts.empty() ? nullptr : s.starts.data(), ptr(s.m), ptr(s.v),
+                       (float*)ptr(value(s.ms)), (float*)ptr(value(s.vs)), s.m.numel(), s.lr, s.beta1, s.beta2, s.eps,
+                       s.decay, s.step, (const float*)ptr(value(norm)), stream_of(s.m)),
        "adamw");
   // what was read of these tensors before (a graph's saved inputs, copies of a weight) is out of date
   const auto changed = [](const Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   };
-  for (const Tensor& t : params) changed(t);
-  for (const Tensor& t : {m, v, value(ms), value(vs)}) changed(t);
+  for (const Tensor& t : s.params) changed(t);
+  for (const Tensor& t : {s.m, s.v, value(s.ms), value(s.vs)}) changed(t);
+}
+
+// All steps with their gradients' common norm held to max_norm, which is returned; all are checked before the first is
+// taken.
+OptTensor take_steps(const std::vector<Step>& steps, const std::optional<double>& max_norm) {
+  TORCH_CHECK_VALUE(!max_norm.has_value() || *max_norm >= 0.0, "adamw: max_norm must be zero or more");
+  std::vector<Lists> lists;
+  List grads;
+  for (const Step& s : steps) {
+    lists.push_back(check_step(s));
+    const List& g = lists.back().g;
+    if (!max_norm.has_value() || g.at.empty()) continue;
+    if (grads.dtype < 0) grads.dtype = g.dtype;
+    TORCH_CHECK_VALUE(g.dtype == grads.dtype && s.m.device() == steps[0].m.device(),
+                      "adamw: gradients of one norm must be of one type and on one device");
+    grads.at.insert(grads.at.end(), g.at.begin(), g.at.end());
+    grads.count.insert(grads.count.end(), g.count.begin(), g.count.end());
+  }
+  OptTensor norm;
+  if (max_norm.has_value() && !steps.empty()) {
+    const c10::DeviceGuard guard(steps[0].m.device());
+    norm = grads.at.empty() ? at::zeros({1}, steps[0].m.options().dtype(at::kFloat))
+                            : gradient_norm(grads, *max_norm, steps[0].m);
+  }
+  for (size_t i = 0; i < steps.size(); ++i) launch_step(steps[i], lists[i], norm);
+  return norm.has_value() ? OptTensor(norm->select(0, 0)) : OptTensor();
 }
 
 OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const Tensor& m,
                      const Tensor& v, const OptTensor& ms, const OptTensor& vs, int64_t step, double lr, double beta1,
                      double beta2, double eps, double decay, const std::optional<double>& max_norm) {
-  check_moments(m, v, ms, vs);
-  OptTensor norm;
-  if (max_norm.has_value()) {
-    TORCH_CHECK_VALUE(*max_norm >= 0.0, "adamw: max_norm must be zero or more");
-    norm = grads.empty() ? at::zeros({1}, m.options().dtype(at::kFloat)) : gradient_norm(grads, *max_norm);
-  }
-  adamw_update(params, grads, m, v, ms, vs, {}, step, lr, beta1, beta2, eps, decay, norm);
-  return norm.has_value() ? OptTensor(norm->select(0, 0)) : OptTensor();
+  const std::vector<int64_t> packed_starts;
+  return take_steps({{params, grads, m, v, ms, vs, packed_starts, step, lr, beta1, beta2, eps, decay}}, max_norm);
+}
+
+using GroupStep = std::tuple<std::vector<Tensor>, std::vector<Tensor>, Tensor, Tensor, OptTensor, OptTensor,
+                             std::vector<int64_t>, int64_t, double, double, double, double, double>;
+
+OptTensor adamw_groups(const std::vector<GroupStep>& groups, const std::optional<double>& max_norm) {
+  std::vector<Step> steps;
+  for (const GroupStep& g : groups) steps.push_back(std::apply([](const auto&... part) -> Step { return {part...}; }, g));
+  return take_steps(steps, max_norm);
 }
 
 std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const Tensor& ms, const Tensor& vs,
@@ -521,8 +561,7 @@ PYBIND11_MODULE(ictc_torch, mod) {
   mod.def("layer_norm", &layer_norm, Free());
   mod.def("expert_order", &expert_order, Free());
   mod.def("expert_linear", &expert_linear, Free());
-  mod.def("gradient_norm", &gradient_norm, Free());
-  mod.def("adamw_update", &adamw_update, Free());
   mod.def("adamw_step", &adamw_step, Free());
+  mod.def("adamw_groups", &adamw_groups, Free());
   mod.def("adamw_moments", &adamw_moments, Free());
 }

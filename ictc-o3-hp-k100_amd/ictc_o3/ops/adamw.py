@@ -7,6 +7,8 @@ bytes an element instead of eight.  Checks and launches are in csrc/torch_ops.cp
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from ictc_o3 import _native as nat
@@ -52,7 +54,8 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits 32 or 8 chooses the type of the moments.  max_norm bounds the 2-norm over the gradients of all groups;
     the norm before the bound is left in ``grad_norm`` (a device scalar).  A parameter without a gradient is skipped:
-    its moments and its count of steps stay as they are.  A group's list of parameters may change between steps."""
+    its moments and its count of steps stay as they are.  A group's list of parameters may change between steps.
+    Parameters must be contiguous; a step that is refused changes nothing."""
 
     _MOMENTS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
@@ -81,10 +84,12 @@ class AdamW(torch.optim.Optimizer):
         are no longer those that they were made for."""
         group = self.param_groups[index]
         ps, eight = group["params"], group["state_bits"] == 8
-        made_for = (eight, ps[0].device, [(id(p), p.numel()) for p in ps])   # (kept parameters keep their ids)
-        if index not in self._flat or self._flat[index][2] != made_for:
+        counts = list(map(torch.Tensor.numel, ps))
+        made_for = (eight, ps[0].device, counts)
+        kept = self._flat.get(index)
+        if kept is None or kept[2] != made_for or not all(map(operator.is_, ps, kept[3])):
             self._flat.pop(index, None)   # (a fault below leaves the state as the only source)
-            starts, total = adamw_segments([p.numel() for p in ps])
+            starts, total = adamw_segments(counts)
             device = ps[0].device
             if eight:
                 flat = [torch.zeros(total, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
@@ -126,8 +131,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        ops = nat.ops()
-        work = []   # (group, flat moments, step, parameters, gradients, segments)
+        work = []   # (parameters, gradients, flat moments, segments, step and the group's numbers)
         for index, group in enumerate(self.param_groups):
             flat, starts = self._moments(index) if group["params"] else (None, ())
             by_step = {}
@@ -137,14 +141,14 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError("AdamW: gradients must be dense")
                     by_step.setdefault(self.state[p]["step"] + 1, []).append((p, p.grad.contiguous(), at))
             for step, rows in by_step.items():
-                work.append((group, flat, step, *map(list, zip(*rows))))
-        norm = None
-        if self.max_norm is not None and work:
-            norm = ops.gradient_norm([g for w in work for g in w[4]], self.max_norm)
-            self.grad_norm = norm[0]
-        for group, (m, v, ms, vs), step, params, grads, starts in work:
-            ops.adamw_update(params, grads, m, v, ms, vs, starts, step, group["lr"], *group["betas"], group["eps"],
-                             group["weight_decay"], norm)
+                params, grads, segments = map(list, zip(*rows))
+                work.append((params, grads, *flat, segments, step, group["lr"], *group["betas"], group["eps"],
+                             group["weight_decay"]))
+        if work:
+            norm = nat.ops().adamw_groups(work, self.max_norm)   # (checks all of it before the first launch)
+            if norm is not None:
+                self.grad_norm = norm
+        for params, *_, step, _, _, _, _, _ in work:
             for p in params:
                 self.state[p]["step"] = step
         return loss

@@ -485,3 +485,39 @@ def test_a_bound_does_not_let_a_bad_call_pass(device):
                 adamw_step(**{**dict(params=[], grads=[], exp_avg=m, exp_avg_sq=v, step=1, max_norm=bound), **bad})
     norm = adamw_step([], [], m, v, step=1, max_norm=1.0)
     assert norm.shape == () and float(norm) == 0
+
+
+def test_a_refused_step_changes_nothing(device):
+    from ictc_o3 import AdamW
+    ps, rs = _pair(device, [(300,), (40, 30), (77,)])
+    hyper = dict(lr=1e-2, weight_decay=0.05)
+    groups = lambda q: [dict(params=q[:1]), dict(params=q[1:])]  # noqa: E731
+    for bound in (None, 1e9):
+        opt = AdamW(groups(ps), max_norm=bound, **hyper)
+        gen = torch.Generator().manual_seed(5)
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=gen).to(device)
+        opt.step()
+        state = lambda: copy.deepcopy([[p.detach() for p in ps],  # noqa: E731
+                                       [[opt.state[p][k] for k in ("step", "exp_avg", "exp_avg_sq")] for p in ps]])
+        before = state()
+
+        def unchanged():
+            flat = lambda s: [x for part in s for x in (part if isinstance(part[0], torch.Tensor) else sum(part, []))]  # noqa: E731
+            return all(torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b
+                       for a, b in zip(flat(before), flat(state())))
+        group = opt.param_groups[1]
+        for name, bad in (("lr", float("nan")), ("betas", (0.9, 1.0)), ("eps", -1.0), ("weight_decay", float("inf"))):
+            good, group[name] = group[name], bad
+            with pytest.raises(ValueError):
+                opt.step()
+            group[name] = good
+            assert unchanged(), name
+        good = ps[1].data
+        ps[1].data, ps[1].grad = good.t().contiguous().t(), ps[1].grad
+        with pytest.raises(ValueError, match="contiguous"):
+            opt.step()
+        assert unchanged()
+        ps[1].data = good
+        opt.step()
+        assert [opt.state[p]["step"] for p in ps] == [2, 2, 2]
