@@ -497,27 +497,42 @@ void launch_step(const Step& s, const Lists& l, const OptTensor& norm) {
   for (const Tensor& t : {s.m, s.v, value(s.ms), value(s.vs)}) changed(t);
 }
 
+// Gradients of one type share a norm's launch; the norms of several types are joined in FP64, and the factor made of them
+// as ictc_gradient_norm makes it (a type's norm past FP32 is infinite here, and the factor zero).
+Tensor common_norm(const std::vector<List>& grads, double max_norm, const Tensor& like) {
+  std::vector<Tensor> norms;
+  for (const List& g : grads) norms.push_back(gradient_norm(g, max_norm, like));
+  if (norms.empty()) return at::zeros({1}, like.options().dtype(at::kFloat));
+  if (norms.size() == 1) return norms[0];
+  for (Tensor& n : norms) n = n.select(0, 0);
+  const Tensor norm = at::stack(norms).to(at::kDouble).square().sum().sqrt();
+  return at::stack({norm, at::clamp_max(max_norm / (norm + 1e-6), 1.0)}).to(at::kFloat);
+}
+
 // All steps with their gradients' common norm held to max_norm, which is returned; all are checked before the first is
 // taken.
 OptTensor take_steps(const std::vector<Step>& steps, const std::optional<double>& max_norm) {
   TORCH_CHECK_VALUE(!max_norm.has_value() || *max_norm >= 0.0, "adamw: max_norm must be zero or more");
   std::vector<Lists> lists;
-  List grads;
+  std::vector<List> grads;   // of each type
   for (const Step& s : steps) {
     lists.push_back(check_step(s));
     const List& g = lists.back().g;
     if (!max_norm.has_value() || g.at.empty()) continue;
-    if (grads.dtype < 0) grads.dtype = g.dtype;
-    TORCH_CHECK_VALUE(g.dtype == grads.dtype && s.m.device() == steps[0].m.device(),
-                      "adamw: gradients of one norm must be of one type and on one device");
-    grads.at.insert(grads.at.end(), g.at.begin(), g.at.end());
-    grads.count.insert(grads.count.end(), g.count.begin(), g.count.end());
+    TORCH_CHECK_VALUE(s.m.device() == steps[0].m.device(), "adamw: gradients of one norm must be on one device");
+    size_t k = 0;
+    while (k < grads.size() && grads[k].dtype != g.dtype) ++k;
+    if (k == grads.size()) {
+      grads.push_back(g);
+      continue;
+    }
+    grads[k].at.insert(grads[k].at.end(), g.at.begin(), g.at.end());
+    grads[k].count.insert(grads[k].count.end(), g.count.begin(), g.count.end());
   }
   OptTensor norm;
   if (max_norm.has_value() && !steps.empty()) {
     const c10::DeviceGuard guard(steps[0].m.device());
-    norm = grads.at.empty() ? at::zeros({1}, steps[0].m.options().dtype(at::kFloat))
-                            : gradient_norm(grads, *max_norm, steps[0].m);
+    norm = common_norm(grads, *max_norm, steps[0].m);
   }
   for (size_t i = 0; i < steps.size(); ++i) launch_step(steps[i], lists[i], norm);
   return norm.has_value() ? OptTensor(norm->select(0, 0)) : OptTensor();

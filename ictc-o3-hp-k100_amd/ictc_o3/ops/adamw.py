@@ -50,7 +50,8 @@ def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, *, dtype
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW with torch.optim's interface on ``adamw_step``'s kernels: all parameters of a group in one launch per 120.
+    """AdamW with torch.optim's interface on ``adamw_step``'s kernels: all parameters of a group that have one type
+    (float32, bfloat16 or float16) in one launch per 120.
 
     state_bits 32 or 8 chooses the type of the moments.  max_norm bounds the 2-norm over the gradients of all groups;
     the norm before the bound is left in ``grad_norm`` (a device scalar).  A parameter without a gradient is skipped:
@@ -134,13 +135,13 @@ class AdamW(torch.optim.Optimizer):
         work = []   # (parameters, gradients, flat moments, segments, step and the group's numbers)
         for index, group in enumerate(self.param_groups):
             flat, starts = self._moments(index) if group["params"] else (None, ())
-            by_step = {}
+            alike = {}   # one step's parameters of one type each
             for p, at in zip(group["params"], starts):
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise ValueError("AdamW: gradients must be dense")
-                    by_step.setdefault(self.state[p]["step"] + 1, []).append((p, p.grad.contiguous(), at))
-            for step, rows in by_step.items():
+                    alike.setdefault((self.state[p]["step"] + 1, p.dtype), []).append((p, p.grad.contiguous(), at))
+            for (step, _), rows in alike.items():
                 params, grads, segments = map(list, zip(*rows))
                 work.append((params, grads, *flat, segments, step, group["lr"], *group["betas"], group["eps"],
                              group["weight_decay"]))

@@ -521,3 +521,45 @@ def test_a_refused_step_changes_nothing(device):
         ps[1].data = good
         opt.step()
         assert [opt.state[p]["step"] for p in ps] == [2, 2, 2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("bound", [None, 0.5])
+def test_parameters_of_several_types(device, bits, split, bound):
+    """FP32, bfloat16 and FP16 in one group or in a group each, one norm over all gradients."""
+    from ictc_o3 import AdamW
+    types = [torch.float32, torch.bfloat16, torch.float32, torch.float16, torch.bfloat16]
+    gen = torch.Generator().manual_seed(7)
+    ps = [torch.nn.Parameter(torch.randn(200 + 77 * i, generator=gen).to(t).to(device)) for i, t in enumerate(types)]
+    gs = [torch.randn(p.shape, generator=gen).to(p.dtype).to(device) for p in ps]
+    groups = [dict(params=[p for p in ps if p.dtype == t]) for t in (torch.bfloat16, torch.float32, torch.float16)]
+    opt = AdamW(groups if split else ps, max_norm=bound, state_bits=bits, **HYPER)
+    zero = [torch.zeros(p.shape, dtype=torch.float64, device=device) for p in ps]
+    (P, _, _), N = _formula([p.detach().double() for p in ps], [g.double() for g in gs], zero, zero, 1, bound, **HYPER)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt.step()
+    if bound is not None:
+        assert opt.grad_norm.dtype == torch.float32 and opt.grad_norm.shape == ()
+        assert abs(float(opt.grad_norm) - float(N)) < 1e-6 * float(N)
+    for p, r in zip(ps, P):
+        assert rel_err(p, r) < TOL[p.dtype]
+
+
+def test_a_common_norm_of_several_types(device):
+    """No bound reached, a bound with one gradient NaN, and norms at both ends of FP32."""
+    from ictc_o3 import AdamW
+    for size in (1e-30, 1.0, 1e25, float("nan")):
+        ps = [torch.nn.Parameter(torch.ones(300, device=device)),
+              torch.nn.Parameter(torch.ones(200, device=device, dtype=torch.bfloat16))]
+        ps[0].grad = torch.full((300,), size, device=device)
+        ps[1].grad = torch.full((200,), 2 * size if size == size else 1.0, device=device, dtype=torch.bfloat16)
+        opt = AdamW(ps, max_norm=1e3, **HYPER)
+        opt.step()
+        if size == size:
+            ref = torch.cat([p.grad.double() for p in ps]).norm()
+            assert abs(float(opt.grad_norm) - float(ref)) < 1e-6 * float(ref)
+            assert all(torch.isfinite(p).all() for p in ps)
+        else:
+            assert torch.isnan(opt.grad_norm) and all(torch.isnan(p).all() for p in ps)
