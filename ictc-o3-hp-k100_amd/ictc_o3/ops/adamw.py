@@ -36,7 +36,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
     ``adamw_moments``).  They are updated in place.  Arithmetic is FP32; a parameter of fewer bits is rounded to
     nearest.  With max_norm the gradients are taken as if clipped to that global norm (they are not changed), and the
     norm before clipping is returned as a float32 scalar on the device; otherwise None.  Non-finite gradients make the
-    parameters that they reach non-finite."""
+    parameters that they reach non-finite.  Captured into a graph, the call replays with the `step` and `lr` it had."""
     return nat.ops().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr,
                                 betas[0], betas[1], eps, weight_decay, max_norm)
 
@@ -56,7 +56,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits 32 or 8 chooses the type of the moments.  max_norm bounds the 2-norm over the gradients of all groups;
     the norm before the bound is left in ``grad_norm`` (a device scalar).  A parameter without a gradient is skipped:
     its moments and its count of steps stay as they are.  A group's list of parameters may change between steps.
-    Parameters must be contiguous; a step that is refused changes nothing."""
+    Parameters must be contiguous; a step that is refused changes nothing.  A step cannot be captured into a graph: a
+    replay would repeat its count of steps and its learning rate."""
 
     _MOMENTS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
@@ -128,6 +129,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step cannot be captured: its count and rate would stay those of the capture")
         loss = None
         if closure is not None:
             with torch.enable_grad():

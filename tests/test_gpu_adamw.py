@@ -563,3 +563,23 @@ def test_a_common_norm_of_several_types(device):
             assert all(torch.isfinite(p).all() for p in ps)
         else:
             assert torch.isnan(opt.grad_norm) and all(torch.isnan(p).all() for p in ps)
+
+
+def test_a_captured_step_is_refused(device):
+    """A graph would replay one step's count and rate for ever."""
+    from ictc_o3 import AdamW
+    p = torch.nn.Parameter(torch.ones(300, device=device))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], max_norm=1.0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    held = torch.zeros(4, device=device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held.add_(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+    assert opt.state[p]["step"] == 1
