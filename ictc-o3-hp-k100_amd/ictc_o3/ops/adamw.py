@@ -63,15 +63,21 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, max_norm=None,
                  state_bits=32):
-        if state_bits not in (32, 8):
-            raise ValueError("AdamW: state_bits must be 32 or 8")
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or lr < 0 or eps < 0 or weight_decay < 0:
-            raise ValueError("AdamW: betas must be in [0, 1); lr, eps and weight_decay zero or more")
         if max_norm is not None and not max_norm >= 0.0:
             raise ValueError("AdamW: max_norm must be zero or more")
         self.max_norm, self.grad_norm, self._flat = max_norm, None, {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits))
+
+    def add_param_group(self, param_group):
+        """torch.optim's, with the group's own numbers held to the same ranges as the defaults."""
+        g = {**self.defaults, **param_group}
+        if g["state_bits"] not in (32, 8):
+            raise ValueError("AdamW: state_bits must be 32 or 8")
+        if (not all(0.0 <= b < 1.0 for b in g["betas"])
+                or not (g["lr"] >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0)):
+            raise ValueError("AdamW: betas must be in [0, 1); lr, eps and weight_decay zero or more")
+        super().add_param_group(param_group)
 
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm}

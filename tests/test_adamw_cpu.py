@@ -53,3 +53,15 @@ def test_native_refusals():
     for norm, ws, nbytes in ((-1.0, 16, 1 << 20), (float("nan"), 16, 1 << 20), (1.0, None, 1 << 20), (1.0, 16, 64)):
         with pytest.raises(ValueError):
             nat.call("ictc_gradient_norm", 0, 1, at(one), at(n), norm, ws, nbytes, None)
+
+
+def test_hyperparameters_of_a_group():
+    from ictc_o3 import AdamW
+    ps = [torch.nn.Parameter(torch.ones(4)) for _ in range(2)]
+    for bad in (dict(state_bits=16), dict(betas=(0.9, 1.0)), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW([dict(params=ps[:1]), dict(params=ps[1:], **bad)])
+        opt = AdamW(ps[:1])
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=ps[1:], **bad))
+        assert len(opt.param_groups) == 1
