@@ -3,8 +3,10 @@
 // in a thread of its own: a node in Python costs two hand-overs of the interpreter's lock there, more than the kernels
 // of a small layer take.  Work goes on the operand's current stream.
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -30,6 +32,17 @@ void done(int rc, const char* what) {
   const std::string said = std::string(what) + ": " + ictc_last_error();
   TORCH_CHECK_VALUE(rc != ICTC_ERR_ARGUMENT && rc != ICTC_ERR_UNSUPPORTED, said);
   TORCH_CHECK(false, said);
+}
+
+// The results are written through raw pointers, which a trace does not see: it would keep their allocation and replay
+// that.  So these operators run eagerly, as the equivariant ones do; forward and backward passes ask.
+void eager(const char* op) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  bool traced = torch::jit::tracer::isTracing();
+  if (Modes::any_modes_set())
+    for (Key key : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) traced |= Modes::get_mode(key).has_value();
+  TORCH_CHECK_VALUE(!traced, op, ": cannot be traced; it requires eager execution");
 }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
@@ -96,6 +109,7 @@ struct NormGrads {
 
 NormGrads norm_backward(const Tensor& x_, const Tensor& w_, const Tensor& g_, const Tensor& stats, bool need_x,
                         bool need_w, bool need_b) {
+  eager("layer_norm");
   const Tensor x = rows_of(x_), w = packed(w_), g = rows_of(g_);
   const int64_t N = x.size(0), C = x.size(1);
   const int dt = dtype_of(x);
@@ -122,6 +136,7 @@ struct NormSeconds {
 
 NormSeconds norm_backward2(const Tensor& x_, const Tensor& w_, const Tensor& g_, const Tensor& v_, const Tensor& vw_,
                            const Tensor& vb_, const Tensor& stats, bool need_x, bool need_w, bool need_g) {
+  eager("layer_norm");
   const Tensor x = rows_of(x_), w = packed(w_), g = rows_of(g_), vw = packed(vw_), vb = packed(vb_);
   const Tensor v = v_.defined() ? rows_of(v_) : at::zeros_like(x, at::MemoryFormat::Contiguous);
   const int64_t N = x.size(0), C = x.size(1);
@@ -244,6 +259,7 @@ struct LayerNorm : Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  eager("layer_norm");
   check_dense(x, "layer_norm", "x");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384,
                     "layer_norm: x must have a last axis of 1 to 16384 elements");
@@ -267,6 +283,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
 
 // (rows sorted by expert, first sorted row of each expert): what the kernels below take.
 std::pair<Tensor, Tensor> expert_order(const Tensor& ids_, int64_t experts) {
+  eager("expert_order");
   TORCH_CHECK_VALUE(ids_.is_cuda() && ids_.scalar_type() == at::kLong && ids_.dim() == 1,
                     "expert_order: ids must be an int64 vector on a ROCm (cuda) device");
   TORCH_CHECK_VALUE(experts >= 1 && experts <= 65535, "expert_order: experts must be an integer from 1 to 65535");
@@ -286,6 +303,7 @@ std::pair<Tensor, Tensor> expert_order(const Tensor& ids_, int64_t experts) {
 
 Tensor linear_rows(const Tensor& x_, const Tensor& W_, const Tensor& b_, const Tensor& perm, const Tensor& off,
                    bool trans) {
+  eager("expert_linear");
   const Tensor x = rows_of(x_), W = packed(W_), b = packed(b_);
   const int64_t N = x.size(0), outputs = W.size(trans ? 2 : 1);
   Tensor out = at::empty({N, outputs}, x.options());
@@ -298,6 +316,7 @@ Tensor linear_rows(const Tensor& x_, const Tensor& W_, const Tensor& b_, const T
 
 std::pair<Tensor, Tensor> linear_outer(const Tensor& g_, const Tensor& x_, const Tensor& perm, const Tensor& off,
                                        bool need_b) {
+  eager("expert_linear");
   const Tensor g = rows_of(g_), x = rows_of(x_);
   const int64_t N = x.size(0), M = g.size(1), K = x.size(1), E = off.size(0) - 2;
   const int dt = dtype_of(x);
@@ -378,6 +397,7 @@ variable_list ExpertLinear::backward(AutogradContext* ctx, variable_list grads) 
 
 Tensor expert_linear(const Tensor& x, const Tensor& W, const OptTensor& b, const Tensor& perm, const Tensor& off,
                      int64_t rows) {
+  eager("expert_linear");
   check_dense(x, "expert_linear", "x");
   check_dense(W, "expert_linear", "weight", &x);
   TORCH_CHECK_VALUE(x.dim() == 2 && W.dim() == 3 && x.size(1) == W.size(2) && W.numel() > 0,
@@ -512,6 +532,7 @@ Tensor common_norm(const std::vector<List>& grads, double max_norm, const Tensor
 // All steps with their gradients' common norm held to max_norm, which is returned; all are checked before the first is
 // taken.
 OptTensor take_steps(const std::vector<Step>& steps, const std::optional<double>& max_norm) {
+  eager("adamw");
   TORCH_CHECK_VALUE(!max_norm.has_value() || *max_norm >= 0.0, "adamw: max_norm must be zero or more");
   std::vector<Lists> lists;
   std::vector<List> grads;   // of each type
@@ -556,6 +577,7 @@ OptTensor adamw_groups(const std::vector<GroupStep>& groups, const std::optional
 
 std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const Tensor& ms, const Tensor& vs,
                                         at::ScalarType type) {
+  eager("adamw");
   check_moments(m, v, ms, vs);
   const c10::DeviceGuard guard(m.device());
   const auto opts = m.options().dtype(type);
