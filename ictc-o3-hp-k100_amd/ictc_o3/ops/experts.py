@@ -23,7 +23,3 @@ class ExpertOrder:
     def __init__(self, ids: torch.Tensor, experts: int):
         self.perm, self.offsets = nat.ops().expert_order(ids, experts)
         self.rows, self.experts = ids.shape[0], experts
-
-
-def expert_linear(x: torch.Tensor, weight: torch.Tensor, order: ExpertOrder, bias=None) -> torch.Tensor:
-    return nat.ops().expert_linear(x, weight, bias, order.perm, order.offsets, order.rows)
