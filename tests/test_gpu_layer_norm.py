@@ -260,3 +260,47 @@ def test_the_same_without_a_graph(device, dtype):
         inference = layer_norm(x, w, b)
     assert kept.requires_grad and not plain.requires_grad and not off.requires_grad
     assert all(torch.equal(t, kept) for t in (plain, off, inference))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width", [(36011, 64), (36011, 120), (20011, 250), (9001, 500), (5003, 1000),
+                                        (5003, 2000), (2531, 2176), (2531, 4096), (1201, 8192), (1201, 9000),
+                                        (601, 16384)])
+def test_rows_that_a_team_takes_in_turn(device, rows, width, dtype):
+    """Rows enough that every team of every kernel has several, the last round part full: results, gradients and
+    gradients of the gradients, the latter two with their sums over rows."""
+    from ictc_o3 import layer_norm
+    x, w, b, gy, v = _inputs(rows, width, dtype, 5, device)
+    vw, vb = _inputs(2, width, dtype, 6, device)[1:3]
+    for t in (x, w, b, gy):
+        t.requires_grad_()
+    X, W, B, G = _double(x, w, b, gy)
+    y, Y = layer_norm(x, w, b, eps=EPS), _formula(X, W, B)
+    first = torch.autograd.grad(y, (x, w, b), gy, create_graph=True)
+    First = torch.autograd.grad(Y, (X, W, B), G, create_graph=True)
+    _check((y, *first), (Y, *First), dtype, ("y", "dx", "dw", "db"))
+    second = torch.autograd.grad(first, (x, gy), (v, vw, vb), retain_graph=True)
+    _check(second, torch.autograd.grad(First, (X, G), (v.double(), vw.double(), vb.double()), retain_graph=True), dtype,
+           ("dx'", "dg'"))
+    second = torch.autograd.grad(first[0], (x, w, gy), v)
+    _check(second, torch.autograd.grad(First[0], (X, W, G), v.double()), dtype, ("dx'", "dw'", "dg'"))
+
+
+@pytest.mark.parametrize("width", [16, 64, 128, 200, 256, 512, 777, 2048, 2176, 8192, 9000])
+def test_gradients_of_the_gradients_in_half(device, width):
+    from ictc_o3 import layer_norm
+    dtype = torch.float16
+    x, w, b, gy, v = _inputs(41, width, dtype, width, device)
+    vw, vb = _inputs(2, width, dtype, width + 1, device)[1:3]
+    for t in (x, w, b, gy):
+        t.requires_grad_()
+    first = torch.autograd.grad(layer_norm(x, w, b, eps=EPS), (x, w, b), gy, create_graph=True)
+    X, W, B, G = _double(x, w, b, gy)
+    First = torch.autograd.grad(_formula(X, W, B), (X, W, B), G, create_graph=True)
+    for outs, cots in (((0,), (v,)), ((0, 1, 2), (v, vw, vb)), ((1,), (vw,)), ((1, 2), (vw, vb))):
+        got = torch.autograd.grad([first[i] for i in outs], (x, gy), cots, retain_graph=True)
+        ref = torch.autograd.grad([First[i] for i in outs], (X, G), [c.double() for c in cots], retain_graph=True)
+        _check(got, ref, dtype, ("dx", "dg"))
+    (got,) = torch.autograd.grad(first[0], w, v, retain_graph=True)
+    (ref,) = torch.autograd.grad(First[0], W, v.double(), retain_graph=True)
+    _check((got,), (ref,), dtype, ("dw",))
