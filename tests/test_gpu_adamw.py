@@ -583,3 +583,34 @@ def test_a_captured_step_is_refused(device):
         with pytest.raises(RuntimeError, match="captured"):
             opt.step()
     assert opt.state[p]["step"] == 1
+
+
+def test_codes_of_8_bit_moments_in_half(device):
+    """FP16 parameters and gradients: codes and scales bit by bit, as of the other types."""
+    from ictc_o3 import adamw_segments, adamw_step
+    sizes = [300, 256, 5, 2304, 1, 700]
+    ps, gs = _lists(sizes, torch.float16, 3, device)
+    gs[1].mul_(1e3)
+    gs[2].zero_()
+    gs[3] *= torch.exp2(-torch.arange(2304, device=device) / 256).half()
+    gs[5][::3] = 0
+    starts, total = adamw_segments(sizes)
+    m8 = torch.zeros(total, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    v8 = torch.zeros(total, dtype=torch.uint8, device=device)
+    sm, sv = torch.ones(total // 256, device=device), torch.ones(total // 256, device=device)
+    m, v = torch.zeros(total), torch.zeros(total)
+    c = [torch.tensor(x, dtype=torch.float32) for x in (HYPER["betas"][0], 1 - HYPER["betas"][0],
+                                                        HYPER["betas"][1], 1 - HYPER["betas"][1])]
+    old = [p.double() for p in ps]
+    adamw_step(ps, gs, m8, v8, step=1, exp_avg_scale=sm, exp_avg_sq_scale=sv, **HYPER)
+    for a, n, g in zip(starts, sizes, gs):
+        g = g.cpu().float()
+        m[a:a + n] = m[a:a + n] * c[0] + g * c[1]
+        v[a:a + n] = v[a:a + n] * c[2] + g * g * c[3]
+    cm, cs, cv, vs = _encode(m, v)
+    live = m.view(-1, 256).abs().amax(1) > 0
+    assert torch.equal(m8.view(torch.uint8).cpu(), cm) and torch.equal(v8.cpu(), cv)
+    assert torch.equal(sm.cpu()[live], cs[live]) and torch.equal(sv.cpu()[live], vs[live])
+    zero = [torch.zeros_like(p) for p in old]
+    (P, _, _), _ = _formula(old, [g.double() for g in gs], zero, zero, 1, None, **HYPER)
+    assert rel_err(torch.cat(ps), torch.cat(P)) < TOL[torch.float16]
