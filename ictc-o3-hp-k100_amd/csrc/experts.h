@@ -20,8 +20,9 @@ __device__ __forceinline__ v4f mma(u32x4 a, u32x4 b, v4f c) {
 }
 
 // split8 (split_bf16.h) with each remainder by one instruction, the pair's dot product with (-1, 0) or (0, -1) added to
-// the value: it is exact as the subtraction is (checked over a million bit patterns), and where one value of a pair is
-// beyond bfloat16's range the other's remainder is NaN too.
+// the value: it is exact as the subtraction is, subnormal numbers included, and where one value of a pair is beyond
+// bfloat16's range the other's remainder is NaN too.  The parts end at bfloat16's last bit, 2^-133: a value under 2^-110
+// is held to 2^-134, not to FP32's precision.
 __device__ __forceinline__ Split split8_pairs(const float* v) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   uint32_t first = 0x0000bf80u, second = 0xbf800000u;

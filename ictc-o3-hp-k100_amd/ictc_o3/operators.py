@@ -388,8 +388,8 @@ def expert_linear(x, weight, order, bias=None):
     """y[n] = weight[id n] x[n] + bias[id n] for rows x [N, inputs] in the caller's order, weight [experts, outputs,
     inputs], bias [experts, outputs] or None, order from ``expert_order``; float32, bfloat16 or float16 throughout.
 
-    Sums are FP32 (FP32 operands keep FP32 accuracy; a row with infinities, or FP32 values above 3.38e38, may give
-    NaN) and each result is rounded once.  A row of no expert gives a zero row and adds to no gradient; an expert
+    Sums are FP32 (FP32 operands keep FP32 accuracy, those under 2^-110, 8e-34, to 2^-134; a row with infinities, or
+    FP32 values above 3.38e38, may give NaN) and each result is rounded once.  A row of no expert gives a zero row and adds to no gradient; an expert
     without rows has zero gradients.
     Differentiable to any order in x, weight and bias; every sum has a fixed order."""
     if not isinstance(order, ExpertOrder):

@@ -769,7 +769,8 @@ int ictc_layer_norm_bwd2(int dtype, const void* x, int64_t ldx, const void* grad
  * expert without rows; sums in a fixed order over a workspace of
  * ictc_expert_outer_workspace_bytes bytes, 16-byte aligned (0: none needed, -1: out of
  * range).  Rows of FP32 values are split into three bfloat16 parts for the matrix units:
- * a row with an infinity, or with a value above 3.38e38, may give NaN.                  */
+ * a row with an infinity, or with a value above 3.38e38, may give NaN, and a value under
+ * 2^-110 is taken to the nearest 2^-133.                                                */
 int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts);
 int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
                       int64_t workspace_bytes, void* stream);

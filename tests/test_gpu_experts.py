@@ -362,3 +362,85 @@ def test_the_same_without_a_graph(device):
         inference = expert_linear(x, W, expert_order(ids, 3), b)
     assert kept.requires_grad and not plain.requires_grad and not off.requires_grad
     assert all(torch.equal(t, kept) for t in (plain, off, inference))
+
+
+@pytest.mark.parametrize("rows,K,M", [(50021, 264, 504), (50021, 504, 264), (50021, 263, 501), (50021, 501, 263), (70000, 256, 256), (70001, 255, 257)])
+def test_many_rows_and_columns_in_fp32(device, rows, K, M):
+    """The largest FP32 tiles of rows, adjoint and weights' gradient, aligned and not, the last ones part full."""
+    data = _inputs(rows, 3, K, M, torch.float32, K, device)
+    _, y, got = _run(*data)
+    _, Y, ref = _reference(*data)
+    _check((y, *got), (Y, *ref), ("y", "gx", "gW", "gb"))
+    _, y2, again = _run(*data)
+    assert torch.equal(y, y2) and all(torch.equal(i, j) for i, j in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("K,M", [(201, 333), (333, 201), (511, 131)])
+def test_odd_rows_of_many_steps(device, dtype, K, M):
+    """Rows that are not 16-byte aligned, reductions of several steps straight and transposed."""
+    data = _inputs(40000, 4, K, M, dtype, K, device)
+    _, y, got = _run(*data)
+    _, Y, ref = _reference(*data)
+    _check((y, *got), (Y, *ref), ("y", "gx", "gW", "gb"))
+
+
+FORMS = [(16, 8, 1024, 256), (900, 2, 3, 5), (900, 3, 64, 96), (3000, 3, 128, 100), (3000, 3, 129, 101), (70000, 3, 256, 256),
+         (70001, 3, 255, 257)]
+
+
+@pytest.mark.parametrize("rows,experts,K,M", FORMS)
+def test_fp32_values_of_any_size(device, rows, experts, K, M):
+    """Values from 2^-60 to 2^60 whose products are of one size, within a row and from row to row.  FP32 operands are split
+    into three parts whatever their exponents, and powers of two change no other rounding, so once they are taken out
+    of the results the bound is that of values of one size."""
+    ids, x, W, b, gy = _inputs(rows, experts, K, M, torch.float32, rows, device)
+    g = torch.Generator().manual_seed(4)
+    s = torch.exp2(torch.randint(-60, 61, (K,), generator=g).float()).to(device)
+    t = torch.exp2(torch.randint(-60, 61, (M,), generator=g).float()).to(device)
+    for first in ("inputs", "outputs"):        # sizes that cancel in y and gW's rows, then in gx
+        if first == "inputs":
+            data = (ids, x * s, W / s, b, gy)
+        else:
+            data = (ids, x, W / t[:, None], b / t, gy * t)
+        _, y, got = _run(*data)
+        _, Y, ref = _reference(*data)
+        gx, gW, gb = got
+        GX, GW, GB = ref
+        if first == "inputs":
+            pairs = ((y, Y), (gx * s, GX * s.double()), (gW / s, GW / s.double()), (gb, GB))
+        else:
+            pairs = ((y * t, Y * t.double()), (gx, GX), (gW / t[:, None], GW / t.double()[:, None]), (gb / t, GB / t.double()))
+        _check([p[0] for p in pairs], [p[1] for p in pairs], ("y", "gx", "gW", "gb"))
+    r = torch.exp2(torch.randint(-60, 61, (rows,), generator=g).float()).to(device)[:, None]    # cancel in gW
+    data = (ids, x * r, W, torch.zeros_like(b), gy / r)
+    _, y, got = _run(*data)
+    _, Y, ref = _reference(*data)
+    _check((y / r, got[0] * r, got[1]), (Y / r.double(), ref[0] * r.double(), ref[1]), ("y", "gx", "gW"))
+
+
+def test_gradients_of_gradients_in_bfloat16(device):
+    """Of several first gradients at once: each second one is a single product, rounded once."""
+    data = _inputs(300, 4, 40, 72, torch.bfloat16, 2, device)
+    args, y, first = _run(*data, create=True)
+    Args, Y, First = _reference(*data)
+    g = torch.Generator().manual_seed(3)
+    v = [torch.randn(t.shape, generator=g).to(torch.bfloat16).to(device) for t in first]
+    got = torch.autograd.grad(first[:2], args[:2], v[:2], create_graph=True)
+    ref = torch.autograd.grad(First[:2], Args[:2], [t.double() for t in v[:2]], create_graph=True)
+    _check(got, ref, ("by x", "by W"))
+
+
+def test_fp32_values_near_the_smallest(device):
+    """A value's third part ends at bfloat16's last bit, 2^-133, so a value is off by up to 2^-134: of K = 64 terms, a
+    result by sum |w| 2^-134 at most; and by the bound of any result.  Results are kept large by the weights."""
+    from ictc_o3 import expert_linear, expert_order
+    for rows in (16, 3000, 70000):
+        ids, x, W, _, _ = _inputs(rows, 2, 64, 256, torch.float32, rows, device, bad=False)
+        order = expert_order(ids, 2)
+        for e in (-100, -110, -118, -126):
+            small, large = x * 2.0 ** e, W * 2.0 ** 90
+            Y = _formula(small.double(), large.double(), None, ids)
+            off = (expert_linear(small, large, order).double() - Y).abs().max()
+            lost = large.double().abs().sum(2).max() * 2.0 ** -134 if e < -110 else 0.0
+            assert off < 2e-5 * Y.abs().max() + lost, (rows, e)
