@@ -19,9 +19,10 @@
 // factor of two at 128 -> 128 (41 against 17 us).  For the weights' gradient a step has 64 rows and two blocks share a
 // unit.
 //
-// At 131,072 rows of 512 -> 512 over ten experts, rows / adjoint / weights' gradient in us: bfloat16 97 / 99 / 118 (709,
-// 694 and 582 TFLOP/s), FP32 520 / 520 / 485 (132 to 142 TFLOP/s, six times that on the matrix cores), bound by the
-// matrix cores' rate at the clock that they leave; 511 -> 511 FP16, through registers, 149 / 177 / 185.
+// At 131,072 rows of 512 -> 512 over ten experts, rows / adjoint / weights' gradient in us: bfloat16 102 / 97 / 116 (674,
+// 708 and 592 TFLOP/s; a library product of these sizes with one matrix 83 / 91 / 363), FP32 394 / 401 / 441 (174, 171 and
+// 156 TFLOP/s, six times that on the matrix cores; 497 / 505 / 640), bound by the matrix cores' rate at the clock that they
+// leave; 511 -> 511 FP16, through registers, 149 / 177 / 185.
 #include <algorithm>
 #include <type_traits>
 
