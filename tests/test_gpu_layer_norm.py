@@ -304,3 +304,21 @@ def test_gradients_of_the_gradients_in_half(device, width):
     (got,) = torch.autograd.grad(first[0], w, v, retain_graph=True)
     (ref,) = torch.autograd.grad(First[0], W, v.double(), retain_graph=True)
     _check((got,), (ref,), dtype, ("dw",))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [40, 100, 250, 500, 1000, 2000, 2176, 8192, 9000])
+def test_rows_whose_squares_leave_the_range(device, width, dtype):
+    """Finite rows spread over up to 2^110, whose variance FP32 does not hold, beside ordinary ones: a power of two
+    changes no rounding, so the bounds are the ordinary ones, row by row."""
+    from ictc_o3 import layer_norm
+    x, w, b, gy, _ = _inputs(40, width, dtype, 3, device)
+    size = torch.exp2(torch.tensor([0.0, 62.0, 66.0, 90.0, 110.0], device=device)).repeat(8)[:, None]
+    x = (x.float() * size).to(dtype).requires_grad_()
+    y = layer_norm(x, w, b)
+    (gx,) = torch.autograd.grad(y, x, gy)
+    X, W, B = _double(x, w, b)
+    Y = _formula(X, W, B)
+    (GX,) = torch.autograd.grad(Y, X, gy.double())
+    _check((y,), (Y,), dtype, ("y",))
+    assert rel_err(gx.double() * size, GX * size) < TOL[dtype]
