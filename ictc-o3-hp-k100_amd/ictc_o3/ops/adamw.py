@@ -55,7 +55,8 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits 32 or 8 chooses the type of the moments.  max_norm bounds the 2-norm over the gradients of all groups;
     the norm before the bound is left in ``grad_norm`` (a device scalar).  A parameter without a gradient is skipped:
-    its moments and its count of steps stay as they are.  A group's list of parameters may change between steps.
+    its moments and its count of steps stay as they are.  A group's list of parameters may change between steps,
+    and ``state`` may be cleared; its tensors are parts of larger ones, to be changed in place.
     Parameters must be contiguous; a step that is refused changes nothing.  A step cannot be captured into a graph: a
     replay would repeat its count of steps and its learning rate."""
 
@@ -89,13 +90,14 @@ class AdamW(torch.optim.Optimizer):
     def _moments(self, index):
         """The flat moments of a group, whose segments are its parameters' state.  Made at the first step, and anew from
         that state whenever the group's parameters (which ones, their order, size and device) or its type of moments
-        are no longer those that they were made for."""
+        are no longer those that they were made for, or the state was cleared."""
         group = self.param_groups[index]
         ps, eight = group["params"], group["state_bits"] == 8
         counts = list(map(torch.Tensor.numel, ps))
         made_for = (eight, ps[0].device, counts)
         kept = self._flat.get(index)
-        if kept is None or kept[2] != made_for or not all(map(operator.is_, ps, kept[3])):
+        if (kept is None or kept[2] != made_for or not all(map(operator.is_, ps, kept[3]))
+                or not all(map(self.state.__contains__, ps))):
             self._flat.pop(index, None)   # (a fault below leaves the state as the only source)
             starts, total = adamw_segments(counts)
             device = ps[0].device

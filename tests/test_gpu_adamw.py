@@ -614,3 +614,32 @@ def test_codes_of_8_bit_moments_in_half(device):
     zero = [torch.zeros_like(p) for p in old]
     (P, _, _), _ = _formula(old, [g.double() for g in gs], zero, zero, 1, None, **HYPER)
     assert rel_err(torch.cat(ps), torch.cat(P)) < TOL[torch.float16]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_cleared_state_starts_anew(device, bits):
+    from ictc_o3 import AdamW
+    start = [p.detach() for p in _pair(device, [(300,), (20, 30)])[0]]
+    gen = torch.Generator().manual_seed(3)
+    grads = [[torch.randn(p.shape, generator=gen).to(device) for p in start] for _ in range(3)]
+
+    def steps(opt, ps):
+        for gs in grads:
+            for p, g in zip(ps, gs):
+                p.grad = g
+            opt.step()
+        return [p.detach().clone() for p in ps]
+
+    ps = [torch.nn.Parameter(p.clone()) for p in start]
+    opt = AdamW(ps, lr=1e-2, state_bits=bits)
+    first = steps(opt, ps)
+    for how in ("clear", "replace"):
+        if how == "clear":
+            opt.state.clear()
+        else:
+            opt.state = type(opt.state)(dict)
+        with torch.no_grad():
+            for p, s in zip(ps, start):
+                p.copy_(s)
+        assert all(torch.equal(a, b) for a, b in zip(steps(opt, ps), first)), how
+        assert [opt.state[p]["step"] for p in ps] == [3, 3]
