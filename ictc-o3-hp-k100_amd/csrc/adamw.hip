@@ -245,12 +245,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table t, Hyper h, void* __re
   }
 }
 
-// out[0] = the norm, out[1] = the factor that holds it to `bound`, from the norm in FP64: one past FP32 still has one.
-// NaN stays NaN.
+// out[0] = the norm, out[1] = the factor that holds it to `bound`, from the norm in FP64: one past FP32 still has one;
+// out[2], out[3] = the FP64 norm.  NaN stays NaN.
 __device__ __forceinline__ void write_norm(double squares, float bound, float* __restrict__ out) {
   const double norm = sqrt(squares), f = (double)bound / (norm + 1e-6);
   out[0] = (float)norm;
   out[1] = f >= 1.0 ? 1.f : (float)f;
+  reinterpret_cast<double*>(out)[1] = norm;
 }
 
 // part[block] = sum of squares of the gradients of this launch's runs blockIdx, blockIdx + gridDim, ...: FP32 over the

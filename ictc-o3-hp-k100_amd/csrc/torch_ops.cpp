@@ -518,14 +518,14 @@ void launch_step(const Step& s, const Lists& l, const OptTensor& norm) {
 }
 
 // Gradients of one type share a norm's launch; the norms of several types are joined in FP64, and the factor made of them
-// as ictc_gradient_norm makes it (a type's norm past FP32 is infinite here, and the factor zero).
+// as ictc_gradient_norm makes it.
 Tensor common_norm(const std::vector<List>& grads, double max_norm, const Tensor& like) {
   std::vector<Tensor> norms;
   for (const List& g : grads) norms.push_back(gradient_norm(g, max_norm, like));
   if (norms.empty()) return at::zeros({1}, like.options().dtype(at::kFloat));
   if (norms.size() == 1) return norms[0];
-  for (Tensor& n : norms) n = n.select(0, 0);
-  const Tensor norm = at::stack(norms).to(at::kDouble).square().sum().sqrt();
+  for (Tensor& n : norms) n = n.narrow(0, 0, 4).view(at::kDouble).select(0, 1);   // (the FP64 norms)
+  const Tensor norm = at::stack(norms).square().sum().sqrt();
   return at::stack({norm, at::clamp_max(max_norm / (norm + 1e-6), 1.0)}).to(at::kFloat);
 }
 

@@ -800,7 +800,8 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  * ictc_gradient_norm: workspace[0] = the 2-norm over all gradients, workspace[1] =
  * min(1, max_norm / (norm + 1e-6)), both FP32 (squares and eight of them added in FP32,
  * in FP64 where FP32's range ends, FP64 above, in a fixed order; the factor holds for a
- * norm past FP32 too); ictc_gradient_norm_workspace_bytes bytes, 16-byte aligned.      */
+ * norm past FP32 too); bytes 8 to 15 = the norm in FP64.
+ * ictc_gradient_norm_workspace_bytes bytes, 16-byte aligned.                           */
 int64_t ictc_gradient_norm_workspace_bytes(int tensors);
 int ictc_gradient_norm(int dtype, int tensors, const int64_t* grads, const int64_t* counts, double max_norm,
                        void* workspace, int64_t workspace_bytes, void* stream);

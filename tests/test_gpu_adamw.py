@@ -643,3 +643,18 @@ def test_a_cleared_state_starts_anew(device, bits):
                 p.copy_(s)
         assert all(torch.equal(a, b) for a, b in zip(steps(opt, ps), first)), how
         assert [opt.state[p]["step"] for p in ps] == [3, 3]
+
+
+def test_a_common_norm_beyond_the_type_still_scales(device):
+    """As with one type: the factor, 2e-41, has 14 bits, and the first step hardly depends on it; the bound is 1e-4, and
+    a bfloat16 parameter's own rounding."""
+    from ictc_o3 import AdamW
+    signs = torch.sign(torch.randn(16384, generator=torch.Generator().manual_seed(0))).to(device)
+    ps = [torch.nn.Parameter(torch.zeros(16384, device=device, dtype=t)) for t in (torch.float32, torch.bfloat16)]
+    for p in ps:
+        p.grad = (3e38 * signs).to(p.dtype)
+    opt = AdamW(ps, max_norm=1.0, **HYPER)
+    opt.step()
+    assert torch.isinf(opt.grad_norm)
+    for p in ps:
+        assert rel_err(p, -HYPER["lr"] * signs.double()) < max(1e-4, TOL[p.dtype])
