@@ -97,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
         made_for = (eight, ps[0].device, counts)
         kept = self._flat.get(index)
         if (kept is None or kept[2] != made_for or not all(map(operator.is_, ps, kept[3]))
-                or not all(map(self.state.__contains__, ps))):
+                or ps[0] not in self.state):
             self._flat.pop(index, None)   # (a fault below leaves the state as the only source)
             starts, total = adamw_segments(counts)
             device = ps[0].device
@@ -143,7 +143,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []   # (parameters, gradients, flat moments, segments, step and the group's numbers)
+        work, stepped = [], []   # (parameters, gradients, flat moments, segments, step, the group's numbers); their states
         for index, group in enumerate(self.param_groups):
             flat, starts = self._moments(index) if group["params"] else (None, ())
             alike = {}   # one step's parameters of one type each
@@ -151,16 +151,18 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise ValueError("AdamW: gradients must be dense")
-                    alike.setdefault((self.state[p]["step"] + 1, p.dtype), []).append((p, p.grad.contiguous(), at))
+                    state = self.state[p]
+                    alike.setdefault((state["step"] + 1, p.dtype), []).append((p, p.grad.contiguous(), at, state))
             for (step, _), rows in alike.items():
-                params, grads, segments = map(list, zip(*rows))
+                params, grads, segments, states = map(list, zip(*rows))
                 work.append((params, grads, *flat, segments, step, group["lr"], *group["betas"], group["eps"],
                              group["weight_decay"]))
+                stepped.append((step, states))
         if work:
             norm = nat.ops().adamw_groups(work, self.max_norm)   # (checks all of it before the first launch)
             if norm is not None:
                 self.grad_norm = norm
-        for params, *_, step, _, _, _, _, _ in work:
-            for p in params:
-                self.state[p]["step"] = step
+        for step, states in stepped:
+            for state in states:
+                state["step"] = step
         return loss
