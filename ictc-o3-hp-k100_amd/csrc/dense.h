@@ -76,6 +76,13 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const floa
   }
 }
 
+// x, rounded to FP32 here: what it is computed by is not joined with a conversion that follows (a product to FP16 is
+// otherwise one instruction that rounds once, and differs from the FP32 product rounded in one case of some thousand).
+__device__ __forceinline__ float held(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));

@@ -2,102 +2,9 @@
 // rows by expert, over the C ABI of libictc_mi355x.so.  The nodes are C++ ones because the engine runs a backward pass
 // in a thread of its own: a node in Python costs two hand-overs of the interpreter's lock there, more than the kernels
 // of a small layer take.  Work goes on the operand's current stream.
-#include <ATen/ATen.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include <cmath>
-#include <limits>
-#include <optional>
-#include <string>
-#include <tuple>
-#include <vector>
-
-#include "../../include/ictc_mi355x.h"
+#include "torch_ops.h"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
-using torch::autograd::variable_list;
-using OptTensor = std::optional<Tensor>;
-
-// Raises what the C ABI reported: an argument's fault as ValueError.
-void done(int rc, const char* what) {
-  if (rc == ICTC_OK) return;
-  const std::string said = std::string(what) + ": " + ictc_last_error();
-  TORCH_CHECK_VALUE(rc != ICTC_ERR_ARGUMENT && rc != ICTC_ERR_UNSUPPORTED, said);
-  TORCH_CHECK(false, said);
-}
-
-// The results are written through raw pointers, which a trace does not see: it would keep their allocation and replay
-// that.  So these operators run eagerly, as the equivariant ones do; forward and backward passes ask.
-void eager(const char* op) {
-  using Modes = c10::impl::TorchDispatchModeTLS;
-  using Key = c10::impl::TorchDispatchModeKey;
-  bool traced = torch::jit::tracer::isTracing();
-  if (Modes::any_modes_set())
-    for (Key key : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) traced |= Modes::get_mode(key).has_value();
-  TORCH_CHECK_VALUE(!traced, op, ": cannot be traced; it requires eager execution");
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-
-int dtype_of(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return ICTC_F32;
-    case at::kBFloat16: return ICTC_BF16;
-    case at::kHalf: return ICTC_F16;
-    default: return -1;
-  }
-}
-
-void check_dense(const Tensor& t, const char* op, const char* name, const Tensor* like = nullptr) {
-  TORCH_CHECK_VALUE(t.is_cuda(), op, ": ", name, " must be on a ROCm (cuda) device");
-  TORCH_CHECK_VALUE(dtype_of(t) >= 0, op, ": ", name, " must be float32, bfloat16 or float16");
-  if (like) {
-    TORCH_CHECK_VALUE(t.get_device() == like->get_device(), op, ": ", name, " must be on ", like->device());
-    TORCH_CHECK_VALUE(t.scalar_type() == like->scalar_type(), op, ": ", name, " must have the type ",
-                      like->scalar_type());
-  }
-}
-
-// t [N, C] itself, or a copy, with unit column stride and a row pitch of at least C.
-Tensor rows_of(const Tensor& t) {
-  if (t.is_contiguous()) return t;
-  if ((t.stride(1) == 1 || t.size(1) == 1) && (t.stride(0) >= t.size(1) || t.size(0) <= 1)) return t;
-  return t.contiguous();
-}
-
-int64_t pitch(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }   // (a single row's stride may be anything)
-
-Tensor packed(const Tensor& t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
-
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-Tensor floats(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
-
-Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-
-// Whether an operator's call has to leave a node behind.  Without (inference) it goes past autograd, and layer norm writes
-// no statistics: order and expert linear of 5 rows 10.7 -> 8.9 us, layer norm of one 5.5 -> 3.8.
-bool tracked(std::initializer_list<const Tensor*> inputs) {
-  for (const Tensor* t : inputs)
-    if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
-  return false;
-}
-
-// Which of a node's inputs the running backward pass asks for; inputs without a variable have no edge.
-std::vector<bool> wanted(AutogradContext* ctx, std::initializer_list<bool> present) {
-  std::vector<bool> out;
-  size_t edge = 0;
-  for (bool p : present) out.push_back(p && ctx->needs_input_grad(edge++));
-  return out;
-}
 
 // ---------------------------------------------------------------------------
 // Layer norm
@@ -200,9 +107,8 @@ struct LayerNormGrad : Function<LayerNormGrad> {
     if (!v[0].defined() && !v[1].defined() && !v[2].defined()) return out;
     const std::vector<bool> want = wanted(ctx, {true, true, w.defined()});
     if (at::GradMode::is_enabled()) {
-      const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
       const variable_list s =
-          LayerNormSecond::apply(x, g, opt(w), opt(v[0]), opt(v[1]), opt(v[2]), stats, want[0], want[2], want[1]);
+          LayerNormSecond::apply(x, g, some(w), some(v[0]), some(v[1]), some(v[2]), stats, want[0], want[2], want[1]);
       size_t k = 0;
       if (want[0]) out[0] = s[k++];
       if (want[2]) out[2] = s[k++];
@@ -243,7 +149,7 @@ struct LayerNorm : Function<LayerNorm> {
     variable_list out(4);
     if (!want[0] && !want[1] && !want[2]) return out;
     if (at::GradMode::is_enabled()) {   // the gradient will be differentiated
-      const variable_list s = LayerNormGrad::apply(x, grads[0], w.defined() ? OptTensor(w) : OptTensor(), stats,
+      const variable_list s = LayerNormGrad::apply(x, grads[0], some(w), stats,
                                                    want[0], want[1], want[2]);
       size_t k = 0;
       for (int i = 0; i < 3; ++i)
@@ -289,16 +195,7 @@ std::pair<Tensor, Tensor> expert_order(const Tensor& ids_, int64_t experts) {
   TORCH_CHECK_VALUE(experts >= 1 && experts <= 65535, "expert_order: experts must be an integer from 1 to 65535");
   TORCH_CHECK_VALUE(ids_.size(0) < (int64_t(1) << 31) - 2, "expert_order: up to 2^31 - 3 rows");
   const c10::DeviceGuard guard(ids_.device());
-  const Tensor ids = packed(ids_);
-  const int64_t N = ids.size(0), bytes = ictc_expert_order_workspace_bytes(N, (int)experts);
-  const auto ints = ids.options().dtype(at::kInt);
-  const Tensor perm = at::empty({std::max<int64_t>(N, 1)}, ints), offsets = at::empty({experts + 2}, ints);
-  Tensor ws;
-  if (bytes > 0) ws = at::empty({bytes}, ids.options().dtype(at::kByte));
-  done(ictc_expert_order(ids.const_data_ptr<int64_t>(), N, (int)experts, perm.mutable_data_ptr<int>(),
-                         offsets.mutable_data_ptr<int>(), ptr(ws), bytes, stream_of(ids)),
-       "expert_order");
-  return {perm, offsets};
+  return rows_by_id(packed(ids_), experts);
 }
 
 Tensor linear_rows(const Tensor& x_, const Tensor& W_, const Tensor& b_, const Tensor& perm, const Tensor& off,
@@ -364,7 +261,7 @@ struct ExpertOuter : Function<ExpertOuter> {
     if (!H.defined() && !h.defined()) return out;
     if (!H.defined()) H = at::zeros({off.size(0) - 2, g.size(1), x.size(1)}, x.options());
     if (ctx->needs_input_grad(0))
-      out[0] = ExpertLinear::apply(x, H, h.defined() ? OptTensor(h) : OptTensor(), perm, off, false);
+      out[0] = ExpertLinear::apply(x, H, some(h), perm, off, false);
     if (ctx->needs_input_grad(1)) out[1] = ExpertLinear::apply(g, H, OptTensor(), perm, off, true);
     return out;
   }
@@ -592,6 +489,8 @@ std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const 
 
 }  // namespace
 
+void bind_layers(pybind11::module_& mod);   // torch_layers.cpp
+
 PYBIND11_MODULE(ictc_torch, mod) {
   // Launches may wait for room in a queue: other Python threads run meanwhile.
   using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
@@ -601,4 +500,5 @@ PYBIND11_MODULE(ictc_torch, mod) {
   mod.def("adamw_step", &adamw_step, Free());
   mod.def("adamw_groups", &adamw_groups, Free());
   mod.def("adamw_moments", &adamw_moments, Free());
+  bind_layers(mod);
 }

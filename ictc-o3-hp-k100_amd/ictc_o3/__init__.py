@@ -6,7 +6,8 @@ needs no GPU; calling an operator needs a ROCm device and the in-tree
 """
 from ictc_o3.operators import (EdgeTensorProduct, GraphMessage, PackedGraphMessage, channel_linear,
                                configure_symmetric_contraction, create_symmetric_contraction,
-                               direction_harmonics, expert_linear, expert_order, layer_norm, normalized_silu)
+                               direction_harmonics, embedding, expert_linear, expert_order, layer_norm,
+                               normalized_silu)
 from ictc_o3.ops.adamw import AdamW, adamw_moments, adamw_segments, adamw_step
 
 __version__ = "0.1.0"
@@ -14,6 +15,6 @@ __version__ = "0.1.0"
 __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
-    "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order",
+    "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order", "embedding",
     "AdamW", "adamw_step", "adamw_moments", "adamw_segments",
 ]

@@ -19,7 +19,7 @@ from ictc_o3.ops.harmonics import harmonics_packed
 __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
-    "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order",
+    "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order", "embedding",
 ]
 
 
@@ -395,3 +395,19 @@ def expert_linear(x, weight, order, bias=None):
     if not isinstance(order, ExpertOrder):
         raise TypeError("expert_linear: order must come from expert_order")
     return nat.ops().expert_linear(x, weight, bias, order.perm, order.offsets, order.rows)
+
+
+def embedding(table, ids, scale=1.0, order=None):
+    """scale * table[ids] for a table [entries, width] (float32, bfloat16 or float16) and int64 ids of any shape, which
+    the result's shape begins with.  An id outside [0, entries) (padding) gives a zero row and adds to no gradient.
+
+    The table's gradient adds the rows of each id in FP32, in a fixed order, and rounds once.  It takes the rows sorted
+    by id: `order` from ``expert_order(ids, entries)`` where one is at hand (ids of one axis), else it sorts them
+    itself.  Differentiable to any order."""
+    if order is None:
+        return nat.ops().embedding(table, ids, scale, None, None)
+    if not isinstance(order, ExpertOrder):
+        raise TypeError("embedding: order must come from expert_order")
+    if ids.numel() != order.rows:
+        raise ValueError("embedding: the order is of other ids")
+    return nat.ops().embedding(table, ids, scale, order.perm, order.offsets)

@@ -782,6 +782,23 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
                       int outputs, int experts, const int32_t* perm, const int32_t* offsets, void* dweight,
                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Rows of a table chosen by an id ---------------------------------------
+ * out[n] = scale table[ids[n]] with table [entries, width] and out [rows, width] packed,
+ * element type dtype; an id outside [0, entries) gives a zero row.  bwd: dtable[v] = scale
+ * times the sum of grad's rows (pitch ldg) whose id is v, FP32 sums in a fixed order, zeros
+ * for an entry without rows.  perm and offsets are the rows' order by id, what
+ * ictc_expert_order and ictc_csr_build give for these ids and `entries` keys; up to as many
+ * rows as ictc_embedding_needs_order denies they may be NULL.  Workspace of
+ * ictc_embedding_bwd_workspace_bytes bytes, 4-byte aligned (0: none needed, -1: an
+ * argument out of range).                                                               */
+int ictc_embedding_fwd(int dtype, const void* table, int64_t entries, int width, const int64_t* ids, int64_t rows,
+                       float scale, void* out, void* stream);
+int ictc_embedding_needs_order(int64_t rows);
+int64_t ictc_embedding_bwd_workspace_bytes(int dtype, int64_t rows, int64_t entries, int width);
+int ictc_embedding_bwd(int dtype, const void* grad, int64_t ldg, int64_t rows, int width, const int64_t* ids,
+                       int64_t entries, const int32_t* perm, const int32_t* offsets, float scale, void* dtable,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- AdamW over a list of tensors ------------------------------------------
  * One step with decoupled weight decay, in FP32 arithmetic:
  *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
