@@ -102,9 +102,48 @@ Tensor embedding(const Tensor& table, const Tensor& ids, double scale, const Opt
   return y.view(shape);
 }
 
+// ---------------------------------------------------------------------------
+// Activations in 8 bits
+// ---------------------------------------------------------------------------
+
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+  std::vector<int64_t> out = sizes.vec();
+  out.back() = last;
+  return out;
+}
+
+std::pair<Tensor, Tensor> encode_activations(const Tensor& x) {
+  eager("encode_activations");
+  check_dense(x, "encode_activations", "x");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= std::numeric_limits<int>::max(),
+                    "encode_activations: x must have a last axis of 1 to 2^31 - 1 elements");
+  const int64_t C = x.size(-1);
+  const Codes k = encode_rows(x.detach().reshape({x.numel() / C, C}));
+  return {k.codes.view(x.sizes()), k.scales.view(with_last(x.sizes(), k.scales.size(1)))};
+}
+
+Tensor decode_activations(const Tensor& codes, const Tensor& scales, at::ScalarType type) {
+  eager("decode_activations");
+  TORCH_CHECK_VALUE(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() >= 1 && codes.size(-1) >= 1 &&
+                        codes.size(-1) <= std::numeric_limits<int>::max(),
+                    "decode_activations: codes must be int8 on a ROCm (cuda) device");
+  TORCH_CHECK_VALUE(scales.scalar_type() == at::kFloat && scales.device() == codes.device() &&
+                        scales.sizes() == with_last(codes.sizes(), (codes.size(-1) + 127) / 128),
+                    "decode_activations: scales must be float32, one for each 128 codes of a row, and on ",
+                    codes.device());
+  TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf,
+                    "decode_activations: dtype must be float32, bfloat16 or float16");
+  const int64_t C = codes.size(-1), N = codes.numel() / C;
+  const c10::DeviceGuard guard(codes.device());
+  return decode_rows(codes.reshape({N, C}).contiguous(), scales.reshape({N, (C + 127) / 128}).contiguous(), type)
+      .view(codes.sizes());
+}
+
 }  // namespace
 
 void bind_layers(pybind11::module_& mod) {
   using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
   mod.def("embedding", &embedding, Free());
+  mod.def("encode_activations", &encode_activations, Free());
+  mod.def("decode_activations", &decode_activations, Free());
 }

@@ -233,9 +233,16 @@ struct ExpertOuter;
 // y[n] = W[e] x[n] + b[e], or with trans W[e]^T x[n].  Its adjoints are the same map with the other orientation and
 // ExpertOuter, whose adjoints are this map again: differentiable to any order.
 struct ExpertLinear : Function<ExpertLinear> {
+  // place, codes and scales: the rows are kept in 8 bits (torch_ops.h)
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& W, const OptTensor& b,
-                        const Tensor& perm, const Tensor& off, bool trans) {
-    ctx->save_for_backward({x, W, perm, off});
+                        const Tensor& perm, const Tensor& off, bool trans, const c10::IValue& place = c10::IValue(),
+                        const Codes& kept = Codes()) {
+    if (kept.codes.defined()) {
+      ctx->save_for_backward({kept.codes, W, perm, off, kept.scales});
+      ctx->saved_data["place"] = place;
+    } else {
+      ctx->save_for_backward({x, W, perm, off});
+    }
     ctx->saved_data["trans"] = trans;
     ctx->saved_data["bias"] = b.has_value();
     return linear_rows(x, W, value(b), perm, off, trans);
@@ -269,11 +276,15 @@ struct ExpertOuter : Function<ExpertOuter> {
 
 variable_list ExpertLinear::backward(AutogradContext* ctx, variable_list grads) {
   const variable_list saved = ctx->get_saved_variables();
-  const Tensor &x = saved[0], &W = saved[1], &perm = saved[2], &off = saved[3], &g = grads[0];
+  const Tensor &W = saved[1], &perm = saved[2], &off = saved[3], &g = grads[0];
   const bool trans = ctx->saved_data["trans"].toBool();
   const std::vector<bool> want = wanted(ctx, {true, true, ctx->saved_data["bias"].toBool()});
   const bool again = at::GradMode::is_enabled();   // the gradient will be differentiated
-  variable_list out(6);
+  Tensor x = saved[0];
+  if (saved.size() > 4 && (want[1] || want[2]))
+    x = again ? Decoded::apply(ctx->saved_data["place"].toTensor(), saved[0], saved[4])
+              : decode_rows(saved[0], saved[4], W.scalar_type());
+  variable_list out(8);
   if (want[0])
     out[0] = again ? ExpertLinear::apply(g, W, OptTensor(), perm, off, !trans)
                    : linear_rows(g, W, Tensor(), perm, off, !trans);
@@ -293,7 +304,7 @@ variable_list ExpertLinear::backward(AutogradContext* ctx, variable_list grads) 
 }
 
 Tensor expert_linear(const Tensor& x, const Tensor& W, const OptTensor& b, const Tensor& perm, const Tensor& off,
-                     int64_t rows) {
+                     int64_t rows, const std::optional<int64_t>& save_bits) {
   eager("expert_linear");
   check_dense(x, "expert_linear", "x");
   check_dense(W, "expert_linear", "weight", &x);
@@ -307,10 +318,13 @@ Tensor expert_linear(const Tensor& x, const Tensor& W, const OptTensor& b, const
     TORCH_CHECK_VALUE(b->dim() == 2 && b->size(0) == W.size(0) && b->size(1) == W.size(1),
                       "expert_linear: bias must have shape [experts, outputs]");
   }
+  const bool eight = in_8_bits(save_bits, "expert_linear");
   const c10::DeviceGuard guard(x.device());
   const Tensor bv = value(b);
-  return tracked({&x, &W, &bv}) ? ExpertLinear::apply(x, W, b, perm, off, false)
-                                : linear_rows(x, W, bv, perm, off, false);
+  if (!tracked({&x, &W, &bv})) return linear_rows(x, W, bv, perm, off, false);
+  // (only the weights' gradient takes the rows)
+  if (!eight || !W.requires_grad()) return ExpertLinear::apply(x, W, b, perm, off, false);
+  return ExpertLinear::apply(x, W, b, perm, off, false, c10::IValue(Place8::apply(x)), encode_rows(x.detach()));
 }
 
 // ---------------------------------------------------------------------------
@@ -496,7 +510,9 @@ PYBIND11_MODULE(ictc_torch, mod) {
   using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
   mod.def("layer_norm", &layer_norm, Free());
   mod.def("expert_order", &expert_order, Free());
-  mod.def("expert_linear", &expert_linear, Free());
+  mod.def("expert_linear", &expert_linear, pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("bias"),
+          pybind11::arg("perm"), pybind11::arg("offsets"), pybind11::arg("rows"),
+          pybind11::arg("save_bits") = pybind11::none(), Free());
   mod.def("adamw_step", &adamw_step, Free());
   mod.def("adamw_groups", &adamw_groups, Free());
   mod.def("adamw_moments", &adamw_moments, Free());

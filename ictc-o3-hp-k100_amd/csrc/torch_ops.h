@@ -117,4 +117,59 @@ std::pair<Tensor, Tensor> rows_by_id(const Tensor& ids, int64_t keys) {
   return {perm, offsets};
 }
 
+// ---------------------------------------------------------------------------
+// Activations in 8 bits
+// ---------------------------------------------------------------------------
+
+struct Codes {
+  Tensor codes, scales;   // int8 [rows, width], float32 [rows, blocks of 128]
+};
+
+Codes encode_rows(const Tensor& x_) {
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = rows_of(x_);
+  const int64_t N = x.size(0), C = x.size(1);
+  Codes out = {at::empty({N, C}, x.options().dtype(at::kChar)),
+               at::empty({N, (C + 127) / 128}, x.options().dtype(at::kFloat))};
+  done(ictc_codes_encode(dtype_of(x), ptr(x), pitch(x), N, (int)C, out.codes.mutable_data_ptr<int8_t>(),
+                         out.scales.mutable_data_ptr<float>(), stream_of(x)),
+       "activations");
+  return out;
+}
+
+Tensor decode_rows(const Tensor& codes, const Tensor& scales, at::ScalarType type) {
+  const c10::DeviceGuard guard(codes.device());
+  const int64_t N = codes.size(0), C = codes.size(1);
+  Tensor out = at::empty({N, C}, codes.options().dtype(type));
+  done(ictc_codes_decode(dtype_of(out), codes.const_data_ptr<int8_t>(), scales.const_data_ptr<float>(), N, (int)C,
+                         ptr(out), stream_of(codes)),
+       "activations");
+  return out;
+}
+
+// Where a graph goes on from rows that are kept in 8 bits: a tensor of their shape without their memory, whose gradient
+// is theirs.  A node keeps it beside the codes, and a backward pass that will be differentiated takes the values as a
+// function of it (Decoded).
+struct Place8 : Function<Place8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x) {
+    ctx->set_materialize_grads(false);
+    return at::empty({1}, x.options()).expand(x.sizes());
+  }
+  static variable_list backward(AutogradContext*, variable_list grads) { return {grads[0]}; }
+};
+
+struct Decoded : Function<Decoded> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& place, const Tensor& codes, const Tensor& scales) {
+    ctx->set_materialize_grads(false);
+    return decode_rows(codes, scales, place.scalar_type());
+  }
+  static variable_list backward(AutogradContext*, variable_list grads) { return {grads[0], Tensor(), Tensor()}; }
+};
+
+// save_bits of an operator: whether its rows are kept in 8 bits.
+bool in_8_bits(const std::optional<int64_t>& save_bits, const char* op) {
+  TORCH_CHECK_VALUE(!save_bits.has_value() || *save_bits == 8, op, ": save_bits must be 8 or None");
+  return save_bits.has_value();
+}
+
 }  // namespace

@@ -20,6 +20,7 @@ __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
     "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order", "embedding",
+    "encode_activations", "decode_activations",
 ]
 
 
@@ -384,17 +385,19 @@ def expert_order(ids, experts):
     return ExpertOrder(ids, experts)
 
 
-def expert_linear(x, weight, order, bias=None):
+def expert_linear(x, weight, order, bias=None, save_bits=None):
     """y[n] = weight[id n] x[n] + bias[id n] for rows x [N, inputs] in the caller's order, weight [experts, outputs,
     inputs], bias [experts, outputs] or None, order from ``expert_order``; float32, bfloat16 or float16 throughout.
 
     Sums are FP32 (FP32 operands keep FP32 accuracy, those under 2^-110, 8e-34, to 2^-134; a row with infinities, or
     FP32 values above 3.38e38, may give NaN) and each result is rounded once.  A row of no expert gives a zero row and adds to no gradient; an expert
     without rows has zero gradients.
-    Differentiable to any order in x, weight and bias; every sum has a fixed order."""
+    Differentiable to any order in x, weight and bias; every sum has a fixed order.
+    With save_bits=8 the backward pass keeps x in 8 bits (``encode_activations``; whole where weight takes no gradient)
+    and the weight's gradient is made of the decoded rows; the result and x's gradient stay as they are."""
     if not isinstance(order, ExpertOrder):
         raise TypeError("expert_linear: order must come from expert_order")
-    return nat.ops().expert_linear(x, weight, bias, order.perm, order.offsets, order.rows)
+    return nat.ops().expert_linear(x, weight, bias, order.perm, order.offsets, order.rows, save_bits)
 
 
 def embedding(table, ids, scale=1.0, order=None):
@@ -411,3 +414,18 @@ def embedding(table, ids, scale=1.0, order=None):
     if ids.numel() != order.rows:
         raise ValueError("embedding: the order is of other ids")
     return nat.ops().embedding(table, ids, scale, order.perm, order.offsets)
+
+
+def encode_activations(x):
+    """x [..., C] (float32, bfloat16 or float16) in 8 bits: (codes int8 [..., C], scales float32 [..., ceil(C / 128)]), as
+    a function of a caller's own keeps what its backward pass needs.
+
+    Blocks of 128 elements along the last axis (the last of a row: what is left) share a scale, their largest magnitude
+    (at least 2^-100) / 127; a code is the nearest whole number of scales.  Values are off by half a scale at most,
+    1/254 of the block's largest magnitude.  A block that holds an infinity or NaN decodes to NaN.  No gradient passes."""
+    return nat.ops().encode_activations(x)
+
+
+def decode_activations(codes, scales, *, dtype=torch.float32):
+    """The values of ``encode_activations``' codes, each code times its scale in FP32, rounded to `dtype` once."""
+    return nat.ops().decode_activations(codes, scales, dtype)

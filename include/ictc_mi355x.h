@@ -799,6 +799,18 @@ int ictc_embedding_bwd(int dtype, const void* grad, int64_t ldg, int64_t rows, i
                        int64_t entries, const int32_t* perm, const int32_t* offsets, float scale, void* dtable,
                        void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Activations in 8 bits -------------------------------------------------
+ * x [rows, width] at pitch ldx, element type dtype, to packed codes [rows, width] and FP32
+ * scales [rows, ceil(width / 128)], one for each 128 consecutive elements of a row (the
+ * last: what is left), and back to packed values of type dtype:
+ *   scale = max(max |x|, 2^-100) / 127 (times 1/127 in FP32), code = x (1 / scale) rounded
+ *   to nearest even and held to [-127, 127], value = code scale rounded to dtype.
+ * A block with an infinity or NaN has the scale NaN and so all of its values.           */
+int ictc_codes_encode(int dtype, const void* x, int64_t ldx, int64_t rows, int width, int8_t* codes, float* scales,
+                      void* stream);
+int ictc_codes_decode(int dtype, const int8_t* codes, const float* scales, int64_t rows, int width, void* out,
+                      void* stream);
+
 /* ---- AdamW over a list of tensors ------------------------------------------
  * One step with decoupled weight decay, in FP32 arithmetic:
  *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
