@@ -135,6 +135,11 @@ _SIGNATURES = {
     "ictc_expert_linear": (_i, [_i, _p, _i64, _i64, _i, _p, _p, _i, _i, _p, _p, _i, _p, _p]),
     "ictc_expert_outer_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i]),
     "ictc_expert_outer": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _p, _p, _i64, _p]),
+    "ictc_group_norm_workspace_bytes": (_i64, [_i, _i, _i64, _i64, _i, _i]),
+    "ictc_group_norm_fwd": (_i, [_i, _p, _i64, _i64, _i, _i, _p, _p, ctypes.c_float, _i, _p, _p, _p, _p, _i64, _p]),
+    "ictc_group_norm_bwd": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "ictc_group_norm_bwd2": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p,
+                                  _p, _i64, _p]),
     "ictc_embedding_fwd": (_i, [_i, _p, _i64, _i, _p, _i64, ctypes.c_float, _p, _p]),
     "ictc_embedding_needs_order": (_i, [_i64]),
     "ictc_embedding_bwd_workspace_bytes": (_i64, [_i, _i64, _i64, _i]),

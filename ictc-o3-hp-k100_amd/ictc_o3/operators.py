@@ -20,7 +20,7 @@ __all__ = [
     "EdgeTensorProduct", "GraphMessage", "PackedGraphMessage", "direction_harmonics",
     "create_symmetric_contraction", "configure_symmetric_contraction",
     "channel_linear", "normalized_silu", "layer_norm", "expert_linear", "expert_order", "embedding",
-    "encode_activations", "decode_activations",
+    "group_norm", "encode_activations", "decode_activations",
 ]
 
 
@@ -429,3 +429,16 @@ def encode_activations(x):
 def decode_activations(codes, scales, *, dtype=torch.float32):
     """The values of ``encode_activations``' codes, each code times its scale in FP32, rounded to `dtype` once."""
     return nat.ops().decode_activations(codes, scales, dtype)
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, save_bits=None):
+    """act((x - mean) / sqrt(var + eps) * weight + bias) for x [samples, ..., channels], channels last: mean and var over
+    all positions of a sample (the axes between; none: a row is a sample) and the channels of a group, of which there are
+    `groups`, alike and consecutive.  activation None, or "silu": z / (1 + exp(-z)).
+
+    x is float32, bfloat16 or float16, weight and bias [channels] of the same type (None: ones / zeros).  Statistics and
+    sums are FP32 or better and each result is rounded once.  Gradients of x, weight and bias, and once more of those (a
+    loss on forces), run on kernels; a third derivative raises.  A sample's group that holds NaN or infinity gives NaN.
+    With save_bits=8 the backward pass keeps x in 8 bits (``encode_activations``, by position) and takes the decoded x in
+    its formulas, with the mean and deviation of x itself; the result stays as it is."""
+    return nat.ops().group_norm(x, groups, weight, bias, eps, activation, save_bits)

@@ -782,6 +782,36 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
                       int outputs, int experts, const int32_t* perm, const int32_t* offsets, void* dweight,
                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Group norm with an activation, channels last ---------------------------
+ * y = act((x - mean) rstd weight + bias) for x [samples, positions, channels], packed,
+ * element type dtype (x, weight, bias, grad and all results alike); mean and rstd are over
+ * all positions and the channels / groups channels of a sample's group; activation 0: none,
+ * 1: z / (1 + exp(-z)).  Statistics and sums in FP32 or FP64, each result rounded once.
+ * weight / bias NULL: ones / zeros.  mean and rstd [samples, groups] FP32 may both be NULL
+ * in fwd.
+ *   bwd:  dx, dweight [channels], dbias [channels], each NULL to skip; no elements give zero
+ *         dweight and dbias.  With codes and scales (ictc_codes_encode of x as rows of
+ *         `channels`) x is not read: h = (value - mean) rstd stands for the normalised x.
+ *   bwd2: the gradients of <v, dx> + <vweight, dweight> + <vbias, dbias> by x (dx), by grad
+ *         (dgrad), by weight and by bias (zero without an activation); vweight / vbias NULL:
+ *         absent.
+ * Sums over samples have a fixed order.  Workspace of ictc_group_norm_workspace_bytes bytes
+ * (pass 0: fwd, 1: bwd, 2: bwd2), 8-byte aligned (0: none needed, -1: out of range).     */
+int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, int64_t positions, int channels,
+                                        int groups);
+int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
+                        const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
+                        float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                        int64_t samples, int64_t positions, int channels, int groups, const void* weight,
+                        const void* bias, int activation, const float* mean, const float* rstd, void* dx, void* dweight,
+                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                         const void* v, const void* vweight, const void* vbias, int64_t samples, int64_t positions,
+                         int channels, int groups, const void* weight, const void* bias, int activation,
+                         const float* mean, const float* rstd, void* dx, void* dgrad, void* dweight, void* dbias,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Rows of a table chosen by an id ---------------------------------------
  * out[n] = scale table[ids[n]] with table [entries, width] and out [rows, width] packed,
  * element type dtype; an id outside [0, entries) gives a zero row.  bwd: dtable[v] = scale
