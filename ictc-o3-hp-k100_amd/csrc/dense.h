@@ -76,6 +76,51 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const floa
   }
 }
 
+// EV elements, 2 to 16 bytes, at any element's address.
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<16> { typedef u32x4 type; typedef u32x4_any any; };
+template <>
+struct RawOf<8> { typedef u32x2 type; typedef u32x2_any any; };
+typedef uint32_t u32_any __attribute__((aligned(2)));
+template <>
+struct RawOf<4> { typedef uint32_t type; typedef u32_any any; };
+template <>
+struct RawOf<2> { typedef uint16_t type; typedef uint16_t any; };
+
+template <typename T, int EV>
+union Pack {
+  typename RawOf<EV * (int)sizeof(T)>::type raw;
+  T e[EV];
+  __device__ Pack() {}
+};
+
+template <typename T, int EV>
+__device__ __forceinline__ Pack<T, EV> load_pack(const T* __restrict__ p, bool ok) {
+  Pack<T, EV> c;
+  if (ok) {
+    c.raw = *reinterpret_cast<const typename RawOf<EV * (int)sizeof(T)>::any*>(p);
+  } else {
+    c.raw = {};
+  }
+  return c;
+}
+
+template <typename T, int EV>
+__device__ __forceinline__ void get(const Pack<T, EV>& c, float (&v)[EV]) {
+#pragma unroll
+  for (int e = 0; e < EV; ++e) v[e] = (float)c.e[e];
+}
+
+template <typename T, int EV>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&v)[EV]) {
+  Pack<T, EV> c;
+#pragma unroll
+  for (int e = 0; e < EV; ++e) c.e[e] = (T)v[e];
+  *reinterpret_cast<typename RawOf<EV * (int)sizeof(T)>::any*>(p) = c.raw;
+}
+
 // x, rounded to FP32 here: what it is computed by is not joined with a conversion that follows (a product to FP16 is
 // otherwise one instruction that rounds once, and differs from the FP32 product rounded in one case of some thousand).
 __device__ __forceinline__ float held(float x) {

@@ -18,63 +18,73 @@ namespace {
 
 constexpr int kMaxWidth = 65536, kUnroll = 4, kFewRows = 128, kMaxBlocks = 1 << 20;
 
-// Lanes of a row's chunks: the power of two that covers the width, at most a wave.
+// Lanes of a row's chunks (16 bytes; of narrower rows single elements): the power of two that covers the width, at most a
+// wave.
+int chunk_of(int64_t width, int chunk) { return width < chunk ? 1 : chunk; }
+
 int team_of(int64_t width, int chunk) {
   int lanes = 1;
   while (lanes < 64 && (int64_t)lanes * chunk < width) lanes *= 2;
   return lanes;
 }
 
-template <typename T, int L>
+// First column of a lane's chunk: a row's last chunk is read back from its end, so that none is in part.  Two lanes then
+// have some columns alike, and write the same there.  (60,013 rows of 1,021 FP16: lookup 61 -> 50 us, gradient 85 -> 65.)
+template <int V>
+__device__ __forceinline__ int column_of(int c, int width) {
+  return min(c, width - V);
+}
+
+template <typename T, int V, int L>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t entries, int width,
                                                         const int64_t* __restrict__ ids, int64_t rows, float scale,
                                                         T* __restrict__ out) {
-  constexpr int V = kChunk<T>, TEAMS = 256 / L;
-  const int c = (blockIdx.y * L + threadIdx.x % L) * V;
-  if (c >= width) return;
+  constexpr int TEAMS = 256 / L;
+  const int c0 = (blockIdx.y * L + threadIdx.x % L) * V, c = column_of<V>(c0, width);
+  if (c0 >= width) return;
   for (int64_t first = ((int64_t)blockIdx.x * TEAMS + threadIdx.x / L) * kUnroll; first < rows;
        first += (int64_t)gridDim.x * TEAMS * kUnroll) {
     int64_t id[kUnroll];
-    u32x4 raw[kUnroll];
+    Pack<T, V> raw[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) id[i] = first + i < rows ? ids[first + i] : -1;
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const bool in = (uint64_t)id[i] < (uint64_t)entries;
-      raw[i] = load_raw(table + (in ? id[i] * width + c : 0), in ? width - c : 0);
+      raw[i] = load_pack<T, V>(table + (in ? id[i] * width + c : 0), in);
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       if (first + i >= rows) break;
       const bool in = (uint64_t)id[i] < (uint64_t)entries;
       float v[V];
-      widen<T>(raw[i], v);
+      get<T, V>(raw[i], v);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = in ? held(v[e] * scale) : 0.f;
-      store_chunk(out + (first + i) * width + c, width - c, v);
+      store_pack<T, V>(out + (first + i) * width + c, v);
     }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void write_scaled(T* __restrict__ p, int n, const float* acc, float scale) {
-  float v[kChunk<T>];
+template <typename T, int V>
+__device__ __forceinline__ void write_scaled(T* __restrict__ p, const float (&acc)[V], float scale) {
+  float v[V];
 #pragma unroll
-  for (int e = 0; e < kChunk<T>; ++e) v[e] = held(acc[e] * scale);
-  store_chunk(p, n, v);
+  for (int e = 0; e < V; ++e) v[e] = held(acc[e] * scale);
+  store_pack<T, V>(p, v);
 }
 
 // Few rows: a team per entry adds the rows whose id is its own, in their order.
-template <typename T, int L>
+template <typename T, int V, int L>
 __global__ __launch_bounds__(256) void embed_few_kernel(const T* __restrict__ g, int64_t ldg, int rows, int width,
                                                         const int64_t* __restrict__ ids, int64_t entries, float scale,
                                                         T* __restrict__ out) {
-  constexpr int V = kChunk<T>, TEAMS = 256 / L;
+  constexpr int TEAMS = 256 / L;
   __shared__ int64_t id[kFewRows];
   if ((int)threadIdx.x < rows) id[threadIdx.x] = ids[threadIdx.x];
   __syncthreads();
-  const int c = (blockIdx.y * L + threadIdx.x % L) * V;
-  if (c >= width) return;
+  const int c0 = (blockIdx.y * L + threadIdx.x % L) * V, c = column_of<V>(c0, width);
+  if (c0 >= width) return;
   for (int64_t v = (int64_t)blockIdx.x * TEAMS + threadIdx.x / L; v < entries; v += (int64_t)gridDim.x * TEAMS) {
     float acc[V] = {};
     for (int r = 0; r < rows;) {
@@ -88,148 +98,181 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const T* __restrict__ g,
         ++r;
         ++n;
       }
-      u32x4 raw[kUnroll];
+      Pack<T, V> raw[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) raw[i] = load_raw(g + (i < n ? row[i] * ldg + c : 0), i < n ? width - c : 0);
+      for (int i = 0; i < kUnroll; ++i) raw[i] = load_pack<T, V>(g + (i < n ? row[i] * ldg + c : 0), i < n);
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
         float x[V];
-        widen<T>(raw[i], x);
+        get<T, V>(raw[i], x);
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] += x[e];
       }
     }
-    write_scaled(out + v * width + c, width - c, acc, scale);
+    write_scaled<T, V>(out + v * width + c, acc, scale);
   }
 }
 
-// part [ranges][2][width]; a block takes `per` sorted rows a team.
-template <typename T, int L>
+// part [ranges][2][width]; a block takes `per` sorted rows a team.  open [ranges]: the id of the run that begins in the
+// range and goes on behind it, or -1.
+template <typename T, int V, int L>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g, int64_t ldg, int width,
                                                          const int64_t* __restrict__ ids, int64_t entries,
                                                          const int* __restrict__ perm, const int* __restrict__ off,
-                                                         float scale, int per, float* __restrict__ part,
-                                                         T* __restrict__ out) {
-  constexpr int V = kChunk<T>, TEAMS = 256 / L, W = L * V;
-  __shared__ float sums[2][TEAMS][W];     // of each team's first run, and of its last where that is another
-  __shared__ int64_t keys[2][TEAMS];
+                                                         float scale, int per, int ranges, float* __restrict__ part,
+                                                         int* __restrict__ open, T* __restrict__ out) {
+  constexpr int TEAMS = 256 / L, W = L * V, AHEAD = 8;
+  extern __shared__ int staged[];         // the range's row numbers, and their ids
+  __shared__ float sums[2][TEAMS][V + W];   // of each team's first run, and of its last where that is another (V: see column_of)
+  __shared__ int keys[2][TEAMS];
   const int lane = threadIdx.x % L, team = threadIdx.x / L;
-  const int c0 = blockIdx.y * W, c = c0 + lane * V, left = width - c;
+  const int c0 = blockIdx.y * W, c = column_of<V>(c0 + lane * V, width);
+  const bool live = c0 + lane * V < width;
+  const int at_lds = V + c - c0;
+  const int64_t n = off[entries], start = (int64_t)blockIdx.x * TEAMS * per;   // (ids outside the table come last)
+  const int count = (int)max<int64_t>(0, min(n - start, (int64_t)TEAMS * per));
+  int *row = staged, *id = staged + TEAMS * per;
+  for (int k = threadIdx.x; k < count; k += 256) {
+    row[k] = perm[start + k];
+    id[k] = (int)ids[row[k]];
+  }
   const float zero[V] = {};
   for (int64_t e = (int64_t)blockIdx.x * TEAMS + team; e < entries; e += (int64_t)gridDim.x * TEAMS)
-    if (off[e] == off[e + 1]) store_chunk(out + e * width + c, left, zero);
-  const int64_t n = off[entries], start = (int64_t)blockIdx.x * TEAMS * per;   // (ids outside the table come last)
-  if (start >= n) return;
-  const int64_t end = min(n, start + (int64_t)TEAMS * per);
-  const int64_t p1 = min(end, start + (int64_t)(team + 1) * per);
-  auto write = [&](int64_t key, const float* acc) {
-    if ((uint64_t)key < (uint64_t)entries) write_scaled(out + key * width + c, left, acc, scale);
+    if (live && off[e] == off[e + 1]) store_pack<T, V>(out + e * width + c, zero);
+  if (open && blockIdx.y == 0 && threadIdx.x == 0 && (int)blockIdx.x < ranges) open[blockIdx.x] = -1;
+  if (count == 0) return;
+  __syncthreads();
+  auto write = [&](int key, const float (&acc)[V]) {
+    if (live && key >= 0 && key < entries) write_scaled<T, V>(out + (int64_t)key * width + c, acc, scale);
   };
   float acc[V] = {};
-  int64_t key = -1;
+  int key = -1;
   bool first = true;
-  for (int64_t p = start + (int64_t)team * per; p < p1; p += kUnroll) {
-    int64_t row[kUnroll], id[kUnroll];
-    u32x4 raw[kUnroll];
+  const int end = min(count, (team + 1) * per);
+  for (int p = team * per; p < end; p += AHEAD) {
+    Pack<T, V> raw[AHEAD];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) row[i] = p + i < p1 ? perm[p + i] : -1;
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      id[i] = row[i] >= 0 ? ids[row[i]] : -1;
-      raw[i] = load_raw(g + (row[i] >= 0 ? row[i] * ldg + c : 0), row[i] >= 0 ? left : 0);
+    for (int i = 0; i < AHEAD; ++i) {
+      const bool in = live && p + i < end;
+      raw[i] = load_pack<T, V>(g + (in ? row[p + i] * ldg + c : 0), in);
     }
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (p + i >= p1) break;
-      if (key != id[i]) {
+    for (int i = 0; i < AHEAD; ++i) {
+      if (p + i >= end) break;
+      const int k = id[p + i];
+      if (key != k) {
         if (key >= 0) {
           if (first) {
+            if (live) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) sums[0][team][lane * V + e] = acc[e];
+              for (int e = 0; e < V; ++e) sums[0][team][at_lds + e] = acc[e];
+            }
             if (lane == 0) keys[0][team] = key;
             first = false;
           } else {
             write(key, acc);
           }
         }
-        key = id[i];
+        key = k;
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.f;
       }
       float x[V];
-      widen<T>(raw[i], x);
+      get<T, V>(raw[i], x);
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += x[e];
     }
   }
+  if (live) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) sums[first ? 0 : 1][team][lane * V + e] = acc[e];
+    for (int e = 0; e < V; ++e) sums[first ? 0 : 1][team][at_lds + e] = acc[e];
+  }
   if (lane == 0) {
     keys[first ? 0 : 1][team] = key;
     if (first) keys[1][team] = -1;
   }
   __syncthreads();
-  // the block's open runs: a column a thread, the teams in order
-  const int64_t before = start > 0 ? ids[perm[start - 1]] : -1, after = end < n ? ids[perm[end]] : -1;
-  for (int col = threadIdx.x; col < W && c0 + col < width; col += 256) {
-    float a = 0.f;
-    int64_t at = keys[0][0];
-    bool begins = at != before;    // the present run begins in this block
-    auto flush = [&](bool ends) {
-      if (at < 0 || at >= entries) return;
-      if (begins && ends)
-        out[at * width + c0 + col] = (T)held(a * scale);
-      else
-        part[((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * width + c0 + col] = a;
-    };
-#pragma unroll 4
-    for (int t = 0; t < TEAMS; ++t) {
+  // The runs that meet other teams', each by the team that it begins in (or the first): its last run takes the first runs of
+  // the teams behind it, in order, as long as they are of its id.
+  if (!live || keys[0][team] < 0) return;
+  const int64_t last = start + count;
+  const int before = start > 0 ? (int)ids[perm[start - 1]] : -1, after = last < n ? (int)ids[perm[last]] : -1;
+  const int k0 = keys[0][team], k1 = keys[1][team];
+  const int previous = team == 0 ? before : keys[1][team - 1] >= 0 ? keys[1][team - 1] : keys[0][team - 1];
+  auto own = [&](int which) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t k = keys[s][t];
-        if (k < 0) continue;
-        const float x = sums[s][t][col];
-        if (k != at) {
-          flush(true);
-          at = k;
-          begins = true;
-          a = x;
-        } else {
-          a += x;
-        }
-      }
+    for (int e = 0; e < V; ++e) acc[e] = sums[which][team][at_lds + e];
+  };
+  auto keep = [&](int slot) {
+    if (!part) return;
+    float* p = part + ((int64_t)blockIdx.x * 2 + slot) * width + c;
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = acc[e];
+  };
+  if (k1 >= 0) {
+    own(0);
+    if (k0 != previous)
+      write(k0, acc);
+    else if (team == 0)
+      keep(0);
+  }
+  const int key_last = k1 >= 0 ? k1 : k0;
+  const bool begins = k1 >= 0 || k0 != previous;
+  if (!begins && team > 0) return;
+  own(k1 >= 0 ? 1 : 0);
+  bool goes_on = true;   // to the end of the block
+  for (int t = team + 1; t < TEAMS && keys[0][t] >= 0; ++t) {
+    if (keys[0][t] != key_last) {
+      goes_on = false;
+      break;
     }
-    flush(at != after);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += sums[0][t][at_lds + e];
+    if (keys[1][t] >= 0) {
+      goes_on = false;
+      break;
+    }
+  }
+  if (!begins) {
+    keep(0);
+  } else if (goes_on && key_last == after) {
+    keep(1);
+    if (open && c == 0) open[blockIdx.x] = key_last < entries ? key_last : -1;
+  } else {
+    write(key_last, acc);
   }
 }
 
-// The runs that cross ranges, each by the block of the first boundary that it crosses: its partial sums added by 32
-// slices and those in order.
+// The runs that cross ranges, each by the blocks of the range that it begins in, 64 columns a block: its partial sums added
+// by 16 slices and those in order.
 template <typename T>
-__global__ __launch_bounds__(512) void embed_join_kernel(const float* __restrict__ part, int width,
-                                                         const int64_t* __restrict__ ids, int64_t entries,
-                                                         const int* __restrict__ perm, const int* __restrict__ off,
-                                                         float scale, int64_t range, T* __restrict__ out) {
-  __shared__ float lds[32][17];
-  const int64_t q = blockIdx.x, p = (q + 1) * range;
-  if (p >= off[entries]) return;
-  const int64_t key = ids[perm[p]];
-  if (ids[perm[p - 1]] != key || (uint64_t)key >= (uint64_t)entries || off[key] / range != q) return;
+__global__ __launch_bounds__(256) void embed_join_kernel(const float* __restrict__ part, const int* __restrict__ open,
+                                                         int width, const int* __restrict__ off, float scale,
+                                                         int64_t range, T* __restrict__ out) {
+  __shared__ float lds[16][64];
+  const int64_t q = blockIdx.x;
+  const int key = open[q];
+  if (key < 0) return;
   const int64_t count = (off[key + 1] - 1) / range - q + 1;
-  const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
-  const int c = blockIdx.y * 16 + col;
-  float a = 0.f;
-  if (c < width) {
-#pragma unroll 4
-    for (int64_t j = slice; j < count; j += 32) a += part[((q + j) * 2 + (j == 0 ? 1 : 0)) * width + c];
+  const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int c = blockIdx.y * 64 + lane * 4, left = width - c;
+  float a[4] = {};
+#pragma unroll 8
+  for (int64_t j = slice; j < count; j += 16) {
+    float x[4];
+    load_chunk<float>(part + ((q + j) * 2 + (j == 0 ? 1 : 0)) * width + c, left, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += x[e];
   }
-  lds[slice][col] = a;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lds[slice][lane * 4 + e] = a[e];
   __syncthreads();
-  if (slice == 0 && c < width) {
+  const int col = threadIdx.x;
+  if (col < 64 && blockIdx.y * 64 + col < width) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) s += lds[i][col];
-    out[key * width + c] = (T)held(s * scale);
+    for (int i = 0; i < 16; ++i) s += lds[i][col];
+    out[(int64_t)key * width + blockIdx.y * 64 + col] = (T)held(s * scale);
   }
 }
 
@@ -241,14 +284,14 @@ struct GradPlan {
 };
 
 GradPlan grad_plan(int dtype, int64_t rows, int64_t entries, int64_t width) {
-  const int chunk = dtype == ICTC_F32 ? 4 : 8;
+  const int chunk = chunk_of(width, dtype == ICTC_F32 ? 4 : 8);
   GradPlan p;
-  p.lanes = team_of(width, chunk);
+  // eight lanes at least, some idle, so that a block has few teams whose runs meet (60,013 rows of one element 45 -> GRAD1 us)
+  p.lanes = std::max(8, team_of(width, chunk));
   p.columns = (int)((width + p.lanes * chunk - 1) / (p.lanes * chunk));
   const int64_t teams = 256 / p.lanes;
   const int64_t want = (rows * p.columns + teams * 2048 - 1) / (teams * 2048);
-  const int64_t most = std::max<int64_t>(32, rows / (teams << 20) + 1);   // (no more than about a million ranges)
-  p.per = (int)((std::min(most, std::max<int64_t>(4, want)) + kUnroll - 1) / kUnroll * kUnroll);
+  p.per = (int)((std::min<int64_t>(32, std::max<int64_t>(4, want)) + 3) / 4 * 4);
   p.range = teams * p.per;
   p.ranges = (rows + p.range - 1) / p.range;
   p.blocks = std::max<int64_t>(std::max<int64_t>(1, p.ranges), std::min<int64_t>(2048, (entries + teams - 1) / teams));
@@ -263,30 +306,52 @@ const char* bad_sizes(int dtype, int64_t rows, int64_t entries, int64_t width) {
   return nullptr;
 }
 
-#define EMBED_CASE(L_, ...)      \
-  case L_: {                     \
-    constexpr int L = L_;        \
-    __VA_ARGS__;                 \
-    break;                       \
+#define EMBED_CASE(V_, L_, ...)           \
+  case L_: {                              \
+    constexpr int V = V_, L = L_;         \
+    __VA_ARGS__;                          \
+    break;                                \
   }
-#define EMBED_LANES(n, ...)                                                                                  \
-  switch (n) {                                                                                               \
-    EMBED_CASE(1, __VA_ARGS__)                                                                               \
-    EMBED_CASE(2, __VA_ARGS__)                                                                               \
-    EMBED_CASE(4, __VA_ARGS__)                                                                               \
-    EMBED_CASE(8, __VA_ARGS__)                                                                               \
-    EMBED_CASE(16, __VA_ARGS__)                                                                              \
-    EMBED_CASE(32, __VA_ARGS__)                                                                              \
-    EMBED_CASE(64, __VA_ARGS__)                                                                              \
+#define EMBED_LANES(width, n, ...)            \
+  if ((width) < kChunk<T>) {                  \
+    switch (n) {                              \
+      EMBED_CASE(1, 1, __VA_ARGS__)           \
+      EMBED_CASE(1, 2, __VA_ARGS__)           \
+      EMBED_CASE(1, 4, __VA_ARGS__)           \
+      EMBED_CASE(1, 8, __VA_ARGS__)           \
+    }                                         \
+  } else {                                    \
+    switch (n) {                              \
+      EMBED_CASE(kChunk<T>, 1, __VA_ARGS__)   \
+      EMBED_CASE(kChunk<T>, 2, __VA_ARGS__)   \
+      EMBED_CASE(kChunk<T>, 4, __VA_ARGS__)   \
+      EMBED_CASE(kChunk<T>, 8, __VA_ARGS__)   \
+      EMBED_CASE(kChunk<T>, 16, __VA_ARGS__)  \
+      EMBED_CASE(kChunk<T>, 32, __VA_ARGS__)  \
+      EMBED_CASE(kChunk<T>, 64, __VA_ARGS__)  \
+    }                                         \
+  }
+#define EMBED_TEAMS(width, n, ...)            \
+  if ((width) < kChunk<T>) {                  \
+    constexpr int V = 1, L = 8;               \
+    __VA_ARGS__;                              \
+  } else {                                    \
+    switch (n) {                              \
+      EMBED_CASE(kChunk<T>, 8, __VA_ARGS__)   \
+      EMBED_CASE(kChunk<T>, 16, __VA_ARGS__)  \
+      EMBED_CASE(kChunk<T>, 32, __VA_ARGS__)  \
+      EMBED_CASE(kChunk<T>, 64, __VA_ARGS__)  \
+    }                                         \
   }
 
 template <typename T>
 void run_fwd(const void* table, int64_t entries, int width, const int64_t* ids, int64_t rows, float scale, void* out,
              hipStream_t st) {
-  const int lanes = team_of(width, kChunk<T>), columns = (width + lanes * kChunk<T> - 1) / (lanes * kChunk<T>);
+  const int chunk = chunk_of(width, kChunk<T>), lanes = team_of(width, chunk);
+  const int columns = (width + lanes * chunk - 1) / (lanes * chunk);
   const int64_t block = 256 / lanes * kUnroll;
   const dim3 grid((unsigned)std::min<int64_t>(kMaxBlocks, (rows + block - 1) / block), columns);
-  EMBED_LANES(lanes, hipLaunchKernelGGL((embed_fwd_kernel<T, L>), grid, dim3(256), 0, st, (const T*)table, entries,
+  EMBED_LANES(width, lanes, hipLaunchKernelGGL((embed_fwd_kernel<T, V, L>), grid, dim3(256), 0, st, (const T*)table, entries,
                                         width, ids, rows, scale, (T*)out))
 }
 
@@ -298,16 +363,18 @@ void run_bwd(const void* g, int64_t ldg, int64_t rows, int width, int64_t entrie
   if (rows <= kFewRows) {
     const int64_t teams = 256 / p.lanes;
     const dim3 grid((unsigned)std::min<int64_t>(kMaxBlocks, (entries + teams - 1) / teams), p.columns);
-    EMBED_LANES(p.lanes, hipLaunchKernelGGL((embed_few_kernel<T, L>), grid, dim3(256), 0, st, (const T*)g, ldg,
+    EMBED_TEAMS(width, p.lanes, hipLaunchKernelGGL((embed_few_kernel<T, V, L>), grid, dim3(256), 0, st, (const T*)g, ldg,
                                             (int)rows, width, ids, entries, scale, (T*)out))
     return;
   }
   const dim3 grid((unsigned)p.blocks, p.columns);
-  EMBED_LANES(p.lanes, hipLaunchKernelGGL((embed_grad_kernel<T, L>), grid, dim3(256), 0, st, (const T*)g, ldg, width,
-                                          ids, entries, perm, off, scale, p.per, part, (T*)out))
-  if (p.ranges > 1)
-    hipLaunchKernelGGL(embed_join_kernel<T>, dim3((unsigned)(p.ranges - 1), (unsigned)((width + 15) / 16)), dim3(512), 0,
-                       st, part, width, ids, entries, perm, off, scale, p.range, (T*)out);
+  int* open = p.ranges > 1 ? (int*)(part + p.ranges * 2 * width) : nullptr;
+  EMBED_TEAMS(width, p.lanes, hipLaunchKernelGGL((embed_grad_kernel<T, V, L>), grid, dim3(256), (unsigned)(p.range * 8), st,
+                                          (const T*)g, ldg, width, ids, entries, perm, off, scale, p.per, (int)p.ranges,
+                                          open ? part : nullptr, open, (T*)out))
+  if (open)
+    hipLaunchKernelGGL(embed_join_kernel<T>, dim3((unsigned)(p.ranges - 1), (unsigned)((width + 63) / 64)), dim3(256), 0,
+                       st, part, open, width, off, scale, p.range, (T*)out);
 }
 
 }  // namespace
@@ -334,7 +401,7 @@ int ictc_embedding_needs_order(int64_t rows) { return rows > kFewRows; }
 int64_t ictc_embedding_bwd_workspace_bytes(int dtype, int64_t rows, int64_t entries, int width) {
   if (bad_sizes(dtype, rows, entries, width)) return -1;
   const GradPlan p = grad_plan(dtype, rows, entries, width);
-  return rows <= kFewRows || p.ranges < 2 ? 0 : p.ranges * 2 * width * (int64_t)sizeof(float);
+  return rows <= kFewRows || p.ranges < 2 ? 0 : p.ranges * (2 * width + 1) * (int64_t)sizeof(float);
 }
 
 int ictc_embedding_bwd(int dtype, const void* grad, int64_t ldg, int64_t rows, int width, const int64_t* ids,

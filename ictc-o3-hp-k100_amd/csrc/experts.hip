@@ -359,64 +359,98 @@ __global__ __launch_bounds__(kFewWaves * 64, 4) void experts_few_kernel(const T*
 // the expert, the lanes of it below and how many there are, is kept in one register, so the ids are read once, all of a
 // lane's at once.  One block does it alone; of several, each has `span` rows and adds up, from all blocks' counts
 // ([blocks, experts + 1], the kernel below), what lies before its own.
+//
+// More than 1,023 experts (entries of a table) are ordered by the low half of the id's bits and then, stably, by the high
+// one: the first pass leaves ids and row numbers, the second row numbers and sorted ids, of which order_offsets_kernel
+// makes the offsets (425,991 rows of 7,921 ids: 31 us, 125 by the general sort).
 constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16, kOrderBlocks = 256;
 constexpr int kOrderRows = kOrderWaves * kOrderAtOnce * 64;
 
-__global__ __launch_bounds__(1024) void experts_count_kernel(const int64_t* __restrict__ ids, int n, int experts,
-                                                             int span, int* __restrict__ counts) {
+// What a pass takes and leaves: row i's id, or of the second pass the key and number that the first left at i.
+enum class Pass { kOnly, kFirst, kSecond };
+struct OrderIn {
+  const int64_t* ids;
+  const int *keys, *rows;
+  int experts, shift, groups;   // digit: key >> shift & (groups - 1); of the only pass the key, groups = experts + 1
+};
+struct OrderOut {
+  int *perm, *keys, *off;
+};
+
+template <Pass P>
+__device__ __forceinline__ uint32_t order_key(const OrderIn& in, int row) {
+  if (P == Pass::kSecond) return in.keys[row];
+  const int64_t id = in.ids[row];
+  return (uint64_t)id < (uint64_t)in.experts ? (uint32_t)id : (uint32_t)in.experts;
+}
+
+template <Pass P>
+__device__ __forceinline__ uint32_t order_digit(const OrderIn& in, uint32_t key) {
+  return P == Pass::kOnly ? key : key >> in.shift & (uint32_t)(in.groups - 1);
+}
+
+template <Pass P>
+__global__ __launch_bounds__(1024) void experts_count_kernel(OrderIn in, int n, int span, int* __restrict__ counts) {
   __shared__ int count[kOrderExperts + 1];
-  if ((int)threadIdx.x <= experts) count[threadIdx.x] = 0;
+  if ((int)threadIdx.x < in.groups) count[threadIdx.x] = 0;
   __syncthreads();
   const int begin = blockIdx.x * span, end = min(n, begin + span);
   for (int r0 = begin + (int)threadIdx.x; r0 < end; r0 += 4096) {
-    int64_t id[4];
+    uint32_t key[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = r0 + i * 1024 < end ? ids[r0 + i * 1024] : -1;
+    for (int i = 0; i < 4; ++i) key[i] = r0 + i * 1024 < end ? order_key<P>(in, r0 + i * 1024) : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (r0 + i * 1024 < end) atomicAdd(&count[(uint64_t)id[i] < (uint64_t)experts ? (int)id[i] : experts], 1);
+      if (r0 + i * 1024 < end) atomicAdd(&count[order_digit<P>(in, key[i])], 1);
   }
   __syncthreads();
-  if ((int)threadIdx.x <= experts) counts[blockIdx.x * (experts + 1) + threadIdx.x] = count[threadIdx.x];
+  if ((int)threadIdx.x < in.groups) counts[blockIdx.x * in.groups + threadIdx.x] = count[threadIdx.x];
 }
 
-__global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __restrict__ ids, int n, int experts,
-                                                             int bits, int span, const int* __restrict__ counts,
-                                                             int* __restrict__ off, int* __restrict__ perm) {
+template <Pass P>
+__global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, int bits, int span,
+                                                             const int* __restrict__ counts, OrderOut out) {
   __shared__ int count[kOrderWaves][kOrderExperts + 1];
   __shared__ int wave_total[kOrderWaves];
-  const int lane = threadIdx.x & 63, groups = experts + 1, group = threadIdx.x;
+  const int lane = threadIdx.x & 63, groups = in.groups, group = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ int totals[kOrderExperts + 1], befores[kOrderExperts + 1];   // of each group: all rows, those of the blocks before
   for (int i = threadIdx.x; i < kOrderWaves * groups; i += 1024) count[i / groups][i % groups] = 0;
-  int total = 0, before = 0;   // of this group: all rows, and those of the blocks before
-  if (counts && group < groups) {
+  totals[threadIdx.x] = befores[threadIdx.x] = 0;
+  __syncthreads();
+  if (counts) {   // the threads left over share a group's blocks
+    const int width = 1 << bits, at = threadIdx.x & (width - 1);
+    int all = 0, earlier = 0;
+    if (at < groups) {
 #pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const int c = counts[b * groups + group];
-      total += c;
-      before += b < (int)blockIdx.x ? c : 0;
+      for (int b = threadIdx.x / width; b < (int)gridDim.x; b += 1024 / width) {
+        const int c = counts[b * groups + at];
+        all += c;
+        earlier += b < (int)blockIdx.x ? c : 0;
+      }
+      atomicAdd(&totals[at], all);
+      atomicAdd(&befores[at], earlier);
     }
   }
-  __syncthreads();
   const int first = blockIdx.x * span, rows = min(span, n - first);
   const int per = ((rows + kOrderWaves - 1) / kOrderWaves + 63) / 64 * 64;
   const int begin = first + wave * per, end = min(first + rows, begin + per);
   int* mine = count[wave];
-  uint32_t place[kOrderAtOnce];   // expert | lanes below << 10 | lanes << 16
-  int64_t id[kOrderAtOnce];
+  uint32_t place[kOrderAtOnce];   // digit | lanes below << 10 | lanes << 16
+  uint32_t key[kOrderAtOnce];
 #pragma unroll
   for (int i = 0; i < kOrderAtOnce; ++i) {
     const int row = begin + i * 64 + lane;
-    id[i] = row < end ? ids[row] : -1;
+    key[i] = row < end ? order_key<P>(in, row) : (uint32_t)in.experts;
   }
 #pragma unroll
   for (int i = 0; i < kOrderAtOnce; ++i) {
     const int r0 = begin + i * 64;
     if (r0 >= end) break;
-    const uint32_t key = (uint64_t)id[i] < (uint64_t)experts ? (uint32_t)id[i] : (uint32_t)experts;
-    const uint64_t in = __ballot(r0 + lane < end);
-    uint32_t lo = (uint32_t)in, hi = (uint32_t)(in >> 32);   // the lanes whose row has this lane's expert
-    int x = (int)(key << (32 - bits));
+    const uint32_t digit = order_digit<P>(in, key[i]);
+    const uint64_t here = __ballot(r0 + lane < end);
+    uint32_t lo = (uint32_t)here, hi = (uint32_t)(here >> 32);   // the lanes whose row has this lane's digit
+    int x = (int)(digit << (32 - bits));
     for (int b = 0; b < bits; ++b, x <<= 1) {
       const uint64_t set = __ballot(x < 0);
       lo &= ~((uint32_t)set ^ (uint32_t)(x >> 31));
@@ -424,11 +458,11 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
     }
     const uint64_t m = (uint64_t)hi << 32 | lo;
     const int below = __popcll(m & ((uint64_t(1) << lane) - 1)), lanes = __popcll(m);
-    place[i] = key | below << 10 | lanes << 16;
-    if (r0 + lane < end && below == 0) atomicAdd(&mine[key], lanes);
+    place[i] = digit | below << 10 | lanes << 16;
+    if (r0 + lane < end && below == 0) atomicAdd(&mine[digit], lanes);
   }
   __syncthreads();
-  int here = 0;
+  int here = 0, total = totals[group], before = befores[group];
   if (group < groups) {
 #pragma unroll
     for (int w = 0; w < kOrderWaves; ++w) {
@@ -444,8 +478,8 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
   for (int w = 0; w < wave; ++w) sum += wave_total[w];
   if (group < groups) {
     const int start = sum - total;
-    if (blockIdx.x == 0) off[group] = start;
-    if (blockIdx.x == 0 && group == experts) off[groups] = n;
+    if (P == Pass::kOnly && blockIdx.x == 0) out.off[group] = start;
+    if (P == Pass::kOnly && blockIdx.x == 0 && group == in.experts) out.off[groups] = n;
 #pragma unroll
     for (int w = 0; w < kOrderWaves; ++w) count[w][group] += start + before;
   }
@@ -454,12 +488,37 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(const int64_t* __re
   for (int i = 0; i < kOrderAtOnce; ++i) {
     const int r0 = begin + i * 64;
     if (r0 >= end) break;
-    const bool in = r0 + lane < end;
-    const int key = place[i] & 1023u, below = place[i] >> 10 & 63u, lanes = place[i] >> 16;
-    if (in) perm[mine[key] + below] = r0 + lane;
+    const bool ok = r0 + lane < end;
+    const int digit = place[i] & 1023u, below = place[i] >> 10 & 63u, lanes = place[i] >> 16;
+    if (ok) {
+      const int to = mine[digit] + below;
+      out.perm[to] = P == Pass::kSecond ? in.rows[r0 + lane] : r0 + lane;
+      if (P != Pass::kOnly) out.keys[to] = (int)key[i];
+    }
     wave_meet();
-    if (in && below == 0) atomicAdd(&mine[key], lanes);   // (before the next rows' reads: LDS keeps a wave's order)
+    if (ok && below == 0) atomicAdd(&mine[digit], lanes);   // (before the next rows' reads: LDS keeps a wave's order)
     wave_meet();
+  }
+}
+
+// off[k] = the first place of sorted keys [n] that holds k or more, for k of 0 .. experts + 1.  A place fills the offsets
+// from the key before it to its own; long gaps are shared by the wave.
+__global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restrict__ keys, int n, int experts,
+                                                            int* __restrict__ off) {
+  const int p = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63;
+  int from = 0, to = 0;   // offsets from .. to - 1 are p
+  if (p <= n) {
+    from = p > 0 ? keys[p - 1] + 1 : 0;
+    to = p < n ? keys[p] + 1 : experts + 2;
+  }
+  const bool wide = to - from > 8;
+  if (!wide)
+    for (int k = from; k < to; ++k) off[k] = p;
+  for (uint64_t m = __ballot(wide); m; m &= m - 1) {
+    const int l = __builtin_ctzll(m);
+    const int a = __builtin_amdgcn_readlane(from, l), b = __builtin_amdgcn_readlane(to, l),
+              q = __builtin_amdgcn_readlane(p, l);
+    for (int k = a + lane; k < b; k += 64) off[k] = q;
   }
 }
 
@@ -475,10 +534,67 @@ int id_bits(int experts) {
 // Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5, 16,384 12.9 / 9.0; 89 experts 6,000
 // rows 8.2 / 8.7, 16,384 16.4 / 10.1.  Several / the general sort, ten experts: 30,011 rows 8.8 / 10.8, 262,145 11.8 / 106,
 // 4.2 million 32 / 83.
-int order_span(int64_t rows, int experts) {
-  if (experts > kOrderExperts || rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
-  if (rows <= kOrderRows && rows * (3 + id_bits(experts)) <= 60000) return (int)std::max<int64_t>(rows, 1);
+int order_span(int64_t rows, int bits) {
+  if (rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
+  if (rows <= kOrderRows && rows * (3 + bits) <= 60000) return (int)std::max<int64_t>(rows, 1);
   return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(4096, (rows / 64 + 1023) / 1024 * 1024));
+}
+
+// The passes over the bits of an id: none (the general sort), one, or two.
+struct OrderPlan {
+  int passes, bits, low, span;   // of an id; of the first digit
+  int64_t blocks, counts;        // of each pass; ints of its counts
+};
+
+OrderPlan order_plan(int64_t rows, int64_t experts) {
+  OrderPlan p = {};
+  if (experts >= 1 << 20) return p;
+  p.bits = id_bits((int)experts);
+  p.passes = experts <= kOrderExperts ? 1 : 2;
+  p.low = p.passes == 1 ? p.bits : (p.bits + 1) / 2;
+  p.span = order_span(rows, p.low);
+  if (p.span == 0) return OrderPlan{};
+  p.blocks = std::max<int64_t>(1, tiles_of(rows, p.span));
+  const int64_t groups = p.passes == 1 ? experts + 1 : int64_t(1) << p.low;
+  p.counts = rows <= p.span ? 0 : p.blocks * groups;
+  return p;
+}
+
+int64_t order_bytes(int64_t rows, int64_t experts) {
+  const OrderPlan p = order_plan(rows, experts);
+  if (p.passes == 0) return ictc_csr_workspace_bytes(rows, experts);
+  return 4 * (p.counts + (p.passes == 2 ? 3 * rows : 0));
+}
+
+template <Pass P>
+void order_pass(const OrderIn& in, int n, int bits, const OrderPlan& p, int* counts, const OrderOut& out, hipStream_t st) {
+  if (counts)
+    hipLaunchKernelGGL(experts_count_kernel<P>, dim3((unsigned)p.blocks), dim3(1024), 0, st, in, n, p.span, counts);
+  hipLaunchKernelGGL(experts_order_kernel<P>, dim3((unsigned)p.blocks), dim3(1024), 0, st, in, n, bits, p.span, counts, out);
+}
+
+// The order of rows by id in [0, experts), those of no id last.
+int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int* off, void* workspace, int64_t bytes,
+               hipStream_t st) {
+  const OrderPlan p = order_plan(rows, experts);
+  if (p.passes == 0) return ictc_csr_build(ids, rows, experts, off, perm, workspace, bytes, st);
+  const int64_t need = order_bytes(rows, experts);
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || bytes < need))
+    return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: workspace smaller than ictc_expert_order_workspace_bytes");
+  const int n = (int)rows;
+  int* counts = p.counts ? (int*)workspace : nullptr;
+  OrderIn in = {ids, nullptr, nullptr, (int)experts, 0, (int)experts + 1};
+  if (p.passes == 1) {
+    order_pass<Pass::kOnly>(in, n, p.bits, p, counts, {perm, nullptr, off}, st);
+    return dense_status("expert_order launch");
+  }
+  int *keys = (int*)workspace + p.counts, *numbers = keys + rows, *sorted = numbers + rows;
+  in.groups = 1 << p.low;
+  order_pass<Pass::kFirst>(in, n, p.low, p, counts, {numbers, keys, nullptr}, st);
+  const OrderIn next = {nullptr, keys, numbers, (int)experts, p.low, 1 << (p.bits - p.low)};
+  order_pass<Pass::kSecond>(next, n, p.bits - p.low, p, counts, {perm, sorted, nullptr}, st);
+  hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, st, sorted, n, (int)experts, off);
+  return dense_status("expert_order launch");
 }
 
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
@@ -722,29 +838,27 @@ extern "C" {
 
 int64_t ictc_expert_order_workspace_bytes(int64_t rows, int experts) {
   if (bad_sizes(ICTC_F32, rows, 1, 1, experts)) return -1;
-  const int span = order_span(rows, experts);
-  if (span == 0) return ictc_csr_workspace_bytes(rows, experts);
-  return rows <= span ? 0 : tiles_of(rows, span) * (experts + 1) * (int64_t)sizeof(int);
+  return order_bytes(rows, experts);
 }
 
 int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* perm, int32_t* offsets, void* workspace,
                       int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(ICTC_F32, rows, 1, 1, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: null operand");
-  const int span = order_span(rows, experts);
-  if (span == 0) return ictc_csr_build(ids, rows, experts, offsets, perm, workspace, workspace_bytes, stream);
-  const bool several = rows > span;
-  if (several && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) ||
-                  workspace_bytes < ictc_expert_order_workspace_bytes(rows, experts)))
-    return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: workspace smaller than ictc_expert_order_workspace_bytes");
-  const dim3 blocks((unsigned)std::max<int64_t>(1, tiles_of(rows, span)));
-  int* counts = several ? (int*)workspace : nullptr;
-  hipStream_t st = (hipStream_t)stream;
-  if (several)
-    hipLaunchKernelGGL(experts_count_kernel, blocks, dim3(1024), 0, st, ids, (int)rows, experts, span, counts);
-  hipLaunchKernelGGL(experts_order_kernel, blocks, dim3(1024), 0, st, ids, (int)rows, experts, id_bits(experts), span,
-                     counts, offsets, perm);
-  return dense_status("expert_order launch");
+  return order_rows(ids, rows, experts, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int64_t ictc_rows_by_id_workspace_bytes(int64_t rows, int64_t entries) {
+  if (rows < 0 || entries < 1 || std::max(rows, entries) >= (int64_t(1) << 31) - 2) return -1;
+  return order_bytes(rows, entries);
+}
+
+int ictc_rows_by_id(const int64_t* ids, int64_t rows, int64_t entries, int32_t* perm, int32_t* offsets, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+  if (ictc_rows_by_id_workspace_bytes(rows, entries) < 0)
+    return dense_fail(ICTC_ERR_ARGUMENT, "rows_by_id: up to 2^31 - 3 rows and entries");
+  if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "rows_by_id: null operand");
+  return order_rows(ids, rows, entries, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int inputs, const void* weight,

@@ -102,17 +102,13 @@ std::vector<bool> wanted(AutogradContext* ctx, std::initializer_list<bool> prese
 
 // (rows in the order of their id, first sorted row of each id) of ids [N] in [0, keys); those outside come last.
 std::pair<Tensor, Tensor> rows_by_id(const Tensor& ids, int64_t keys) {
-  const int64_t N = ids.size(0);
-  const bool few = keys <= 65535;   // what ictc_expert_order takes
-  const int64_t bytes = few ? ictc_expert_order_workspace_bytes(N, (int)keys) : ictc_csr_workspace_bytes(N, keys);
+  const int64_t N = ids.size(0), bytes = ictc_rows_by_id_workspace_bytes(N, keys);
   const auto ints = ids.options().dtype(at::kInt);
   const Tensor perm = at::empty({std::max<int64_t>(N, 1)}, ints), offsets = at::empty({keys + 2}, ints);
   Tensor ws;
   if (bytes > 0) ws = at::empty({bytes}, ids.options().dtype(at::kByte));
-  int *p = perm.mutable_data_ptr<int>(), *o = offsets.mutable_data_ptr<int>();
-  const int64_t* at = ids.const_data_ptr<int64_t>();
-  done(few ? ictc_expert_order(at, N, (int)keys, p, o, ptr(ws), bytes, stream_of(ids))
-           : ictc_csr_build(at, N, keys, o, p, ptr(ws), bytes, stream_of(ids)),
+  done(ictc_rows_by_id(ids.const_data_ptr<int64_t>(), N, keys, perm.mutable_data_ptr<int>(),
+                       offsets.mutable_data_ptr<int>(), ptr(ws), bytes, stream_of(ids)),
        "expert_order");
   return {perm, offsets};
 }

@@ -140,6 +140,8 @@ _SIGNATURES = {
     "ictc_group_norm_bwd": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_group_norm_bwd2": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p,
                                   _p, _i64, _p]),
+    "ictc_rows_by_id_workspace_bytes": (_i64, [_i64, _i64]),
+    "ictc_rows_by_id": (_i, [_p, _i64, _i64, _p, _p, _p, _i64, _p]),
     "ictc_embedding_fwd": (_i, [_i, _p, _i64, _i, _p, _i64, ctypes.c_float, _p, _p]),
     "ictc_embedding_needs_order": (_i, [_i64]),
     "ictc_embedding_bwd_workspace_bytes": (_i64, [_i, _i64, _i64, _i]),

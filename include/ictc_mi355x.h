@@ -820,7 +820,10 @@ int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const fl
  * ictc_expert_order and ictc_csr_build give for these ids and `entries` keys; up to as many
  * rows as ictc_embedding_needs_order denies they may be NULL.  Workspace of
  * ictc_embedding_bwd_workspace_bytes bytes, 4-byte aligned (0: none needed, -1: an
- * argument out of range).                                                               */
+ * argument out of range).  ictc_rows_by_id is ictc_expert_order for any number of entries. */
+int64_t ictc_rows_by_id_workspace_bytes(int64_t rows, int64_t entries);
+int ictc_rows_by_id(const int64_t* ids, int64_t rows, int64_t entries, int32_t* perm, int32_t* offsets, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 int ictc_embedding_fwd(int dtype, const void* table, int64_t entries, int width, const int64_t* ids, int64_t rows,
                        float scale, void* out, void* stream);
 int ictc_embedding_needs_order(int64_t rows);

@@ -57,3 +57,19 @@ def test_native_refusals():
                 dict(out=None), dict(ws=None), dict(ws=18), dict(bytes=4)):
         with pytest.raises(ValueError):
             bwd(**bad)
+
+
+def test_order_refusals():
+    nat = _built()
+    size = nat.lib().ictc_rows_by_id_workspace_bytes
+    assert size(100, 5) == 0 and size(100000, 200000) > 0
+    for bad in ((-1, 5), (5, 0), (2 ** 31, 5), (5, 2 ** 31)):
+        assert size(*bad) == -1, bad
+
+    def order(ids=16, rows=100000, entries=200000, perm=16, off=16, ws=16, bytes=1 << 30):
+        nat.call("ictc_rows_by_id", ids, rows, entries, perm, off, ws, bytes, None)
+
+    for bad in (dict(ids=None), dict(rows=-1), dict(entries=0), dict(perm=None), dict(off=None), dict(ws=None),
+                dict(ws=18), dict(bytes=100)):
+        with pytest.raises(ValueError):
+            order(**bad)

@@ -248,3 +248,27 @@ def test_offsets_past_32_bits(device):
     (got,) = torch.autograd.grad(y, table, torch.ones_like(y))
     assert (got[0] == 0).all() and (got[2] == 5).all()
     assert ((got[1].double() - 16999998).abs() <= 16999998 * 700 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("rows,entries", [(0, 1024), (1, 1023), (1, 1024), (5, 65535), (300, 140003), (16384, 1500),
+                                          (20000, 5000), (425991, 7921), (70000, 1048575), (70000, 1048576),
+                                          (4300000, 2000)])
+def test_order_of_many_entries(device, rows, entries):
+    """The rows' order by id: stable, ids outside last, and where each id begins, whichever passes make it."""
+    from ictc_o3 import _native as nat
+    g = torch.Generator().manual_seed(rows + entries)
+    ids = torch.randint(-2, entries + 3, (rows,), generator=g).to(device)
+    if rows > 100:
+        ids[rows // 3: rows // 2] = entries // 2        # one id of many
+    lib = nat.lib()
+    size = lib.ictc_rows_by_id_workspace_bytes(rows, entries)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+    perm = torch.full((max(rows, 1),), -7, dtype=torch.int32, device=device)
+    off = torch.full((entries + 2,), -7, dtype=torch.int32, device=device)
+    nat.call("ictc_rows_by_id", ids.data_ptr(), rows, entries, perm.data_ptr(), off.data_ptr(), ws.data_ptr(), size,
+             torch.cuda.current_stream().cuda_stream)
+    key = torch.where((ids >= 0) & (ids < entries), ids, torch.full_like(ids, entries))
+    ref = torch.sort(key, stable=True)
+    assert torch.equal(perm[:rows].long(), ref.indices)
+    counts = torch.bincount(key, minlength=entries + 1)
+    assert torch.equal(off.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
