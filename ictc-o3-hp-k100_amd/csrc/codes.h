@@ -87,4 +87,16 @@ __device__ __forceinline__ uint32_t lane_top(uint32_t x) {
   return x;
 }
 
+// The same over `lanes` lanes, a power of two up to 32 that all agree on.
+__device__ __forceinline__ uint32_t lanes_top(uint32_t x, int lanes) {
+  switch (lanes) {
+    case 1: return x;
+    case 2: return lane_top<2>(x);
+    case 4: return lane_top<4>(x);
+    case 8: return lane_top<8>(x);
+    case 16: return lane_top<16>(x);
+    default: return lane_top<32>(x);
+  }
+}
+
 }  // namespace

@@ -154,6 +154,12 @@ __device__ __forceinline__ void wave_meet() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Block `b` of `blocks` in an order that gives each of the eight dies (blocks go to them in turn) a contiguous part.
+__device__ __forceinline__ int die_order(int b, int blocks) {
+  const int per = blocks / 8, rest = blocks % 8, die = b & 7;
+  return die * per + min(die, rest) + (b >> 3);
+}
+
 inline int dense_fail(int code, const char* msg) { return ictc::set_error(code, msg); }
 
 inline int dense_status(const char* what) {

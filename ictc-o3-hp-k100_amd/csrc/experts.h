@@ -159,12 +159,6 @@ __device__ __forceinline__ bool find_segment(const int* __restrict__ off, int ex
   return true;
 }
 
-// Block `b` of `blocks` in an order that gives each of the eight dies (blocks go to them in turn) a contiguous part.
-__device__ __forceinline__ int die_order(int b, int blocks) {
-  const int per = blocks / 8, rest = blocks % 8, die = b & 7;
-  return die * per + min(die, rest) + (b >> 3);
-}
-
 // Zeros in the tile at (m0, k0) of gW [M, K] and, of the first column tile, of gb [M].
 template <typename T, int TILE, int THREADS>
 __device__ __forceinline__ void zero_tile(T* __restrict__ gW, T* __restrict__ gb, int M, int K, int m0, int k0) {

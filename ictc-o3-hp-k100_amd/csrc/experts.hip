@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 4) void experts_few_kernel(const T*
 //
 // More than 1,023 experts (entries of a table) are ordered by the low half of the id's bits and then, stably, by the high
 // one: the first pass leaves ids and row numbers, the second row numbers and sorted ids, of which order_offsets_kernel
-// makes the offsets (425,991 rows of 7,921 ids: 31 us, 125 by the general sort).
+// makes the offsets (425,991 rows of 7,921 ids: 36 us, 125 by the general sort).
 constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16, kOrderBlocks = 256;
 constexpr int kOrderRows = kOrderWaves * kOrderAtOnce * 64;
 
@@ -530,14 +530,16 @@ int id_bits(int experts) {
   return bits;
 }
 
-// Rows of a block: all of few rows; 4,096; more once those would be more than 64 blocks; and zero: the general sort.
-// Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5, 16,384 12.9 / 9.0; 89 experts 6,000
-// rows 8.2 / 8.7, 16,384 16.4 / 10.1.  Several / the general sort, ten experts: 30,011 rows 8.8 / 10.8, 262,145 11.8 / 106,
-// 4.2 million 32 / 83.
+// Rows of a block: all of few rows; 1,024, and more once those would be more than 256 blocks (over 255 ids 2,048 and 128);
+// and zero: the general sort.  Measured in us, one block / several: ten experts 500 rows 4.6 / 8.0, 8,192 8.0 / 8.5.
+// Both kernels at 64 / 128 / 256 blocks and 4,096 / 2,048 / 1,024 rows at least: 131,072 rows of ten experts 10.5 / 8.9 /
+// 8.3, 30,011 of 89 11.1 / 9.5 / 9.0, 425,991 of 1,000 25 / 24 / 29; both passes of 60,013 rows of 50,021 ids 34 / 28 / 22,
+// of 425,991 of 7,921 42 / 35 / 32.  Several / the general sort, ten experts: 4.2 million rows 32 / 83.
 int order_span(int64_t rows, int bits) {
   if (rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
   if (rows <= kOrderRows && rows * (3 + bits) <= 60000) return (int)std::max<int64_t>(rows, 1);
-  return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(4096, (rows / 64 + 1023) / 1024 * 1024));
+  const int blocks = bits <= 8 ? 256 : 128;
+  return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(262144 / blocks, (rows / blocks + 1023) / 1024 * 1024));
 }
 
 // The passes over the bits of an id: none (the general sort), one, or two.

@@ -59,18 +59,21 @@ int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, in
 
 int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
                         const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
-                        float* rstd, void* workspace, int64_t workspace_bytes, void* stream) {
+                        float* rstd, int8_t* codes, float* scales, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(dtype, samples, positions, channels, groups)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!(eps >= 0.f)) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: eps must not be negative");
   if (activation != 0 && activation != 1) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: activation must be 0 or 1");
   if (samples == 0 || positions == 0) return ICTC_OK;
-  if (!x || !y || !mean != !rstd) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
+  if (!x || !y || !mean != !rstd || !codes != !scales) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
   ictc::GroupNormCall a = {};
   a.samples = samples, a.positions = positions, a.channels = channels, a.groups = groups;
   a.x = x, a.w = weight, a.b = bias, a.eps = eps, a.silu = activation, a.out = y, a.mean = mean, a.rstd = rstd;
+  a.codes_out = codes, a.scales_out = scales;
   a.ws = workspace, a.ws_bytes = workspace_bytes, a.stream = (hipStream_t)stream;
   if (!workspace_fits(a, dtype, 0))
     return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: workspace smaller than ictc_group_norm_workspace_bytes");
+  if (codes && !plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups).coded)
+    if (const int rc = ictc_codes_encode(dtype, x, channels, samples * positions, channels, codes, scales, stream)) return rc;
   GN_TYPED(group_norm_fwd)
   return dense_status("group_norm_fwd launch");
 }

@@ -256,7 +256,7 @@ struct GroupNormGrad : Function<GroupNormGrad> {
 
 // stats: the groups' mean and 1 / deviation, or undefined
 Tensor group_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, const Tensor& stats,
-                     const NormShape& n) {
+                     const NormShape& n, const Codes& codes = Codes()) {
   const Tensor x = packed(x_), w = packed(w_), b = packed(b_);
   Tensor y = at::empty(x.sizes(), x.options());
   float* st = stats.defined() ? stats.mutable_data_ptr<float>() : nullptr;
@@ -264,21 +264,24 @@ Tensor group_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, doubl
       ictc_group_norm_workspace_bytes(dtype_of(x), 0, n.samples, n.positions, n.channels, (int)n.groups);
   const Tensor ws = workspace(bytes, x);
   done(ictc_group_norm_fwd(dtype_of(x), ptr(x), n.samples, n.positions, n.channels, (int)n.groups, ptr(w), ptr(b),
-                           (float)eps, n.silu, ptr(y), st, st ? st + n.samples * n.groups : nullptr, ptr(ws), bytes,
-                           stream_of(x)),
+                           (float)eps, n.silu, ptr(y), st, st ? st + n.samples * n.groups : nullptr,
+                           (int8_t*)ptr(codes.codes), (float*)ptr(codes.scales), ptr(ws), bytes, stream_of(x)),
        "group_norm");
   return y;
 }
 
 struct GroupNorm : Function<GroupNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps,
-                        const NormShape& n, const c10::IValue& place, const Codes& codes) {
+                        const NormShape& n, const c10::IValue& place) {
     const Tensor stats = floats(2 * n.samples * n.groups, x);
-    if (codes.codes.defined())
+    Codes codes;
+    if (!place.isNone()) {
       ctx->saved_data["place"] = place;
+      codes = empty_codes(n.samples * n.positions, n.channels, x);
+    }
     ctx->save_for_backward({codes.codes.defined() ? Tensor() : x, value(w), value(b), stats, codes.codes, codes.scales});
     keep(ctx, n);
-    return group_forward(x, value(w), value(b), eps, stats, n);
+    return group_forward(x, value(w), value(b), eps, stats, n, codes);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
@@ -286,7 +289,7 @@ struct GroupNorm : Function<GroupNorm> {
     const Kept kept = {saved[0], saved[4], saved[5]};
     const NormShape n = kept_shape(ctx);
     const std::vector<bool> want = wanted(ctx, {true, w.defined(), b.defined()});
-    variable_list out(7);
+    variable_list out(6);
     if (!want[0] && !want[1] && !want[2]) return out;
     if (at::GradMode::is_enabled()) {   // the gradient will be differentiated
       const Tensor x = kept.codes.defined() ? ctx->saved_data["place"].toTensor() : kept.x;
@@ -326,9 +329,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& w, const Opt
   const NormShape n = {x.size(0), positions, groups, (int)C, activation.has_value()};
   const Tensor wv = value(w), bv = value(b);
   if (!tracked({&x, &wv, &bv})) return group_forward(x, wv, bv, eps, Tensor(), n);
-  if (!eight) return GroupNorm::apply(x, w, b, eps, n, c10::IValue(), Codes());
-  return GroupNorm::apply(x, w, b, eps, n, c10::IValue(Place8::apply(x)),
-                          encode_rows(x.detach().reshape({n.samples * n.positions, C})));
+  return GroupNorm::apply(x, w, b, eps, n, eight ? c10::IValue(Place8::apply(x)) : c10::IValue());
 }
 
 // ---------------------------------------------------------------------------

@@ -121,12 +121,15 @@ struct Codes {
   Tensor codes, scales;   // int8 [rows, width], float32 [rows, blocks of 128]
 };
 
+Codes empty_codes(int64_t N, int64_t C, const Tensor& like) {
+  return {at::empty({N, C}, like.options().dtype(at::kChar)), at::empty({N, (C + 127) / 128}, like.options().dtype(at::kFloat))};
+}
+
 Codes encode_rows(const Tensor& x_) {
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = rows_of(x_);
   const int64_t N = x.size(0), C = x.size(1);
-  Codes out = {at::empty({N, C}, x.options().dtype(at::kChar)),
-               at::empty({N, (C + 127) / 128}, x.options().dtype(at::kFloat))};
+  Codes out = empty_codes(N, C, x);
   done(ictc_codes_encode(dtype_of(x), ptr(x), pitch(x), N, (int)C, out.codes.mutable_data_ptr<int8_t>(),
                          out.scales.mutable_data_ptr<float>(), stream_of(x)),
        "activations");

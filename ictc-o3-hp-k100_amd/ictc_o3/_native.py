@@ -136,7 +136,8 @@ _SIGNATURES = {
     "ictc_expert_outer_workspace_bytes": (_i64, [_i, _i64, _i, _i, _i]),
     "ictc_expert_outer": (_i, [_i, _p, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_group_norm_workspace_bytes": (_i64, [_i, _i, _i64, _i64, _i, _i]),
-    "ictc_group_norm_fwd": (_i, [_i, _p, _i64, _i64, _i, _i, _p, _p, ctypes.c_float, _i, _p, _p, _p, _p, _i64, _p]),
+    "ictc_group_norm_fwd": (_i, [_i, _p, _i64, _i64, _i, _i, _p, _p, ctypes.c_float, _i, _p, _p, _p, _p, _p, _p, _i64,
+                                 _p]),
     "ictc_group_norm_bwd": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_group_norm_bwd2": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p,
                                   _p, _i64, _p]),

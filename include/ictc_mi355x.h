@@ -788,10 +788,9 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  * all positions and the channels / groups channels of a sample's group; activation 0: none,
  * 1: z / (1 + exp(-z)).  Statistics and sums in FP32 or FP64, each result rounded once.
  * weight / bias NULL: ones / zeros.  mean and rstd [samples, groups] FP32 may both be NULL
- * in fwd.
+ * in fwd; codes and scales NULL, or what ictc_codes_encode gives of x as rows of `channels`.
  *   bwd:  dx, dweight [channels], dbias [channels], each NULL to skip; no elements give zero
- *         dweight and dbias.  With codes and scales (ictc_codes_encode of x as rows of
- *         `channels`) x is not read: h = (value - mean) rstd stands for the normalised x.
+ *         dweight and dbias.  With codes and scales x is not read: h = (value - mean) rstd stands for the normalised x.
  *   bwd2: the gradients of <v, dx> + <vweight, dweight> + <vbias, dbias> by x (dx), by grad
  *         (dgrad), by weight and by bias (zero without an activation); vweight / vbias NULL:
  *         absent.
@@ -801,7 +800,8 @@ int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, in
                                         int groups);
 int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
                         const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
-                        float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+                        float* rstd, int8_t* codes, float* scales, void* workspace, int64_t workspace_bytes,
+                        void* stream);
 int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
                         int64_t samples, int64_t positions, int channels, int groups, const void* weight,
                         const void* bias, int activation, const float* mean, const float* rstd, void* dx, void* dweight,

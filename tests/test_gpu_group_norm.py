@@ -142,7 +142,9 @@ def test_larger(device, shape, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(37, 1, 64, 8), (9, 1, 35, 5), (5, 1, 600, 200), (3, 1, 2176, 1), (7, 9, 64, 8),
                                    (5, 33, 30, 5), (2, 257, 330, 11), (3, 300, 64, 8), (2, 4099, 30, 5), (1, 700, 2304, 1),
-                                   (9, 1, 384, 3), (9, 1, 392, 4), (0, 1, 16, 4)])
+                                   (9, 1, 384, 3), (9, 1, 392, 4), (0, 1, 16, 4),
+                                   (700, 1, 16, 4), (11, 1, 128, 1), (37, 1, 256, 8), (1030, 1, 512, 64), (5, 1, 1024, 2),
+                                   (3, 1, 2048, 2), (6, 1, 768, 2), (9, 1, 640, 40), (4, 1, 2048, 256), (3, 1, 96, 3)])
 def test_x_in_8_bits(device, shape, dtype):
     """The result is that of whole rows, bit for bit; the derivatives are the formulas at the decoded x."""
     from ictc_o3 import decode_activations, encode_activations, group_norm

@@ -51,12 +51,13 @@ def test_native_refusals():
         assert size(*bad) == -1, bad
 
     def fwd(dtype=0, x=16, samples=2, positions=3, channels=8, groups=2, eps=1e-5, act=0, y=16, mean=None, rstd=None,
-            ws=None, bytes=0):
+            codes=None, scales=None, ws=None, bytes=0):
         nat.call("ictc_group_norm_fwd", dtype, x, samples, positions, channels, groups, None, None, eps, act, y, mean,
-                 rstd, ws, bytes, None)
+                 rstd, codes, scales, ws, bytes, None)
 
     for bad in (dict(dtype=4), dict(x=None), dict(samples=-1), dict(positions=-1), dict(channels=0), dict(groups=3),
                 dict(eps=-1.0), dict(eps=float("nan")), dict(act=2), dict(y=None), dict(mean=16),
+                dict(codes=16), dict(scales=16),
                 dict(samples=1, positions=100000)):
         with pytest.raises(ValueError):
             fwd(**bad)
