@@ -201,3 +201,9 @@ bool experts_direct_outer_fits(int dtype, int M, int K);
 void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x,
                           int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
                           float* part, hipStream_t st);
+
+// The same of rows in 8 bits, and whether it takes these.
+bool experts_codes_outer_fits(int dtype, const void* gy, int64_t ldg, int M, int K);
+void experts_codes_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const int8_t* codes,
+                         const float* scales, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
+                         float* part, hipStream_t st);

@@ -834,6 +834,43 @@ void launch_sum(const OuterPlan& plan, int M, int K, int experts, const int* off
                      part, MK, M, off, experts, plan.rows, plan.ranges, (T*)gW, (T*)gb);
 }
 
+// The weights' gradient of rows x, or of codes; the caller has looked at these.
+int run_outer(int dtype, const void* grad, int64_t ldg, const void* x, int64_t ldx, const int8_t* codes, const float* scales,
+              int64_t rows, int inputs, int outputs, int experts, const int* perm, const int* offsets, void* dweight,
+              void* dbias, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  if (ldg < outputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: row pitch below the row");
+  if (!offsets || !dweight || (rows > 0 && (!grad || !perm)))
+    return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
+  const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, outputs, inputs),
+                                    dtype, rows, outputs, inputs, experts);
+  if (outer_bytes(plan, outputs, inputs) > 0 &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+       workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
+    return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: workspace smaller than ictc_expert_outer_workspace_bytes");
+  float* part = (float*)workspace;
+  if (codes)
+    experts_codes_outer(dtype, plan, grad, ldg, outputs, codes, scales, inputs, experts, perm, offsets, dweight, dbias, part,
+                        st);
+  else if (plan.direct)
+    experts_direct_outer(dtype, plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part,
+                         st);
+  else if (dtype == ICTC_F32)
+    launch_outer<float>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
+  else if (dtype == ICTC_BF16)
+    launch_outer<bf16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
+  else
+    launch_outer<f16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
+  if (plan.sums) {
+    if (dtype == ICTC_F32)
+      launch_sum<float>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+    else if (dtype == ICTC_BF16)
+      launch_sum<bf16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+    else
+      launch_sum<f16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
+  }
+  return dense_status("expert_outer launch");
+}
+
 }  // namespace
 
 extern "C" {
@@ -907,36 +944,26 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
                       int outputs, int experts, const int32_t* perm, const int32_t* offsets, void* dweight,
                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(dtype, rows, inputs, outputs, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
-  if ((ldx < inputs || ldg < outputs) && rows > 1)
-    return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: row pitch below the row");
-  if (!offsets || !dweight || (rows > 0 && (!grad || !x || !perm)))
-    return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
-  const OuterPlan plan = outer_plan(rows > 0 && experts_direct_outer_fits(dtype, outputs, inputs),
-                                    dtype, rows, outputs, inputs, experts);
-  if (outer_bytes(plan, outputs, inputs) > 0 &&
-      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-       workspace_bytes < ictc_expert_outer_workspace_bytes(dtype, rows, inputs, outputs, experts)))
-    return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: workspace smaller than ictc_expert_outer_workspace_bytes");
-  hipStream_t st = (hipStream_t)stream;
-  float* part = (float*)workspace;
-  if (plan.direct)
-    experts_direct_outer(dtype, plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part,
-                         st);
-  else if (dtype == ICTC_F32)
-    launch_outer<float>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
-  else if (dtype == ICTC_BF16)
-    launch_outer<bf16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
-  else
-    launch_outer<f16>(plan, grad, ldg, outputs, x, ldx, inputs, experts, perm, offsets, dweight, dbias, part, st);
-  if (plan.sums) {
-    if (dtype == ICTC_F32)
-      launch_sum<float>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
-    else if (dtype == ICTC_BF16)
-      launch_sum<bf16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
-    else
-      launch_sum<f16>(plan, outputs, inputs, experts, offsets, dweight, dbias, part, st);
-  }
-  return dense_status("expert_outer launch");
+  if (ldx < inputs && rows > 1) return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: row pitch below the row");
+  if (rows > 0 && !x) return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
+  return run_outer(dtype, grad, ldg, x, ldx, nullptr, nullptr, rows, inputs, outputs, experts, perm, offsets, dweight, dbias,
+                   workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int ictc_expert_outer_takes_codes(int dtype, const void* grad, int64_t ldg, int64_t rows, int inputs, int outputs) {
+  return !bad_sizes(dtype, rows, inputs, outputs, 1) && rows > 0 && experts_direct_outer_fits(dtype, outputs, inputs) &&
+         experts_codes_outer_fits(dtype, grad, ldg, outputs, inputs);
+}
+
+int ictc_expert_outer_codes(int dtype, const void* grad, int64_t ldg, const int8_t* codes, const float* scales, int64_t rows,
+                            int inputs, int outputs, int experts, const int32_t* perm, const int32_t* offsets,
+                            void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const char* e = bad_sizes(dtype, rows, inputs, outputs, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
+  if (!codes || !scales) return dense_fail(ICTC_ERR_ARGUMENT, "expert_outer: null operand");
+  if (!ictc_expert_outer_takes_codes(dtype, grad, ldg, rows, inputs, outputs))
+    return dense_fail(ICTC_ERR_UNSUPPORTED, "expert_outer: codes need rows, and whole aligned 16-byte chunks of them");
+  return run_outer(dtype, grad, ldg, nullptr, inputs, codes, scales, rows, inputs, outputs, experts, perm, offsets, dweight,
+                   dbias, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "codes.h"
 #include "experts.h"
 
 namespace {
@@ -399,14 +400,29 @@ void direct_rows(const void* x, int64_t ldx, int64_t rows, int K, const void* W,
   launch_direct<T, ALIGNED, TRANS, 128, 128, LARGE>(x, ldx, rows, K, W, bias, N, experts, perm, off, out, st);
 }
 
+// Rows kept in 8 bits: a chunk's codes and scale as they lie in memory, and the chunk that they stand for.
+template <typename T>
+struct CodeChunk {
+  Codes<kChunk<T>> codes;
+  float scale;
+  __device__ __forceinline__ u32x4 values() const {
+    Chunk<T> c;
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) c.e[e] = (T)held((float)codes.e[e] * scale);
+    return c.raw;
+  }
+};
+
 // Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
-// range of rows: see experts_outer_kernel.
-template <typename T, bool ALIGNED, int TA, int TB, int S, int GA, int GB>
+// range of rows: see experts_outer_kernel.  CODES: x is codes [rows, K], with scales; its chunks become values on their way
+// to LDS (131,072 rows of 512 -> 512 bfloat16: CODES_US us, and 40 + 124 decoded to memory first).
+template <typename T, bool ALIGNED, bool CODES, int TA, int TB, int S, int GA, int GB>
 __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
-    const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, int K, int experts, int ranges,
-    const int* __restrict__ perm, const int* __restrict__ off, T* __restrict__ gW, T* __restrict__ gb,
-    float* __restrict__ part) {
+    const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ codes,
+    const float* __restrict__ scales, int K, int experts, int ranges, const int* __restrict__ perm,
+    const int* __restrict__ off, T* __restrict__ gW, T* __restrict__ gb, float* __restrict__ part) {
   static_assert(TA == TB, "one row number serves both operands");
+  static_assert(!CODES || (ALIGNED && TA <= kCodeBlock && kCodeBlock % TA == 0), "a row of a tile has one scale");
   constexpr int WAVES = GA * GB, L = kLoads<T, TA, S, WAVES>, V = kChunk<T>, CH = TA / V, PER = 64 / CH;
   constexpr int KB = 64 * V;   // elements of a load
   constexpr int NA = TA / GA / 16, NB = TB / GB / 16;
@@ -438,6 +454,7 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
       }
     };
     u32x4 ra[L], rb[L];   // (not ALIGNED)
+    CodeChunk<T> rc[L];   // (CODES)
     auto column = [&](int i) { return ((lane % CH) ^ across_swap<T, TA>((wave * L + i) * PER + sub)) * V; };
     auto load = [&](Word<T>* A, Word<T>* B) {
 #pragma unroll
@@ -446,7 +463,12 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
         const bool ok = node[i] >= 0;
         const T *px = x + (int64_t)node[i] * ldx + ca, *pg = gy + (int64_t)node[i] * ldg + cb;
         if (ALIGNED) {
-          to_lds(ok ? (const void*)px : (const void*)kZeros, A + (wave * L + i) * KB);
+          if constexpr (CODES) {
+            rc[i].codes = load_codes<V>(codes + (ok ? (int64_t)node[i] * K + ca : 0), ok ? V : 0);
+            rc[i].scale = ok ? scales[(int64_t)node[i] * ((K + kCodeBlock - 1) / kCodeBlock) + k0 / kCodeBlock] : 0.f;
+          } else {
+            to_lds(ok ? (const void*)px : (const void*)kZeros, A + (wave * L + i) * KB);
+          }
           to_lds(ok ? (const void*)pg : (const void*)kZeros, B + (wave * L + i) * KB);
         } else {
           ra[i] = load_chunk_of(px, ok ? K - k0 - c : 0);
@@ -454,9 +476,13 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
         }
       }
     };
-    auto put = [&](Word<T>* A, Word<T>* B) {   // not ALIGNED: what load read
+    auto put = [&](Word<T>* A, Word<T>* B) {   // what load read into registers
 #pragma unroll
       for (int i = 0; i < L; ++i) {
+        if constexpr (CODES) {
+          *reinterpret_cast<u32x4*>(A + (wave * L + i) * KB + lane * V) = rc[i].values();
+          continue;
+        }
         *reinterpret_cast<u32x4*>(A + (wave * L + i) * KB + lane * V) = move_chunk<T>(ra[i], K - k0 - column(i));
         *reinterpret_cast<u32x4*>(B + (wave * L + i) * KB + lane * V) = move_chunk<T>(rb[i], M - m0 - column(i));
       }
@@ -468,9 +494,10 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
 #pragma unroll
       for (int i = 0; i < NA; ++i) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
+    constexpr bool PUTS = !ALIGNED || CODES;
     name(0);
     load(A0, B0);
-    if (!ALIGNED) put(A0, B0);
+    if (PUTS) put(A0, B0);
     name(S);
     for (int row = 0; row < seg.count; row += 2 * S) {
       meet<ALIGNED>();
@@ -480,14 +507,14 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
       }
       direct_step<T, true, true, TA, TB, S, GA, GB, true>(A0, B0, wa, wb, acc, bias, accb);
       if (row + S < seg.count) {
-        if (!ALIGNED) put(A1, B1);
+        if (PUTS) put(A1, B1);
         meet<ALIGNED>();
         if (row + 2 * S < seg.count) {
           load(A0, B0);
           name(row + 3 * S);
         }
         direct_step<T, true, true, TA, TB, S, GA, GB, true>(A1, B1, wa, wb, acc, bias, accb);
-        if (!ALIGNED && row + 2 * S < seg.count) put(A0, B0);
+        if (PUTS && row + 2 * S < seg.count) put(A0, B0);
       }
     }
     meet<false>();   // the next segment's first load overwrites what a wave may still read
@@ -531,24 +558,33 @@ __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
   }
 }
 
-template <typename T, bool ALIGNED, int TILE, int S>
-void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
-                  int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
+// The rows of a weights' gradient: x at pitch ldx, or in 8 bits.
+struct OuterRows {
+  const void* x;
+  int64_t ldx;
+  const int8_t* codes;
+  const float* scales;
+};
+
+template <typename T, bool ALIGNED, bool CODES, int TILE, int S>
+void launch_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const OuterRows& r, int K, int experts,
+                  const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   const int64_t tiles = (int64_t)((M + TILE - 1) / TILE) * ((K + TILE - 1) / TILE);
   const dim3 grid((unsigned)(std::max(plan.ranges, plan.fill) * tiles));
-  hipLaunchKernelGGL((experts_direct_outer_kernel<T, ALIGNED, TILE, TILE, S, 2, 2>), grid, dim3(256), 0, st, (const T*)gy,
-                     ldg, M, (const T*)x, ldx, K, experts, plan.ranges, perm, off, (T*)gW, (T*)gb, part);
+  hipLaunchKernelGGL((experts_direct_outer_kernel<T, ALIGNED, CODES, TILE, TILE, S, 2, 2>), grid, dim3(256), 0, st,
+                     (const T*)gy, ldg, M, (const T*)r.x, r.ldx, r.codes, r.scales, K, experts, plan.ranges, perm, off,
+                     (T*)gW, (T*)gb, part);
 }
 
-template <typename T, bool ALIGNED>
-void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const void* x, int64_t ldx, int K,
-                  int experts, const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
+template <typename T, bool ALIGNED, bool CODES>
+void direct_outer(const OuterPlan& plan, const void* gy, int64_t ldg, int M, const OuterRows& r, int K, int experts,
+                  const int* perm, const int* off, void* gW, void* gb, float* part, hipStream_t st) {
   if constexpr (sizeof(T) == 2)
-    launch_outer<T, ALIGNED, 128, 64>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    launch_outer<T, ALIGNED, CODES, 128, 64>(plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
   else if (plan.tile == 64)
-    launch_outer<T, ALIGNED, 64, 64>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    launch_outer<T, ALIGNED, CODES, 64, 64>(plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
   else
-    launch_outer<T, ALIGNED, 128, 32>(plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    launch_outer<T, ALIGNED, CODES, 128, 32>(plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
 }
 
 bool whole16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -571,14 +607,14 @@ void either_rows(int dtype, bool transpose, A... a) {
     typed_rows<ALIGNED, false>(dtype, a...);
 }
 
-template <bool ALIGNED, typename... A>
+template <bool ALIGNED, bool CODES, typename... A>
 void typed_outer(int dtype, A... a) {
   if (dtype == ICTC_F32)
-    direct_outer<float, ALIGNED>(a...);
+    direct_outer<float, ALIGNED, CODES>(a...);
   else if (dtype == ICTC_BF16)
-    direct_outer<bf16, ALIGNED>(a...);
+    direct_outer<bf16, ALIGNED, CODES>(a...);
   else
-    direct_outer<f16, ALIGNED>(a...);
+    direct_outer<f16, ALIGNED, CODES>(a...);
 }
 
 }  // namespace
@@ -606,8 +642,21 @@ void experts_direct_outer(int dtype, const OuterPlan& plan, const void* gy, int6
                           int64_t ldx, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
                           float* part, hipStream_t st) {
   const int v = chunk_of(dtype);
+  const OuterRows r = {x, ldx, nullptr, nullptr};
   if (whole16(gy) && whole16(x) && ldg % v == 0 && ldx % v == 0 && M % v == 0 && K % v == 0)
-    typed_outer<true>(dtype, plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    typed_outer<true, false>(dtype, plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
   else
-    typed_outer<false>(dtype, plan, gy, ldg, M, x, ldx, K, experts, perm, off, gW, gb, part, st);
+    typed_outer<false, false>(dtype, plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
+}
+
+bool experts_codes_outer_fits(int dtype, const void* gy, int64_t ldg, int M, int K) {
+  const int v = chunk_of(dtype);
+  return whole16(gy) && ldg % v == 0 && M % v == 0 && K % v == 0;
+}
+
+void experts_codes_outer(int dtype, const OuterPlan& plan, const void* gy, int64_t ldg, int M, const int8_t* codes,
+                         const float* scales, int K, int experts, const int* perm, const int* off, void* gW, void* gb,
+                         float* part, hipStream_t st) {
+  const OuterRows r = {nullptr, K, codes, scales};
+  typed_outer<true, true>(dtype, plan, gy, ldg, M, r, K, experts, perm, off, gW, gb, part, st);
 }

@@ -211,19 +211,24 @@ Tensor linear_rows(const Tensor& x_, const Tensor& W_, const Tensor& b_, const T
   return out;
 }
 
+// x: rows; or codes of them with their scales.
 std::pair<Tensor, Tensor> linear_outer(const Tensor& g_, const Tensor& x_, const Tensor& perm, const Tensor& off,
-                                       bool need_b) {
+                                       bool need_b, const Tensor& scales = Tensor()) {
   eager("expert_linear");
-  const Tensor g = rows_of(g_), x = rows_of(x_);
-  const int64_t N = x.size(0), M = g.size(1), K = x.size(1), E = off.size(0) - 2;
-  const int dt = dtype_of(x);
-  Tensor gW = at::empty({E, M, K}, x.options()), gb, ws;
-  if (need_b) gb = at::empty({E, M}, x.options());
+  const Tensor g = rows_of(g_);
+  const int64_t N = g.size(0), M = g.size(1), K = x_.size(1), E = off.size(0) - 2;
+  const int dt = dtype_of(g);
+  const bool codes = scales.defined() && ictc_expert_outer_takes_codes(dt, ptr(g), pitch(g), N, (int)K, (int)M);
+  const Tensor x = codes ? x_ : scales.defined() ? decode_rows(x_, scales, g.scalar_type()) : rows_of(x_);
+  Tensor gW = at::empty({E, M, K}, g.options()), gb, ws;
+  if (need_b) gb = at::empty({E, M}, g.options());
   const int64_t bytes = ictc_expert_outer_workspace_bytes(dt, N, (int)K, (int)M, (int)E);
-  if (bytes > 0) ws = floats(bytes / 4, x);
-  done(ictc_expert_outer(dt, ptr(g), pitch(g), ptr(x), pitch(x), N, (int)K, (int)M, (int)E,
-                         perm.const_data_ptr<int>(), off.const_data_ptr<int>(), ptr(gW), ptr(gb), ptr(ws), bytes,
-                         stream_of(x)),
+  if (bytes > 0) ws = floats(bytes / 4, g);
+  const int *p = perm.const_data_ptr<int>(), *o = off.const_data_ptr<int>();
+  done(codes ? ictc_expert_outer_codes(dt, ptr(g), pitch(g), x.const_data_ptr<int8_t>(), scales.const_data_ptr<float>(), N,
+                                       (int)K, (int)M, (int)E, p, o, ptr(gW), ptr(gb), ptr(ws), bytes, stream_of(g))
+             : ictc_expert_outer(dt, ptr(g), pitch(g), ptr(x), pitch(x), N, (int)K, (int)M, (int)E, p, o, ptr(gW), ptr(gb),
+                                 ptr(ws), bytes, stream_of(g)),
        "expert_linear");
   return {gW, gb};
 }
@@ -281,9 +286,9 @@ variable_list ExpertLinear::backward(AutogradContext* ctx, variable_list grads) 
   const std::vector<bool> want = wanted(ctx, {true, true, ctx->saved_data["bias"].toBool()});
   const bool again = at::GradMode::is_enabled();   // the gradient will be differentiated
   Tensor x = saved[0];
-  if (saved.size() > 4 && (want[1] || want[2]))
-    x = again ? Decoded::apply(ctx->saved_data["place"].toTensor(), saved[0], saved[4])
-              : decode_rows(saved[0], saved[4], W.scalar_type());
+  const Tensor scales = saved.size() > 4 ? saved[4] : Tensor();   // (of codes, which are not transposed)
+  if (scales.defined() && again && (want[1] || want[2]))
+    x = Decoded::apply(ctx->saved_data["place"].toTensor(), saved[0], scales);
   variable_list out(8);
   if (want[0])
     out[0] = again ? ExpertLinear::apply(g, W, OptTensor(), perm, off, !trans)
@@ -295,7 +300,7 @@ variable_list ExpertLinear::backward(AutogradContext* ctx, variable_list grads) 
       if (want[1]) out[1] = s[0];
       if (want[2]) out[2] = s[1];
     } else {
-      auto [gW, gb] = linear_outer(a, b, perm, off, want[2]);
+      auto [gW, gb] = linear_outer(a, b, perm, off, want[2], scales);
       if (want[1]) out[1] = gW;
       out[2] = gb;
     }

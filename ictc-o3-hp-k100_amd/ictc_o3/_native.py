@@ -147,6 +147,8 @@ _SIGNATURES = {
     "ictc_embedding_needs_order": (_i, [_i64]),
     "ictc_embedding_bwd_workspace_bytes": (_i64, [_i, _i64, _i64, _i]),
     "ictc_embedding_bwd": (_i, [_i, _p, _i64, _i64, _i, _p, _i64, _p, _p, ctypes.c_float, _p, _p, _i64, _p]),
+    "ictc_expert_outer_takes_codes": (_i, [_i, _p, _i64, _i64, _i, _i]),
+    "ictc_expert_outer_codes": (_i, [_i, _p, _i64, _p, _p, _i64, _i, _i, _i, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_codes_encode": (_i, [_i, _p, _i64, _i64, _i, _p, _p, _p]),
     "ictc_codes_decode": (_i, [_i, _p, _p, _i64, _i, _p, _p]),
     "ictc_gradient_norm_workspace_bytes": (_i64, [_i]),

@@ -843,6 +843,13 @@ int ictc_codes_encode(int dtype, const void* x, int64_t ldx, int64_t rows, int w
                       void* stream);
 int ictc_codes_decode(int dtype, const int8_t* codes, const float* scales, int64_t rows, int width, void* out,
                       void* stream);
+/* ictc_expert_outer with the values of codes [rows, inputs] for x, and the same workspace:
+ * where grad begins at a multiple of 16 bytes and its pitch, `inputs` and `outputs` are
+ * multiples of 16 bytes of elements (ictc_expert_outer_takes_codes).                     */
+int ictc_expert_outer_takes_codes(int dtype, const void* grad, int64_t ldg, int64_t rows, int inputs, int outputs);
+int ictc_expert_outer_codes(int dtype, const void* grad, int64_t ldg, const int8_t* codes, const float* scales, int64_t rows,
+                            int inputs, int outputs, int experts, const int32_t* perm, const int32_t* offsets,
+                            void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- AdamW over a list of tensors ------------------------------------------
  * One step with decoupled weight decay, in FP32 arithmetic:

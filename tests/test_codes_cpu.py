@@ -36,3 +36,23 @@ def test_refusals():
             decode(**bad)
     encode(rows=0, x=None, codes=None, scales=None)
     decode(rows=0, codes=None, scales=None, out=None)
+
+
+def test_outer_refusals():
+    from ictc_o3 import _native as nat
+    if not os.path.exists(nat.library_path()):
+        pytest.skip("library not built")
+    takes = nat.lib().ictc_expert_outer_takes_codes
+    assert takes(0, 32, 64, 10, 64, 32) and takes(1, 16, 8, 10, 8, 8)
+    for bad in ((5, 32, 64, 10, 64, 32), (0, 8, 64, 10, 64, 32), (0, 32, 63, 10, 64, 32), (0, 32, 64, 0, 64, 32),
+                (0, 32, 64, 10, 62, 32), (0, 32, 64, 10, 64, 30), (1, 32, 64, 10, 4, 8), (0, 32, 64, 10, 0, 32)):
+        assert not takes(*bad), bad
+
+    def outer(dtype=0, grad=16, ldg=8, codes=16, scales=16, rows=4, inputs=8, outputs=8, perm=16, off=16, out=16):
+        nat.call("ictc_expert_outer_codes", dtype, grad, ldg, codes, scales, rows, inputs, outputs, 2, perm, off, out, None,
+                 16, 1 << 30, None)
+
+    for bad in (dict(dtype=3), dict(grad=None), dict(grad=20), dict(ldg=4), dict(ldg=9), dict(codes=None), dict(scales=None),
+                dict(rows=0), dict(inputs=6), dict(outputs=6), dict(perm=None), dict(off=None), dict(out=None)):
+        with pytest.raises(ValueError):
+            outer(**bad)

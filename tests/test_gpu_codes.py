@@ -134,7 +134,9 @@ def _linear(rows, experts, inputs, outputs, dtype, device):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,experts,inputs,outputs", [(0, 2, 8, 8), (1, 3, 16, 5), (70, 4, 7, 33), (300, 10, 128, 128),
-                                                         (5000, 3, 200, 333), (4096, 2, 512, 256), (999, 1, 1, 1)])
+                                                         (5000, 3, 200, 333), (4096, 2, 512, 256), (999, 1, 1, 1),
+                                                         (2000, 7, 136, 72), (20000, 10, 264, 128), (60000, 3, 520, 264),
+                                                         (333, 90, 128, 64), (7, 1, 8, 8)])
 def test_expert_linear(device, rows, experts, inputs, outputs, dtype):
     """Result and row gradient are those of whole rows, bit for bit; the weights' and biases' gradients those that the
     decoded rows have."""
