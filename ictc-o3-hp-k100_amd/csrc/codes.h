@@ -24,9 +24,22 @@ __device__ __forceinline__ int code_of(float x, float inverse) {
   return (int)fminf(fmaxf(rintf(held(x * inverse)), -127.f), 127.f);
 }
 
-template <typename T>
-__device__ __forceinline__ float code_value(int code, float scale) {
-  return (float)(T)held((float)code * scale);
+// N code values in FP32, code times scale.  A code is taken as code + 128, which one instruction makes a float of, and the
+// product's surplus of 128 scales, a power of two of them, leaves by the same rounding: fma(code + 128, scale, -128 scale)
+// is code times scale rounded once.  Where 128 scales are past FP32, code by code.
+template <int N>
+__device__ __forceinline__ void code_products(const uint32_t* raw, float scale, float (&v)[N]) {
+  if (__builtin_amdgcn_ballot_w64(scale > 0x1p120f)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = held((float)(int8_t)(raw[e / 4] >> 8 * (e % 4)) * scale);
+    return;
+  }
+  const float surplus = -128.f * scale;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const uint32_t biased = raw[e / 4] ^ 0x80808080u;
+    v[e] = held(__builtin_fmaf((float)(biased >> 8 * (e % 4) & 255u), scale, surplus));
+  }
 }
 
 typedef uint32_t u32_byte __attribute__((aligned(1)));

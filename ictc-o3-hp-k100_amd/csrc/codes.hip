@@ -83,8 +83,7 @@ __global__ __launch_bounds__(256) void decode_kernel(const int8_t* __restrict__ 
     for (int i = 0; i < kAtOnce; ++i) {
       if (b0 + i * TEAMS >= blocks) break;
       float v[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = held((float)q[i].e[e] * scale[i]);
+      code_products<V>(q[i].raw, scale[i], v);
       const int c = at[i].column + lane * V;
       store_chunk(out + at[i].row * width + c, width - c, v);
     }

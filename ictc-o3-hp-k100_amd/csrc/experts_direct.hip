@@ -407,15 +407,18 @@ struct CodeChunk {
   float scale;
   __device__ __forceinline__ u32x4 values() const {
     Chunk<T> c;
+    float v[kChunk<T>];
+    code_products<kChunk<T>>(codes.raw, scale, v);
 #pragma unroll
-    for (int e = 0; e < kChunk<T>; ++e) c.e[e] = (T)held((float)codes.e[e] * scale);
+    for (int e = 0; e < kChunk<T>; ++e) c.e[e] = (T)v[e];
     return c.raw;
   }
 };
 
 // Gradients of W (g^T x; operand A is x, so a lane ends with four consecutive columns of one row) and of b over one
 // range of rows: see experts_outer_kernel.  CODES: x is codes [rows, K], with scales; its chunks become values on their way
-// to LDS (131,072 rows of 512 -> 512 bfloat16: CODES_US us, and 40 + 124 decoded to memory first).
+// to LDS, behind the step's products (131,072 rows of 512 -> 512 bfloat16: 143 us, and 40 + 124 decoded to memory first; with
+// the codes asked for two steps ahead, and so one more set of row numbers, 165).
 template <typename T, bool ALIGNED, bool CODES, int TA, int TB, int S, int GA, int GB>
 __global__ __launch_bounds__(GA * GB * 64, 2) void experts_direct_outer_kernel(
     const T* __restrict__ gy, int64_t ldg, int M, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ codes,

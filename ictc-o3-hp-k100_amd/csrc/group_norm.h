@@ -88,7 +88,7 @@ struct Source<T, EV, true> {
   union {
     int8_t e[8];
     uint16_t b2;
-    uint32_t b4;
+    uint32_t b4, word[2];
     u32x2 b8;
   } raw;
   float scale;
@@ -105,8 +105,9 @@ struct Source<T, EV, true> {
     scale = a.scales[block];
   }
   __device__ __forceinline__ void values(float (&v)[EV]) const {
+    code_products<EV>(raw.word, scale, v);
 #pragma unroll
-    for (int e = 0; e < EV; ++e) v[e] = code_value<T>(raw.e[e], scale);
+    for (int e = 0; e < EV; ++e) v[e] = (float)(T)v[e];
   }
 };
 
