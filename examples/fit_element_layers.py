@@ -1,12 +1,14 @@
 """Fits a small interatomic potential whose atomic layers are chosen by element, on energies and forces.
 
-    python examples/fit_element_layers.py [--steps 300] [--state-bits 8] [--cells 4]
+    python examples/fit_element_layers.py [--steps 300] [--state-bits 8] [--cells 4] [--groups 8 [--save-bits 8]]
 
 Each atom gathers its neighbours with the graph message (degree 0 and 1 harmonics, radial gates), the invariants of
 the result go through layer norm, a linear of the atom's own element, SiLU and a second such linear to an atomic
 energy, and forces are minus the gradient by the positions.  The loss on forces differentiates that gradient again, so
 the norm and the element linears run forward, backward and through their second derivatives; AdamW updates all
-parameters at once with the gradients' norm bounded.  The data are jittered FCC cells of four elements under a pair
+parameters at once with the gradients' norm bounded.  With --groups the element's features come of the embedding operator
+and the first linear is followed by a group norm with its SiLU in one, and with --save-bits 8 these layers keep their rows
+in 8 bits between the passes.  The data are jittered FCC cells of four elements under a pair
 potential with element-dependent strengths.
 """
 from __future__ import annotations
@@ -22,8 +24,8 @@ PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 
 if PKG not in sys.path:
     sys.path.insert(0, PKG)
 
-from ictc_o3 import (AdamW, PackedGraphMessage, direction_harmonics, expert_linear, expert_order,  # noqa: E402
-                     layer_norm, normalized_silu)
+from ictc_o3 import (AdamW, PackedGraphMessage, direction_harmonics, embedding, expert_linear, expert_order,  # noqa: E402
+                     group_norm, layer_norm, normalized_silu)
 from ictc_o3.ops.activation import radial_embedding  # noqa: E402
 from mace_ictc.hp import radius_graph_pbc  # noqa: E402
 
@@ -61,8 +63,9 @@ def systems(cells, n, seed, device):
 
 
 class ElementPotential(torch.nn.Module):
-    def __init__(self, channels=32, hidden=64, seed=0, device="cuda"):
+    def __init__(self, channels=32, hidden=64, seed=0, device="cuda", groups=None, save_bits=None):
         super().__init__()
+        self.groups, self.save_bits = groups, save_bits
         self.message = PackedGraphMessage.create(channels=channels, input_lmax=0, edge_lmax=1, output_lmax=1,
                                                  device=device)
         self.channels = channels
@@ -81,6 +84,7 @@ class ElementPotential(torch.nn.Module):
         self.node_norm = norm(2 * channels)
         self.weight_1, self.bias_1 = weight(ELEMENTS, hidden, 2 * channels), weight(ELEMENTS, hidden)
         self.weight_2, self.bias_2 = weight(ELEMENTS, 1, hidden), weight(ELEMENTS, 1)
+        self.hidden_norm = norm(hidden) if groups else None
 
     def forward(self, pos, element, order, src, dst, shift):
         """Atomic energies [N]; `order` is expert_order(element, ELEMENTS), shared by every step of a batch."""
@@ -90,18 +94,23 @@ class ElementPotential(torch.nn.Module):
         radial = normalized_silu(layer_norm(radial_embedding(r, CUTOFF) @ self.radial_1.t(), *self.radial_norm))
         # (the norm undoes the basis' decay towards the cutoff: the gates get it back)
         gates = (radial @ self.radial_2.t()) * (0.5 + 0.5 * torch.cos(math.pi * r / CUTOFF))[:, None]
-        m = self.message(self.embedding[element], harmonics, gates, src, dst)
+        rows = embedding(self.embedding, element, order=order) if self.groups else self.embedding[element]
+        m = self.message(rows, harmonics, gates, src, dst)
         scalars, vectors = m[:, :self.channels], m[:, self.channels:].reshape(-1, 3, self.channels)
         x = layer_norm(torch.cat([scalars, (vectors * vectors).sum(1)], 1), *self.node_norm)
-        x = normalized_silu(expert_linear(x, self.weight_1, order, self.bias_1))
-        return expert_linear(x, self.weight_2, order, self.bias_2).squeeze(1)
+        x = expert_linear(x, self.weight_1, order, self.bias_1, save_bits=self.save_bits)
+        if self.groups:
+            x = group_norm(x, self.groups, *self.hidden_norm, activation="silu", save_bits=self.save_bits)
+        else:
+            x = normalized_silu(x)
+        return expert_linear(x, self.weight_2, order, self.bias_2, save_bits=self.save_bits).squeeze(1)
 
 
-def train(steps=300, cells=4, n=3, state_bits=32, lr=4e-3, seed=0, device="cuda", log=None):
+def train(steps=300, cells=4, n=3, state_bits=32, lr=4e-3, seed=0, device="cuda", log=None, groups=None, save_bits=None):
     """(model, [(energy loss, force loss, gradient norm) of each step])."""
     torch.manual_seed(seed)
     data = systems(cells, n, seed, device)
-    model = ElementPotential(seed=seed, device=device)
+    model = ElementPotential(seed=seed, device=device, groups=groups, save_bits=save_bits)
     opt = AdamW([p for p in model.parameters() if p.requires_grad], lr=lr, weight_decay=1e-4, max_norm=10.0,
                 state_bits=state_bits)
     order = expert_order(data["element"], ELEMENTS)
@@ -131,5 +140,8 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=300)
     ap.add_argument("--cells", type=int, default=4)
     ap.add_argument("--state-bits", type=int, choices=(8, 32), default=32)
+    ap.add_argument("--groups", type=int, default=None)
+    ap.add_argument("--save-bits", type=int, choices=(8,), default=None)
     a = ap.parse_args()
-    train(a.steps, a.cells, state_bits=a.state_bits, log=lambda text: print(text, flush=True))
+    train(a.steps, a.cells, state_bits=a.state_bits, log=lambda text: print(text, flush=True), groups=a.groups,
+          save_bits=a.save_bits)
