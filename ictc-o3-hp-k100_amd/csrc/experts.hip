@@ -360,14 +360,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 4) void experts_few_kernel(const T*
 // lane's at once.  One block does it alone; of several, each has `span` rows and adds up, from all blocks' counts
 // ([blocks, experts + 1], the kernel below), what lies before its own.
 //
-// More than 1,023 experts (entries of a table) are ordered by the low half of the id's bits and then, stably, by the high
-// one: the first pass leaves ids and row numbers, the second row numbers and sorted ids, of which order_offsets_kernel
-// makes the offsets (425,991 rows of 7,921 ids: 36 us, 125 by the general sort).
-constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16, kOrderBlocks = 256;
+// More than 1,023 experts (entries of a table) are ordered by the low bits of the id and then, stably, by the ones above, up
+// to ten at a time: each pass leaves ids and row numbers, the last the row numbers and sorted ids, of which
+// order_offsets_kernel makes the offsets (425,991 rows of 7,921 ids: 36 us, 125 by the general sort).
+constexpr int kOrderExperts = 1023, kOrderWaves = 16, kOrderAtOnce = 16, kOrderBlocks = 1024;
 constexpr int kOrderRows = kOrderWaves * kOrderAtOnce * 64;
 
-// What a pass takes and leaves: row i's id, or of the second pass the key and number that the first left at i.
-enum class Pass { kOnly, kFirst, kSecond };
+// What a pass takes and leaves: row i's id, or of a later pass the key and number that the one before left at i.
+enum class Pass { kOnly, kFirst, kLater };
 struct OrderIn {
   const int64_t* ids;
   const int *keys, *rows;
@@ -379,7 +379,7 @@ struct OrderOut {
 
 template <Pass P>
 __device__ __forceinline__ uint32_t order_key(const OrderIn& in, int row) {
-  if (P == Pass::kSecond) return in.keys[row];
+  if (P == Pass::kLater) return in.keys[row];
   const int64_t id = in.ids[row];
   return (uint64_t)id < (uint64_t)in.experts ? (uint32_t)id : (uint32_t)in.experts;
 }
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, 
     const int digit = place[i] & 1023u, below = place[i] >> 10 & 63u, lanes = place[i] >> 16;
     if (ok) {
       const int to = mine[digit] + below;
-      out.perm[to] = P == Pass::kSecond ? in.rows[r0 + lane] : r0 + lane;
+      out.perm[to] = P == Pass::kLater ? in.rows[r0 + lane] : r0 + lane;
       if (P != Pass::kOnly) out.keys[to] = (int)key[i];
     }
     wave_meet();
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restric
 
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
-int id_bits(int experts) {
+int id_bits(int64_t experts) {
   int bits = 1;
   while (experts >> bits) ++bits;
   return bits;
@@ -542,30 +542,30 @@ int order_span(int64_t rows, int bits) {
   return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(262144 / blocks, (rows / blocks + 1023) / 1024 * 1024));
 }
 
-// The passes over the bits of an id: none (the general sort), one, or two.
+// The passes over the bits of an id, none: the general sort.
 struct OrderPlan {
-  int passes, bits, low, span;   // of an id; of the first digit
-  int64_t blocks, counts;        // of each pass; ints of its counts
+  int passes, bits, digit, span;   // bits of an id and of a pass; rows of a block
+  int64_t blocks, counts;          // of each pass; ints of its counts
 };
 
 OrderPlan order_plan(int64_t rows, int64_t experts) {
   OrderPlan p = {};
-  if (experts >= 1 << 20) return p;
-  p.bits = id_bits((int)experts);
-  p.passes = experts <= kOrderExperts ? 1 : 2;
-  p.low = p.passes == 1 ? p.bits : (p.bits + 1) / 2;
-  p.span = order_span(rows, p.low);
+  p.bits = id_bits(experts);
+  p.passes = experts <= kOrderExperts ? 1 : (p.bits + 9) / 10;
+  p.digit = (p.bits + p.passes - 1) / p.passes;
+  p.span = order_span(rows, p.digit);
   if (p.span == 0) return OrderPlan{};
   p.blocks = std::max<int64_t>(1, tiles_of(rows, p.span));
-  const int64_t groups = p.passes == 1 ? experts + 1 : int64_t(1) << p.low;
+  const int64_t groups = p.passes == 1 ? experts + 1 : int64_t(1) << p.digit;
   p.counts = rows <= p.span ? 0 : p.blocks * groups;
   return p;
 }
 
+// Ids and row numbers between two passes, both twice where there are more than two; the sorted ids.
 int64_t order_bytes(int64_t rows, int64_t experts) {
   const OrderPlan p = order_plan(rows, experts);
   if (p.passes == 0) return ictc_csr_workspace_bytes(rows, experts);
-  return 4 * (p.counts + (p.passes == 2 ? 3 * rows : 0));
+  return 4 * (p.counts + (p.passes == 1 ? 0 : p.passes == 2 ? 3 : 4) * rows);
 }
 
 template <Pass P>
@@ -590,12 +590,18 @@ int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int
     order_pass<Pass::kOnly>(in, n, p.bits, p, counts, {perm, nullptr, off}, st);
     return dense_status("expert_order launch");
   }
-  int *keys = (int*)workspace + p.counts, *numbers = keys + rows, *sorted = numbers + rows;
-  in.groups = 1 << p.low;
-  order_pass<Pass::kFirst>(in, n, p.low, p, counts, {numbers, keys, nullptr}, st);
-  const OrderIn next = {nullptr, keys, numbers, (int)experts, p.low, 1 << (p.bits - p.low)};
-  order_pass<Pass::kSecond>(next, n, p.bits - p.low, p, counts, {perm, sorted, nullptr}, st);
-  hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, st, sorted, n, (int)experts, off);
+  int* half[2][2];   // ids and row numbers that pass 0, 2, .. and 1, 3, .. leave; the last pass: sorted ids
+  for (int k = 0; k < 4; ++k) half[k / 2][k % 2] = (int*)workspace + p.counts + k * rows;
+  in.groups = 1 << p.digit;
+  order_pass<Pass::kFirst>(in, n, p.digit, p, counts, {half[0][1], half[0][0], nullptr}, st);
+  for (int k = 1; k < p.passes; ++k) {
+    int *const *from = half[(k - 1) % 2], *const *to = half[k % 2];
+    const int shift = k * p.digit, bits = std::min(p.digit, p.bits - shift);
+    const OrderIn next = {nullptr, from[0], from[1], (int)experts, shift, 1 << bits};
+    order_pass<Pass::kLater>(next, n, bits, p, counts, {k + 1 < p.passes ? to[1] : perm, to[0], nullptr}, st);
+  }
+  hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, st, half[(p.passes - 1) % 2][0],
+                     n, (int)experts, off);
   return dense_status("expert_order launch");
 }
 

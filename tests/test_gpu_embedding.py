@@ -252,7 +252,8 @@ def test_offsets_past_32_bits(device):
 
 @pytest.mark.parametrize("rows,entries", [(0, 1024), (1, 1023), (1, 1024), (5, 65535), (300, 140003), (16384, 1500),
                                           (20000, 5000), (425991, 7921), (70000, 1048575), (70000, 1048576),
-                                          (4300000, 2000)])
+                                          (4300000, 2000), (5000, 33554431), (3, 40000000), (16777216, 10),
+                                          (16777217, 10)])
 def test_order_of_many_entries(device, rows, entries):
     """The rows' order by id: stable, ids outside last, and where each id begins, whichever passes make it."""
     from ictc_o3 import _native as nat
@@ -272,3 +273,31 @@ def test_order_of_many_entries(device, rows, entries):
     assert torch.equal(perm[:rows].long(), ref.indices)
     counts = torch.bincount(key, minlength=entries + 1)
     assert torch.equal(off.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+
+
+def test_graph_replays_of_very_many_rows(device):
+    """More rows than the counted passes take: the general sort, captured and replayed."""
+    from ictc_o3 import embedding
+    table = torch.randn(50, 2, device=device, requires_grad=True)
+    ids = torch.randint(-1, 50, (16777300,), device=device, generator=torch.Generator(device).manual_seed(1))
+    gy = torch.ones(16777300, 2, device=device)
+
+    def step():
+        return torch.autograd.grad(embedding(table, ids), table, gy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        ids.copy_(ids.roll(1001) if k else ids.flip(0))
+        ids[: 1000 * (k + 1)] = k
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager), k
+        ref = torch.bincount(ids[ids >= 0], minlength=50)
+        assert ((held[:, 0].double() - ref).abs() <= 700 * 2.0 ** -24 * ref).all()
