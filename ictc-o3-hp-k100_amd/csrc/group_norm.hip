@@ -1,5 +1,5 @@
 // The group norm's entry points: checks, workspaces and the choice of the element type (group_norm.h has the kernels).
-#include "group_norm.h"
+#include "group_norm_launch.h"
 
 namespace {
 

@@ -1,0 +1,6 @@
+// The group norm's kernels of the second derivative for one element type.
+#include "group_norm_launch.h"
+
+namespace ictc {
+template void group_norm_bwd2<float>(const GroupNormCall&);
+}  // namespace ictc

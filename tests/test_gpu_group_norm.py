@@ -24,11 +24,15 @@ SHAPES = [  # samples, positions, channels, groups: one position
     (1, 1, 4, 1), (37, 1, 64, 8), (3, 1, 64, 64), (5, 1, 30, 5), (9, 1, 35, 5), (9, 1, 96, 4), (33, 1, 13, 1),
     (3, 1, 512, 1), (4, 1, 1024, 2), (3, 1, 1000, 1), (3, 1, 2048, 1), (5, 1, 600, 200), (1100, 1, 24, 3),
     (3, 1, 2176, 1), (5, 1, 8192, 2), (2, 1, 5001, 1), (0, 1, 16, 4),
+    (3, 1, 8192, 1), (5, 1, 4096, 1), (4, 1, 6144, 2), (2, 1, 16384, 1), (4, 1, 999, 3), (7, 1, 77, 7), (3, 1, 1010, 1),
+    (5, 1, 45, 5), (3, 1, 2001, 1), (6, 1, 18, 3), (4, 1, 33, 3),
     # a few positions
+    (9, 5, 45, 5), (7, 3, 77, 7), (5, 4, 26, 2), (11, 9, 128, 8), (5, 16, 90, 3), (3, 25, 27, 3), (4, 7, 1022, 2),
     (7, 9, 64, 8), (3, 128, 16, 2), (5, 33, 30, 5), (6, 2, 7, 7), (4, 16, 64, 2), (2, 3, 256, 1), (50, 5, 36, 12),
     # blocks, one sample after another or many
     (3, 300, 64, 8), (2, 257, 330, 11), (40, 200, 48, 2), (700, 140, 40, 1), (3, 513, 5, 5), (2, 100, 900, 3),
     (1, 65, 2048, 8),
+    (30, 70, 64, 64), (3, 400, 14, 7), (5, 300, 36, 12),
     # parts
     (1, 5000, 64, 8), (2, 4099, 30, 5), (1, 700, 2304, 1), (2, 3, 8000, 2), (1, 20011, 12, 4), (3, 1, 65536, 1),
     (2, 0, 8, 2)]
