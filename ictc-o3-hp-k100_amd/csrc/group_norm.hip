@@ -5,7 +5,7 @@ namespace {
 
 int64_t workspace_bytes(int dtype, int pass, int64_t samples, int64_t positions, int channels, int groups) {
   if (samples == 0 || positions == 0) samples = 0, positions = 1;   // (as the calls take them)
-  const Plan p = plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups);
+  const Plan p = plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups, pass == 2);
   const bool parts = p.form == Form::kParts;
   const int64_t units = samples * groups, each = units * p.tile.splits * p.tile.tiles_per;
   if (pass == 0) return parts ? each * 16 + units * 8 : 0;
@@ -72,7 +72,7 @@ int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t posit
   a.ws = workspace, a.ws_bytes = workspace_bytes, a.stream = (hipStream_t)stream;
   if (!workspace_fits(a, dtype, 0))
     return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: workspace smaller than ictc_group_norm_workspace_bytes");
-  if (codes && !plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups).coded)
+  if (codes && !plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups, false).coded)
     if (const int rc = ictc_codes_encode(dtype, x, channels, samples * positions, channels, codes, scales, stream)) return rc;
   GN_TYPED(group_norm_fwd)
   return dense_status("group_norm_fwd launch");

@@ -1,7 +1,7 @@
 // Which form of the group norm's kernels a call takes, and its launches.
 #pragma once
 #include "group_norm_rows.h"
-#include "group_norm_tiles.h"
+#include "group_norm_span.h"
 
 namespace {
 
@@ -10,7 +10,7 @@ enum class Form { kRows, kTiles, kParts };
 struct Plan {
   Form form;
   int ev, n;   // elements of a chunk; rows: chunks a lane
-  bool part;   // rows: a group's last chunk is not whole
+  bool part;   // rows: a group's last chunk is not whole; tiles: whole chunks over groups (group_norm_span.h)
   RowsPlan rows;
   TilePlan tile;
   int64_t parts;   // rows of partial sums by channel
@@ -24,12 +24,13 @@ inline int power_of_two(int64_t n) {
 }
 
 // A team for samples of so many positions of chunks: its lanes along a position and in all, and the chunks of a lane (0: too
-// large).  Of teams that divide the positions differently the one with the fewest idle lanes, then the largest.
+// large).  Of teams that divide the positions differently the one with the fewest idle lanes, then the largest.  (1,024
+// samples of 256 x 64 FP32 channels, each its own group, by teams of a wave, each load 64 lines: 168 us forward.)
 struct RowsChoice {
   int across, team, n;
 };
 
-inline RowsChoice rows_choice(int64_t positions, int chunks) {
+inline RowsChoice rows_choice(int64_t positions, int chunks, int groups, int bytes) {
   const int across = std::min(64, power_of_two(chunks));
   if (positions == 1) {
     if (chunks <= 256) return {across, across, (chunks + 63) / 64};
@@ -43,12 +44,15 @@ inline RowsChoice rows_choice(int64_t positions, int chunks) {
     const int64_t n = (positions + strips - 1) / strips;
     const double used = (double)positions / (double)(strips * n);
     if (n > 4 || (strips > 1 && strips / 2 >= positions)) continue;
+    // a wave's groups side by side: 64 bytes of a position, or all there are
+    if (std::min(64 / (across * strips), groups) * bytes < std::min(64, groups * bytes)) continue;
     if (used > most + 0.01) most = used, best = {across, across * strips, (int)n};
   }
   return best;
 }
 
-inline Plan plan_of(int element, int64_t samples, int64_t positions, int channels, int groups) {
+// second: of the gradients of the gradients
+inline Plan plan_of(int element, int64_t samples, int64_t positions, int channels, int groups, bool second) {
   Plan p = {};
   const int per = channels / groups;
   p.ev = 16 / element;
@@ -57,7 +61,7 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
   // have one or two channels.  (Fours of eight: there are one fewer of these than twice the others.)
   const int whole = 16 / element;
   const bool part = p.ev < 4 && p.ev < whole && per >= whole;
-  RowsChoice choice = rows_choice(positions, part ? (per + whole - 1) / whole : per / p.ev);
+  RowsChoice choice = rows_choice(positions, part ? (per + whole - 1) / whole : per / p.ev, groups, per * element);
   if (choice.team == 256 && (part || p.ev != whole || choice.n * p.ev > 32)) choice = {};   // (kernels there are none of)
   if (choice.n > 0) {
     p.form = Form::kRows;
@@ -89,18 +93,27 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
       p.coded = lanes;
     return p;
   }
-  const int chunks = per / p.ev;
   TilePlan& t = p.tile;
+  // whole groups of 128 bytes a position or more, where there are; of samples that a block takes whole down to 64 while there
+  // are few blocks; and of whole chunks over groups 768.  These where a chunk that divides a group is a quarter of 16 bytes or
+  // less, and from eight million elements: chunks of a group / over groups in us, forward and gradients: 1,024 samples of 256
+  // x 64 FP32, each channel its group, 110 / 95, bfloat16 121 / 78; 500 of 1,000 x 30 bfloat16 in five 120 / 75; 300 of 3,000
+  // x 35 in seven 230 / 172; one of 131,072 x 65 in thirteen 110 / 97; the other way 300 of 300 x 35 in seven 41 / 46, three
+  // of 40,000 x 21 49 / 56; FP32 by twos, 5,000 of 100 x 30 in three 101 / 110.
+  const int want = std::max(1, 128 / (per * element)), span = std::max(1, std::min(64, 768 / (per * element)));
+  p.part = !second && p.ev * 4 <= whole && samples * positions * channels >= 1 << 23 &&
+           (span * per + whole - 1) / whole <= kThreads;
+  if (p.part) p.ev = whole;
+  const int chunks = (per + p.ev - 1) / p.ev;   // (of a group alone)
+  const int at_once = p.ev >= 8 || p.part ? 2 : 4, few = 10 * at_once;   // positions of a thread that are few
   t.chunks = chunks;
-  t.tiles_per = (chunks + kThreads - 1) / kThreads;
+  t.tiles_per = p.part ? 1 : (chunks + kThreads - 1) / kThreads;
   if (t.tiles_per == 1) {
-    // whole groups of 128 bytes a position or more, where there are
-    const int want = std::max(1, 128 / (per * element));
-    t.groups = std::min(groups, std::min(want, kThreads / chunks));
-    // down to 32 bytes while there are few blocks, of samples that a block takes whole
-    while (positions <= 32 * (kThreads / chunks) && t.groups > 1 && t.groups * per * element > 64 && samples * ((groups + t.groups - 1) / t.groups) < 512)
+    t.groups = std::min(groups, p.part ? span : std::min(want, kThreads / chunks));
+    while (positions <= few * (kThreads / chunks) && t.groups > 1 && t.groups * per * element > 64 &&
+           samples * ((groups + t.groups - 1) / t.groups) < 512)
       t.groups = (t.groups + 1) / 2;
-    t.lanes = t.groups * chunks;
+    t.lanes = p.part ? (t.groups * per + whole - 1) / whole : t.groups * chunks;
     t.tiles = (groups + t.groups - 1) / t.groups;
   } else {
     t.groups = 1;
@@ -111,16 +124,16 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
   t.splits = 1;
   t.per_split = positions;
   const int64_t blocks = samples * t.tiles, steps = (positions + t.rows - 1) / t.rows;
-  if (t.tiles_per == 1 && (blocks >= 512 || steps <= 32)) {
+  if (t.tiles_per == 1 && (blocks >= 512 || steps <= few)) {
     p.form = Form::kTiles;
   } else {
     p.form = Form::kParts;
-    const int64_t most = (steps + 3) / 4;   // (four positions a thread at least)
+    const int64_t most = (steps + at_once - 1) / at_once;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(most, (2048 + blocks) / (blocks + 1)));
     t.per_split = (steps + splits - 1) / splits * t.rows;
     t.splits = (int)((positions + t.per_split - 1) / t.per_split);
   }
-  t.powers = t.lanes <= 64 && power_of_two(t.lanes) == t.lanes && power_of_two(chunks) == chunks;
+  t.powers = t.lanes <= 64 && power_of_two(t.lanes) == t.lanes && (p.part || power_of_two(chunks) == chunks);
   t.slots = (int)std::max<int64_t>(1, std::min<int64_t>(samples, 2048 / (t.tiles * t.splits)));
   p.parts = (int64_t)t.slots * t.splits;
   return p;
@@ -130,7 +143,10 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
 inline dim3 unit_blocks(int64_t units) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(1 << 20, (units + 3) / 4))); }
 
 // Few parts of a group, for tiles of few whole groups: the blocks that need their sums add them.
-inline bool own_parts(const TilePlan& p) { return p.tiles_per == 1 && p.splits <= kOwnParts && p.groups <= kOwnGroups; }
+inline bool own_parts(const Plan& p) {
+  const TilePlan& t = p.tile;
+  return t.tiles_per == 1 && t.splits <= kOwnParts && (p.part || t.groups <= kOwnGroups);
+}
 
 #define GN_LAUNCH(kernel, ...) hipLaunchKernelGGL((kernel), grid, dim3(256), 0, a.stream, __VA_ARGS__)
 #define GN_TEAM(N_, WIDE_, PART_, kernel, ...)                        \
@@ -175,6 +191,10 @@ void launch_fwd(const ictc::GroupNormCall& a, const Plan& p) {
     return;
   }
   const dim3 grid((unsigned)p.tile.slots * p.tile.splits * p.tile.tiles);
+  if (p.form == Form::kTiles && p.part) {
+    if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_fwd_kernel<T, EV, SILU>), a, p.tile, per, (double*)nullptr);
+    return;
+  }
   if (p.form == Form::kTiles) {
     hipLaunchKernelGGL((gn_tile_fwd_kernel<T, EV, SILU>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per);
     return;
@@ -184,13 +204,21 @@ void launch_fwd(const ictc::GroupNormCall& a, const Plan& p) {
   double* part = (double*)a.ws;
   float* mean = a.mean ? a.mean : (float*)(part + units * parts * 2);
   float* rstd = a.mean ? a.rstd : mean + units;
-  hipLaunchKernelGGL((gn_part_stats_kernel<T, EV>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per, part);
-  const bool own = own_parts(p.tile);
+  if (p.part) {
+    if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_fwd_kernel<T, EV, SILU>), a, p.tile, per, part);
+  } else {
+    GN_LAUNCH((gn_part_stats_kernel<T, EV>), a, p.tile, per, part);
+  }
+  const bool own = own_parts(p);
   if (!own)
     hipLaunchKernelGGL(gn_part_moments_kernel, unit_blocks(units), dim3(256), 0, a.stream, part, units, parts,
                        (double)per * (double)a.positions, a.eps, mean, rstd);
-  hipLaunchKernelGGL((gn_part_fwd_kernel<T, EV, SILU>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per,
-                     own ? part : nullptr, mean, rstd);
+  const double* parts_of = own ? part : nullptr;
+  if (p.part) {
+    if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of, mean, rstd);
+  } else {
+    GN_LAUNCH((gn_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of, mean, rstd);
+  }
 }
 
 template <typename T>
@@ -232,18 +260,28 @@ void launch_bwd(const ictc::GroupNormCall& a, const Plan& p) {
     const dim3 grid(p.rows.blocks_x, p.rows.blocks_y);
     GN_ROWS((gn_rows_bwd_kernel<T, EV, N, WIDE, PART, SILU, EIGHT>), a, p.rows, per, pw, pb)
   } else {
-    const bool parts = p.form == Form::kParts, own = own_parts(p.tile);
+    const bool parts = p.form == Form::kParts, own = own_parts(p);
     const dim3 grid((unsigned)p.tile.slots * p.tile.splits * p.tile.tiles);
-    if (parts)
-      hipLaunchKernelGGL((gn_tile_bwd_kernel<T, EV, SILU, EIGHT, false>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per,
-                         ws.part, pw, pb);
-    else
-      hipLaunchKernelGGL((gn_tile_bwd_kernel<T, EV, SILU, EIGHT, true>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per,
-                         (float*)nullptr, pw, pb);
+    float* none = nullptr;
+    if (p.part) {
+      if constexpr (EV == kChunk<T>) {
+        if (parts)
+          GN_LAUNCH((gn_span_bwd_kernel<T, EV, SILU, EIGHT, false>), a, p.tile, per, ws.part, pw, pb);
+        else
+          GN_LAUNCH((gn_span_bwd_kernel<T, EV, SILU, EIGHT, true>), a, p.tile, per, none, pw, pb);
+      }
+    } else if (parts) {
+      GN_LAUNCH((gn_tile_bwd_kernel<T, EV, SILU, EIGHT, false>), a, p.tile, per, ws.part, pw, pb);
+    } else {
+      GN_LAUNCH((gn_tile_bwd_kernel<T, EV, SILU, EIGHT, true>), a, p.tile, per, none, pw, pb);
+    }
     if (parts && a.out) {
       const float* sums = launch_sums<2>(a, p, ws, own);
-      hipLaunchKernelGGL((gn_part_bwd_kernel<T, EV, SILU, EIGHT>), grid, dim3(kThreads), 0, a.stream, a, p.tile, per, sums,
-                         own);
+      if (p.part) {
+        if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_part_bwd_kernel<T, EV, SILU, EIGHT>), a, p.tile, per, sums, own);
+      } else {
+        GN_LAUNCH((gn_part_bwd_kernel<T, EV, SILU, EIGHT>), a, p.tile, per, sums, own);
+      }
     }
   }
   launch_channels<T>(a, p, pw, pb);
@@ -258,7 +296,7 @@ void launch_bwd2(const ictc::GroupNormCall& a, const Plan& p) {
     const dim3 grid(p.rows.blocks_x, p.rows.blocks_y);
     GN_ROWS((gn_rows_bwd2_kernel<T, EV, N, WIDE, PART, SILU, EIGHT>), a, p.rows, per, pw, pb)
   } else {
-    const bool own = own_parts(p.tile);
+    const bool own = own_parts(p);
     const dim3 grid((unsigned)p.tile.slots * p.tile.splits * p.tile.tiles);
     float* none = nullptr;
     const float* sums = nullptr;
@@ -280,8 +318,8 @@ void launch_bwd2(const ictc::GroupNormCall& a, const Plan& p) {
 
 namespace ictc {
 
-#define GN_CHUNKS(launch)                                      \
-  const Plan p = plan_of((int)sizeof(T), a.samples, a.positions, a.channels, a.groups); \
+#define GN_CHUNKS(launch, second)                              \
+  const Plan p = plan_of((int)sizeof(T), a.samples, a.positions, a.channels, a.groups, second); \
   if constexpr (sizeof(T) == 2) {                              \
     if (p.ev == 8) { constexpr int EV = 8; return launch; }    \
   }                                                            \
@@ -292,7 +330,7 @@ namespace ictc {
 
 template <typename T>
 void group_norm_fwd(const GroupNormCall& a) {
-  GN_CHUNKS((a.silu ? launch_fwd<T, EV, true>(a, p) : launch_fwd<T, EV, false>(a, p)))
+  GN_CHUNKS((a.silu ? launch_fwd<T, EV, true>(a, p) : launch_fwd<T, EV, false>(a, p)), false)
 }
 
 #define GN_KIND(f) \
@@ -301,11 +339,11 @@ void group_norm_fwd(const GroupNormCall& a) {
 
 template <typename T>
 void group_norm_bwd(const GroupNormCall& a) {
-  GN_CHUNKS(GN_KIND(launch_bwd))
+  GN_CHUNKS(GN_KIND(launch_bwd), false)
 }
 template <typename T>
 void group_norm_bwd2(const GroupNormCall& a) {
-  GN_CHUNKS(GN_KIND(launch_bwd2))
+  GN_CHUNKS(GN_KIND(launch_bwd2), true)
 }
 
 }  // namespace ictc

@@ -54,8 +54,8 @@ struct TileAt {
 };
 
 // K values of every thread, added over the positions' threads: in those of row 0, left in lds [K][256].
-template <typename V, int K>
-__device__ __forceinline__ void sum_rows(V (&s)[K], const TilePlan& p, const TileAt& at, V* lds) {
+template <typename V, int K, typename At>
+__device__ __forceinline__ void sum_rows(V (&s)[K], const TilePlan& p, const At& at, V* lds) {
   __syncthreads();
   if (p.powers) {   // over a wave's lanes, then the waves in order
     sum_high(s, p.lanes);
@@ -129,8 +129,8 @@ __device__ __forceinline__ void sum_all(V (&s)[K], const TilePlan& p, const Tile
 }
 
 // A thread's walk over its positions, U of them at once: f(first element of each, which of them there are, how many).
-template <int U, typename F>
-__device__ __forceinline__ void walk(const TilePlan& p, const TileAt& at, int64_t S, int C, F&& f) {
+template <int U, typename At, typename F>
+__device__ __forceinline__ void walk(const TilePlan& p, const At& at, int64_t S, int C, F&& f) {
   if (!at.on) return;
   const int64_t step = (int64_t)p.rows * C, bstep = (int64_t)p.rows * code_blocks(C);
   const int64_t row = at.sample * S + at.begin + at.row;

@@ -116,7 +116,9 @@ def test_gradients_of_the_gradients(device, shape, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(20011, 1, 64, 8), (30000, 1, 30, 5), (5003, 9, 64, 8), (3001, 70, 40, 5),
-                                   (1, 131072, 32, 4), (4, 9001, 72, 3), (2003, 1, 4096, 1)])
+                                   (1, 131072, 32, 4), (4, 9001, 72, 3), (2003, 1, 4096, 1),
+                                   (1, 131072, 65, 13), (500, 1000, 30, 5), (1030, 130, 63, 63), (21, 1999, 330, 11),
+                                   (3001, 401, 7, 7), (37, 4001, 60, 2)])
 def test_larger(device, shape, dtype):
     from ictc_o3 import group_norm
     x, w, b, gy, v, vw, vb = _inputs(shape, dtype, device)
@@ -148,7 +150,9 @@ def test_larger(device, shape, dtype):
                                    (5, 33, 30, 5), (2, 257, 330, 11), (3, 300, 64, 8), (2, 4099, 30, 5), (1, 700, 2304, 1),
                                    (9, 1, 384, 3), (9, 1, 392, 4), (0, 1, 16, 4),
                                    (700, 1, 16, 4), (11, 1, 128, 1), (37, 1, 256, 8), (1030, 1, 512, 64), (5, 1, 1024, 2),
-                                   (3, 1, 2048, 2), (6, 1, 768, 2), (9, 1, 640, 40), (4, 1, 2048, 256), (3, 1, 96, 3)])
+                                   (3, 1, 2048, 2), (6, 1, 768, 2), (9, 1, 640, 40), (4, 1, 2048, 256), (3, 1, 96, 3),
+                                   (1, 131072, 65, 13), (501, 1000, 30, 5), (2100, 65, 130, 26), (9, 1, 999, 3),
+                                   (5, 3, 77, 7)])
 def test_x_in_8_bits(device, shape, dtype):
     """The result is that of whole rows, bit for bit; the derivatives are the formulas at the decoded x."""
     from ictc_o3 import decode_activations, encode_activations, group_norm
