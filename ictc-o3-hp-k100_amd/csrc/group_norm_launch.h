@@ -30,7 +30,7 @@ struct RowsChoice {
   int across, team, n;
 };
 
-inline RowsChoice rows_choice(int64_t positions, int chunks, int groups, int bytes) {
+inline RowsChoice rows_choice(int64_t positions, int chunks, int groups, int bytes, int most_chunks) {
   const int across = std::min(64, power_of_two(chunks));
   if (positions == 1) {
     if (chunks <= 256) return {across, across, (chunks + 63) / 64};
@@ -43,7 +43,7 @@ inline RowsChoice rows_choice(int64_t positions, int chunks, int groups, int byt
   for (int strips = 64 / across; strips >= 1; strips /= 2) {
     const int64_t n = (positions + strips - 1) / strips;
     const double used = (double)positions / (double)(strips * n);
-    if (n > 4 || (strips > 1 && strips / 2 >= positions)) continue;
+    if (n > most_chunks || (strips > 1 && strips / 2 >= positions)) continue;
     // a wave's groups side by side: 64 bytes of a position, or all there are
     if (std::min(64 / (across * strips), groups) * bytes < std::min(64, groups * bytes)) continue;
     if (used > most + 0.01) most = used, best = {across, across * strips, (int)n};
@@ -61,7 +61,12 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
   // have one or two channels.  (Fours of eight: there are one fewer of these than twice the others.)
   const int whole = 16 / element;
   const bool part = p.ev < 4 && p.ev < whole && per >= whole;
-  RowsChoice choice = rows_choice(positions, part ? (per + whole - 1) / whole : per / p.ev, groups, per * element);
+  RowsChoice choice = rows_choice(positions, part ? (per + whole - 1) / whole : per / p.ev, groups, per * element, 4);
+  // (the second derivative keeps too much of three and four chunks of eight: 131,072 samples of 9 x 64 bfloat16 655 us, by two 542)
+  if (second && positions > 1 && choice.n > 2 && (part ? whole : p.ev) == 8) {
+    const RowsChoice two = rows_choice(positions, part ? (per + whole - 1) / whole : per / p.ev, groups, per * element, 2);
+    if (two.n > 0) choice = two;
+  }
   if (choice.team == 256 && (part || p.ev != whole || choice.n * p.ev > 32)) choice = {};   // (kernels there are none of)
   if (choice.n > 0) {
     p.form = Form::kRows;
@@ -129,7 +134,7 @@ inline Plan plan_of(int element, int64_t samples, int64_t positions, int channel
   } else {
     p.form = Form::kParts;
     const int64_t most = (steps + at_once - 1) / at_once;
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(most, (2048 + blocks) / (blocks + 1)));
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(most, (1024 + blocks) / (blocks + 1)));
     t.per_split = (steps + splits - 1) / splits * t.rows;
     t.splits = (int)((positions + t.per_split - 1) / t.per_split);
   }
