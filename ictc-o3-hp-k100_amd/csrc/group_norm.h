@@ -75,10 +75,10 @@ __device__ __forceinline__ Pack<T, EV> load_part(const T* __restrict__ p, int64_
 }
 
 template <bool PART, int EV>
-__device__ __forceinline__ void cut(float (&v)[EV], int n) {
+__device__ __forceinline__ void cut(float (&v)[EV], int n, float none = 0.f) {
   if constexpr (PART) {
 #pragma unroll
-    for (int e = 0; e < EV; ++e) v[e] = e < n ? v[e] : 0.f;
+    for (int e = 0; e < EV; ++e) v[e] = e < n ? v[e] : none;
   }
 }
 

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
   __shared__ float cross[WIDE ? 8 : 1];
   const RowsAt at(p, a.groups);
   const int C = a.channels, S = (int)a.positions;
-  const float inv = 1.f / ((float)per * (float)S);
+  const float count = (float)per * (float)S, inv = 1.f / count;
   const RowsChunks<EV, N, PART> k(p, at, per, S, C);
   float w[N][EV], b[N][EV];
 #pragma unroll
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
       }
     }
     rows_sum<WIDE>(s, p.team, cross);
-    // The deviations' own mean corrects the rounded one (a group of one value far from zero has no deviation left).
+    // The deviations' own mean corrects the rounded one, a quotient to the last bit (a group of one value far from zero has
+    // no deviation left).
     const float first = s[0] * inv;
     float q[2] = {0.f, 0.f};
 #pragma unroll
@@ -117,20 +118,22 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
         q[1] += v[i][e] * v[i][e];
       }
     rows_sum<WIDE>(q, p.team, cross);
-    const float rest = q[0] * inv, mu = first + rest;
+    const float about = q[0] * inv, rest = __builtin_fmaf(__builtin_fmaf(-about, count, q[0]), inv, about), mu = first + rest;
     float r = 1.f / sqrtf(fmaxf(q[1] * inv - rest * rest, 0.f) + a.eps);
-    if (q[1] == __builtin_inff()) {   // (the whole team) finite deviations whose squares are past FP32: added again, scaled
-      constexpr float SCALE = 0x1p-80f;
+    // (the whole team) squares past FP32 of finite deviations, or hardly any but the mean's: added again, without that, scaled
+    if (q[1] == __builtin_inff() || 2.f * rest * rest > q[1] * inv) {
+      const bool past = q[1] == __builtin_inff();
+      const float scale = past ? 0x1p-80f : 1.f;
       s[0] = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
-          const float d = (v[i][e] - rest) * SCALE;
+          const float d = (v[i][e] - rest) * scale;
           s[0] += (PART ? e : 0) < k.n[i] ? d * d : 0.f;
         }
       rows_sum<WIDE>(s, p.team, cross);
-      r = SCALE / sqrtf(s[0] * inv + a.eps * SCALE * SCALE);
+      r = past ? fminf(scale / sqrtf(s[0] * inv), 1.f / sqrtf(a.eps)) : 1.f / sqrtf(s[0] * inv + a.eps);
     }
     if (q[1] != q[1]) r = q[1];   // (fmaxf drops a NaN)
 #pragma unroll
@@ -209,11 +212,12 @@ __global__ __launch_bounds__(256) void gn_rows_bwd_kernel(ictc::GroupNormCall a,
     for (int i = 0; i < N; ++i) {
       rx[i].values(h[i]);
       get<T, EV>(rg[i], u[i]);
-      cut<PART>(h[i], k.n[i]);
+      cut<PART>(h[i], k.n[i], mu);   // (nothing is the mean: a large one times r may be infinite)
       cut<PART>(u[i], k.n[i]);
+      const float mean = PART || k.n[i] > 0 ? mu : 0.f;
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        h[i][e] = (h[i][e] - mu) * r;
+        h[i][e] = (h[i][e] - mean) * r;
         const float ga = u[i][e] * Act<SILU>(h[i][e] * w[i][e] + b[i][e]).slope();
         dw[i][e] += ga * h[i][e];
         db[i][e] += ga;
@@ -279,14 +283,15 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
     const float mu = a.mean[n * a.groups + at.group], r = a.rstd[n * a.groups + at.group];
     float s[kSums] = {};
     Point kept[KEEP ? EV : 1];
-    float x[EV], g[EV], v[EV];
+    float x[EV], g[EV], v[EV], mean;   // (mean: see the first derivative)
     auto unpack = [&](int i) {
       rx[i].values(x);
       get<T, EV>(rg[i], g);
       get<T, EV>(rv[i], v);
-      cut<PART>(x, k.n[i]);
+      cut<PART>(x, k.n[i], mu);
       cut<PART>(g, k.n[i]);
       cut<PART>(v, k.n[i]);
+      mean = PART || k.n[i] > 0 ? mu : 0.f;
       if (!KEEP) q.load(a, k.c[i], k.n[i]);
     };
 #pragma unroll
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       unpack(i);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const Point o = point<SILU>((x[e] - mu) * r, g[e], q.w[e], q.b[e]);
+        const Point o = point<SILU>((x[e] - mean) * r, g[e], q.w[e], q.b[e]);
         if (KEEP) kept[KEEP ? e : 0] = o;
         add_sums<SILU>(o, r, v[e], q.w[e], q.vw[e], q.vb[e], s);
       }
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       if (!KEEP) unpack(i);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const Point o = KEEP ? kept[KEEP ? e : 0] : point<SILU>((x[e] - mu) * r, g[e], q.w[e], q.b[e]);
+        const Point o = KEEP ? kept[KEEP ? e : 0] : point<SILU>((x[e] - mean) * r, g[e], q.w[e], q.b[e]);
         float pw, pb;
         of.element(o, r, v[e], q.w[e], q.vw[e], q.vb[e], x[e], v[e], pw, pb);
         dw[i][e] += (PART ? e : 0) < k.n[i] ? pw : 0.f;

@@ -329,8 +329,10 @@ __device__ __forceinline__ void tile_channels(const ictc::GroupNormCall& a, cons
     Pack<T, EV> rg[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      rx[i].load(a, from + i * step, block + i * bstep, EV, i < count ? EV : 0, 0);
-      rg[i] = load_pack<T, EV>((const T*)a.g + (i < count ? from + i * step : from), i < count);
+      // (x of a position that there is: zero less a large mean may be infinite)
+      const int64_t f = i < count ? from + i * step : from;
+      rx[i].load(a, f, i < count ? block + i * bstep : block, EV, EV, 0);
+      rg[i] = load_pack<T, EV>((const T*)a.g + f, i < count);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -481,7 +483,7 @@ __device__ __forceinline__ void tile_sums(const ictc::GroupNormCall& a, const Ti
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int64_t f = i < count ? from + i * step : from;
-      rx[i].load(a, f, block + i * bstep, EV, i < count ? EV : 0, 0);
+      rx[i].load(a, f, i < count ? block + i * bstep : block, EV, EV, 0);
       rg[i] = load_pack<T, EV>((const T*)a.g + f, i < count);
       rv[i] = load_pack<T, EV>((const T*)a.v + f, i < count);
     }

@@ -285,6 +285,33 @@ def test_samples_whose_squares_leave_the_range(device, shape, dtype):
     _close(gx.double() * size, ref * size, TOL[dtype], "dx")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(40, 9, 32, 4), (40, 3, 35, 5), (9, 1, 36, 3), (7, 9, 64, 8), (33, 301, 32, 4),
+                                   (3, 300, 30, 5), (2, 9001, 16, 2)])
+def test_samples_of_one_large_value(device, shape, dtype):
+    """2^121 everywhere: means and deviations are exact, so the bounds are the ordinary ones; the mean over the deviation
+    is past FP32, which lanes and positions that hold nothing must not see."""
+    from ictc_o3 import group_norm
+    x, w, b, gy, v, vw, vb = _inputs(shape, dtype, device, 5)
+    x = torch.full_like(x, 2.0 ** 121)
+    for t in (x, w, b, gy):
+        t.requires_grad_()
+    y = group_norm(x, shape[3], w, b, eps=EPS, activation="silu")
+    first = torch.autograd.grad(y, (x, w, b), gy, create_graph=True)
+    second = torch.autograd.grad(first, (x, gy, w, b), (v, vw, vb))
+    d = Derivatives(x.detach(), shape[3], w.detach(), b.detach(), EPS, "silu", gy.detach())
+    (dx, dw, db), (sw, sb) = d.first()
+    ref, sizes = d.second(v, vw, vb)
+    _close(y, torch.nn.functional.silu(b.double()).expand(x.shape), TOL[dtype], "y")
+    _close(first[0], dx, TOL[dtype], "dx")
+    _close_sum(first[1], dw, sw, "dw")
+    _close_sum(first[2], db, sb, "db")
+    _close(second[0], ref[0], SECOND[dtype], "dx'")
+    _close(second[1], ref[1], SECOND[dtype], "dg'")
+    _close_sum(second[2], ref[2], sizes[0], "dw'")
+    _close_sum(second[3], ref[3], sizes[1], "db'")
+
+
 @pytest.mark.parametrize("shape", [(33, 1, 64, 8), (33, 6, 32, 4), (33, 300, 32, 4), (33, 5000, 16, 2), (33, 1, 2176, 1)])
 def test_nan_and_infinity_stay_in_their_group(device, shape):
     from ictc_o3 import group_norm
