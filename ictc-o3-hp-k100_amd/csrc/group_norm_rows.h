@@ -214,10 +214,9 @@ __global__ __launch_bounds__(256) void gn_rows_bwd_kernel(ictc::GroupNormCall a,
       get<T, EV>(rg[i], u[i]);
       cut<PART>(h[i], k.n[i], mu);   // (nothing is the mean: a large one times r may be infinite)
       cut<PART>(u[i], k.n[i]);
-      const float mean = PART || k.n[i] > 0 ? mu : 0.f;
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        h[i][e] = (h[i][e] - mean) * r;
+        h[i][e] = (PART || k.n[i] > 0 ? h[i][e] - mu : 0.f) * r;
         const float ga = u[i][e] * Act<SILU>(h[i][e] * w[i][e] + b[i][e]).slope();
         dw[i][e] += ga * h[i][e];
         db[i][e] += ga;
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
     const float mu = a.mean[n * a.groups + at.group], r = a.rstd[n * a.groups + at.group];
     float s[kSums] = {};
     Point kept[KEEP ? EV : 1];
-    float x[EV], g[EV], v[EV], mean;   // (mean: see the first derivative)
+    float x[EV], g[EV], v[EV];
     auto unpack = [&](int i) {
       rx[i].values(x);
       get<T, EV>(rg[i], g);
@@ -291,7 +290,6 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       cut<PART>(x, k.n[i], mu);
       cut<PART>(g, k.n[i]);
       cut<PART>(v, k.n[i]);
-      mean = PART || k.n[i] > 0 ? mu : 0.f;
       if (!KEEP) q.load(a, k.c[i], k.n[i]);
     };
 #pragma unroll
@@ -299,7 +297,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       unpack(i);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const Point o = point<SILU>((x[e] - mean) * r, g[e], q.w[e], q.b[e]);
+        const Point o = point<SILU>((PART || k.n[i] > 0 ? x[e] - mu : 0.f) * r, g[e], q.w[e], q.b[e]);
         if (KEEP) kept[KEEP ? e : 0] = o;
         add_sums<SILU>(o, r, v[e], q.w[e], q.vw[e], q.vb[e], s);
       }
@@ -311,7 +309,8 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       if (!KEEP) unpack(i);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const Point o = KEEP ? kept[KEEP ? e : 0] : point<SILU>((x[e] - mean) * r, g[e], q.w[e], q.b[e]);
+        const Point o = KEEP ? kept[KEEP ? e : 0]
+                             : point<SILU>((PART || k.n[i] > 0 ? x[e] - mu : 0.f) * r, g[e], q.w[e], q.b[e]);
         float pw, pb;
         of.element(o, r, v[e], q.w[e], q.vw[e], q.vb[e], x[e], v[e], pw, pb);
         dw[i][e] += (PART ? e : 0) < k.n[i] ? pw : 0.f;
