@@ -377,11 +377,18 @@ struct OrderOut {
   int *perm, *keys, *off;
 };
 
+// A row's id or key as it lies in memory (-1: there is no row), and the key.  (Apart, so that loads are not waited for one
+// by one.)
 template <Pass P>
-__device__ __forceinline__ uint32_t order_key(const OrderIn& in, int row) {
-  if (P == Pass::kLater) return in.keys[row];
-  const int64_t id = in.ids[row];
-  return (uint64_t)id < (uint64_t)in.experts ? (uint32_t)id : (uint32_t)in.experts;
+__device__ __forceinline__ int64_t order_raw(const OrderIn& in, int row, bool there) {
+  if (P == Pass::kLater) return there ? in.keys[row] : -1;
+  return there ? in.ids[row] : -1;
+}
+
+template <Pass P>
+__device__ __forceinline__ uint32_t order_key(const OrderIn& in, int64_t raw) {
+  if (P == Pass::kLater) return (uint32_t)raw;
+  return (uint64_t)raw < (uint64_t)in.experts ? (uint32_t)raw : (uint32_t)in.experts;
 }
 
 template <Pass P>
@@ -396,12 +403,12 @@ __global__ __launch_bounds__(1024) void experts_count_kernel(OrderIn in, int n, 
   __syncthreads();
   const int begin = blockIdx.x * span, end = min(n, begin + span);
   for (int r0 = begin + (int)threadIdx.x; r0 < end; r0 += 4096) {
-    uint32_t key[4];
+    int64_t raw[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = r0 + i * 1024 < end ? order_key<P>(in, r0 + i * 1024) : 0;
+    for (int i = 0; i < 4; ++i) raw[i] = order_raw<P>(in, r0 + i * 1024, r0 + i * 1024 < end);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (r0 + i * 1024 < end) atomicAdd(&count[order_digit<P>(in, key[i])], 1);
+      if (r0 + i * 1024 < end) atomicAdd(&count[order_digit<P>(in, order_key<P>(in, raw[i]))], 1);
   }
   __syncthreads();
   if ((int)threadIdx.x < in.groups) counts[blockIdx.x * in.groups + threadIdx.x] = count[threadIdx.x];
@@ -437,17 +444,14 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, 
   const int begin = first + wave * per, end = min(first + rows, begin + per);
   int* mine = count[wave];
   uint32_t place[kOrderAtOnce];   // digit | lanes below << 10 | lanes << 16
-  uint32_t key[kOrderAtOnce];
+  int64_t raw[kOrderAtOnce];
 #pragma unroll
-  for (int i = 0; i < kOrderAtOnce; ++i) {
-    const int row = begin + i * 64 + lane;
-    key[i] = row < end ? order_key<P>(in, row) : (uint32_t)in.experts;
-  }
+  for (int i = 0; i < kOrderAtOnce; ++i) raw[i] = order_raw<P>(in, begin + i * 64 + lane, begin + i * 64 + lane < end);
 #pragma unroll
   for (int i = 0; i < kOrderAtOnce; ++i) {
     const int r0 = begin + i * 64;
     if (r0 >= end) break;
-    const uint32_t digit = order_digit<P>(in, key[i]);
+    const uint32_t digit = order_digit<P>(in, order_key<P>(in, raw[i]));
     const uint64_t here = __ballot(r0 + lane < end);
     uint32_t lo = (uint32_t)here, hi = (uint32_t)(here >> 32);   // the lanes whose row has this lane's digit
     int x = (int)(digit << (32 - bits));
@@ -493,7 +497,7 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, 
     if (ok) {
       const int to = mine[digit] + below;
       out.perm[to] = P == Pass::kLater ? in.rows[r0 + lane] : r0 + lane;
-      if (P != Pass::kOnly) out.keys[to] = (int)key[i];
+      if (P != Pass::kOnly) out.keys[to] = (int)order_key<P>(in, raw[i]);
     }
     wave_meet();
     if (ok && below == 0) atomicAdd(&mine[digit], lanes);   // (before the next rows' reads: LDS keeps a wave's order)
