@@ -12,15 +12,20 @@
 // Where x is kept in 8 bits (codes.h) its values stand in h; mean and r are those of x itself.
 //
 // All of it is bound by memory.  Three forms, by the size of a sample's group:
-//  * Rows: up to 256 chunks of it.  A team of up to 64 lanes holds it in registers: one read, no barrier.  A team keeps its
-//    group, so the parameters stay in registers and their gradients are added per lane.
+//  * Rows: up to four chunks a lane of up to 64 lanes; of single positions, up to 32 elements a lane of a block.  This team
+//    holds it in registers: one read.  It keeps its group, so the parameters stay in registers and their gradients are
+//    added per lane.  (425,991 x 64 FP32 in eight groups: forward 48 us, gradients 60, 5.1 and 5.9 TB/s; one position of
+//    4,096 bfloat16 channels by a block's team, 8,192 samples: gradients 106 us, by parts 204.)
 //  * Tiles: a block takes some whole groups of a sample and reads them twice, for the sums and for the result, the second
-//    time from the caches; one launch.
-//  * Parts: few large samples.  The sums by many blocks, a small kernel that adds their parts in order, and the result by
-//    as many blocks again.
+//    time from the caches; one launch.  (32 x 256 positions x 128 FP32: forward 6 us, gradients 8, second derivative 13.)
+//  * Parts: few large samples.  The sums by many blocks, a small kernel that adds their parts in order (few parts are added
+//    by every block that needs them), and the result by as many blocks again.  (One sample of 131,072 x 256 bfloat16:
+//    statistics 15 us, 4.5 TB/s; result 25, its x from the caches; gradients' sums 32 and result 37.)
 // A chunk is the largest power of two of a group's channels up to 16 bytes, so each lies in one group and in one block of
-// codes.  Statistics of tiles and parts are sums of x and of its squares in FP64, which costs nothing beside memory,
-// loses nothing to a mean far from zero and holds squares past FP32's range.  Every sum has a fixed order.
+// codes.  Groups that only small chunks divide are cut into 16-byte chunks, the last in part (rows), or their tile is,
+// whatever the groups (group_norm_span.h).  Statistics of tiles and parts are sums of x and of its squares in FP64, which
+// costs nothing beside memory, loses nothing to a mean far from zero and holds squares past FP32's range.  Every sum has a
+// fixed order.
 #pragma once
 #include <algorithm>
 
