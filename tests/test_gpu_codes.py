@@ -186,3 +186,32 @@ def test_expert_linear_keeps_a_byte_an_element(device):
     slack = 1 << 20
     assert full > rows * width * 4 - slack and eight < rows * (width + 8) + slack
     assert kept(8, W) > full - slack      # (the rows are not needed, and whole ones are kept as without the argument)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_function_that_keeps_its_input_in_8_bits(device, dtype):
+    """A caller's own backward pass: the gradient is its formula at the decoded values, bit by bit."""
+    from ictc_o3 import decode_activations, encode_activations
+
+    class Gate(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            ctx.save_for_backward(*encode_activations(x))
+            ctx.dtype = x.dtype
+            return x * torch.tanh(x)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, g):
+            x = decode_activations(*ctx.saved_tensors, dtype=ctx.dtype)
+            t = torch.tanh(x)
+            return g * (t + x * (1 - t * t))
+
+    generator = torch.Generator().manual_seed(8)
+    x, g = (torch.randn(37, 5, 130, generator=generator).to(dtype).to(device) for _ in range(2))
+    x.requires_grad_()
+    y = Gate.apply(x)
+    (got,) = torch.autograd.grad(y, x, g)
+    d = decode_activations(*encode_activations(x), dtype=dtype)
+    t = torch.tanh(d)
+    assert torch.equal(got, g * (t + d * (1 - t * t))) and not torch.equal(d, x)
