@@ -198,3 +198,38 @@ def test_example_with_group_norm(device):
         with torch.no_grad():
             diff = (energy(data["pos"] + h * d) - energy(data["pos"] - h * d)) / (2 * h)
         assert (diff - (grad.double() * d.double()).sum()).abs() < 1e-2 * grad.double().norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [64, 130])
+def test_operands_that_begin_anywhere(device, width, dtype):
+    """Contiguous operands one element behind an aligned address: the results of aligned ones, bit by bit."""
+    from ictc_o3 import decode_activations, embedding, encode_activations, group_norm
+    generator = torch.Generator().manual_seed(width)
+
+    def make(*size):
+        return torch.randn(*size, generator=generator).to(dtype).to(device)
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=device)
+        flat[1:] = t.detach().reshape(-1)
+        return flat[1:].view(t.shape).requires_grad_(t.requires_grad)
+
+    ids = torch.randint(-1, 12, (700,), generator=generator).to(device)
+
+    def run(at):
+        table, g = at(make_table).requires_grad_(), at(make_g)
+        rows = embedding(table, at(ids), 0.75)
+        out = [rows, *torch.autograd.grad(rows, table, g)]
+        for x, gy, bits in ((make_x, make_g, None), (make_cells, make_cells_g, None), (make_x, make_g, 8)):
+            x, w, b, gy, v = at(x).requires_grad_(), at(make_w).requires_grad_(), at(make_b).requires_grad_(), at(gy), at(gy)
+            y = group_norm(x, 2, w, b, activation="silu", save_bits=bits)
+            first = torch.autograd.grad(y, (x, w, b), gy, create_graph=True)
+            out += [y, *first, *torch.autograd.grad(first[0], (x, w), v)]
+        codes, scales = encode_activations(at(make_x))
+        return [*out, codes, scales, decode_activations(at(codes), at(scales), dtype=dtype)]
+
+    make_table, make_g, make_x, make_w, make_b = make(12, width), make(700, width), make(700, width), make(width), make(width)
+    make_cells, make_cells_g = make(3, 500, width), make(3, 500, width)
+    for a, b in zip(run(lambda t: t.detach()), run(moved)):
+        assert torch.equal(a, b)
