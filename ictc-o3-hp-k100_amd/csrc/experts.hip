@@ -430,11 +430,17 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, 
     const int width = 1 << bits, at = threadIdx.x & (width - 1);
     int all = 0, earlier = 0;
     if (at < groups) {
-#pragma unroll 8
-      for (int b = threadIdx.x / width; b < (int)gridDim.x; b += 1024 / width) {
-        const int c = counts[b * groups + at];
-        all += c;
-        earlier += b < (int)blockIdx.x ? c : 0;
+      constexpr int AT_ONCE = 16;
+      const int step = 1024 / width;
+      for (int b0 = threadIdx.x / width; b0 < (int)gridDim.x; b0 += AT_ONCE * step) {
+        int c[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) c[i] = b0 + i * step < (int)gridDim.x ? counts[(b0 + i * step) * groups + at] : 0;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          all += c[i];
+          earlier += b0 + i * step < (int)blockIdx.x ? c[i] : 0;
+        }
       }
       atomicAdd(&totals[at], all);
       atomicAdd(&befores[at], earlier);
