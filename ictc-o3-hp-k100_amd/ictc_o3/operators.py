@@ -438,7 +438,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, sav
 
     x is float32, bfloat16 or float16, weight and bias [channels] of the same type (None: ones / zeros).  Statistics and
     sums are FP32 or better and each result is rounded once.  Gradients of x, weight and bias, and once more of those (a
-    loss on forces), run on kernels; a third derivative raises.  A sample's group that holds NaN or infinity gives NaN.
+    loss on forces), run on kernels; a third derivative raises.  A sample's group that holds NaN or infinity gives NaN; one
+    whose sum passes FP32's range may.
     With save_bits=8 the backward pass keeps x in 8 bits (``encode_activations``, by position) and takes the decoded x in
     its formulas, with the mean and deviation of x itself; the result stays as it is."""
     return nat.ops().group_norm(x, groups, weight, bias, eps, activation, save_bits)
