@@ -91,6 +91,9 @@ __global__ __launch_bounds__(256) void decode_kernel(const int8_t* __restrict__ 
   }
 }
 
+// Blocks of a row.  (Of any width that an int holds: a row of 2^31 - 1 elements has 2^24, the last chunk's column is below 2^31.)
+int blocks_of(int width) { return (width - 1) / kCodeBlock + 1; }
+
 // Lanes of a block's chunks: all of 128 elements, fewer where rows are shorter.
 int team_of(int width, int chunk) {
   int lanes = 1;
@@ -125,14 +128,14 @@ dim3 grid_of(int64_t blocks, int team) {
 
 template <typename T>
 void run_encode(const void* x, int64_t ldx, int64_t rows, int width, int8_t* codes, float* scales, hipStream_t st) {
-  const int per = (width + kCodeBlock - 1) / kCodeBlock, team = team_of(width, kChunk<T>);
+  const int per = blocks_of(width), team = team_of(width, kChunk<T>);
   CODES_TEAMS(team, hipLaunchKernelGGL((encode_kernel<T, TEAM>), grid_of(rows * per, team), dim3(256), 0, st,
                                        (const T*)x, ldx, rows, width, per, codes, scales))
 }
 
 template <typename T>
 void run_decode(const int8_t* codes, const float* scales, int64_t rows, int width, void* out, hipStream_t st) {
-  const int per = (width + kCodeBlock - 1) / kCodeBlock, team = team_of(width, kChunk<T>);
+  const int per = blocks_of(width), team = team_of(width, kChunk<T>);
   CODES_TEAMS(team, hipLaunchKernelGGL((decode_kernel<T, TEAM>), grid_of(rows * per, team), dim3(256), 0, st, codes,
                                        scales, rows, width, per, (T*)out))
 }

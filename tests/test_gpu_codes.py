@@ -215,3 +215,21 @@ def test_a_function_that_keeps_its_input_in_8_bits(device, dtype):
     d = decode_activations(*encode_activations(x), dtype=dtype)
     t = torch.tanh(d)
     assert torch.equal(got, g * (t + d * (1 - t * t))) and not torch.equal(d, x)
+
+
+def test_longest_last_axis(device):
+    """A row of 2^31 - 1 elements, the longest that is taken: its first, middle and last blocks against the definition."""
+    from ictc_o3 import decode_activations, encode_activations
+    width = 2 ** 31 - 1
+    x = torch.zeros(1, width, dtype=torch.bfloat16, device=device)
+    spans = [(0, 4096), (2 ** 30 - 1280, 2 ** 30 + 1280), (width - 4223, width)]   # (from whole blocks on)
+    for k, (a, b) in enumerate(spans):
+        x[:, a:b] = _rows(1, b - a, torch.bfloat16, device, k)
+    codes, scales = encode_activations(x)
+    assert codes.shape == (1, width) and scales.shape == (1, 2 ** 24)
+    values = decode_activations(codes, scales, dtype=torch.bfloat16)
+    for a, b in spans:
+        ref, ref_scales, ref_values = _definition(x[:, a:b])
+        assert torch.equal(codes[:, a:b].cpu(), ref) and torch.equal(values[:, a:b].cpu(), ref_values)
+        assert torch.equal(scales[:, a // 128:(b + 127) // 128].cpu(), ref_scales)
+    assert not codes[:, 4096:2 ** 30 - 1280].any() and not codes[:, 2 ** 30 + 1280:width - 4223].any()
