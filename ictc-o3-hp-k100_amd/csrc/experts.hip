@@ -512,24 +512,56 @@ __global__ __launch_bounds__(1024) void experts_order_kernel(OrderIn in, int n, 
   }
 }
 
+// First place of sorted keys [n] that holds `key` or more, by a wave: 64 places looked at together, then 64 of the part
+// between two of them.
+__device__ __forceinline__ int first_place(const int* __restrict__ keys, int n, uint32_t key) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t m = __ballot(at < hi && (uint32_t)keys[at < hi ? at : lo] >= key);
+    const int f = m ? __builtin_ctzll(m) : (hi - lo - 1) / step + 1;   // looked at: f are below the key
+    if (m) hi = lo + f * step;
+    if (f > 0) lo += (f - 1) * step + 1;
+  }
+  return lo;
+}
+
 // off[k] = the first place of sorted keys [n] that holds k or more, for k of 0 .. experts + 1.  A place fills the offsets
-// from the key before it to its own; long gaps are shared by the wave.
-__global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restrict__ keys, int n, int experts,
-                                                            int* __restrict__ off) {
-  const int p = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63;
-  int from = 0, to = 0;   // offsets from .. to - 1 are p
+// from the key before it to its own, long gaps with its wave; but of a gap the whole spans of kSpan offsets (from multiples
+// of it) are filled by a wave each, of the blocks behind the places', so that few rows, or ids side by side, of many entries
+// do not keep one wave (the whole order of 5 rows of a million entries 484 -> 16 us, of 33.5 million 15.8 ms ->
+// 34 us).  Offsets are
+// unsigned: experts + 2 may be 2^31 - 1, and a step past it.
+constexpr uint32_t kSpan = 1024;
+__global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restrict__ keys, int n, uint32_t experts,
+                                                            int place_blocks, int* __restrict__ off) {
+  const int lane = threadIdx.x & 63;
+  if ((int)blockIdx.x >= place_blocks) {
+    const uint32_t first = ((blockIdx.x - place_blocks) * 4 + (threadIdx.x >> 6)) * kSpan;
+    if (first + kSpan > experts + 2) return;
+    const int p = first_place(keys, n, first);
+    if (p < n && (uint32_t)keys[p] + 1 < first + kSpan) return;   // a key within it
+    for (uint32_t k = lane; k < kSpan; k += 64) off[first + k] = p;
+    return;
+  }
+  const int p = blockIdx.x * 256 + threadIdx.x;
+  uint32_t from = 0, to = 0;   // offsets from .. to - 1 are p
   if (p <= n) {
-    from = p > 0 ? keys[p - 1] + 1 : 0;
-    to = p < n ? keys[p] + 1 : experts + 2;
+    from = p > 0 ? (uint32_t)keys[p - 1] + 1 : 0;
+    to = p < n ? (uint32_t)keys[p] + 1 : experts + 2;
   }
   const bool wide = to - from > 8;
   if (!wide)
-    for (int k = from; k < to; ++k) off[k] = p;
+    for (uint32_t k = from; k < to; ++k) off[k] = p;
   for (uint64_t m = __ballot(wide); m; m &= m - 1) {
     const int l = __builtin_ctzll(m);
-    const int a = __builtin_amdgcn_readlane(from, l), b = __builtin_amdgcn_readlane(to, l),
-              q = __builtin_amdgcn_readlane(p, l);
-    for (int k = a + lane; k < b; k += 64) off[k] = q;
+    const uint32_t a = __builtin_amdgcn_readlane(from, l), b = __builtin_amdgcn_readlane(to, l),
+                   q = __builtin_amdgcn_readlane(p, l);
+    uint32_t spans = (a + kSpan - 1) / kSpan * kSpan, behind = b / kSpan * kSpan;   // whole ones: from, to
+    if (behind <= spans) spans = behind = b;
+    for (uint32_t k = a + lane; k < spans; k += 64) off[k] = q;
+    for (uint32_t k = behind + lane; k < b; k += 64) off[k] = q;
   }
 }
 
@@ -611,8 +643,10 @@ int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int
     const OrderIn next = {nullptr, from[0], from[1], (int)experts, shift, 1 << bits};
     order_pass<Pass::kLater>(next, n, bits, p, counts, {k + 1 < p.passes ? to[1] : perm, to[0], nullptr}, st);
   }
-  hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, st, half[(p.passes - 1) % 2][0],
-                     n, (int)experts, off);
+  const int places = (int)(rows / 256) + 1;
+  const int64_t spans = (experts + 2) / kSpan;
+  hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(places + tiles_of(spans, 4))), dim3(256), 0, st,
+                     half[(p.passes - 1) % 2][0], n, (uint32_t)experts, places, off);
   return dense_status("expert_order launch");
 }
 

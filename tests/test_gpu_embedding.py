@@ -301,3 +301,54 @@ def test_graph_replays_of_very_many_rows(device):
         assert torch.equal(held, eager), k
         ref = torch.bincount(ids[ids >= 0], minlength=50)
         assert ((held[:, 0].double() - ref).abs() <= 700 * 2.0 ** -24 * ref).all()
+
+
+@pytest.mark.parametrize("rows,entries,kind", [(5, 1024, "near"), (5, 2047, "near"), (300, 3000, "none"), (20000, 4100, "near"),
+                                               (129, 1000003, "ends"), (70000, 1000003, "near"), (70000, 1000003, "none"),
+                                               (5000, 65535, "spread"), (40000, 33554431, "spread"),
+                                               (260, 2 ** 31 - 3, "ends"), (5, 2 ** 31 - 3, "none")])
+def test_order_of_ids_side_by_side(device, rows, entries, kind):
+    """Ids in one part of a large table, at its ends, or none within it: where each id begins, up to the largest tables."""
+    from ictc_o3 import _native as nat
+    g = torch.Generator().manual_seed(rows + entries)
+    first = entries - 7 if kind == "ends" else entries // 3
+    ids = torch.randint(first, min(first + 40, entries + 5), (rows,), generator=g)
+    if kind == "ends":
+        ids[: rows // 2] = torch.randint(-2, 5, (rows // 2,), generator=g)
+    elif kind == "none":
+        ids = torch.full((rows,), entries)
+    elif kind == "spread":
+        ids = torch.randint(0, entries, (rows,), generator=g)
+    ids = ids.to(device)
+    size = nat.lib().ictc_rows_by_id_workspace_bytes(rows, entries)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+    perm = torch.full((rows,), -7, dtype=torch.int32, device=device)
+    off = torch.full((entries + 2,), -7, dtype=torch.int32, device=device)
+    nat.call("ictc_rows_by_id", ids.data_ptr(), rows, entries, perm.data_ptr(), off.data_ptr(), ws.data_ptr(), size,
+             torch.cuda.current_stream().cuda_stream)
+    key = torch.where((ids >= 0) & (ids < entries), ids, torch.full_like(ids, entries))
+    ref = torch.sort(key, stable=True)
+    assert torch.equal(perm.long(), ref.indices)
+    for k in range(0, entries + 2, 1 << 26):
+        ks = torch.arange(k, min(entries + 2, k + (1 << 26)), device=device)
+        assert torch.equal(off[k:k + (1 << 26)], torch.searchsorted(ref.values, ks, out_int32=True)), k
+
+
+def test_largest_table(device):
+    """A table of 2^31 - 3 entries, the most that are taken: lookup and gradient at its ends."""
+    from ictc_o3 import embedding
+    entries = 2 ** 31 - 3
+    table = torch.zeros(entries, 1, dtype=torch.bfloat16, device=device)
+    ids = torch.cat([torch.arange(100), entries - 1 - torch.arange(100), torch.tensor([5, 5, entries, -1, entries - 1])]).to(device)
+    inside = (ids >= 0) & (ids < entries)
+    gy = torch.randint(-8, 9, (205, 1), generator=torch.Generator().manual_seed(1)).bfloat16().to(device)
+    table[ids[inside]] = 1.5
+    table.requires_grad_()
+    y = embedding(table, ids)
+    assert torch.equal(y[:, 0], 1.5 * inside)
+    (got,) = torch.autograd.grad(y, table, gy)
+    ref = torch.zeros(200, dtype=torch.float64, device=device)     # the ends' entries; sums of whole numbers are exact
+    ref.index_add_(0, torch.where(ids < 100, ids, ids - entries + 200)[inside], gy[inside, 0].double())
+    assert torch.equal(torch.cat([got[:100, 0], got[-100:, 0]]).double(), ref)
+    for part in got[100:-100].split(1 << 28):
+        assert not part.any()
