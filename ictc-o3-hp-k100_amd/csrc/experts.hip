@@ -530,12 +530,12 @@ __device__ __forceinline__ int first_place(const int* __restrict__ keys, int n, 
 // off[k] = the first place of sorted keys [n] that holds k or more, for k of 0 .. experts + 1.  A place fills the offsets
 // from the key before it to its own, long gaps with its wave; but of a gap the whole spans of kSpan offsets (from multiples
 // of it) are filled by a wave each, of the blocks behind the places', so that few rows, or ids side by side, of many entries
-// do not keep one wave (the whole order of 5 rows of a million entries 484 -> 16 us, of 33.5 million 15.8 ms ->
+// do not keep one wave; and a wave has only eight places where most gaps are long (the whole order of 5 rows of a million entries 484 -> 16 us, of 33.5 million 15.8 ms ->
 // 34 us).  Offsets are
 // unsigned: experts + 2 may be 2^31 - 1, and a step past it.
 constexpr uint32_t kSpan = 1024;
 __global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restrict__ keys, int n, uint32_t experts,
-                                                            int place_blocks, int* __restrict__ off) {
+                                                            int each, int place_blocks, int* __restrict__ off) {
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x >= place_blocks) {
     const uint32_t first = ((blockIdx.x - place_blocks) * 4 + (threadIdx.x >> 6)) * kSpan;
@@ -545,9 +545,9 @@ __global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restric
     for (uint32_t k = lane; k < kSpan; k += 64) off[first + k] = p;
     return;
   }
-  const int p = blockIdx.x * 256 + threadIdx.x;
+  const int p = (blockIdx.x * 4 + (threadIdx.x >> 6)) * each + lane;
   uint32_t from = 0, to = 0;   // offsets from .. to - 1 are p
-  if (p <= n) {
+  if (lane < each && p <= n) {
     from = p > 0 ? (uint32_t)keys[p - 1] + 1 : 0;
     to = p < n ? (uint32_t)keys[p] + 1 : experts + 2;
   }
@@ -578,8 +578,12 @@ int id_bits(int64_t experts) {
 // Both kernels at 64 / 128 / 256 blocks and 4,096 / 2,048 / 1,024 rows at least: 131,072 rows of ten experts 10.5 / 8.9 /
 // 8.3, 30,011 of 89 11.1 / 9.5 / 9.0, 425,991 of 1,000 25 / 24 / 29; both passes of 60,013 rows of 50,021 ids 34 / 28 / 22,
 // of 425,991 of 7,921 42 / 35 / 32.  Several / the general sort, ten experts: 4.2 million rows 32 / 83.
-int order_span(int64_t rows, int bits) {
-  if (rows > (int64_t)kOrderBlocks * kOrderRows) return 0;
+//
+// Every block reads all blocks' counts, so very many rows go to the general sort: over ten bits from 12.6 million on (1,000
+// experts: 12 million rows 256 / 264, 16.8 million 425 / 350; 500: 259 / 348), in several passes from 2.1 million (2 and 4.2
+// million rows of 7,921 ids 67 / 93 and 144 / 115, of 65,535 86 / 92 and 184 / 116, of a million 134 / 137 and 259 / 165).
+int order_span(int64_t rows, int bits, int passes) {
+  if (rows > (int64_t)kOrderBlocks * kOrderRows || (passes > 1 && rows > 1 << 21) || (bits > 9 && rows > 12 << 20)) return 0;
   if (rows <= kOrderRows && rows * (3 + bits) <= 60000) return (int)std::max<int64_t>(rows, 1);
   const int blocks = bits <= 8 ? 256 : 128;
   return (int)std::min<int64_t>(kOrderRows, std::max<int64_t>(262144 / blocks, (rows / blocks + 1023) / 1024 * 1024));
@@ -596,7 +600,7 @@ OrderPlan order_plan(int64_t rows, int64_t experts) {
   p.bits = id_bits(experts);
   p.passes = experts <= kOrderExperts ? 1 : (p.bits + 9) / 10;
   p.digit = (p.bits + p.passes - 1) / p.passes;
-  p.span = order_span(rows, p.digit);
+  p.span = order_span(rows, p.digit, p.passes);
   if (p.span == 0) return OrderPlan{};
   p.blocks = std::max<int64_t>(1, tiles_of(rows, p.span));
   const int64_t groups = p.passes == 1 ? experts + 1 : int64_t(1) << p.digit;
@@ -643,10 +647,10 @@ int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int
     const OrderIn next = {nullptr, from[0], from[1], (int)experts, shift, 1 << bits};
     order_pass<Pass::kLater>(next, n, bits, p, counts, {k + 1 < p.passes ? to[1] : perm, to[0], nullptr}, st);
   }
-  const int places = (int)(rows / 256) + 1;
+  const int each = experts >= 8 * rows ? 8 : 64, places = (int)tiles_of(rows + 1, 4 * each);
   const int64_t spans = (experts + 2) / kSpan;
   hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(places + tiles_of(spans, 4))), dim3(256), 0, st,
-                     half[(p.passes - 1) % 2][0], n, (uint32_t)experts, places, off);
+                     half[(p.passes - 1) % 2][0], n, (uint32_t)experts, each, places, off);
   return dense_status("expert_order launch");
 }
 

@@ -73,3 +73,14 @@ def test_order_refusals():
                 dict(ws=18), dict(bytes=100)):
         with pytest.raises(ValueError):
             order(**bad)
+
+
+def test_order_of_very_many_rows():
+    """Where the general sort is the faster, the order takes it (and its workspace)."""
+    lib = _built().lib()
+    for rows, entries, general in ((16777216, 10, False), (16777216, 511, False), (16777217, 10, True),
+                                   (12 << 20, 1000, False), ((12 << 20) + 1, 1000, True), (1 << 21, 65535, False),
+                                   ((1 << 21) + 1, 65535, True), ((1 << 21) + 1, 1024, True), ((1 << 21) + 1, 40000000, True)):
+        assert (lib.ictc_rows_by_id_workspace_bytes(rows, entries) == lib.ictc_csr_workspace_bytes(rows, entries)) == general
+        if entries <= 65535:
+            assert lib.ictc_expert_order_workspace_bytes(rows, entries) == lib.ictc_rows_by_id_workspace_bytes(rows, entries)

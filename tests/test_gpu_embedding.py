@@ -352,3 +352,25 @@ def test_largest_table(device):
     assert torch.equal(torch.cat([got[:100, 0], got[-100:, 0]]).double(), ref)
     for part in got[100:-100].split(1 << 28):
         assert not part.any()
+
+
+@pytest.mark.parametrize("rows,entries", [((1 << 21) + 1, 7921), ((12 << 20) + 5, 1000)])
+def test_graph_replays_of_the_general_sort(device, rows, entries):
+    """Very many rows take the general sort: the order captured and replayed, against the eager one and its definition."""
+    from ictc_o3 import expert_order
+    ids = torch.randint(-1, entries + 1, (rows,), device=device, generator=torch.Generator(device).manual_seed(1))
+    expert_order(ids, entries)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = expert_order(ids, entries)
+    for k in range(4):
+        ids.copy_(ids.roll(1001) if k else ids.flip(0))
+        ids[: 1000 * (k + 1)] = k
+        graph.replay()
+        eager = expert_order(ids, entries)
+        torch.cuda.synchronize()
+        assert torch.equal(held.perm, eager.perm) and torch.equal(held.offsets, eager.offsets), k
+        key = torch.where((ids >= 0) & (ids < entries), ids, torch.full_like(ids, entries))
+        assert torch.equal(held.perm.long(), torch.sort(key, stable=True).indices), k
+        counts = torch.bincount(key, minlength=entries + 1)
+        assert torch.equal(held.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)])), k
