@@ -622,20 +622,24 @@ void order_pass(const OrderIn& in, int n, int bits, const OrderPlan& p, int* cou
   hipLaunchKernelGGL(experts_order_kernel<P>, dim3((unsigned)p.blocks), dim3(1024), 0, st, in, n, bits, p.span, counts, out);
 }
 
-// The order of rows by id in [0, experts), those of no id last.
+// The order of rows by id in [0, experts), those of no id last.  small, launch: what the caller says of too small a workspace
+// and of a launch that fails.
 int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int* off, void* workspace, int64_t bytes,
-               hipStream_t st) {
+               hipStream_t st, const char* small, const char* launch) {
   const OrderPlan p = order_plan(rows, experts);
-  if (p.passes == 0) return ictc_csr_build(ids, rows, experts, off, perm, workspace, bytes, st);
+  if (p.passes == 0) {   // (what is left for it to refuse is the workspace)
+    const int rc = ictc_csr_build(ids, rows, experts, off, perm, workspace, bytes, st);
+    return rc == ICTC_ERR_ARGUMENT ? dense_fail(rc, small) : rc;
+  }
   const int64_t need = order_bytes(rows, experts);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || bytes < need))
-    return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: workspace smaller than ictc_expert_order_workspace_bytes");
+    return dense_fail(ICTC_ERR_ARGUMENT, small);
   const int n = (int)rows;
   int* counts = p.counts ? (int*)workspace : nullptr;
   OrderIn in = {ids, nullptr, nullptr, (int)experts, 0, (int)experts + 1};
   if (p.passes == 1) {
     order_pass<Pass::kOnly>(in, n, p.bits, p, counts, {perm, nullptr, off}, st);
-    return dense_status("expert_order launch");
+    return dense_status(launch);
   }
   int* half[2][2];   // ids and row numbers that pass 0, 2, .. and 1, 3, .. leave; the last pass: sorted ids
   for (int k = 0; k < 4; ++k) half[k / 2][k % 2] = (int*)workspace + p.counts + k * rows;
@@ -651,7 +655,7 @@ int order_rows(const int64_t* ids, int64_t rows, int64_t experts, int* perm, int
   const int64_t spans = (experts + 2) / kSpan;
   hipLaunchKernelGGL(order_offsets_kernel, dim3((unsigned)(places + tiles_of(spans, 4))), dim3(256), 0, st,
                      half[(p.passes - 1) % 2][0], n, (uint32_t)experts, each, places, off);
-  return dense_status("expert_order launch");
+  return dense_status(launch);
 }
 
 // Gradients of W ([M, K], g^T x) and of b ([M], the product of g with ones, by the blocks of column tile 0): one tile
@@ -939,7 +943,8 @@ int ictc_expert_order(const int64_t* ids, int64_t rows, int experts, int32_t* pe
                       int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(ICTC_F32, rows, 1, 1, experts)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "expert_order: null operand");
-  return order_rows(ids, rows, experts, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream);
+  return order_rows(ids, rows, experts, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream,
+                    "expert_order: workspace smaller than ictc_expert_order_workspace_bytes", "expert_order launch");
 }
 
 int64_t ictc_rows_by_id_workspace_bytes(int64_t rows, int64_t entries) {
@@ -952,7 +957,8 @@ int ictc_rows_by_id(const int64_t* ids, int64_t rows, int64_t entries, int32_t* 
   if (ictc_rows_by_id_workspace_bytes(rows, entries) < 0)
     return dense_fail(ICTC_ERR_ARGUMENT, "rows_by_id: up to 2^31 - 3 rows and entries");
   if (!offsets || (rows > 0 && (!ids || !perm))) return dense_fail(ICTC_ERR_ARGUMENT, "rows_by_id: null operand");
-  return order_rows(ids, rows, entries, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream);
+  return order_rows(ids, rows, entries, perm, offsets, workspace, workspace_bytes, (hipStream_t)stream,
+                    "rows_by_id: workspace smaller than ictc_rows_by_id_workspace_bytes", "rows_by_id launch");
 }
 
 int ictc_expert_linear(int dtype, const void* x, int64_t ldx, int64_t rows, int inputs, const void* weight,

@@ -26,7 +26,7 @@ Tensor embedding_sums(const Tensor& g_, const Tensor& ids, const Tensor& perm_, 
   const int64_t N = g.size(0), C = g.size(1);
   const int dt = dtype_of(g);
   Tensor perm = perm_, off = off_, ws;
-  if (!perm.defined() && ictc_embedding_needs_order(N)) std::tie(perm, off) = rows_by_id(ids, entries);
+  if (!perm.defined() && ictc_embedding_needs_order(N)) std::tie(perm, off) = rows_by_id(ids, entries, "embedding");
   Tensor out = at::empty({entries, C}, g.options());
   const int64_t bytes = ictc_embedding_bwd_workspace_bytes(dt, N, entries, (int)C);
   if (bytes > 0) ws = floats(bytes / 4, g);

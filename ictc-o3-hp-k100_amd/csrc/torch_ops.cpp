@@ -195,7 +195,7 @@ std::pair<Tensor, Tensor> expert_order(const Tensor& ids_, int64_t experts) {
   TORCH_CHECK_VALUE(experts >= 1 && experts <= 65535, "expert_order: experts must be an integer from 1 to 65535");
   TORCH_CHECK_VALUE(ids_.size(0) < (int64_t(1) << 31) - 2, "expert_order: up to 2^31 - 3 rows");
   const c10::DeviceGuard guard(ids_.device());
-  return rows_by_id(packed(ids_), experts);
+  return rows_by_id(packed(ids_), experts, "expert_order");
 }
 
 Tensor linear_rows(const Tensor& x_, const Tensor& W_, const Tensor& b_, const Tensor& perm, const Tensor& off,

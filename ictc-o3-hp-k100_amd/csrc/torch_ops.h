@@ -100,8 +100,9 @@ std::vector<bool> wanted(AutogradContext* ctx, std::initializer_list<bool> prese
   return out;
 }
 
-// (rows in the order of their id, first sorted row of each id) of ids [N] in [0, keys); those outside come last.
-std::pair<Tensor, Tensor> rows_by_id(const Tensor& ids, int64_t keys) {
+// (rows in the order of their id, first sorted row of each id) of ids [N] in [0, keys); those outside come last.  op: the
+// operator that asks.
+std::pair<Tensor, Tensor> rows_by_id(const Tensor& ids, int64_t keys, const char* op) {
   const int64_t N = ids.size(0), bytes = ictc_rows_by_id_workspace_bytes(N, keys);
   const auto ints = ids.options().dtype(at::kInt);
   const Tensor perm = at::empty({std::max<int64_t>(N, 1)}, ints), offsets = at::empty({keys + 2}, ints);
@@ -109,7 +110,7 @@ std::pair<Tensor, Tensor> rows_by_id(const Tensor& ids, int64_t keys) {
   if (bytes > 0) ws = at::empty({bytes}, ids.options().dtype(at::kByte));
   done(ictc_rows_by_id(ids.const_data_ptr<int64_t>(), N, keys, perm.mutable_data_ptr<int>(),
                        offsets.mutable_data_ptr<int>(), ptr(ws), bytes, stream_of(ids)),
-       "expert_order");
+       op);
   return {perm, offsets};
 }
 

@@ -84,3 +84,13 @@ def test_order_of_very_many_rows():
         assert (lib.ictc_rows_by_id_workspace_bytes(rows, entries) == lib.ictc_csr_workspace_bytes(rows, entries)) == general
         if entries <= 65535:
             assert lib.ictc_expert_order_workspace_bytes(rows, entries) == lib.ictc_rows_by_id_workspace_bytes(rows, entries)
+
+
+def test_refusals_name_their_own_operator():
+    nat = _built()
+    for rows, entries in ((100000, 200000), (100000, 1000), (3000000, 200000)):     # passes, one pass, the general sort
+        with pytest.raises(ValueError, match="ictc_rows_by_id_workspace_bytes"):
+            nat.call("ictc_rows_by_id", 16, rows, entries, 16, 16, None, 0, None)
+    for rows, experts in ((100000, 65535), (100000, 1000), (3000000, 65535)):
+        with pytest.raises(ValueError, match="ictc_expert_order_workspace_bytes"):
+            nat.call("ictc_expert_order", 16, rows, experts, 16, 16, None, 0, None)
