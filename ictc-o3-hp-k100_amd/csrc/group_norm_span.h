@@ -277,8 +277,10 @@ __global__ __launch_bounds__(kThreads) void gn_span_bwd_kernel(ictc::GroupNormCa
       Pack<T, EV> rg[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        rx[i].load(a, from + i * step, block + i * bstep, at.border, i < count ? at.n : 0, total);
-        rg[i] = load_part<T, EV, true>((const T*)a.g, from + i * step, i < count ? at.n : 0, total);
+        // (x of a position that there is: zero less a large mean may be infinite)
+        const int64_t f = i < count ? from + i * step : from;
+        rx[i].load(a, f, i < count ? block + i * bstep : block, at.border, at.n, total);
+        rg[i] = load_part<T, EV, true>((const T*)a.g, f, i < count ? at.n : 0, total);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {

@@ -454,3 +454,26 @@ def test_offsets_past_32_bits(device):
     r = 1 / torch.sqrt(squares / count - mean ** 2 + EPS)
     ref = (X[ends].double() - mean[:, None]) * r[:, None]
     assert rel_err(y.view(N, 8, 8)[ends], ref) < TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("bits", [None, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1030, 130, 63, 63), (3001, 401, 7, 7), (501, 1001, 30, 15), (1, 131072, 65, 13)])
+def test_samples_of_one_large_value_in_many_small_groups(device, shape, dtype, bits):
+    """2^121 everywhere, as in the test of one large value, where a tile's chunks reach over groups; 127 (2^121 / 127), which
+    its codes stand for, is 2^121 again."""
+    from ictc_o3 import decode_activations, encode_activations, group_norm
+    x, w, b, gy, *_ = _inputs(shape, dtype, device, 5)
+    x = torch.full_like(x, 2.0 ** 121)
+    assert torch.equal(decode_activations(*encode_activations(x), dtype=dtype), x)
+    for t in (x, w, b):
+        t.requires_grad_()
+    for activation in (None, "silu"):
+        y = group_norm(x, shape[3], w, b, eps=EPS, activation=activation, save_bits=bits)
+        first = torch.autograd.grad(y, (x, w, b), gy)
+        ref, sizes = Derivatives(x.detach(), shape[3], w.detach(), b.detach(), EPS, activation, gy).first()
+        z = b.detach().double()
+        _close(y, (torch.nn.functional.silu(z) if activation else z).expand(x.shape), TOL[dtype], "y")
+        _close(first[0], ref[0], TOL[dtype], "dx")
+        _close_sum(first[1], ref[1], sizes[0], "dw")
+        _close_sum(first[2], ref[2], sizes[1], "db")
