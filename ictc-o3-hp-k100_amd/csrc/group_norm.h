@@ -23,9 +23,16 @@
 //    statistics 15 us, 4.5 TB/s; result 25, its x from the caches; gradients' sums 32 and result 37.)
 // A chunk is the largest power of two of a group's channels up to 16 bytes, so each lies in one group and in one block of
 // codes.  Groups that only small chunks divide are cut into 16-byte chunks, the last in part (rows), or their tile is,
-// whatever the groups (group_norm_span.h).  Statistics of tiles and parts are sums of x and of its squares in FP64, which
-// costs nothing beside memory, loses nothing to a mean far from zero and holds squares past FP32's range.  Every sum has a
-// fixed order.
+// whatever the groups (group_norm_span.h).
+//
+// Means far from zero: statistics of tiles and parts are sums in FP64 of x less the group's first element (FP32; the sums of
+// 16-bit values near one another and of their squares are exact) and of its squares, which costs little beside memory, loses
+// nothing to what all of a group have in common and holds squares past FP32's range.  Of FP32 x a mean has two FP32 values,
+// itself and what its rounding left, and both are taken from x wherever h is made: x less the rounded mean is exact where
+// they are near, so h is as good as x is.  (By the rounded mean alone every h of a group is off by half a unit of the mean:
+// with a mean of 2^20 deviations 3 to 8 % of the results.)  The rows' backward passes find the second value anew, where it
+// counts, for there is one for every few elements; tiles and parts read it.  Half a unit of the mean is at most 2^-14 of the largest deviation of 16-bit x, and
+// 2^-17 of the error of x kept in 8 bits, so there it is left.  Every sum has a fixed order.
 #pragma once
 #include <algorithm>
 
@@ -44,6 +51,7 @@ struct GroupNormCall {
   float eps;
   int silu;
   float *mean, *rstd;   // [samples, groups]; forward writes them (null: nobody wants them)
+  float* rest;          // of the means, their FP32 value taken off (null: nobody wants them, or not taken)
   void *out, *out_g, *out_w, *out_b;
   void* ws;
   int64_t ws_bytes;
@@ -80,10 +88,10 @@ __device__ __forceinline__ Pack<T, EV> load_part(const T* __restrict__ p, int64_
 }
 
 template <bool PART, int EV>
-__device__ __forceinline__ void cut(float (&v)[EV], int n, float none = 0.f) {
+__device__ __forceinline__ void cut(float (&v)[EV], int n) {
   if constexpr (PART) {
 #pragma unroll
-    for (int e = 0; e < EV; ++e) v[e] = e < n ? v[e] : none;
+    for (int e = 0; e < EV; ++e) v[e] = e < n ? v[e] : 0.f;
   }
 }
 
@@ -259,6 +267,18 @@ struct Seconds {
     db = zz;
   }
 };
+
+// A mean in two FP32 values, and what it leaves of x.
+struct Mean {
+  float hi, lo;
+  __device__ __forceinline__ float off(float x) const { return (x - hi) - lo; }
+};
+
+// Of sample's group u, by one value or two.
+template <bool TWO>
+__device__ __forceinline__ Mean mean_of(const ictc::GroupNormCall& a, int64_t u) {
+  return {a.mean[u], TWO && a.rest ? a.rest[u] : 0.f};
+}
 
 // 1 / sqrt(var + eps) of a variance that may be past FP32
 __device__ __forceinline__ float deviation(double var, float eps) { return (float)(1.0 / sqrt(var + (double)eps)); }

@@ -8,7 +8,7 @@ int64_t workspace_bytes(int dtype, int pass, int64_t samples, int64_t positions,
   const Plan p = plan_of(dtype == ICTC_F32 ? 4 : 2, samples, positions, channels, groups, pass == 2);
   const bool parts = p.form == Form::kParts;
   const int64_t units = samples * groups, each = units * p.tile.splits * p.tile.tiles_per;
-  if (pass == 0) return parts ? each * 16 + units * 8 : 0;
+  if (pass == 0) return parts ? each * 16 + units * 12 : 0;
   const int K = pass == 1 ? 2 : kSums;
   return 4 * (2 * p.parts * channels + (parts ? (each + units) * K : 0));
 }
@@ -57,17 +57,24 @@ int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, in
   return workspace_bytes(dtype, pass, samples, positions, channels, groups);
 }
 
-int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
-                        const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
-                        float* rstd, int8_t* codes, float* scales, void* workspace, int64_t workspace_bytes, void* stream) {
+int ictc_group_norm_keeps_rest(int dtype, int64_t samples, int64_t positions, int channels, int groups) {
+  return !bad_sizes(dtype, samples, positions, channels, groups) && samples > 0 && positions > 0 && dtype == ICTC_F32 &&
+         plan_of(4, samples, positions, channels, groups, false).form != Form::kRows;
+}
+
+int ictc_group_norm_fwd_rest(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
+                             const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
+                             float* rest, float* rstd, int8_t* codes, float* scales, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(dtype, samples, positions, channels, groups)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (!(eps >= 0.f)) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: eps must not be negative");
   if (activation != 0 && activation != 1) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: activation must be 0 or 1");
   if (samples == 0 || positions == 0) return ICTC_OK;
-  if (!x || !y || !mean != !rstd || !codes != !scales) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
+  if (!x || !y || !mean != !rstd || (rest && !mean) || !codes != !scales) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
   ictc::GroupNormCall a = {};
   a.samples = samples, a.positions = positions, a.channels = channels, a.groups = groups;
-  a.x = x, a.w = weight, a.b = bias, a.eps = eps, a.silu = activation, a.out = y, a.mean = mean, a.rstd = rstd;
+  a.x = x, a.w = weight, a.b = bias, a.eps = eps, a.silu = activation, a.out = y, a.mean = mean, a.rest = rest,
+  a.rstd = rstd;
   a.codes_out = codes, a.scales_out = scales;
   a.ws = workspace, a.ws_bytes = workspace_bytes, a.stream = (hipStream_t)stream;
   if (!workspace_fits(a, dtype, 0))
@@ -78,10 +85,11 @@ int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t posit
   return dense_status("group_norm_fwd launch");
 }
 
-int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
-                        int64_t samples, int64_t positions, int channels, int groups, const void* weight,
-                        const void* bias, int activation, const float* mean, const float* rstd, void* dx, void* dweight,
-                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+int ictc_group_norm_bwd_rest(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                             int64_t samples, int64_t positions, int channels, int groups, const void* weight,
+                             const void* bias, int activation, const float* mean, const float* rest, const float* rstd,
+                             void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
   if (const char* e = bad_sizes(dtype, samples, positions, channels, groups)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (activation != 0 && activation != 1) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: activation must be 0 or 1");
   const bool none = samples == 0 || positions == 0;
@@ -91,7 +99,7 @@ int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const flo
   ictc::GroupNormCall a = {};
   a.samples = none ? 0 : samples, a.positions = none ? 1 : positions, a.channels = channels, a.groups = groups;
   a.x = x, a.codes = codes, a.scales = scales, a.g = grad, a.w = weight, a.b = bias, a.silu = activation;
-  a.mean = (float*)mean, a.rstd = (float*)rstd, a.out = dx, a.out_w = dweight, a.out_b = dbias;
+  a.mean = (float*)mean, a.rest = (float*)rest, a.rstd = (float*)rstd, a.out = dx, a.out_w = dweight, a.out_b = dbias;
   a.ws = workspace, a.ws_bytes = workspace_bytes, a.stream = (hipStream_t)stream;
   if (!workspace_fits(a, dtype, 1))
     return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: workspace smaller than ictc_group_norm_workspace_bytes");
@@ -99,11 +107,11 @@ int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const flo
   return dense_status("group_norm_bwd launch");
 }
 
-int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
-                         const void* v, const void* vweight, const void* vbias, int64_t samples, int64_t positions,
-                         int channels, int groups, const void* weight, const void* bias, int activation,
-                         const float* mean, const float* rstd, void* dx, void* dgrad, void* dweight, void* dbias,
-                         void* workspace, int64_t workspace_bytes, void* stream) {
+int ictc_group_norm_bwd2_rest(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                              const void* v, const void* vweight, const void* vbias, int64_t samples, int64_t positions,
+                              int channels, int groups, const void* weight, const void* bias, int activation,
+                              const float* mean, const float* rest, const float* rstd, void* dx, void* dgrad,
+                              void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const char* e = bad_sizes(dtype, samples, positions, channels, groups)) return dense_fail(ICTC_ERR_ARGUMENT, e);
   if (activation != 0 && activation != 1) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: activation must be 0 or 1");
   const bool none = samples == 0 || positions == 0;
@@ -113,13 +121,38 @@ int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const fl
   ictc::GroupNormCall a = {};
   a.samples = none ? 0 : samples, a.positions = none ? 1 : positions, a.channels = channels, a.groups = groups;
   a.x = x, a.codes = codes, a.scales = scales, a.g = grad, a.v = v, a.vw = vweight, a.vb = vbias;
-  a.w = weight, a.b = bias, a.silu = activation, a.mean = (float*)mean, a.rstd = (float*)rstd;
+  a.w = weight, a.b = bias, a.silu = activation, a.mean = (float*)mean, a.rest = (float*)rest, a.rstd = (float*)rstd;
   a.out = dx, a.out_g = dgrad, a.out_w = dweight, a.out_b = dbias;
   a.ws = workspace, a.ws_bytes = workspace_bytes, a.stream = (hipStream_t)stream;
   if (!workspace_fits(a, dtype, 2))
     return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: workspace smaller than ictc_group_norm_workspace_bytes");
   GN_TYPED(group_norm_bwd2)
   return dense_status("group_norm_bwd2 launch");
+}
+
+int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
+                        const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
+                        float* rstd, int8_t* codes, float* scales, void* workspace, int64_t workspace_bytes, void* stream) {
+  return ictc_group_norm_fwd_rest(dtype, x, samples, positions, channels, groups, weight, bias, eps, activation, y, mean,
+                                  nullptr, rstd, codes, scales, workspace, workspace_bytes, stream);
+}
+
+int ictc_group_norm_bwd(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                        int64_t samples, int64_t positions, int channels, int groups, const void* weight,
+                        const void* bias, int activation, const float* mean, const float* rstd, void* dx, void* dweight,
+                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  return ictc_group_norm_bwd_rest(dtype, x, codes, scales, grad, samples, positions, channels, groups, weight, bias,
+                                  activation, mean, nullptr, rstd, dx, dweight, dbias, workspace, workspace_bytes, stream);
+}
+
+int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                         const void* v, const void* vweight, const void* vbias, int64_t samples, int64_t positions,
+                         int channels, int groups, const void* weight, const void* bias, int activation,
+                         const float* mean, const float* rstd, void* dx, void* dgrad, void* dweight, void* dbias,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  return ictc_group_norm_bwd2_rest(dtype, x, codes, scales, grad, v, vweight, vbias, samples, positions, channels, groups,
+                                   weight, bias, activation, mean, nullptr, rstd, dx, dgrad, dweight, dbias, workspace,
+                                   workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -182,7 +182,7 @@ inline bool own_parts(const Plan& p) {
   }
 
 template <typename T, int EV, bool SILU>
-void launch_fwd(const ictc::GroupNormCall& a, const Plan& p) {
+void launch_fwd(ictc::GroupNormCall a, const Plan& p) {
   const int per = a.channels / a.groups;
   if (p.form == Form::kRows) {
     const dim3 grid(p.rows.blocks_fwd, p.rows.blocks_y);
@@ -207,22 +207,23 @@ void launch_fwd(const ictc::GroupNormCall& a, const Plan& p) {
   const int64_t units = a.samples * a.groups;
   const int parts = p.tile.splits * p.tile.tiles_per;
   double* part = (double*)a.ws;
-  float* mean = a.mean ? a.mean : (float*)(part + units * parts * 2);
-  float* rstd = a.mean ? a.rstd : mean + units;
   if (p.part) {
     if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_fwd_kernel<T, EV, SILU>), a, p.tile, per, part);
   } else {
     GN_LAUNCH((gn_part_stats_kernel<T, EV>), a, p.tile, per, part);
   }
   const bool own = own_parts(p);
-  if (!own)
-    hipLaunchKernelGGL(gn_part_moments_kernel, unit_blocks(units), dim3(256), 0, a.stream, part, units, parts,
-                       (double)per * (double)a.positions, a.eps, mean, rstd);
   const double* parts_of = own ? part : nullptr;
+  if (!own) {   // means that nobody wants, or in one value each, go behind the parts
+    float* kept = (float*)(part + units * parts * 2);
+    if (!a.rest) a.rest = kept;
+    if (!a.mean) a.mean = kept + units, a.rstd = kept + 2 * units;
+    hipLaunchKernelGGL(gn_part_moments_kernel<T>, unit_blocks(units), dim3(256), 0, a.stream, a, part, units, parts, per);
+  }
   if (p.part) {
-    if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of, mean, rstd);
+    if constexpr (EV == kChunk<T>) GN_LAUNCH((gn_span_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of);
   } else {
-    GN_LAUNCH((gn_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of, mean, rstd);
+    GN_LAUNCH((gn_part_fwd_kernel<T, EV, SILU>), a, p.tile, per, parts_of);
   }
 }
 

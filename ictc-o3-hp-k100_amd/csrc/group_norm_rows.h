@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
     }
     rows_sum<WIDE>(s, p.team, cross);
     // The deviations' own mean corrects the rounded one, a quotient to the last bit (a group of one value far from zero has
-    // no deviation left).
-    const float first = s[0] * inv;
+    // no deviation left).  (Held: one value wherever it is used, none of them joined with the product.)
+    const float first = held(s[0] * inv);
     float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
         q[1] += v[i][e] * v[i][e];
       }
     rows_sum<WIDE>(q, p.team, cross);
-    const float about = q[0] * inv, rest = __builtin_fmaf(__builtin_fmaf(-about, count, q[0]), inv, about), mu = first + rest;
+    const float about = q[0] * inv, rest = __builtin_fmaf(__builtin_fmaf(-about, count, q[0]), inv, about);
     float r = 1.f / sqrtf(fmaxf(q[1] * inv - rest * rest, 0.f) + a.eps);
     // (the whole team) squares past FP32 of finite deviations, or hardly any but the mean's: added again, without that, scaled
     if (q[1] == __builtin_inff() || 2.f * rest * rest > q[1] * inv) {
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void gn_rows_fwd_kernel(ictc::GroupNormCall a,
       if (k.n[i] > 0) store_part<T, EV, PART>((T*)a.out + base + k.from[i], k.n[i], v[i]);
     }
     if (at.lane == 0 && a.mean) {
-      a.mean[n * a.groups + at.group] = mu;
+      a.mean[n * a.groups + at.group] = first + rest;
       a.rstd[n * a.groups + at.group] = r;
     }
   }
@@ -180,6 +180,25 @@ __device__ __forceinline__ void rows_channels(float (&acc)[N][EV], const RowsPla
   }
 }
 
+// The team's mean as the backward passes take it: of FP32 x with what its rounding to `mean` left, the mean of x less it,
+// where that counts: half a unit of a mean of up to eight deviations 1 / r is 2^-22 of one.  (425,991 x 64 in eight groups,
+// gradients 60 us; looked for by every team, or read from memory, 66.)
+template <typename T, int EV, int N, bool WIDE, bool PART, bool EIGHT, typename X>
+__device__ __forceinline__ Mean rows_mean(const X (&rx)[N], const int (&n)[N], float mean, float r, float inv, int team,
+                                          float* cross) {
+  if (sizeof(T) == 2 || EIGHT || !(fabsf(mean) * r > 8.f)) return {mean, 0.f};   // (the whole team)
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float v[EV];
+    rx[i].values(v);
+#pragma unroll
+    for (int e = 0; e < EV; ++e) s[0] += (PART ? e : 0) < n[i] ? v[e] - mean : 0.f;
+  }
+  rows_sum<WIDE>(s, team, cross);
+  return {mean, s[0] * inv};
+}
+
 template <typename T, int EV, int N, bool WIDE, bool PART, bool SILU, bool EIGHT>
 __global__ __launch_bounds__(256) void gn_rows_bwd_kernel(ictc::GroupNormCall a, RowsPlan p, int per,
                                                           float* __restrict__ part_w, float* __restrict__ part_b) {
@@ -206,17 +225,18 @@ __global__ __launch_bounds__(256) void gn_rows_bwd_kernel(ictc::GroupNormCall a,
       rx[i].load(a, base + k.from[i], n * blocks + k.block[i], k.border[i], k.n[i], end);
       rg[i] = load_part<T, EV, PART>((const T*)a.g, base + k.from[i], k.n[i], end);
     }
-    const float mu = a.mean[n * a.groups + at.group], r = a.rstd[n * a.groups + at.group];
+    const float r = a.rstd[n * a.groups + at.group];
+    const Mean mu = rows_mean<T, EV, N, WIDE, PART, EIGHT>(rx, k.n, a.mean[n * a.groups + at.group], r, inv, p.team, lds);
     float h[N][EV], u[N][EV], s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       rx[i].values(h[i]);
       get<T, EV>(rg[i], u[i]);
-      cut<PART>(h[i], k.n[i], mu);   // (nothing is the mean: a large one times r may be infinite)
       cut<PART>(u[i], k.n[i]);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        h[i][e] = (PART || k.n[i] > 0 ? h[i][e] - mu : 0.f) * r;
+        // (what there is not has no deviation: zero less a large mean, times r, may be infinite)
+        h[i][e] = ((PART ? e : 0) < k.n[i] ? mu.off(h[i][e]) : 0.f) * r;
         const float ga = u[i][e] * Act<SILU>(h[i][e] * w[i][e] + b[i][e]).slope();
         dw[i][e] += ga * h[i][e];
         db[i][e] += ga;
@@ -279,7 +299,8 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       rg[i] = load_part<T, EV, PART>((const T*)a.g, base + k.from[i], k.n[i], end);
       rv[i] = load_part<T, EV, PART>((const T*)a.v, base + k.from[i], k.n[i], end);
     }
-    const float mu = a.mean[n * a.groups + at.group], r = a.rstd[n * a.groups + at.group];
+    const float r = a.rstd[n * a.groups + at.group];
+    const Mean mu = rows_mean<T, EV, N, WIDE, PART, EIGHT>(rx, k.n, a.mean[n * a.groups + at.group], r, inv, p.team, lds);
     float s[kSums] = {};
     Point kept[KEEP ? EV : 1];
     float x[EV], g[EV], v[EV];
@@ -287,7 +308,6 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       rx[i].values(x);
       get<T, EV>(rg[i], g);
       get<T, EV>(rv[i], v);
-      cut<PART>(x, k.n[i], mu);
       cut<PART>(g, k.n[i]);
       cut<PART>(v, k.n[i]);
       if (!KEEP) q.load(a, k.c[i], k.n[i]);
@@ -297,7 +317,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
       unpack(i);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const Point o = point<SILU>((PART || k.n[i] > 0 ? x[e] - mu : 0.f) * r, g[e], q.w[e], q.b[e]);
+        const Point o = point<SILU>(((PART ? e : 0) < k.n[i] ? mu.off(x[e]) : 0.f) * r, g[e], q.w[e], q.b[e]);
         if (KEEP) kept[KEEP ? e : 0] = o;
         add_sums<SILU>(o, r, v[e], q.w[e], q.vw[e], q.vb[e], s);
       }
@@ -310,7 +330,7 @@ __global__ __launch_bounds__(256) void gn_rows_bwd2_kernel(ictc::GroupNormCall a
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
         const Point o = KEEP ? kept[KEEP ? e : 0]
-                             : point<SILU>((PART || k.n[i] > 0 ? x[e] - mu : 0.f) * r, g[e], q.w[e], q.b[e]);
+                             : point<SILU>(((PART ? e : 0) < k.n[i] ? mu.off(x[e]) : 0.f) * r, g[e], q.w[e], q.b[e]);
         float pw, pb;
         of.element(o, r, v[e], q.w[e], q.vw[e], q.vb[e], x[e], v[e], pw, pb);
         dw[i][e] += (PART ? e : 0) < k.n[i] ? pw : 0.f;

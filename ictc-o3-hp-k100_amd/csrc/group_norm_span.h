@@ -86,11 +86,14 @@ __device__ __forceinline__ void span_parts(const V* __restrict__ part, int split
   __syncthreads();
 }
 
-// Sums by group of the tile's x and of its squares.
+// Sums by group of the tile's x less the group's first element and of their squares.
 template <typename T, int EV>
 __device__ __forceinline__ void span_statistics(const ictc::GroupNormCall& a, const TilePlan& p, const SpanAt<EV>& at, int per,
                                                 int64_t total, double* lds, double (*sums)[2]) {
   double s[2 * EV] = {};
+  float zero[EV];
+#pragma unroll
+  for (int e = 0; e < EV; ++e) zero[e] = at.on ? first_of<T>(a, at.sample, at.first_group + at.local[e], per) : 0.f;
   constexpr int U = 2;
   walk<U>(p, at, a.positions, a.channels, [&](int64_t from, int64_t step, int64_t, int64_t, int count) {
     Pack<T, EV> raw[U];
@@ -98,12 +101,12 @@ __device__ __forceinline__ void span_statistics(const ictc::GroupNormCall& a, co
     for (int i = 0; i < U; ++i) raw[i] = load_part<T, EV, true>((const T*)a.x, from + i * step, i < count ? at.n : 0, total);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
+      if (i >= count) break;   // (past n: sums that nobody reads)
       float v[EV];
       get<T, EV>(raw[i], v);
-      cut<true>(v, at.n);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const double d = v[e];
+        const double d = (double)v[e] - (double)zero[e];
         s[e] += d;
         s[EV + e] += d * d;
       }
@@ -115,12 +118,21 @@ __device__ __forceinline__ void span_statistics(const ictc::GroupNormCall& a, co
 
 template <int EV>
 struct SpanMoments {
-  float mean[EV], rstd[EV];
-  __device__ __forceinline__ void load(const float* __restrict__ m, const float* __restrict__ r, const SpanAt<EV>& at) {
+  Mean mean[EV];
+  float rstd[EV];
+  __device__ __forceinline__ void load(const Moments* m, const SpanAt<EV>& at) {   // the tile's groups'
 #pragma unroll
     for (int e = 0; e < EV; ++e) {
-      mean[e] = m[at.local[e]];
-      rstd[e] = r[at.local[e]];
+      mean[e] = m[at.local[e]].mean;
+      rstd[e] = m[at.local[e]].rstd;
+    }
+  }
+  template <bool TWO>
+  __device__ __forceinline__ void load(const ictc::GroupNormCall& a, int64_t u, const SpanAt<EV>& at) {   // u: its first group
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      mean[e] = mean_of<TWO>(a, u + at.local[e]);
+      rstd[e] = a.rstd[u + at.local[e]];
     }
   }
 };
@@ -142,7 +154,7 @@ __device__ __forceinline__ void span_result(const ictc::GroupNormCall& a, const 
       float v[EV];
       get<T, EV>(raw[i], v);
 #pragma unroll
-      for (int e = 0; e < EV; ++e) v[e] = Act<SILU>((v[e] - m.mean[e]) * m.rstd[e] * w[e] + b[e]).value();
+      for (int e = 0; e < EV; ++e) v[e] = Act<SILU>(m.mean[e].off(v[e]) * m.rstd[e] * w[e] + b[e]).value();
       store_part<T, EV, true>((T*)a.out + from + i * step, at.n, v);
     }
   });
@@ -154,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void gn_span_fwd_kernel(ictc::GroupNormCa
                                                                double* __restrict__ part) {
   __shared__ double lds[2 * EV * kThreads];
   __shared__ double sums[kSpanGroups][2];
-  __shared__ float mean[kSpanGroups], rstd[kSpanGroups];
+  __shared__ Moments groups[kSpanGroups];
   SpanAt<EV> at(p, per, a.groups, a.positions);
   const int64_t total = a.samples * a.positions * a.channels;
   for (; at.sample < a.samples; at.sample += p.slots) {
@@ -169,17 +181,13 @@ __global__ __launch_bounds__(kThreads) void gn_span_fwd_kernel(ictc::GroupNormCa
       continue;   // (the next sample's sums are behind a barrier)
     }
     if (g < at.groups) {
-      const Moments m = moments(sums[g][0], sums[g][1], (double)per * (double)a.positions, a.eps);
-      mean[g] = m.mean;
-      rstd[g] = m.rstd;
-      if (a.mean) {
-        a.mean[u + g] = m.mean;
-        a.rstd[u + g] = m.rstd;
-      }
+      const float zero = first_of<T>(a, at.sample, at.first_group + g, per);
+      groups[g] = moments<T>(zero, sums[g][0], sums[g][1], (double)per * (double)a.positions, a.eps);
+      if (a.mean) keep(a, u + g, groups[g]);
     }
     __syncthreads();
     SpanMoments<EV> m;
-    m.load(mean, rstd, at);
+    m.load(groups, at);
     span_result<T, EV, SILU>(a, p, at, m, total);
   }
 }
@@ -187,11 +195,9 @@ __global__ __launch_bounds__(kThreads) void gn_span_fwd_kernel(ictc::GroupNormCa
 // part: the statistics' parts, which the blocks add (those of split 0 write mean and rstd, if they are wanted); or null
 template <typename T, int EV, bool SILU>
 __global__ __launch_bounds__(kThreads) void gn_span_part_fwd_kernel(ictc::GroupNormCall a, TilePlan p, int per,
-                                                                    const double* __restrict__ part,
-                                                                    const float* __restrict__ mean_,
-                                                                    const float* __restrict__ rstd_) {
+                                                                    const double* __restrict__ part) {
   __shared__ double sums[kSpanGroups][2];
-  __shared__ float mean[kSpanGroups], rstd[kSpanGroups];
+  __shared__ Moments groups[kSpanGroups];
   SpanAt<EV> at(p, per, a.groups, a.positions);
   const int64_t total = a.samples * a.positions * a.channels;
   for (; at.sample < a.samples; at.sample += p.slots) {
@@ -201,18 +207,14 @@ __global__ __launch_bounds__(kThreads) void gn_span_part_fwd_kernel(ictc::GroupN
       span_parts(part + u * p.splits * 2, p.splits, at.groups, sums);
       const int g = threadIdx.x;
       if (g < at.groups) {
-        const Moments o = moments(sums[g][0], sums[g][1], (double)per * (double)a.positions, a.eps);
-        mean[g] = o.mean;
-        rstd[g] = o.rstd;
-        if (a.mean && at.split == 0) {
-          a.mean[u + g] = o.mean;
-          a.rstd[u + g] = o.rstd;
-        }
+        const float zero = first_of<T>(a, at.sample, at.first_group + g, per);
+        groups[g] = moments<T>(zero, sums[g][0], sums[g][1], (double)per * (double)a.positions, a.eps);
+        if (a.mean && at.split == 0) keep(a, u + g, groups[g]);
       }
       __syncthreads();
-      m.load(mean, rstd, at);
+      m.load(groups, at);
     } else {
-      m.load(mean_ + u, rstd_ + u, at);
+      m.template load<sizeof(T) == 4>(a, u, at);
     }
     span_result<T, EV, SILU>(a, p, at, m, total);
   }
@@ -245,7 +247,7 @@ __device__ __forceinline__ void span_gradient(const ictc::GroupNormCall& a, cons
       get<T, EV>(rg[i], g);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const float h = (x[e] - m.mean[e]) * m.rstd[e], ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
+        const float h = m.mean[e].off(x[e]) * m.rstd[e], ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
         x[e] = m.rstd[e] * (ga * w[e] - u[e] - h * uh[e]);
       }
       store_part<T, EV, true>((T*)a.out + from + i * step, at.n, x);
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void gn_span_bwd_kernel(ictc::GroupNormCa
   for (; at.sample < a.samples; at.sample += p.slots) {
     const int64_t group = at.sample * a.groups + at.first_group;
     SpanMoments<EV> m;
-    m.load(a.mean + group, a.rstd + group, at);
+    m.template load<sizeof(T) == 4 && !EIGHT>(a, group, at);
     float s[2 * EV] = {};
     constexpr int U = 2;
     walk<U>(p, at, a.positions, a.channels, [&](int64_t from, int64_t step, int64_t block, int64_t bstep, int count) {
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void gn_span_bwd_kernel(ictc::GroupNormCa
         cut<true>(g, at.n);
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
-          const float h = (x[e] - m.mean[e]) * m.rstd[e], ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
+          const float h = m.mean[e].off(x[e]) * m.rstd[e], ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
           s[e] += ga;
           s[EV + e] += ga * h;
         }
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void gn_span_part_bwd_kernel(ictc::GroupN
       __syncthreads();
     }
     SpanMoments<EV> m;
-    m.load(a.mean + group, a.rstd + group, at);
+    m.template load<sizeof(T) == 4 && !EIGHT>(a, group, at);
     span_gradient<T, EV, SILU, EIGHT>(a, p, at, m, w, b, sums, 1.f / ((float)per * (float)a.positions), total);
   }
 }

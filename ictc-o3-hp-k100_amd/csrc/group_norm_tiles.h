@@ -139,11 +139,20 @@ __device__ __forceinline__ void walk(const TilePlan& p, const At& at, int64_t S,
     f(from, step, block, bstep, (int)min<int64_t>(U, (left + p.rows - 1) / p.rows));
 }
 
+// What the statistics of sample n's group are counted from: its first element, zero of 16 bits.
+template <typename T>
+__device__ __forceinline__ float first_of(const ictc::GroupNormCall& a, int64_t n, int group, int per) {
+  if constexpr (sizeof(T) == 2) return 0.f;
+  return (float)((const T*)a.x)[n * a.positions * a.channels + (int64_t)group * per];
+}
+
+// Sums over the tile's group of x less its first element and of their squares; returns that.
 template <typename T, int EV>
-__device__ __forceinline__ void tile_statistics(const ictc::GroupNormCall& a, const TilePlan& p, const TileAt& at,
-                                                double (&s)[2], double* lds) {
+__device__ __forceinline__ float tile_statistics(const ictc::GroupNormCall& a, const TilePlan& p, const TileAt& at, int per,
+                                                 double (&s)[2], double* lds) {
   constexpr int U = kRowsAtOnce<EV>;
   s[0] = s[1] = 0.0;
+  const float zero = at.on ? first_of<T>(a, at.sample, at.group, per) : 0.f;
   walk<U>(p, at, a.positions, a.channels, [&](int64_t from, int64_t step, int64_t, int64_t, int count) {
     Pack<T, EV> raw[U];
 #pragma unroll
@@ -151,26 +160,43 @@ __device__ __forceinline__ void tile_statistics(const ictc::GroupNormCall& a, co
       raw[i] = load_pack<T, EV>((const T*)a.x + (i < count ? from + i * step : from), i < count);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
+      if (i >= count) break;
       float v[EV];
       get<T, EV>(raw[i], v);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const double d = v[e];
+        const double d = (double)v[e] - (double)zero;
         s[0] += d;
         s[1] += d * d;
       }
     }
   });
   sum_all(s, p, at, lds);
+  return zero;
 }
 
 struct Moments {
-  float mean, rstd;
+  Mean mean;
+  float rstd;
 };
 
-__device__ __forceinline__ Moments moments(double sum, double squares, double count, float eps) {
-  const double mean = sum / count, var = squares / count - mean * mean;
-  return {(float)mean, deviation(var < 0.0 ? 0.0 : var, eps)};
+// Of sums of values less `zero`.
+template <typename T>
+__device__ __forceinline__ Moments moments(float zero, double sum, double squares, double count, float eps) {
+  const double off = sum / count, var = squares / count - off * off, mean = zero + off;
+  return {{(float)mean, sizeof(T) == 4 ? (float)(mean - (float)mean) : 0.f}, deviation(var < 0.0 ? 0.0 : var, eps)};
+}
+
+template <typename T, bool EIGHT>
+__device__ __forceinline__ Moments moments_of(const ictc::GroupNormCall& a, int64_t u) {
+  return {mean_of<sizeof(T) == 4 && !EIGHT>(a, u), a.rstd[u]};
+}
+
+// To where they are wanted.
+__device__ __forceinline__ void keep(const ictc::GroupNormCall& a, int64_t u, const Moments& m) {
+  a.mean[u] = m.mean.hi;
+  if (a.rest) a.rest[u] = m.mean.lo;
+  a.rstd[u] = m.rstd;
 }
 
 template <typename T, int EV, bool SILU>
@@ -191,7 +217,7 @@ __device__ __forceinline__ void tile_result(const ictc::GroupNormCall& a, const 
       float v[EV];
       get<T, EV>(raw[i], v);
 #pragma unroll
-      for (int e = 0; e < EV; ++e) v[e] = Act<SILU>((v[e] - m.mean) * m.rstd * w[e] + b[e]).value();
+      for (int e = 0; e < EV; ++e) v[e] = Act<SILU>(m.mean.off(v[e]) * m.rstd * w[e] + b[e]).value();
       store_pack<T, EV>((T*)a.out + from + i * step, v);
     }
   });
@@ -203,12 +229,9 @@ __global__ __launch_bounds__(kThreads) void gn_tile_fwd_kernel(ictc::GroupNormCa
   TileAt at(p, EV, per, a.groups, a.positions);
   for (; at.sample < a.samples; at.sample += p.slots) {
     double s[2];
-    tile_statistics<T, EV>(a, p, at, s, lds);
-    const Moments m = moments(s[0], s[1], (double)per * (double)a.positions, a.eps);
-    if (a.mean && at.first) {
-      a.mean[at.sample * a.groups + at.group] = m.mean;
-      a.rstd[at.sample * a.groups + at.group] = m.rstd;
-    }
+    const float zero = tile_statistics<T, EV>(a, p, at, per, s, lds);
+    const Moments m = moments<T>(zero, s[0], s[1], (double)per * (double)a.positions, a.eps);
+    if (a.mean && at.first) keep(a, at.sample * a.groups + at.group, m);
     tile_result<T, EV, SILU>(a, p, at, m);
   }
 }
@@ -221,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void gn_part_stats_kernel(ictc::GroupNorm
   TileAt at(p, EV, per, a.groups, a.positions);
   for (; at.sample < a.samples; at.sample += p.slots) {
     double s[2];
-    tile_statistics<T, EV>(a, p, at, s, lds);
+    tile_statistics<T, EV>(a, p, at, per, s, lds);
     if (at.first) {
       double* to = part + ((at.sample * a.groups + at.group) * (p.splits * p.tiles_per) + at.part) * 2;
       to[0] = s[0];
@@ -244,17 +267,17 @@ __device__ __forceinline__ void wave_parts(const V* __restrict__ part, int parts
     for (int d = 32; d > 0; d /= 2) s[i] += __shfl_xor(s[i], d);
 }
 
-// A wave a sample's group.
-__global__ __launch_bounds__(256) void gn_part_moments_kernel(const double* __restrict__ part, int64_t units, int parts,
-                                                              double count, float eps, float* __restrict__ mean,
-                                                              float* __restrict__ rstd) {
+// A wave a sample's group; to a's mean, rest and rstd.
+template <typename T>
+__global__ __launch_bounds__(256) void gn_part_moments_kernel(ictc::GroupNormCall a, const double* __restrict__ part,
+                                                              int64_t units, int parts, int per) {
   for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (int64_t)gridDim.x * 4) {
     double s[2];
     wave_parts<2>(part + u * parts * 2, parts, s);
     if ((threadIdx.x & 63) == 0) {
-      const Moments m = moments(s[0], s[1], count, eps);
-      mean[u] = m.mean;
-      rstd[u] = m.rstd;
+      const int64_t n = u / a.groups;
+      const float zero = first_of<T>(a, n, (int)(u - n * a.groups), per);
+      keep(a, u, moments<T>(zero, s[0], s[1], (double)per * (double)a.positions, a.eps));
     }
   }
 }
@@ -295,24 +318,20 @@ __device__ __forceinline__ void tile_parts(const V* __restrict__ part, int64_t s
 // are wanted); else null, and mean and rstd are read
 template <typename T, int EV, bool SILU>
 __global__ __launch_bounds__(kThreads) void gn_part_fwd_kernel(ictc::GroupNormCall a, TilePlan p, int per,
-                                                               const double* __restrict__ part,
-                                                               const float* __restrict__ mean,
-                                                               const float* __restrict__ rstd) {
+                                                               const double* __restrict__ part) {
   __shared__ double lds[kOwnGroups][2];
   TileAt at(p, EV, per, a.groups, a.positions);
   for (; at.sample < a.samples; at.sample += p.slots) {
-    Moments m = {0.f, 0.f};
+    Moments m = {{0.f, 0.f}, 0.f};
     const int64_t u = at.sample * a.groups + at.group;
     if (part) {
       double s[2];
       tile_parts(part, at.sample, a.groups, p, at, s, lds);
-      m = moments(s[0], s[1], (double)per * (double)a.positions, a.eps);
-      if (a.mean && at.first && at.split == 0) {
-        a.mean[u] = m.mean;
-        a.rstd[u] = m.rstd;
-      }
+      const float zero = at.on ? first_of<T>(a, at.sample, at.group, per) : 0.f;
+      m = moments<T>(zero, s[0], s[1], (double)per * (double)a.positions, a.eps);
+      if (a.mean && at.first && at.split == 0) keep(a, u, m);
     } else if (at.on) {
-      m = {mean[u], rstd[u]};
+      m = moments_of<T, false>(a, u);
     }
     tile_result<T, EV, SILU>(a, p, at, m);
   }
@@ -341,7 +360,7 @@ __device__ __forceinline__ void tile_channels(const ictc::GroupNormCall& a, cons
       get<T, EV>(rg[i], g);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const float h = (x[e] - m.mean) * m.rstd, ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
+        const float h = m.mean.off(x[e]) * m.rstd, ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
         s[e] += ga;
         s[EV + e] += ga * h;
       }
@@ -371,7 +390,7 @@ __device__ __forceinline__ void tile_gradient(const ictc::GroupNormCall& a, cons
       get<T, EV>(rg[i], g);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const float h = (x[e] - m.mean) * m.rstd, ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
+        const float h = m.mean.off(x[e]) * m.rstd, ga = g[e] * Act<SILU>(h * w[e] + b[e]).slope();
         x[e] = m.rstd * (ga * w[e] - mu - h * muh);
       }
       store_pack<T, EV>((T*)a.out + from + i * step, x);
@@ -418,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void gn_tile_bwd_kernel(ictc::GroupNormCa
   ChannelSums<EV> channels;
   for (; at.sample < a.samples; at.sample += p.slots) {
     const int64_t u = at.on ? at.sample * a.groups + at.group : 0;
-    const Moments m = {a.mean[u], a.rstd[u]};
+    const Moments m = moments_of<T, EIGHT>(a, u);
     tile_channels<T, EV, SILU, EIGHT>(a, p, at, m, w, b, lds);
     float s[2] = {0.f, 0.f};
     if (at.on && at.row == 0) {
@@ -465,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void gn_part_bwd_kernel(ictc::GroupNormCa
       s[0] = sums[u * 2];
       s[1] = sums[u * 2 + 1];
     }
-    tile_gradient<T, EV, SILU, EIGHT>(a, p, at, Moments{a.mean[u], a.rstd[u]}, w, b, s[0] * inv, s[1] * inv);
+    tile_gradient<T, EV, SILU, EIGHT>(a, p, at, moments_of<T, EIGHT>(a, u), w, b, s[0] * inv, s[1] * inv);
   }
 }
 
@@ -495,7 +514,7 @@ __device__ __forceinline__ void tile_sums(const ictc::GroupNormCall& a, const Ti
       get<T, EV>(rv[i], v);
 #pragma unroll
       for (int e = 0; e < EV; ++e)
-        add_sums<SILU>(point<SILU>((x[e] - m.mean) * m.rstd, g[e], w[e], b[e]), m.rstd, v[e], w[e], vw[e], vb[e], s);
+        add_sums<SILU>(point<SILU>(m.mean.off(x[e]) * m.rstd, g[e], w[e], b[e]), m.rstd, v[e], w[e], vw[e], vb[e], s);
     }
   });
   sum_all(s, p, at, lds);
@@ -527,7 +546,7 @@ __device__ __forceinline__ void tile_second(const ictc::GroupNormCall& a, const 
       get<T, EV>(rv[i], v);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        of.element(point<SILU>((x[e] - m.mean) * m.rstd, g[e], w[e], b[e]), m.rstd, v[e], w[e], vw[e], vb[e], x[e], v[e], pw,
+        of.element(point<SILU>(m.mean.off(x[e]) * m.rstd, g[e], w[e], b[e]), m.rstd, v[e], w[e], vw[e], vb[e], x[e], v[e], pw,
                    pb);
         s[e] += pb;
         s[EV + e] += pw;
@@ -559,7 +578,7 @@ __global__ __launch_bounds__(kThreads) void gn_tile_bwd2_kernel(ictc::GroupNormC
   ChannelSums<EV> channels;
   for (; at.sample < a.samples; at.sample += p.slots) {
     const int64_t u = at.on ? at.sample * a.groups + at.group : 0;
-    const Moments m = {a.mean[u], a.rstd[u]};
+    const Moments m = moments_of<T, EIGHT>(a, u);
     float s[kSums];
     if constexpr (PHASE != Phase::kResults) {
       tile_sums<T, EV, SILU, EIGHT>(a, p, at, m, w, b, vw, vb, s, lds);

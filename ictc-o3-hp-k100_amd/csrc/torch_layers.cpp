@@ -110,6 +110,15 @@ struct NormShape {
   int64_t samples, positions, groups;
   int channels;
   bool silu;
+  int64_t units() const { return samples * groups; }
+};
+
+// Of a sample's groups: means and 1 / deviations [2 units], and where it counts what their rounding left of the means [units].
+struct Stats {
+  Tensor both, rest;
+  float* mean() const { return both.defined() ? both.mutable_data_ptr<float>() : nullptr; }
+  float* rstd(const NormShape& n) const { return both.defined() ? mean() + n.units() : nullptr; }
+  float* left() const { return rest.defined() ? rest.mutable_data_ptr<float>() : nullptr; }
 };
 
 // What a backward pass has of x [samples, positions, channels]: itself, or codes and scales of its rows of channels.
@@ -127,7 +136,7 @@ struct GroupGrads {
   Tensor x, w, b;
 };
 
-GroupGrads group_backward(const Kept& kept, const Tensor& g_, const Tensor& w_, const Tensor& b_, const Tensor& stats,
+GroupGrads group_backward(const Kept& kept, const Tensor& g_, const Tensor& w_, const Tensor& b_, const Stats& stats,
                           const NormShape& n, bool need_x, bool need_w, bool need_b) {
   eager("group_norm");
   const c10::DeviceGuard guard(g_.device());
@@ -139,10 +148,9 @@ GroupGrads group_backward(const Kept& kept, const Tensor& g_, const Tensor& w_, 
   if (need_b) out.b = at::empty({n.channels}, g.options());
   const int64_t bytes = ictc_group_norm_workspace_bytes(dt, 1, n.samples, n.positions, n.channels, (int)n.groups);
   const Tensor ws = workspace(bytes, g);
-  const float* st = stats.const_data_ptr<float>();
-  done(ictc_group_norm_bwd(dt, ptr(x), kept.code(), kept.scale(), ptr(g), n.samples, n.positions, n.channels,
-                           (int)n.groups, ptr(w), ptr(b), n.silu, st, st + n.samples * n.groups, ptr(out.x), ptr(out.w),
-                           ptr(out.b), ptr(ws), bytes, stream_of(g)),
+  done(ictc_group_norm_bwd_rest(dt, ptr(x), kept.code(), kept.scale(), ptr(g), n.samples, n.positions, n.channels,
+                                (int)n.groups, ptr(w), ptr(b), n.silu, stats.mean(), stats.left(), stats.rstd(n),
+                                ptr(out.x), ptr(out.w), ptr(out.b), ptr(ws), bytes, stream_of(g)),
        "group_norm");
   return out;
 }
@@ -152,7 +160,7 @@ struct GroupSeconds {
 };
 
 GroupSeconds group_backward2(const Kept& kept, const Tensor& g_, const Tensor& w_, const Tensor& b_, const Tensor& v_,
-                             const Tensor& vw_, const Tensor& vb_, const Tensor& stats, const NormShape& n, bool need_x,
+                             const Tensor& vw_, const Tensor& vb_, const Stats& stats, const NormShape& n, bool need_x,
                              bool need_g, bool need_w, bool need_b) {
   eager("group_norm");
   const c10::DeviceGuard guard(g_.device());
@@ -166,11 +174,10 @@ GroupSeconds group_backward2(const Kept& kept, const Tensor& g_, const Tensor& w
   if (need_b) out.b = at::empty({n.channels}, g.options());
   const int64_t bytes = ictc_group_norm_workspace_bytes(dt, 2, n.samples, n.positions, n.channels, (int)n.groups);
   const Tensor ws = workspace(bytes, g);
-  const float* st = stats.const_data_ptr<float>();
-  done(ictc_group_norm_bwd2(dt, ptr(x), kept.code(), kept.scale(), ptr(g), ptr(v), ptr(vw), ptr(vb), n.samples,
-                            n.positions, n.channels, (int)n.groups, ptr(w), ptr(b), n.silu, st,
-                            st + n.samples * n.groups, ptr(out.x), ptr(out.g), ptr(out.w), ptr(out.b), ptr(ws), bytes,
-                            stream_of(g)),
+  done(ictc_group_norm_bwd2_rest(dt, ptr(x), kept.code(), kept.scale(), ptr(g), ptr(v), ptr(vw), ptr(vb), n.samples,
+                                 n.positions, n.channels, (int)n.groups, ptr(w), ptr(b), n.silu, stats.mean(),
+                                 stats.left(), stats.rstd(n), ptr(out.x), ptr(out.g), ptr(out.w), ptr(out.b), ptr(ws),
+                                 bytes, stream_of(g)),
        "group_norm");
   return out;
 }
@@ -179,7 +186,7 @@ GroupSeconds group_backward2(const Kept& kept, const Tensor& g_, const Tensor& w
 struct GroupNormSecond : Function<GroupNormSecond> {
   static variable_list forward(AutogradContext*, const OptTensor& place, const Tensor& g, const OptTensor& w,
                                const OptTensor& b, const OptTensor& v, const OptTensor& vw, const OptTensor& vb,
-                               const Kept& kept, const Tensor& stats, const NormShape& n, bool need_x, bool need_g,
+                               const Kept& kept, const Stats& stats, const NormShape& n, bool need_x, bool need_g,
                                bool need_w, bool need_b) {
     const GroupSeconds s = group_backward2(kept, g, value(w), value(b), value(v), value(vw), value(vb), stats, n, need_x,
                                            need_g, need_w, need_b);
@@ -211,10 +218,10 @@ NormShape kept_shape(AutogradContext* ctx) {
 // the bias.
 struct GroupNormGrad : Function<GroupNormGrad> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const OptTensor& w,
-                               const OptTensor& b, const Kept& kept, const Tensor& stats, const NormShape& n, bool need_x,
+                               const OptTensor& b, const Kept& kept, const Stats& stats, const NormShape& n, bool need_x,
                                bool need_w, bool need_b) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, g, value(w), value(b), stats, kept.codes, kept.scales});
+    ctx->save_for_backward({x, g, value(w), value(b), stats.both, stats.rest, kept.codes, kept.scales});
     ctx->saved_data["needs"] = (int64_t)(need_x | need_w << 1 | need_b << 2);
     keep(ctx, n);
     const GroupGrads s = group_backward(kept, g, value(w), value(b), stats, n, need_x, need_w, need_b);
@@ -225,9 +232,10 @@ struct GroupNormGrad : Function<GroupNormGrad> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &g = saved[1], &w = saved[2], &b = saved[3], &stats = saved[4];
-    const bool eight = saved[5].defined();
-    const Kept kept = {eight ? Tensor() : x, saved[5], saved[6]};
+    const Tensor &x = saved[0], &g = saved[1], &w = saved[2], &b = saved[3];
+    const Stats stats = {saved[4], saved[5]};
+    const bool eight = saved[6].defined();
+    const Kept kept = {eight ? Tensor() : x, saved[6], saved[7]};
     const int64_t needs = ctx->saved_data["needs"].toInt();
     const NormShape n = kept_shape(ctx);
     Tensor v[3];
@@ -254,18 +262,17 @@ struct GroupNormGrad : Function<GroupNormGrad> {
   }
 };
 
-// stats: the groups' mean and 1 / deviation, or undefined
-Tensor group_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, const Tensor& stats,
+// stats: may be undefined
+Tensor group_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, const Stats& stats,
                      const NormShape& n, const Codes& codes = Codes()) {
   const Tensor x = packed(x_), w = packed(w_), b = packed(b_);
   Tensor y = at::empty(x.sizes(), x.options());
-  float* st = stats.defined() ? stats.mutable_data_ptr<float>() : nullptr;
   const int64_t bytes =
       ictc_group_norm_workspace_bytes(dtype_of(x), 0, n.samples, n.positions, n.channels, (int)n.groups);
   const Tensor ws = workspace(bytes, x);
-  done(ictc_group_norm_fwd(dtype_of(x), ptr(x), n.samples, n.positions, n.channels, (int)n.groups, ptr(w), ptr(b),
-                           (float)eps, n.silu, ptr(y), st, st ? st + n.samples * n.groups : nullptr,
-                           (int8_t*)ptr(codes.codes), (float*)ptr(codes.scales), ptr(ws), bytes, stream_of(x)),
+  done(ictc_group_norm_fwd_rest(dtype_of(x), ptr(x), n.samples, n.positions, n.channels, (int)n.groups, ptr(w), ptr(b),
+                                (float)eps, n.silu, ptr(y), stats.mean(), stats.left(), stats.rstd(n),
+                                (int8_t*)ptr(codes.codes), (float*)ptr(codes.scales), ptr(ws), bytes, stream_of(x)),
        "group_norm");
   return y;
 }
@@ -273,20 +280,24 @@ Tensor group_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, doubl
 struct GroupNorm : Function<GroupNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps,
                         const NormShape& n, const c10::IValue& place) {
-    const Tensor stats = floats(2 * n.samples * n.groups, x);
+    Stats stats = {floats(2 * n.units(), x), Tensor()};
     Codes codes;
     if (!place.isNone()) {
       ctx->saved_data["place"] = place;
       codes = empty_codes(n.samples * n.positions, n.channels, x);
+    } else if (ictc_group_norm_keeps_rest(dtype_of(x), n.samples, n.positions, n.channels, (int)n.groups)) {
+      stats.rest = floats(n.units(), x);
     }
-    ctx->save_for_backward({codes.codes.defined() ? Tensor() : x, value(w), value(b), stats, codes.codes, codes.scales});
+    ctx->save_for_backward({codes.codes.defined() ? Tensor() : x, value(w), value(b), stats.both, stats.rest, codes.codes,
+                            codes.scales});
     keep(ctx, n);
     return group_forward(x, value(w), value(b), eps, stats, n, codes);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &w = saved[1], &b = saved[2], &stats = saved[3];
-    const Kept kept = {saved[0], saved[4], saved[5]};
+    const Tensor &w = saved[1], &b = saved[2];
+    const Stats stats = {saved[3], saved[4]};
+    const Kept kept = {saved[0], saved[5], saved[6]};
     const NormShape n = kept_shape(ctx);
     const std::vector<bool> want = wanted(ctx, {true, w.defined(), b.defined()});
     variable_list out(6);
@@ -328,7 +339,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& w, const Opt
   for (int64_t i = 1; i + 1 < x.dim(); ++i) positions *= x.size(i);
   const NormShape n = {x.size(0), positions, groups, (int)C, activation.has_value()};
   const Tensor wv = value(w), bv = value(b);
-  if (!tracked({&x, &wv, &bv})) return group_forward(x, wv, bv, eps, Tensor(), n);
+  if (!tracked({&x, &wv, &bv})) return group_forward(x, wv, bv, eps, Stats(), n);
   return GroupNorm::apply(x, w, b, eps, n, eight ? c10::IValue(Place8::apply(x)) : c10::IValue());
 }
 

@@ -141,6 +141,13 @@ _SIGNATURES = {
     "ictc_group_norm_bwd": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "ictc_group_norm_bwd2": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p,
                                   _p, _i64, _p]),
+    "ictc_group_norm_keeps_rest": (_i, [_i, _i64, _i64, _i, _i]),
+    "ictc_group_norm_fwd_rest": (_i, [_i, _p, _i64, _i64, _i, _i, _p, _p, ctypes.c_float, _i, _p, _p, _p, _p, _p, _p, _p,
+                                      _i64, _p]),
+    "ictc_group_norm_bwd_rest": (_i, [_i, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                      _p]),
+    "ictc_group_norm_bwd2_rest": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p,
+                                       _p, _p, _p, _i64, _p]),
     "ictc_rows_by_id_workspace_bytes": (_i64, [_i64, _i64]),
     "ictc_rows_by_id": (_i, [_p, _i64, _i64, _p, _p, _p, _i64, _p]),
     "ictc_embedding_fwd": (_i, [_i, _p, _i64, _i, _p, _i64, ctypes.c_float, _p, _p]),

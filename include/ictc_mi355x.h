@@ -795,7 +795,12 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  *         (dgrad), by weight and by bias (zero without an activation); vweight / vbias NULL:
  *         absent.
  * Sums over samples have a fixed order.  Workspace of ictc_group_norm_workspace_bytes bytes
- * (pass 0: fwd, 1: bwd, 2: bwd2), 8-byte aligned (0: none needed, -1: out of range).     */
+ * (pass 0: fwd, 1: bwd, 2: bwd2), 8-byte aligned (0: none needed, -1: out of range).
+ * The calls with _rest also give and take mean_rest [samples, groups] FP32, what the means'
+ * rounding to FP32 left of them (NULL: nothing), so that the backward passes' h is as exact as
+ * x, as fwd's is.  Without, half a unit of the mean may be in every h of a group: 2^-25 times
+ * the mean over the deviation.  Only where ictc_group_norm_keeps_rest says so (FP32, samples
+ * that are not held in registers) is it written or read; codes need none.                */
 int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, int64_t positions, int channels,
                                         int groups);
 int ictc_group_norm_fwd(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
@@ -811,6 +816,21 @@ int ictc_group_norm_bwd2(int dtype, const void* x, const int8_t* codes, const fl
                          int channels, int groups, const void* weight, const void* bias, int activation,
                          const float* mean, const float* rstd, void* dx, void* dgrad, void* dweight, void* dbias,
                          void* workspace, int64_t workspace_bytes, void* stream);
+int ictc_group_norm_keeps_rest(int dtype, int64_t samples, int64_t positions, int channels, int groups);
+int ictc_group_norm_fwd_rest(int dtype, const void* x, int64_t samples, int64_t positions, int channels, int groups,
+                             const void* weight, const void* bias, float eps, int activation, void* y, float* mean,
+                             float* mean_rest, float* rstd, int8_t* codes, float* scales, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+int ictc_group_norm_bwd_rest(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                             int64_t samples, int64_t positions, int channels, int groups, const void* weight,
+                             const void* bias, int activation, const float* mean, const float* mean_rest,
+                             const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+int ictc_group_norm_bwd2_rest(int dtype, const void* x, const int8_t* codes, const float* scales, const void* grad,
+                              const void* v, const void* vweight, const void* vbias, int64_t samples, int64_t positions,
+                              int channels, int groups, const void* weight, const void* bias, int activation,
+                              const float* mean, const float* mean_rest, const float* rstd, void* dx, void* dgrad,
+                              void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Rows of a table chosen by an id ---------------------------------------
  * out[n] = scale table[ids[n]] with table [entries, width] and out [rows, width] packed,

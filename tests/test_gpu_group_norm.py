@@ -477,3 +477,62 @@ def test_samples_of_one_large_value_in_many_small_groups(device, shape, dtype, b
         _close(first[0], ref[0], TOL[dtype], "dx")
         _close_sum(first[1], ref[1], sizes[0], "dw")
         _close_sum(first[2], ref[2], sizes[1], "db")
+
+
+@pytest.mark.parametrize("spread", [2.0 ** -12, 2.0 ** -17, 2.0 ** -20])
+@pytest.mark.parametrize("shape", [(40, 1, 64, 8), (33, 1, 60, 5), (3, 1, 8192, 1), (40, 6, 32, 4), (9, 5, 45, 5),
+                                   (40, 300, 32, 4), (3, 513, 5, 5), (1, 9000, 16, 2), (1, 131072, 64, 64),
+                                   (1, 700, 2304, 1), (3001, 401, 7, 7), (1, 131072, 65, 13)])
+def test_means_far_from_zero_as_near_ones(device, shape, spread):
+    """Means of up to 2^20 deviations, in every form and pass.  x less its mean is as exact as x is: less the mean in FP32
+    without an error (the operands are within a factor of two), less what that rounding left with one of half a unit of
+    the result.  So the bounds are the ordinary ones, and those of sums count h itself and not x and the mean; ga
+    depends on h by the activation, with a slope of at most 1/2."""
+    from ictc_o3 import group_norm
+    x, w, b, gy, v, vw, vb = _inputs(shape, torch.float32, device, 6)
+    x = x + 1.2345 / spread * (1 + torch.rand(shape[0], *[1] * (x.dim() - 1), device=device,
+                                               generator=torch.Generator(device).manual_seed(3)))
+    for t in (x, w, b, gy):
+        t.requires_grad_()
+    for activation in (None, "silu"):
+        y = group_norm(x, shape[3], w, b, eps=EPS, activation=activation)
+        first = torch.autograd.grad(y, (x, w, b), gy, create_graph=True)
+        second = torch.autograd.grad(first, (x, gy, w, b), (v, vw, vb), allow_unused=True)
+        d = Derivatives(x.detach(), shape[3], w.detach(), b.detach(), EPS, activation, gy.detach())
+        ref, _ = d.first()
+        _close(y, definition(x.detach().double(), shape[3], w.detach().double(), b.detach().double(), EPS, activation), 1e-5,
+               "y")
+        _close(first[0], ref[0], 1e-5, "dx")
+        size = d.g.abs() * (1.1 + d.h.abs() / 2)
+        _close_sum(first[1], ref[1], d._channels(size * (1 + d.h.abs())), "dw")
+        _close_sum(first[2], ref[2], d._channels(size), "db")
+        ref, _ = d.second(v, vw, vb)
+        _close(second[0], ref[0], 4e-5, "dx'")
+        _close(second[1], ref[1], 4e-5, "dg'")
+
+
+@pytest.mark.parametrize("shape", [(40, 1, 64, 8), (40, 300, 32, 4), (1, 9000, 16, 2), (1, 131072, 64, 64)])
+def test_one_value_of_a_mean(device, shape):
+    """The entry points without the means' rest: the same output; gradients off by half a unit of the mean in h."""
+    from ictc_o3 import _native as nat
+    from ictc_o3 import group_norm
+    samples, positions, channels, groups = shape
+    x, w, b, gy, *_ = _inputs(shape, torch.float32, device, 6)
+    x = (x + 100.0).requires_grad_()
+    y = group_norm(x, groups, w, b, eps=EPS, activation="silu")
+    (dx,) = torch.autograd.grad(y, x, gy)
+    mean, rstd = torch.empty(2, samples, groups, device=device)
+    out, got = torch.empty_like(x), torch.empty_like(x)
+    size = nat.lib().ictc_group_norm_workspace_bytes
+    sizes = [size(0, k, samples, positions, channels, groups) for k in (0, 1)]
+    ws = torch.empty(max(*sizes, 8), dtype=torch.uint8, device=device)
+    at = (samples, positions, channels, groups, w.data_ptr(), b.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    nat.call("ictc_group_norm_fwd", 0, x.data_ptr(), *at, EPS, 1, out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), None, None,
+             ws.data_ptr(), sizes[0], stream)
+    nat.call("ictc_group_norm_bwd", 0, x.data_ptr(), None, None, gy.data_ptr(), *at, 1, mean.data_ptr(), rstd.data_ptr(),
+             got.data_ptr(), None, None, ws.data_ptr(), sizes[1], stream)
+    X = x.detach().double().view(samples, -1, groups, channels // groups)
+    assert torch.equal(out, y) and rel_err(mean, X.mean((1, 3))) < 2.0 ** -23
+    # half a unit of the mean times r, in h and with a slope of two or less in all that follows; and the ordinary bound
+    assert rel_err(got, dx.double()) < 1e-5 + 2 * 2.0 ** -25 * (X.mean((1, 3)).abs() * rstd).max() * 4

@@ -77,3 +77,27 @@ def test_native_refusals():
     with pytest.raises(ValueError):
         bwd(**{**second, "v": (None, None, None)})
     bwd(out=(None, None, None))
+
+
+def test_native_refusals_of_the_means_rest():
+    from ictc_o3 import _native as nat
+    if not os.path.exists(nat.library_path()):
+        pytest.skip("library not built")
+    keeps = nat.lib().ictc_group_norm_keeps_rest
+    assert keeps(0, 3, 300, 64, 8) and keeps(0, 1, 100000, 64, 8) and not keeps(0, 100, 1, 64, 8)
+    for none in ((1, 3, 300, 64, 8), (2, 3, 300, 64, 8), (0, 0, 300, 64, 8), (0, 3, 0, 64, 8), (0, 3, 300, 64, 7), (4, 3, 300, 64, 8)):
+        assert not keeps(*none), none
+
+    def fwd(mean=16, rest=16, rstd=16, x=16, samples=2):
+        nat.call("ictc_group_norm_fwd_rest", 0, x, samples, 3, 8, 2, None, None, 1e-5, 0, 16, mean, rest, rstd, None, None,
+                 None, 0, None)
+
+    for bad in (dict(mean=None), dict(mean=None, rstd=None), dict(rstd=None), dict(x=None), dict(samples=-1)):
+        with pytest.raises(ValueError):
+            fwd(**bad)
+    fwd(samples=0)
+    for name, v, out in (("ictc_group_norm_bwd_rest", (), (16, 16, 16)),
+                         ("ictc_group_norm_bwd2_rest", (16, None, None), (16, 16, 16, 16))):
+        for mean, rstd, ws in ((None, 16, 16), (16, None, 16), (16, 16, None)):
+            with pytest.raises(ValueError):
+                nat.call(name, 0, 16, None, None, 16, *v, 2, 3, 8, 2, None, None, 0, mean, 16, rstd, *out, ws, 1 << 20, None)
