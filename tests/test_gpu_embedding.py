@@ -374,3 +374,22 @@ def test_graph_replays_of_the_general_sort(device, rows, entries):
         assert torch.equal(held.perm.long(), torch.sort(key, stable=True).indices), k
         counts = torch.bincount(key, minlength=entries + 1)
         assert torch.equal(held.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)])), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [3, 9, 64, 130, 256, 1021])
+def test_gradient_of_few_rows_in_a_large_table(device, width, dtype):
+    """Up to 128 rows take no order: ids that repeat within and between what a lane holds, single ones, and the table's ends."""
+    from ictc_o3 import embedding
+    entries = 30011
+    for rows in (1, 7, 8, 63, 64, 65, 100, 127, 128):
+        g = torch.Generator().manual_seed(rows + width)
+        ids = torch.randint(0, entries, (rows,), generator=g)
+        ids[::3] = 77
+        ids[1::7] = entries - 1
+        ids[2::9] = torch.tensor([0, -1, entries, 2 ** 40 + 77, 5]).repeat(26)[: len(ids[2::9])]
+        ids = ids.to(device)
+        gy = torch.randn(rows, width, generator=g).to(dtype).to(device)
+        table = torch.zeros(entries, width, dtype=dtype, device=device, requires_grad=True)
+        (got,) = torch.autograd.grad(embedding(table, ids, 1.7), table, gy)
+        _check_sums(got, gy, ids, entries, 1.7)
