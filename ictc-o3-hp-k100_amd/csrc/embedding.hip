@@ -11,7 +11,7 @@
 // ones.  A team of lanes holds a chunk of columns in registers and adds consecutive sorted rows; a run of one id that
 // lies within the team's rows is written at once, the first and the last run of a team meet the neighbours' in LDS, and
 // those of a block that continue in other blocks leave FP32 partial sums (slot 0: continued from before; slot 1: begun
-// here) that a second kernel adds in order.  Every sum has a fixed order.  Up to 128 rows are added by one kernel that
+// here) that a second kernel adds in order, in FP64.  Every sum has a fixed order.  Up to 128 rows are added by one kernel that
 // looks the ids over itself.
 #include <algorithm>
 
@@ -261,19 +261,20 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const T* __restrict__ g
 }
 
 // The runs that cross ranges, each by the blocks of the range that it begins in, 64 columns a block: its partial sums added
-// by 16 slices and those in order.
+// by 16 slices and those in order, in FP64, for a run may have a tenth of all rows and more (4.2 million rows of 256 in a run
+// are 2,048 sums a slice: values alike lose 480 units of 2^-24 in FP32).
 template <typename T>
 __global__ __launch_bounds__(256) void embed_join_kernel(const float* __restrict__ part, const int* __restrict__ open,
                                                          int width, const int* __restrict__ off, float scale,
                                                          int64_t range, T* __restrict__ out) {
-  __shared__ float lds[16][64];
+  __shared__ double lds[16][64];
   const int64_t q = blockIdx.x;
   const int key = open[q];
   if (key < 0) return;
   const int64_t count = (off[key + 1] - 1) / range - q + 1;
   const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4;
   const int c = blockIdx.y * 64 + lane * 4, left = width - c;
-  float a[4] = {};
+  double a[4] = {};
 #pragma unroll 8
   for (int64_t j = slice; j < count; j += 16) {
     float x[4];
@@ -286,10 +287,10 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const float* __restrict
   __syncthreads();
   const int col = threadIdx.x;
   if (col < 64 && blockIdx.y * 64 + col < width) {
-    float s = 0.f;
+    double s = 0.0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += lds[i][col];
-    out[(int64_t)key * width + blockIdx.y * 64 + col] = (T)held(s * scale);
+    out[(int64_t)key * width + blockIdx.y * 64 + col] = (T)held(held((float)s) * scale);
   }
 }
 

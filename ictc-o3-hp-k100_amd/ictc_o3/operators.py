@@ -404,7 +404,7 @@ def embedding(table, ids, scale=1.0, order=None):
     """scale * table[ids] for a table [entries, width] (float32, bfloat16 or float16) and int64 ids of any shape, which
     the result's shape begins with.  An id outside [0, entries) (padding) gives a zero row and adds to no gradient.
 
-    The table's gradient adds the rows of each id in FP32, in a fixed order, and rounds once.  It takes the rows sorted
+    The table's gradient adds the rows of each id in FP32 or better, in a fixed order, and rounds once.  It takes the rows sorted
     by id: `order` from ``expert_order(ids, entries)`` where one is at hand (ids of one axis), else it sorts them
     itself.  Differentiable to any order."""
     if order is None:

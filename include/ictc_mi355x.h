@@ -835,7 +835,7 @@ int ictc_group_norm_bwd2_rest(int dtype, const void* x, const int8_t* codes, con
 /* ---- Rows of a table chosen by an id ---------------------------------------
  * out[n] = scale table[ids[n]] with table [entries, width] and out [rows, width] packed,
  * element type dtype; an id outside [0, entries) gives a zero row.  bwd: dtable[v] = scale
- * times the sum of grad's rows (pitch ldg) whose id is v, FP32 sums in a fixed order, zeros
+ * times the sum of grad's rows (pitch ldg) whose id is v, sums in FP32 or better in a fixed order, zeros
  * for an entry without rows.  perm and offsets are the rows' order by id, what
  * ictc_expert_order and ictc_csr_build give for these ids and `entries` keys; up to as many
  * rows as ictc_embedding_needs_order denies they may be NULL.  Workspace of

@@ -393,3 +393,24 @@ def test_gradient_of_few_rows_in_a_large_table(device, width, dtype):
         table = torch.zeros(entries, width, dtype=dtype, device=device, requires_grad=True)
         (got,) = torch.autograd.grad(embedding(table, ids, 1.7), table, gy)
         _check_sums(got, gy, ids, entries, 1.7)
+
+
+@pytest.mark.parametrize("values", ["alike", "random"])
+@pytest.mark.parametrize("rows,width", [(4200001, 256), (4200001, 7)])
+def test_sums_of_very_many_rows(device, rows, width, values):
+    """Millions of rows of one id.  A sum's additions in FP32: up to 32 rows of a team and 32 teams of a block; its blocks' are
+    in FP64, and two roundings follow.  Values alike of 19 bits make every FP32 sum of a block exact, and would lose nearly
+    half a unit of a long FP32 sum of blocks in the same direction each time (256 wide 480 units of 2^-24)."""
+    from ictc_o3 import embedding
+    table = torch.zeros(3, width, device=device, requires_grad=True)
+    ids = torch.ones(rows, dtype=torch.int64, device=device)
+    ids[:300], ids[-5000:] = 0, 2
+    if values == "alike":
+        gy = torch.full((rows, width), 1 + 2.0 ** -14 - 2.0 ** -19, device=device)
+    else:
+        gy = torch.rand(rows, width, device=device, generator=torch.Generator(device).manual_seed(width))
+    (got,) = torch.autograd.grad(embedding(table, ids), table, gy)
+    parts = gy[:300], gy[300:-5000], gy[-5000:]
+    ref = torch.stack([sum(t.double().sum(0) for t in part.split(1 << 18)) for part in parts])
+    units = 2 if values == "alike" else 66
+    assert ((got.double() - ref).abs() <= units * 2.0 ** -24 * ref).all()
