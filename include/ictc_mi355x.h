@@ -790,7 +790,9 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  * weight / bias NULL: ones / zeros.  mean and rstd [samples, groups] FP32 may both be NULL
  * in fwd; codes and scales NULL, or what ictc_codes_encode gives of x as rows of `channels`.
  *   bwd:  dx, dweight [channels], dbias [channels], each NULL to skip; no elements give zero
- *         dweight and dbias.  With codes and scales x is not read: h = (value - mean) rstd stands for the normalised x.
+ *         dweight and dbias.  With codes and scales x is not read: h = (value - mean) rstd stands
+ *         for the normalised x, off by up to half a scale times rstd (means of many deviations, or
+ *         groups much smaller than others of their block of 128, leave little of it).
  *   bwd2: the gradients of <v, dx> + <vweight, dweight> + <vbias, dbias> by x (dx), by grad
  *         (dgrad), by weight and by bias (zero without an activation); vweight / vbias NULL:
  *         absent.

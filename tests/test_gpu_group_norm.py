@@ -536,3 +536,25 @@ def test_one_value_of_a_mean(device, shape):
     assert torch.equal(out, y) and rel_err(mean, X.mean((1, 3))) < 2.0 ** -23
     # half a unit of the mean times r, in h and with a slope of two or less in all that follows; and the ordinary bound
     assert rel_err(got, dx.double()) < 1e-5 + 2 * 2.0 ** -25 * (X.mean((1, 3)).abs() * rstd).max() * 4
+
+
+@pytest.mark.parametrize("shape", [(300, 1, 64, 8), (9, 5, 45, 5), (40, 300, 32, 4), (1, 9000, 160, 2), (501, 1000, 30, 5)])
+@pytest.mark.parametrize("far", [0.0, 3.0, 30.0])
+def test_error_of_gradients_from_8_bits(device, shape, far):
+    """What is promised of x kept in 8 bits: h is off by at most half a scale (1/254 of the largest magnitude of its block of
+    128 channels) times r, so without an activation dw is off by as much of each of its terms, and dx by r (|eh| <u h> +
+    |h| <u eh>) with both h's; and by the ordinary bounds."""
+    from ictc_o3 import encode_activations, group_norm
+    x, w, b, gy, *_ = _inputs(shape, torch.float32, device, 4)
+    x = x + far
+    scales = encode_activations(x)[1].double().repeat_interleave(128, -1)[..., :shape[2]]
+    x, w = x.requires_grad_(), w.requires_grad_()
+    got = torch.autograd.grad(group_norm(x, shape[3], w, b, eps=EPS, save_bits=8), (x, w), gy)
+    d = Derivatives(x.detach(), shape[3], w.detach(), b, EPS, None, gy)
+    (dx, dw, _), (sw, _) = d.first()
+    off = (scales * (0.5 + 127 * 2.0 ** -21)).view(d.h.shape) * d.r
+    mean = lambda t: t.abs().mean((1, 3), keepdim=True)
+    u = d.ga * d.w
+    bound = d.r * (off * (mean(u * d.h) + mean(u * off)) + d.h.abs() * mean(u * off))
+    assert ((got[1].double() - dw).abs() <= d._channels(d.ga.abs() * off) + 600 * 2.0 ** -24 * (sw + d._channels(d.ga.abs() * off))).all()
+    assert ((got[0].double() - dx).abs() <= bound.view(x.shape) + 1e-5 * (dx.abs().max() + bound.max())).all()
