@@ -15,7 +15,7 @@
 //  * Rows: up to four chunks a lane of up to 64 lanes; of single positions, up to 32 elements a lane of a block.  This team
 //    holds it in registers: one read.  It keeps its group, so the parameters stay in registers and their gradients are
 //    added per lane.  (425,991 x 64 FP32 in eight groups: forward 48 us, gradients 60, 5.1 and 5.9 TB/s; one position of
-//    4,096 bfloat16 channels by a block's team, 8,192 samples: gradients 106 us, by parts 204.)
+//    4,096 bfloat16 channels by a block's team, 8,192 samples: forward 29 us and gradients 72, both by parts 204.)
 //  * Tiles: a block takes some whole groups of a sample and reads them twice, for the sums and for the result, the second
 //    time from the caches; one launch.  (32 x 256 positions x 128 FP32: forward 6 us, gradients 8, second derivative 13.)
 //  * Parts: few large samples.  The sums by many blocks, a small kernel that adds their parts in order (few parts are added
@@ -192,7 +192,9 @@ __device__ __forceinline__ int code_blocks(int C) { return (C + kCodeBlock - 1) 
 // The formulas, element by element
 // ---------------------------------------------------------------------------
 
-// act(z), and its derivatives.  (An exponential past FP32 makes the sigmoid zero, as it is to within 2^-128.)
+// act(z), and its derivatives.  The sigmoid is the hardware's reciprocal of 1 + its power of two, each off by up to one unit
+// of FP32 where a correctly rounded quotient is off by half; with the argument's rounding (1.5 |z| units) FP32 results are off
+// by 1.0 to 1.6 times what rounded steps give, inside the bounds of the row results.  (An exponential past FP32 makes the sigmoid zero, as it is to within 2^-128.)
 template <bool SILU>
 struct Act {
   float s, z;
