@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256) void decode_kernel(const int8_t* __restrict__ 
   }
 }
 
-// Blocks of a row.  (Of any width that an int holds: a row of 2^31 - 1 elements has 2^24, the last chunk's column is below 2^31.)
+// Blocks of a row.  (Of any width that an int holds: a row of 2^31 - 1 elements has 2^24, the last chunk's column is
+// below 2^31.)
 int blocks_of(int width) { return (width - 1) / kCodeBlock + 1; }
 
 // Lanes of a block's chunks: all of 128 elements, fewer where rows are shorter.

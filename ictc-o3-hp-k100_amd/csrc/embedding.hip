@@ -11,8 +11,8 @@
 // ones.  A team of lanes holds a chunk of columns in registers and adds consecutive sorted rows; a run of one id that
 // lies within the team's rows is written at once, the first and the last run of a team meet the neighbours' in LDS, and
 // those of a block that continue in other blocks leave FP32 partial sums (slot 0: continued from before; slot 1: begun
-// here) that a second kernel adds in order, in FP64.  Every sum has a fixed order.  Up to 128 rows are added by one kernel that
-// looks the ids over itself.
+// here) that a second kernel adds in order, in FP64.  Every sum has a fixed order.  Up to 128 rows are added by one kernel
+// that looks the ids over itself.
 #include <algorithm>
 
 #include "dense.h"
@@ -77,9 +77,9 @@ __device__ __forceinline__ void write_scaled(T* __restrict__ p, const float (&ac
   store_pack<T, V>(p, v);
 }
 
-// Few rows: a team per entry adds the rows whose id is its own, in their order.  Its lanes hold the ids, kFewRows / L each, and
-// compare them with the entry all at once, so an entry without rows costs a ballot and its store.  Measured
-// in us, 128 rows this way / 129 in order with the order's launches, FP32: ten entries of 64 5 / 12; 10,000 5 / 19; 150,000
+// Few rows: a team per entry adds the rows whose id is its own, in their order.  Its lanes hold the ids, kFewRows / L
+// each, and compare them with the entry all at once, so an entry without rows costs a ballot and its store.  Measured in
+// us, 128 rows this way / 129 in order with the order's launches, FP32: ten entries of 64 5 / 12; 10,000 5 / 19; 150,000
 // 14 / 28; a million 67 / 66, of 128 78 / 121.  (Each team looking all ids over in LDS: 28, 29, 133, 774 and 1,533.)
 template <typename T, int V, int L>
 __global__ __launch_bounds__(256) void embed_few_kernel(const T* __restrict__ g, int64_t ldg, int rows, int width,

@@ -528,11 +528,11 @@ __device__ __forceinline__ int first_place(const int* __restrict__ keys, int n, 
 }
 
 // off[k] = the first place of sorted keys [n] that holds k or more, for k of 0 .. experts + 1.  A place fills the offsets
-// from the key before it to its own, long gaps with its wave; but of a gap the whole spans of kSpan offsets (from multiples
-// of it) are filled by a wave each, of the blocks behind the places', so that few rows, or ids side by side, of many entries
-// do not keep one wave; and a wave has only eight places where most gaps are long (the whole order of 5 rows of a million entries 484 -> 16 us, of 33.5 million 15.8 ms ->
-// 34 us).  Offsets are
-// unsigned: experts + 2 may be 2^31 - 1, and a step past it.
+// from the key before it to its own, long gaps with its wave; but of a gap the whole spans of kSpan offsets (from
+// multiples of it) are filled by a wave each, of the blocks behind the places', so that few rows, or ids side by side, of
+// many entries do not keep one wave; and a wave has only eight places where most gaps are long (the whole order of 5 rows
+// of a million entries 484 -> 16 us, of 33.5 million 15.8 ms -> 34 us).  Offsets are unsigned: experts + 2 may be
+// 2^31 - 1, and a step past it.
 constexpr uint32_t kSpan = 1024;
 __global__ __launch_bounds__(256) void order_offsets_kernel(const int* __restrict__ keys, int n, uint32_t experts,
                                                             int each, int place_blocks, int* __restrict__ off) {

@@ -25,14 +25,15 @@
 // codes.  Groups that only small chunks divide are cut into 16-byte chunks, the last in part (rows), or their tile is,
 // whatever the groups (group_norm_span.h).
 //
-// Means far from zero: statistics of tiles and parts are sums in FP64 of x less the group's first element (FP32; the sums of
-// 16-bit values near one another and of their squares are exact) and of its squares, which costs little beside memory, loses
-// nothing to what all of a group have in common and holds squares past FP32's range.  Of FP32 x a mean has two FP32 values,
-// itself and what its rounding left, and both are taken from x wherever h is made: x less the rounded mean is exact where
-// they are near, so h is as good as x is.  (By the rounded mean alone every h of a group is off by half a unit of the mean:
-// with a mean of 2^20 deviations 3 to 8 % of the results.)  The rows' backward passes find the second value anew, where it
-// counts, for there is one for every few elements; tiles and parts read it.  Half a unit of the mean is at most 2^-14 of the largest deviation of 16-bit x, and
-// 2^-17 of the error of x kept in 8 bits, so there it is left.  Every sum has a fixed order.
+// Means far from zero: statistics of tiles and parts are sums in FP64 of x less the group's first element (FP32; the sums
+// of 16-bit values near one another and of their squares are exact) and of its squares, which costs little beside memory,
+// loses nothing to what all of a group have in common and holds squares past FP32's range.  Of FP32 x a mean has two FP32
+// values, itself and what its rounding left, and both are taken from x wherever h is made: x less the rounded mean is
+// exact where they are near, so h is as good as x is.  (By the rounded mean alone every h of a group is off by half a
+// unit of the mean: with a mean of 2^20 deviations 3 to 8 % of the results.)  The rows' backward passes find the second
+// value anew, where it counts, for there is one for every few elements; tiles and parts read it.  Half a unit of the mean
+// is at most 2^-13 of the largest deviation of 16-bit x, and 2^-16 of the error of x kept in 8 bits, so there it is left.
+// Every sum has a fixed order.
 #pragma once
 #include <algorithm>
 
@@ -192,9 +193,10 @@ __device__ __forceinline__ int code_blocks(int C) { return (C + kCodeBlock - 1) 
 // The formulas, element by element
 // ---------------------------------------------------------------------------
 
-// act(z), and its derivatives.  The sigmoid is the hardware's reciprocal of 1 + its power of two, each off by up to one unit
-// of FP32 where a correctly rounded quotient is off by half; with the argument's rounding (1.5 |z| units) FP32 results are off
-// by 1.0 to 1.6 times what rounded steps give, inside the bounds of the row results.  (An exponential past FP32 makes the sigmoid zero, as it is to within 2^-128.)
+// act(z), and its derivatives.  The sigmoid is the hardware's reciprocal of 1 + its power of two, each off by up to one
+// unit of FP32 where a correctly rounded quotient is off by half; with the argument's rounding (1.5 |z| units) FP32
+// results are off by 1.0 to 1.6 times what rounded steps give, inside the bounds of the row results.  (An exponential
+// past FP32 makes the sigmoid zero, as it is to within 2^-128.)
 template <bool SILU>
 struct Act {
   float s, z;

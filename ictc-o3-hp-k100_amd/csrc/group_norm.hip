@@ -70,7 +70,8 @@ int ictc_group_norm_fwd_rest(int dtype, const void* x, int64_t samples, int64_t 
   if (!(eps >= 0.f)) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: eps must not be negative");
   if (activation != 0 && activation != 1) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: activation must be 0 or 1");
   if (samples == 0 || positions == 0) return ICTC_OK;
-  if (!x || !y || !mean != !rstd || (rest && !mean) || !codes != !scales) return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
+  if (!x || !y || !mean != !rstd || (rest && !mean) || !codes != !scales)
+    return dense_fail(ICTC_ERR_ARGUMENT, "group_norm: null operand");
   ictc::GroupNormCall a = {};
   a.samples = samples, a.positions = positions, a.channels = channels, a.groups = groups;
   a.x = x, a.w = weight, a.b = bias, a.eps = eps, a.silu = activation, a.out = y, a.mean = mean, a.rest = rest,

@@ -181,7 +181,7 @@ __device__ __forceinline__ void rows_channels(float (&acc)[N][EV], const RowsPla
 }
 
 // The team's mean as the backward passes take it: of FP32 x with what its rounding to `mean` left, the mean of x less it,
-// where that counts: half a unit of a mean of up to eight deviations 1 / r is 2^-22 of one.  (425,991 x 64 in eight groups,
+// where that counts: half a unit of a mean of up to eight deviations 1 / r is 2^-21 of one.  (425,991 x 64 in eight groups,
 // gradients 60 us; looked for by every team, or read from memory, 66.)
 template <typename T, int EV, int N, bool WIDE, bool PART, bool EIGHT, typename X>
 __device__ __forceinline__ Mean rows_mean(const X (&rx)[N], const int (&n)[N], float mean, float r, float inv, int team,

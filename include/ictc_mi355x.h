@@ -800,7 +800,7 @@ int ictc_expert_outer(int dtype, const void* grad, int64_t ldg, const void* x, i
  * (pass 0: fwd, 1: bwd, 2: bwd2), 8-byte aligned (0: none needed, -1: out of range).
  * The calls with _rest also give and take mean_rest [samples, groups] FP32, what the means'
  * rounding to FP32 left of them (NULL: nothing), so that the backward passes' h is as exact as
- * x, as fwd's is.  Without, half a unit of the mean may be in every h of a group: 2^-25 times
+ * x, as fwd's is.  Without, half a unit of the mean may be in every h of a group: 2^-24 times
  * the mean over the deviation.  Only where ictc_group_norm_keeps_rest says so (FP32, samples
  * that are not held in registers) is it written or read; codes need none.                */
 int64_t ictc_group_norm_workspace_bytes(int dtype, int pass, int64_t samples, int64_t positions, int channels,
